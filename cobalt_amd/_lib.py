@@ -10,6 +10,21 @@ import os
 
 from .format import CbkDesc  # noqa: F401 (re-exported for callers that build descriptor arrays)
 
+
+class CbkCache(ctypes.Structure):
+    """struct cbk_cache (include/cbk.h)"""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_meta", ctypes.c_void_p),
+                ("v_meta", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
+class CbkRows(ctypes.Structure):
+    """struct cbk_rows (include/cbk.h)"""
+    _fields_ = [("table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("lens", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("seqs", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+                ("tokens", ctypes.c_int64)]
+
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcbk_hip.so")
 _lib = None
@@ -18,6 +33,8 @@ _P = ctypes.c_void_p
 _DP = ctypes.POINTER(CbkDesc)
 _MM = [_DP, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64, _P, _P,
        ctypes.c_size_t, _P]
+_CP, _RP = ctypes.POINTER(CbkCache), ctypes.POINTER(CbkRows)
+_ROWS = [_P, ctypes.c_int64, ctypes.c_int64]                        # a dense tensor: address, strides of rows and heads
 SIGNATURES = {
     "cbk_abi_version": (ctypes.c_int, []),
     "cbk_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -39,6 +56,13 @@ SIGNATURES = {
     "cbk_linear": (ctypes.c_int, _MM),
     "cbk_linear_act_workspace_bytes": (ctypes.c_size_t, [_DP, ctypes.c_int, ctypes.c_int]),
     "cbk_linear_act": (ctypes.c_int, _MM[:9] + [ctypes.c_int] + _MM[9:]),
+    "cbk_cache_code_bytes": (ctypes.c_size_t, [_CP]),
+    "cbk_cache_meta_bytes": (ctypes.c_size_t, [_CP]),
+    "cbk_cache_write": (ctypes.c_int, [_CP, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache_read": (ctypes.c_int, [_CP, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache_attention_workspace_bytes": (ctypes.c_size_t, [_CP, _RP, ctypes.c_int]),
+    "cbk_cache_attention": (ctypes.c_int, [_CP, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                                                      ctypes.c_int, _P, ctypes.c_size_t, _P]),
 }
 ACT_CODE = {"gelu_tanh": 0, "silu": 1}
 

@@ -572,6 +572,186 @@ PyObject* py_pack_end(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------ the 4-bit key/value cache
+// The pool as Python holds it: (k_codes, v_codes, k_meta, v_meta, pages, page, heads, head_dim, group).
+struct Cache { at::Tensor t[4]; cbk_cache c; };
+Cache as_cache(PyObject* o) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 9) fail(PyExc_TypeError, "a KVCache is expected");
+  Cache r;
+  void* p[4];
+  for (int i = 0; i < 4; ++i) {
+    r.t[i] = as_tensor(PyTuple_GET_ITEM(o, i), "an array of the cache");
+    if (!r.t[i].defined()) fail(PyExc_TypeError, "a KVCache is expected");
+    p[i] = r.t[i].mutable_data_ptr();
+  }
+  long long v[5];
+  for (int i = 0; i < 5; ++i) v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, 4 + i));
+  if (PyErr_Occurred()) throw Fail{};
+  r.c = cbk_cache{p[0], p[1], p[2], p[3], (int64_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4]};
+  const size_t codes = cbk_cache_code_bytes(&r.c), meta = cbk_cache_meta_bytes(&r.c);
+  if (!codes || r.t[0].nbytes() < codes || r.t[1].nbytes() < codes || r.t[2].nbytes() < meta || r.t[3].nbytes() < meta)
+    fail(PyExc_ValueError, "the arrays of the cache do not hold what its description says");
+  if (!r.t[0].is_cuda()) fail(g_error, "the cache must live on the GPU; this package has no CPU execution path");
+  return r;
+}
+void same_device(const Cache& c, const at::Tensor& t) {
+  if (t.defined() && t.device() != c.t[0].device())
+    fail(g_error, "tensor on " + t.device().str() + ", cache on " + c.t[0].device().str());
+}
+struct RowMap { at::Tensor table, lens, starts; cbk_rows r; };
+RowMap as_rows(const Cache& c, PyObject* table, PyObject* lens, PyObject* starts, int64_t tokens) {
+  RowMap m;
+  m.table = as_tensor(table, "table");
+  m.lens = as_tensor(lens, "lens");
+  m.starts = as_tensor(starts, "starts");
+  if (!m.table.defined() || !m.lens.defined()) fail(PyExc_TypeError, "table and lens must be tensors");
+  for (const at::Tensor* t : {&m.table, &m.lens, &m.starts})
+    if (t->defined()) {
+      same_device(c, *t);
+      if (t->scalar_type() != at::kInt) fail(PyExc_TypeError, "table, lens and starts are int32 tensors");
+    }
+  if (m.table.dim() != 2 || m.lens.dim() != 1 || m.table.size(0) != m.lens.size(0))
+    fail(PyExc_ValueError, "table is [sequences, pages] and lens [sequences]");
+  const int64_t seqs = m.lens.size(0);
+  if (m.starts.defined() && (m.starts.dim() != 1 || m.starts.size(0) != seqs + 1))
+    fail(PyExc_ValueError, "starts has one entry more than there are sequences");
+  if (!m.starts.defined() && (seqs ? tokens % seqs : tokens))
+    fail(PyExc_ValueError, std::to_string(tokens) + " rows do not divide into " + std::to_string(seqs) + " sequences: give starts");
+  if ((m.table.size(1) > 1 && m.table.stride(1) != 1) || (seqs > 1 && m.lens.stride(0) != 1) ||
+      (m.starts.defined() && m.starts.size(0) > 1 && m.starts.stride(0) != 1))
+    fail(PyExc_ValueError, "lens, starts and the rows of table have unit stride");
+  if (seqs > INT32_MAX || m.table.size(1) > INT32_MAX) check(CBK_ERR_SHAPE, "cbk_rows");
+  const int64_t ld = seqs > 1 ? m.table.stride(0) : m.table.size(1);
+  m.r = cbk_rows{m.table.const_data_ptr(), ld, m.lens.const_data_ptr(), m.starts.defined() ? m.starts.const_data_ptr() : nullptr,
+                 (int32_t)seqs, (int32_t)m.table.size(1), tokens};
+  return m;
+}
+void check_heads(const at::Tensor& x, int64_t heads, int64_t dim, const char* what) {
+  if (x.dim() != 3 || x.size(2) != dim || (heads ? x.size(1) != heads : x.size(1) < 1))
+    fail(PyExc_ValueError, std::string(what) + " is [rows, heads, head_dim]");
+}
+bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+int64_t row_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : 0; }
+int64_t head_stride(const at::Tensor& x) { return x.size(1) > 1 ? x.stride(1) : 0; }
+bool readable16(const at::Tensor& x) {                              // by 16-byte pieces of its rows
+  const int64_t n = 16 / x.element_size();
+  return x.stride(2) == 1 && row_stride(x) % n == 0 && head_stride(x) % n == 0 && row_stride(x) >= 0 && head_stride(x) >= 0 &&
+         ((uintptr_t)x.const_data_ptr() & 15) == 0;
+}
+at::Tensor dense_in(const at::Tensor& x) { return readable16(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
+void check_out(const at::Tensor& o, int64_t rows, int64_t heads, int64_t dim, at::ScalarType t, const char* what) {
+  check_heads(o, heads, dim, what);
+  if (o.size(0) != rows || o.scalar_type() != t)
+    fail(PyExc_ValueError, std::string(what) + " must have " + std::to_string(rows) + " rows of type " + c10::toString(t));
+  const int64_t rs = row_stride(o), hs = head_stride(o);
+  const bool apart = (rows <= 1 || rs >= (heads - 1) * hs + dim || (heads > 1 && hs >= (rows - 1) * rs + dim)) &&
+                     (heads <= 1 || hs >= dim) && (rows <= 1 || rs >= dim);
+  if (rows && (!readable16(o) || !apart))
+    fail(PyExc_ValueError, std::string(what) + " must have unit stride along head_dim, rows that do not overlap and 16-byte aligned heads");
+}
+
+// cache_write(cache, k, v, table, lens, starts or None)
+PyObject* py_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 6)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Cache c = as_cache(a[0]);
+    at::Tensor k = as_tensor(a[1], "k"), v = as_tensor(a[2], "v");
+    if (!k.defined() || !v.defined()) fail(PyExc_TypeError, "k and v must be tensors");
+    same_device(c, k);
+    same_device(c, v);
+    check_heads(k, c.c.heads, c.c.head_dim, "k");
+    check_heads(v, c.c.heads, c.c.head_dim, "v");
+    if (k.size(0) != v.size(0) || k.scalar_type() != v.scalar_type() || !half_type(k.scalar_type()))
+      fail(PyExc_ValueError, "k and v have the same number of rows and are both float16 or both bfloat16");
+    const RowMap m = as_rows(c, a[3], a[4], a[5], k.size(0));
+    const int dt = dtype_code(k.scalar_type());
+    int rc = CBK_OK;
+    if (k.size(0)) {
+      const GilRelease other_threads_run;
+      const c10::DeviceGuard guard(k.device());
+      k = dense_in(k);
+      v = dense_in(v);
+      rc = cbk_cache_write(&c.c, &m.r, k.const_data_ptr(), row_stride(k), head_stride(k), v.const_data_ptr(), row_stride(v),
+                           head_stride(v), dt, stream_of(k));
+    }
+    check(rc, "cbk_cache_write");
+    Py_RETURN_NONE;
+  });
+}
+
+// cache_read(cache, table, lens, starts or None, rows, dtype, k or None, v or None) -> (k, v)
+PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 8)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Cache c = as_cache(a[0]);
+    const long long rows = PyLong_AsLongLong(a[4]);
+    if (PyErr_Occurred()) throw Fail{};
+    if (rows < 0) fail(PyExc_ValueError, "the number of rows is negative");
+    const RowMap m = as_rows(c, a[1], a[2], a[3], rows);
+    if (!THPDtype_Check(a[5])) fail(PyExc_TypeError, "dtype must be a torch.dtype");
+    const at::ScalarType t = ((THPDtype*)a[5])->scalar_type;
+    const int dt = dtype_code(t);
+    at::Tensor out[2] = {as_tensor(a[6], "k"), as_tensor(a[7], "v")};
+    for (at::Tensor& o : out)
+      if (o.defined()) {
+        same_device(c, o);
+        check_out(o, rows, c.c.heads, c.c.head_dim, t, "the output");
+      }
+    int rc = CBK_OK;
+    {
+      const GilRelease other_threads_run;
+      const c10::DeviceGuard guard(c.t[0].device());
+      for (at::Tensor& o : out)
+        if (!o.defined()) o = at::empty({(int64_t)rows, c.c.heads, c.c.head_dim}, c.t[0].options().dtype(t));
+      if (rows)
+        rc = cbk_cache_read(&c.c, &m.r, out[0].mutable_data_ptr(), row_stride(out[0]), head_stride(out[0]), out[1].mutable_data_ptr(),
+                            row_stride(out[1]), head_stride(out[1]), dt, stream_of(c.t[0]));
+    }
+    check(rc, "cbk_cache_read");
+    return Py_BuildValue("NN", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+  });
+}
+
+// cache_attention(cache, q, table, lens, starts or None, scale, window, sinks, out or None) -> out
+PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 9)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Cache c = as_cache(a[0]);
+    at::Tensor q = as_tensor(a[1], "q"), out = as_tensor(a[8], "out");
+    if (!q.defined()) fail(PyExc_TypeError, "q must be a tensor");
+    same_device(c, q);
+    same_device(c, out);
+    check_heads(q, 0, c.c.head_dim, "q");
+    if (!half_type(q.scalar_type())) fail(PyExc_TypeError, "q is float16 or bfloat16");
+    const int64_t heads = q.size(1);
+    if (heads % c.c.heads)
+      fail(PyExc_ValueError, std::to_string(heads) + " query heads are no multiple of the cache's " + std::to_string(c.c.heads));
+    if (out.defined()) check_out(out, q.size(0), heads, c.c.head_dim, q.scalar_type(), "out");
+    const RowMap m = as_rows(c, a[2], a[3], a[4], q.size(0));
+    const double scale = PyFloat_AsDouble(a[5]);
+    const long long window = PyLong_AsLongLong(a[6]), sinks = PyLong_AsLongLong(a[7]);
+    if (PyErr_Occurred()) throw Fail{};
+    if (heads > INT32_MAX || window < 0 || sinks < 0) check(CBK_ERR_SHAPE, "cbk_cache_attention");
+    const int dt = dtype_code(q.scalar_type());
+    int rc = CBK_OK;
+    {
+      const GilRelease other_threads_run;
+      const c10::DeviceGuard guard(q.device());
+      if (!out.defined()) out = at::empty({q.size(0), heads, (int64_t)c.c.head_dim}, q.options().requires_grad(false));
+      if (q.size(0)) {
+        q = dense_in(q);
+        const at::Tensor ws = scratch(q, cbk_cache_attention_workspace_bytes(&c.c, &m.r, (int)heads));
+        rc = cbk_cache_attention(&c.c, &m.r, q.const_data_ptr(), row_stride(q), head_stride(q), out.mutable_data_ptr(),
+                                 row_stride(out), head_stride(out), dt, (int)heads, (float)scale,
+                                 (int)(window < INT32_MAX ? window : INT32_MAX), (int)(sinks < INT32_MAX ? sinks : INT32_MAX),
+                                 ws.defined() ? ws.mutable_data_ptr() : nullptr, ws.defined() ? ws.nbytes() : 0, stream_of(q));
+      }
+    }
+    check(rc, "cbk_cache_attention");
+    return THPVariable_Wrap(out);
+  });
+}
+
 PyObject* py_set_error(PyObject*, PyObject* e) {
   Py_INCREF(e);
   Py_XSETREF(g_error, e);
@@ -591,6 +771,9 @@ PyMethodDef methods[] = {
     {"dequant", (PyCFunction)(void (*)())py_dequant, METH_FASTCALL, nullptr},
     {"pack_begin", (PyCFunction)(void (*)())py_pack_begin, METH_FASTCALL, nullptr},
     {"pack_end", (PyCFunction)(void (*)())py_pack_end, METH_FASTCALL, nullptr},
+    {"cache_write", (PyCFunction)(void (*)())py_cache_write, METH_FASTCALL, nullptr},
+    {"cache_read", (PyCFunction)(void (*)())py_cache_read, METH_FASTCALL, nullptr},
+    {"cache_attention", (PyCFunction)(void (*)())py_cache_attention, METH_FASTCALL, nullptr},
     {"set_error", py_set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

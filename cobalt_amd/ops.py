@@ -188,3 +188,37 @@ def transcode(pm: PackedMatrix, layout: int, bits=None, group=None, keep=None, t
                    cs, layout, bits, group, keep, fix_zero=False, cs_splits=rm.cs_splits, tiled=tiled)
     out.n_survivors = pm.n_survivors
     return out
+
+
+# ------------------------------------------------------------------ the key/value cache held in 4 bits (cache.py)
+def cache_write(cache, k, v, rows) -> None:
+    """The rows' keys and values (float16 or bfloat16, [rows, heads, head_dim]) into the cache, rounded to 4 bits per
+    group: codes c = rint((x - m) / s) with the fp16 minimum m and scale s of the group, held value m + c s.  Magnitudes above
+    65280 are held as 65280; a NaN makes its token's key and value of that head NaN.  Rows whose token has no page are
+    left out.  Two rows of a call must not be the same token of the same page."""
+    _lib.native().cache_write(cache.native(), k, v, rows.table, rows.lens, rows.starts)
+
+
+def cache_read(cache, rows, count: int, dtype=torch.float16, out=None):
+    """(k, v), the held values of the rows' tokens as dense [count, heads, head_dim] tensors of `dtype` (float32, float16
+    or bfloat16; `out`: into these two).  A token that no page holds reads as 0; rows that belong to no sequence
+    are not written."""
+    k, v = out if out is not None else (None, None)
+    return _lib.native().cache_read(cache.native(), rows.table, rows.lens, rows.starts, count, dtype, k, v)
+
+
+def cache_attention(cache, q, rows, scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0, out=None):
+    """Causal attention of the rows' queries ([rows, query heads, head_dim], float16 or bfloat16) over the cache, which
+    holds their own tokens already (`cache_write` first).  `scale`: of the scores, head_dim ** -0.5 by default.  `window`: a row
+    sees the last `window` tokens up to its own only, and the first `sinks` tokens of its sequence.  Query
+    heads share the cache's heads in groups, consecutive ones the same.  Returns a tensor like q (or `out`, which must
+    not overlap q); a row that sees nothing is 0, and rows that belong to no sequence are not written."""
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, or None for all tokens, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    return _lib.native().cache_attention(cache.native(), q, rows.table, rows.lens, rows.starts, scale, window or 0, sinks, out)

@@ -265,6 +265,69 @@ int cbk_linear_act(const cbk_desc* d, const void* x, int x_dtype, int M, int64_t
                    void* y, int y_dtype, int64_t ldy, const void* bias, int act,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- key/value cache held in 4 bits
+ * Keys and values of attention in the framework's own terms: groups of `group` consecutive channels of one token and head,
+ * 4-bit codes rounded to nearest, an fp16 scale and an fp16 minimum per group (4 + 32 / group bits a value):
+ *
+ *     x' = x clamped to +-65280,  m = fp16(min x'),  s = fp16((max x' - m) / 15),
+ *     c = clamp(rint((x' - m) / s), 0, 15)  (0 where s = 0),     held value m + c s,
+ *
+ * in float32 steps.  A NaN anywhere in a token's key or value of a head makes that token's key and value of the head
+ * NaN; infinities are held as +-65280.
+ *
+ * The cache is a pool of pages of `page` tokens, all heads of a token on one page.  Of the four arrays the caller owns
+ * cbk_cache_code_bytes() (k_codes, v_codes) and cbk_cache_meta_bytes() (k_meta, v_meta) each, 16-byte aligned and
+ * cleared to zero once before their first use; what stands where is the library's own (cbk_cache.h). */
+typedef struct cbk_cache {
+  void *k_codes, *v_codes, *k_meta, *v_meta;
+  int64_t pages;
+  int32_t page;        /* tokens a page: 16, 32, 64, 128 or 256                       */
+  int32_t heads;       /* key/value heads                                             */
+  int32_t head_dim;    /* 64, 128 or 256                                              */
+  int32_t group;       /* 32, 64 or 128, at most head_dim                             */
+} cbk_cache;
+
+/* Whose tokens the rows of a call are.  Dense tensors are [tokens, heads, head_dim] with the newest tokens of the
+ * sequences packed one behind the other: sequence b owns rows starts[b] .. starts[b+1]-1 (starts NULL: tokens / seqs
+ * rows each), and the last of them is its token lens[b] - 1, so lens counts them.  Token j is on page
+ * table[b * ld_table + j / page] of the pool.  All of these are DEVICE arrays of int32, read when the kernels
+ * run: a recorded call follows them.  Nothing in them can lead outside the arrays: a table entry outside
+ * [0, pages), or a token behind the table's last column, is a token the cache does not hold.  A row before
+ * starts[0] or behind starts[seqs] belongs to no sequence and stays as it was. */
+typedef struct cbk_rows {
+  const void* table;
+  int64_t ld_table;
+  const void* lens;
+  const void* starts;
+  int32_t seqs, table_cols;
+  int64_t tokens;      /* rows of the dense tensors, below 2^30                       */
+} cbk_rows;
+
+size_t cbk_cache_code_bytes(const cbk_cache* cache);   /* 0: not a valid description */
+size_t cbk_cache_meta_bytes(const cbk_cache* cache);
+
+/* The rows' keys and values (fp16 or bf16; strides of rows and heads in elements, 16-byte aligned as the pointers are) go
+ * into the cache.  Tokens the table has no page for are left out.  Two rows must not be the same token of the same page. */
+int cbk_cache_write(const cbk_cache* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
+                    const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+
+/* And back, as dense fp32, fp16 or bf16: the held value, rounded once.  A token the cache does not hold reads as 0. */
+int cbk_cache_read(const cbk_cache* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
+                   void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+
+/* Attention of the rows over the cache (their own tokens are in it: cbk_cache_write comes first):
+ *   out[t, hq] = sum_j softmax_j(scale q[t, hq] . k_j) v_j,   head hq reads cache head hq / (q_heads / heads),
+ * over the tokens j <= i that the cache holds, i the row's own position, and with window > 0 only those with j > i - window
+ * or j < sinks.  A row that sees no token is 0.  fp16 or bf16 in and out; scores, their maximum and all sums
+ * in float32, operands of the products in fp16 (a key or value is rounded once to fp16, a bf16 query is
+ * scaled by a power of two and stays exact).  scale > 0.  The result is the same from call to call, also on
+ * another workspace.  The workspace holds nothing between calls and needs no clearing:
+ * cbk_cache_attention_workspace_bytes(), 256-byte aligned, one per call in flight. */
+size_t cbk_cache_attention_workspace_bytes(const cbk_cache* cache, const cbk_rows* rows, int q_heads);
+int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
+                        void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
+                        int sinks, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
