@@ -82,6 +82,9 @@ def shift_hazards(code_object):
 MFMA_TO_READ = {"v_mfma_f32_16x16x32_f16": 8, "v_mfma_f32_32x32x16_f16": 12}   # until anything but the next product of the same sums touches them
 VALU_TO_MFMA = 2                                                       # a vector register written -> a matrix instruction reads it
 VALU_TO_VMEM = 5                                                       # a scalar register written by a vector instruction -> a memory instruction reads it
+# Kernels whose products the compiler has placed among its own instructions: it also adds to sums that stand in other registers than the
+# result, or reuses those of sums that the next product takes over, which the hardware keeps in order.  Operands still have to wait.
+COMPILED = ("cache_attn_kernel", "cache_prompt_kernel")
 _REG = re.compile(r"(?<![\w])([vas])(?:(\d+)\b|\[(\d+):(\d+)\])")
 _TARGET = re.compile(r"<(\S+?)(?:\+0x([0-9a-f]+))?>$")
 
@@ -123,6 +126,7 @@ def wait_hazards(code_object):
     for fn, body in _functions(code_object):
         at = {b[0]: i for i, b in enumerate(body)}
         regs = [None] * len(body)
+        compiled = any(n in fn for n in COMPILED)
 
         def touched(i):
             if regs[i] is None:
@@ -157,7 +161,7 @@ def wait_hazards(code_object):
                     hit = dst & touched(j)
                     if hit and body[j][1] == op:
                         d, a, b, c = body[j][2].split(", ")[:4]
-                        if c == d == sums:                             # the next product of the same sums: chained by the hardware
+                        if compiled or c == d == sums:                 # the next product of the same sums: chained by the hardware
                             hit = dst & _registers(a + " " + b)
                     if hit:
                         out.append((fn, addr, op, "%s%d" % min(hit), body[j][1]))

@@ -3,7 +3,8 @@
 //
 // A page holds `page` tokens of `heads` heads; block (p, h) is page p's part of head h, p * heads + h.  Of a block,
 // with D channels and groups of G of them:
-//   keys    codes: token-major, D/2 bytes a token; dword w of a token holds channels 8w .. 8w+7
+//   keys    codes: token-major, D/2 bytes a token; a dword holds eight consecutive channels, and the dwords stand in the order
+//           of key_dword: the lane that multiplies channels 8h .. 8h+7 of every 32 finds its dwords side by side
 //   values  codes: by four tokens, dword n (channels 8n .. 8n+7) of tokens 4i .. 4i+3 side by side: 16 bytes at
 //           (i * D/8 + n) * 16.  A matrix instruction that sums over tokens takes for one channel the codes of several
 //           tokens from one lane, and finds them in one 16-byte load.
@@ -16,6 +17,7 @@
 namespace cbk {
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr float CACHE_TOP = 65280.f;        // larger magnitudes are held as this one: 15 rounded steps above a rounded minimum stay finite
@@ -40,6 +42,12 @@ struct CacheIo {                            // dense side: rows [tokens, heads, 
   int64_t kt, kh, vt, vh;                   // strides of rows and heads, in elements
 };
 
+// Where channels 8w .. 8w+7 of a key stand among its dwords
+template <int D>
+__host__ __device__ constexpr int key_dword(int w) {
+  return D == 64 ? 2 * (w % 4) + w / 4 : w / 16 * 16 + 4 * (w % 4) + w % 16 / 4;
+}
+
 // The rows of sequence b: [first, first + n) of the call, token positions pos0 .. pos0 + n - 1, and the tokens the table
 // has pages for.  Offsets that are not ascending give rows that do not belong together, never rows outside the call.
 struct Seq { int first, n, pos0, held; };
@@ -56,31 +64,34 @@ __device__ inline Seq seq_of(const DRows& r, int b) {
 }
 
 // page of token `pos` (not negative) of sequence b; -1: the table has none
-__device__ inline int64_t page_of(const DCache& c, const DRows& r, int b, int pos) {
+__device__ inline int page_of(const DCache& c, const DRows& r, int b, int pos) {
   const int i = pos >> c.shift;
   if (i >= r.cols) return -1;
-  const int p = r.table[(int64_t)b * r.ld + i];
+  const int p = ((const __attribute__((address_space(4))) int32_t*)r.table)[(int64_t)b * r.ld + i];   // (never written by a kernel that reads it)
   return p >= 0 && p < c.pages ? p : -1;
 }
 
 // ------------------------------------------------------------------ codes to fp16
-// m + c s for two codes that stand in the low four bits of each half of w (hi: in the next four), rounded once to
-// fp16.  The bits under an exponent of 2^10 (2^6) are the number 1024 + c (64 + c); the difference is exact.
-template <bool HI>
-__device__ inline v2h code_pair(uint32_t w, v2h s, v2h m) {
-  const uint32_t u = HI ? ((w & 0x00f000f0u) | 0x54005400u) : ((w & 0x000f000fu) | 0x64006400u);
-  const v2h off = HI ? v2h{(_Float16)64.f, (_Float16)64.f} : v2h{(_Float16)1024.f, (_Float16)1024.f};
-  const v2h c = __builtin_bit_cast(v2h, u) - off;
-  return __builtin_elementwise_fma(c, s, m);
+// The low four bits of each half of a dword (hi: the next four) under the exponent of 2^10 (2^6) are the numbers 1024 + c
+// (64 + c), and the difference is c, exactly.  One instruction masks and sets the exponent if the exponent is in a vector register: a
+// constant would be a second scalar operand, which this architecture does not take.
+struct Exponents { uint32_t lo, hi; };
+__device__ inline Exponents exponents() {
+  Exponents e;
+  asm("v_mov_b32 %0, 0x64006400" : "=v"(e.lo));
+  asm("v_mov_b32 %0, 0x54005400" : "=v"(e.hi));
+  return e;
 }
-__device__ inline v2h pair_of(_Float16 x) { return v2h{x, x}; }
-
-// dword w of a key: its eight channels in order
-__device__ inline v8h key_octet(uint32_t w, uint32_t meta) {
-  const v2h sm = __builtin_bit_cast(v2h, meta);
-  const v2h s = pair_of(sm.x), m = pair_of(sm.y);
+template <bool HI>
+__device__ inline v2h codes_of(uint32_t w, const Exponents& e) {
+  const uint32_t u = HI ? ((w & 0x00f000f0u) | e.hi) : ((w & 0x000f000fu) | e.lo);
+  const v2h off = HI ? v2h{(_Float16)64.f, (_Float16)64.f} : v2h{(_Float16)1024.f, (_Float16)1024.f};
+  return __builtin_bit_cast(v2h, u) - off;
+}
+// the eight codes of a dword in the order of their channels
+__device__ inline v8h code_octet(uint32_t w, const Exponents& e) {
   const uint32_t u = w >> 8;
-  const v2h a = code_pair<false>(w, s, m), b = code_pair<true>(w, s, m), c = code_pair<false>(u, s, m), d = code_pair<true>(u, s, m);
+  const v2h a = codes_of<false>(w, e), b = codes_of<true>(w, e), c = codes_of<false>(u, e), d = codes_of<true>(u, e);
   return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(DCache c, DRows r, Cac
   if (bad) { wk = wv = mv = 0; mk = 0x7e000000u; }
   if (blk < 0) return;
   const int64_t bytes = (int64_t)c.page * (D / 2);
-  *(uint32_t*)(c.kc + blk * bytes + at * (D / 2) + e * 4) = wk;
+  *(uint32_t*)(c.kc + blk * bytes + at * (D / 2) + key_dword<D>(e) * 4) = wk;
   *(uint32_t*)(c.vc + blk * bytes + (at >> 2) * (2 * D) + e * 16 + (at & 3) * 4) = wv;
   if (e % GL == 0) {
     const int64_t i = blk * ((int64_t)c.page * (D / (8 * GL))) + (e / GL) * c.page + at;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(DCache c, DRows r, Cach
   uint32_t wk = 0, wv = 0, mk = 0, mv = 0;
   if (blk >= 0) {
     const int64_t bytes = (int64_t)c.page * (D / 2), i = blk * ((int64_t)c.page * c.groups) + (e * 8 / c.group) * c.page + at;
-    wk = *(const uint32_t*)(c.kc + blk * bytes + at * (D / 2) + e * 4);
+    wk = *(const uint32_t*)(c.kc + blk * bytes + at * (D / 2) + key_dword<D>(e) * 4);
     wv = *(const uint32_t*)(c.vc + blk * bytes + (at >> 2) * (2 * D) + e * 16 + (at & 3) * 4);
     mk = c.km[i];
     mv = c.vm[i];

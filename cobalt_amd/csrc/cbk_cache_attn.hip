@@ -10,9 +10,13 @@
 // step are numbered 4h + r of the first and of the second 16, so nothing passes through LDS until a wavefront has done
 // its share.
 //
-// Operands are fp16: a key or value m + c s is rounded once (2^-11; its scale and minimum are fp16 already), a bf16
-// query row is brought to [1, 2) by a power of two and is then exact, and p is kept at 2^8 times its size against the
-// running maximum, so that what an fp16 cannot hold lies 2^-32 below the largest.  The sum adds the rounded p.
+// Scores are exact up to float32: the codes themselves are the operands, one product per group of channels, and its sum is
+// multiplied by the token's scale; the minima, which are fp16 already, meet the sums of q over the groups in a product
+// of their own.  (Keys rounded to fp16 put 5e-4 of error into an fp16 result, which itself rounds by 2e-4.)  fp16 queries are
+// operands as they are, and a bf16 row is brought to [1, 2) by a power of two and is exact in fp16 then.
+// Values m + c s are rounded once to fp16 (2^-11).  p is kept at 2^8 times its size against the running maximum, so that what
+// an fp16 cannot hold lies 2^-32 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
+// bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
 //
 // The tokens of all sequences and heads are one list of units of 128 tokens, cut into equal pieces, one a workgroup;
 // what a workgroup has of a head it does not finish goes to the workspace with its maximum and sum, and a second
@@ -40,15 +44,23 @@ __device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
   return g;
 }
 
-// Sequences are walked in 256 parts, one a thread: total units of all, and where unit `want` lies
-struct Cursor { int b; int64_t base; };     // sequence and its first unit
-struct Walk {
-  int64_t sums[256];
-};
 __device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads, int b, int rows) {
+  if (b >= r.seqs) return 0;
   const Seq s = seq_of(r, b);
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
   return tiles * heads * range_of(s, a).units;
+}
+__device__ inline int64_t shift_up(int64_t x, int by, int lane) {   // the value of the lane `by` below, 0 at the start
+  const int lo = __shfl_up((int)x, by), hi = __shfl_up((int)(x >> 32), by);
+  return lane >= by ? (int64_t)hi << 32 | (uint32_t)lo : 0;
+}
+__device__ inline int64_t of_lane(int64_t x, int l) {
+  return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+}
+__device__ inline int64_t scan64(int64_t x, int lane) {             // sum of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) x += shift_up(x, o, lane);
+  return x;
 }
 
 __device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
@@ -67,39 +79,25 @@ __device__ inline float rounded_product(float a, float b) {
   return a * b;
 }
 
-template <int D>
+template <int D, int G>
 struct Held {                               // a wavefront's 32 tokens: two sixteens
   uint32_t k[2][D / 32];
-  uint32_t km[2][D > 128 ? D / 128 : 1];
+  uint32_t km[2][(D / G + 3) / 4];
   v4u v[2][D > 128 ? D / 128 : 1], vm[2][D > 128 ? D / 128 : 1];
 };
 
-template <int D, int NT>
-__global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, AttnArgs a) {
-  constexpr int R = 16 * NT, KS = D / 32, VU = D > 128 ? D / 128 : 1, TILES = D / 16;
+template <int D, int G, int NT, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCache c, DRows r, AttnArgs a) {
+  constexpr int R = 16 * NT, KS = D / 32, GS = D / G, GU = (GS + 3) / 4, VU = D > 128 ? D / 128 : 1, TILES = D / 16;
   __shared__ float o_sh[4][R][D + 4];
   __shared__ float m_sh[4][R], l_sh[4][R];
-  __shared__ int64_t walk[256];
-  __shared__ int64_t found[4];
+  __shared__ v2u scale_sh[4][2][GS][4];       // a wavefront's own: scales of its 32 keys, by group, four in a piece
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, h4 = lane >> 4;
 
-  // ---- this workgroup's piece of the list
-  const int per = (r.seqs + 255) / 256;
-  int64_t mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < r.seqs) mine += units_of(r, a, c.heads, b, R);
-  }
-  walk[tid] = mine;
-  __syncthreads();
-  for (int o = 1; o < 256; o *= 2) {
-    const int64_t x = tid >= o ? walk[tid - o] : 0;
-    __syncthreads();
-    walk[tid] += x;
-    __syncthreads();
-  }
-  const int64_t total = walk[255];
+  // ---- this workgroup's piece of the list; every wavefront looks for itself, 64 sequences at a time
+  int64_t sum = scan64(units_of(r, a, c.heads, lane, R), lane), total = of_lane(sum, 63);
+  for (int j = 64; j < r.seqs; j += 64) total += of_lane(scan64(units_of(r, a, c.heads, j + lane, R), lane), 63);
   const int64_t pieces = min((int64_t)gridDim.x, (total + a.least - 1) / a.least);
   const int64_t w = blockIdx.x;
   AttnPiece* const desc = (AttnPiece*)a.ws + w;
@@ -108,20 +106,22 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
     return;
   }
   const int64_t begin = w * total / pieces, end = (w + 1) * total / pieces;
-  if (walk[tid] - mine <= begin && begin < walk[tid]) {             // one thread
-    int b = tid * per;
-    int64_t base = walk[tid] - mine;
-    for (;; ++b) {
-      const int64_t u = units_of(r, a, c.heads, b, R);
-      if (begin < base + u) break;
-      base += u;
+  int64_t base = 0;
+  int b = 0;
+  for (int j = 0;; j += 64) {                                       // (begin < total: it is found)
+    if (j) sum = scan64(units_of(r, a, c.heads, j + lane, R), lane);
+    const int64_t here = of_lane(sum, 63);
+    if (begin < base + here) {
+      const int l = __popcll(__ballot(base + sum <= begin));        // sequences that end before it
+      b = j + l;
+      if (l) base += of_lane(sum, l - 1);
+      break;
     }
-    found[0] = b; found[1] = base;
+    base += here;
   }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane((int)found[0]);
-  int64_t base = found[1], at = begin;
+  int64_t at = begin;
   int joined = 0;
+  const Exponents ex = exponents();
 
   while (at < end) {
     // ---- one head's tile of rows and the units of it that are this workgroup's
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
     const int valid = min(R, rows - row0);
 
     // ---- queries: fragments, positions and factors
-    v8h q[NT][KS];
+    v8h q[NT][KS], qm[NT];
     float cs[NT];
     int pos[NT];
 #pragma unroll
@@ -147,33 +147,46 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
       const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
       pos[n] = s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio);
       const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
-      float x[KS][8], top = 0.f;
+      v4u raw[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int d = D >= 128 ? 128 * (k / 4) + 32 * h4 + 8 * (k % 4) : 16 * h4 + 8 * k;
-        const v4u v = is ? *(const v4u*)(qp + d) : v4u{};
-        if (a.bf) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[k][2 * i] = __uint_as_float(v[i] << 16);
-            x[k][2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-            top = fmaxf(top, fmaxf(fabsf(x[k][2 * i]), fabsf(x[k][2 * i + 1])));
-          }
-        } else {
-          q[n][k] = __builtin_bit_cast(v8h, v);
-        }
-      }
+      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
       cs[n] = a.scale;
-      if (a.bf) {
-        top = across_max(top);
-        int e = 0;
-        if (top > 0.f && top < __builtin_inff()) e = max((int)(__float_as_uint(top) >> 23), 1) - 127;
+      if constexpr (BF) {
+        uint32_t big = 0;                                           // the largest magnitude, as bits
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big = max(big, max(raw[k][i] << 16 & 0x7fff0000u, raw[k][i] & 0x7fff0000u));
+        big = max(big, (uint32_t)__shfl_xor((int)big, 16));
+        big = max(big, (uint32_t)__shfl_xor((int)big, 32));
+        int e = max((int)(big >> 23), 1) - 127;
+        if (big == 0 || big >= 0x7f800000u) e = 0;
         const float down = __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);   // 2^-e, e = 127: 2^-126 leaves [2, 4)
         cs[n] = a.scale * __uint_as_float((uint32_t)(min(e, 126) + 127) << 23);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) q[n][k][i] = (_Float16)(x[k][i] * down);
+          for (int i = 0; i < 4; ++i) {
+            q[n][k][2 * i] = (_Float16)(__uint_as_float(raw[k][i] << 16) * down);
+            q[n][k][2 * i + 1] = (_Float16)(__uint_as_float(raw[k][i] & 0xffff0000u) * down);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[n][k] = __builtin_bit_cast(v8h, raw[k]);
+      }
+      // sums of q over the groups: as two fp16 that meet the minima
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qm[n][i] = (_Float16)0.f;
+#pragma unroll
+      for (int g = 0; g < GS; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum += (float)q[n][k][i];
+        sum = across_sum(sum);
+        const _Float16 hi = (_Float16)sum;
+        if (h4 == g % 4) { qm[n][2 * (g / 4)] = hi; qm[n][2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
       }
       cs[n] = fmaxf(cs[n], 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
     }
@@ -188,73 +201,107 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
       for (int t = 0; t < TILES; ++t) o[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    const int64_t kblk = (int64_t)c.page * (D / 2), mblk = (int64_t)c.page * c.groups;
+    // where the cache head's part of page 0 is, and what a page takes; offsets of the lane from a sixteen's first token
+    const uint32_t code_page = (uint32_t)c.heads * c.page * (D / 2), meta_page = (uint32_t)c.heads * c.page * (GS * 4);
+    const int64_t code_head = (int64_t)h * c.page * (D / 2), meta_head = (int64_t)h * c.page * (GS * 4);
+    const uint8_t *const kc = c.kc + code_head, *const vc = c.vc + code_head;
+    const uint8_t *const km = (const uint8_t*)c.km + meta_head, *const vm = (const uint8_t*)c.vm + meta_head;
+    const uint32_t k_at = col * (D / 2) + h4 * (D == 64 ? 8 : 16);
+    const uint32_t v_at = h4 * (2 * D) + (D == 64 ? col & 7 : col) * 16;
+    const uint32_t km_at = 4 * (min(h4, GS - 1) * c.page + col), vm_at = 4 * ((8 * (D == 64 ? col & 7 : col) / G) * c.page + 4 * h4);
     auto token_of = [&](int u) { return ((u < g.head ? u : u + g.skip) * 4 + wave) * 32; };
-    auto pages_of = [&](int tok, int64_t (&pg)[2]) {
+    auto pages_of = [&](int tok, int (&pg)[2]) {                    // pages of the two sixteens of a step
 #pragma unroll
       for (int t = 0; t < 2; ++t) pg[t] = tok + 16 * t < s.held ? page_of(c, r, b, tok + 16 * t) : -1;
     };
-    auto fetch = [&](int tok, const int64_t (&pg)[2], Held<D>& x) {
+    Held<D, G> x;
+    auto fetch_keys = [&](int tok, const int (&pg)[2]) {            // (a page that is not there: page 0, and masked)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int in = (tok + 16 * t) & (c.page - 1);
-        const int64_t blk = max(pg[t], (int64_t)0) * c.heads + h;
-        const uint8_t* kp = c.kc + blk * kblk + (in + col) * (D / 2);
-        const uint8_t* vp = c.vc + blk * kblk + ((in >> 2) + h4) * (2 * D);
-        const uint32_t* kmp = c.km + blk * mblk + in + col;
-        const uint32_t* vmp = c.vm + blk * mblk + in + 4 * h4;
+        const uint32_t in = (tok + 16 * t) & (c.page - 1), page = max(pg[t], 0);
+        const uint8_t* kp = kc + ((uint64_t)page * code_page + in * (D / 2));
+        const uint8_t* mp = km + ((uint64_t)page * meta_page + in * 4);
+#pragma unroll
+        for (int i = 0; i < GU; ++i) x.km[t][i] = *(const uint32_t*)(mp + (uint32_t)(i * 16) * c.page + km_at);
         if constexpr (D == 64) {
-          const uint2 d = *(const uint2*)(kp + h4 * 8);
+          const uint2 d = *(const uint2*)(kp + k_at);
           x.k[t][0] = d.x; x.k[t][1] = d.y;
-          x.km[t][0] = kmp[(16 * h4 / c.group) * c.page];
-          const int n = col & 7;
-          x.v[t][0] = *(const v4u*)(vp + n * 16);
-          x.vm[t][0] = *(const v4u*)(vmp + (8 * n / c.group) * c.page);
         } else {
 #pragma unroll
           for (int i = 0; i < VU; ++i) {
-            const v4u d = *(const v4u*)(kp + 64 * i + h4 * 16);
+            const v4u d = *(const v4u*)(kp + 64 * i + k_at);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = d[j];
-            x.km[t][i] = kmp[((128 * i + 32 * h4) / c.group) * c.page];
-            const int n = col + 16 * i;
-            x.v[t][i] = *(const v4u*)(vp + n * 16);
-            x.vm[t][i] = *(const v4u*)(vmp + (8 * n / c.group) * c.page);
           }
         }
       }
     };
+    auto fetch_values = [&](int tok, const int (&pg)[2]) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t in = (tok + 16 * t) & (c.page - 1), page = max(pg[t], 0);
+        const uint8_t* vp = vc + ((uint64_t)page * code_page + in * (D / 2));
+        const uint8_t* mp = vm + ((uint64_t)page * meta_page + in * 4);
+#pragma unroll
+        for (int i = 0; i < VU; ++i) {
+          x.v[t][i] = *(const v4u*)(vp + 256 * i + v_at);
+          x.vm[t][i] = *(const v4u*)(mp + (uint32_t)(i * (128 / G) * 4) * c.page + vm_at);
+        }
+      }
+    };
 
-    Held<D> next;
-    int64_t pg[2], pg_next[2];
+    // keys of the next step are under way while this one's values are worked on, and the other way round
+    int pg[2], pg_next[2];
     pages_of(token_of(u0), pg);
-    fetch(token_of(u0), pg, next);
+    fetch_keys(token_of(u0), pg);
+    fetch_values(token_of(u0), pg);
     pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
     for (int u = u0; u < u1; ++u) {
-      Held<D> x = next;
-      const int tok = token_of(u);
+      const int tok = token_of(u), tok_next = token_of(min(u + 1, u1 - 1));
       const bool p0 = pg[0] >= 0, p1 = pg[1] >= 0;
-      if (u + 1 < u1) {
-        pg[0] = pg_next[0]; pg[1] = pg_next[1];
-        fetch(token_of(u + 1), pg, next);
-        pages_of(token_of(min(u + 2, u1 - 1)), pg_next);
-      }
-      if (tok >= s.held) continue;
       // every row sees all 32 tokens, and all of them are there
       const bool whole = p0 && p1 && tok + 32 <= s.held && tok + 31 <= pos_lo &&
                          (a.window <= 0 || tok > pos_hi - a.window || tok + 32 <= a.sinks);
       v4f sc[NT][2];
+      uint16_t* const mine_sh = (uint16_t*)scale_sh[wave];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < GU; ++i)
+          if (4 * i + h4 < GS) mine_sh[(t * GS + 4 * i + h4) * 16 + col] = (uint16_t)x.km[t][i];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        v8h mins;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 8; ++i) mins[i] = i < 2 * GU ? __builtin_bit_cast(v2h, x.km[t][i / 2 % GU]).y : (_Float16)0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const v8h f = key_octet(x.k[t][k], x.km[t][k / 4]);
+        for (int n = 0; n < NT; ++n) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mins, qm[n], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[n][k], sc[n][t], 0, 0, 0);
+        for (int g = 0; g < GS; ++g) {
+          v4f part[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) part[n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k) {
+            const v8h f = code_octet(x.k[t][k], ex);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[n][k], part[n], 0, 0, 0);
+          }
+          const v2u sm = scale_sh[wave][t][g][h4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t two = sm[i >> 1];                      // (a bit cast of a vector's element reads its first)
+              sc[n][t][i] = fmaf((float)__builtin_bit_cast(v2h, two)[i & 1], part[n][i], sc[n][t][i]);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);                          // (or the second sixteen's operands take registers early)
       }
+      if (u + 1 < u1) fetch_keys(tok_next, pg_next);
       if (!whole) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -272,7 +319,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
               for (int v = 0; v < VU; ++v) x.vm[t][v][i] = 0;       // whatever stands there: its value is 0
           }
       }
-      v8h p[NT];
+      v8h p[NT], rest[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float e[8], top;
@@ -295,6 +342,11 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
           const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
           l[n] = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
           p[n][2 * i] = ph.x; p[n][2 * i + 1] = ph.y;
+          if constexpr (!BF) {
+            const v2h pl = {(_Float16)(e[2 * i] - (float)ph.x), (_Float16)(e[2 * i + 1] - (float)ph.y)};
+            rest[n][2 * i] = pl.x; rest[n][2 * i + 1] = pl.y;
+            l[n] = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
+          }
         }
       }
 #pragma unroll
@@ -313,23 +365,35 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(DCache c, DRows r, Attn
           for (int i = 0; i < 4; ++i) wd[t][i] = D == 64 ? x.v[t][0][i] >> (4 * (col >> 3)) : x.v[t][v][i];
 #pragma unroll
         for (int by = 0; by < 4; ++by) {
+          __builtin_amdgcn_sched_barrier(0);
           uint32_t pr[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             pr[i] = __builtin_amdgcn_perm(wd[i >> 1][2 * (i & 1) + 1], wd[i >> 1][2 * (i & 1)], 0x0c040c00u + by * 0x00010001u);
           v8h f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { const v2h y = code_pair<false>(pr[i], s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
+          for (int i = 0; i < 4; ++i) { const v2h y = __builtin_elementwise_fma(codes_of<false>(pr[i], ex), s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
           const int t0 = D == 64 ? by : 2 * by * VU + v;
 #pragma unroll
           for (int n = 0; n < NT; ++n) o[n][t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[n], o[n][t0], 0, 0, 0);
+          if constexpr (!BF)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest[n], o[n][t0], 0, 0, 0);
           if constexpr (D > 64) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const v2h y = code_pair<true>(pr[i], s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
+            for (int i = 0; i < 4; ++i) { const v2h y = __builtin_elementwise_fma(codes_of<true>(pr[i], ex), s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[n][t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[n], o[n][t0 + VU], 0, 0, 0);
+            if constexpr (!BF)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) o[n][t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest[n], o[n][t0 + VU], 0, 0, 0);
           }
         }
+      }
+      if (u + 1 < u1) {
+        fetch_values(tok_next, pg_next);
+        pg[0] = pg_next[0]; pg[1] = pg_next[1];
+        pages_of(token_of(min(u + 2, u1 - 1)), pg_next);
       }
     }
 
@@ -443,9 +507,16 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
 }
 size_t cache_attn_workspace(const DCache& c, const DRows& r, int ratio) { return plan_attn(c, r, ratio).bytes; }
 
+template <int D, int G>
+static void attn2(const AttnPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  if (a.bf) hipLaunchKernelGGL((cache_attn_kernel<D, G, 1, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  else hipLaunchKernelGGL((cache_attn_kernel<D, G, 1, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+}
 template <int D>
 static void attn1(const AttnPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((cache_attn_kernel<D, 1>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  if (c.group == 32) attn2<D, 32>(p, c, r, a, st);
+  else if (c.group == 64) attn2<D, 64>(p, c, r, a, st);
+  else if constexpr (D > 64) attn2<D, 128>(p, c, r, a, st);
   if (p.split) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16>), dim3(p.grid, 16), dim3(256), 0, st, a, p.grid);
 }
 int launch_cache_attn(const DCache& c, const DRows& r, AttnArgs a, size_t ws_bytes, hipStream_t st) {
