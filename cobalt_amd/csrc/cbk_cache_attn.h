@@ -4,6 +4,9 @@
 
 namespace cbk {
 
+constexpr float FLOOR = -3.0e38f;           // running maximum before the first token: below every score that is one
+constexpr float P_BITS = 8.f, P_SLACK = 6.f;   // p = 2^(t - M + P_BITS) with t <= M + P_SLACK: at most 2^14
+
 struct AttnArgs {
   const void* q;                            // [tokens, ratio * heads, D] fp16 or bf16
   void* out;
@@ -22,12 +25,42 @@ struct AttnPiece { int count, slot, first, row0, valid, head, pad[2]; };
 
 // rows of a part: D sums, the maximum they stand against, the sum of p, padding to 16 bytes
 constexpr int attn_row(int dim) { return dim + 4; }
-inline size_t attn_bytes(int grid, int rows, int dim) {
-  return ((size_t)grid * sizeof(AttnPiece) + 255) / 256 * 256 + (size_t)grid * 2 * rows * attn_row(dim) * sizeof(float);
+inline size_t attn_bytes(int grid, int rows, int slots, int dim) {   // slots: parts a workgroup may leave
+  return ((size_t)grid * sizeof(AttnPiece) + 255) / 256 * 256 + (size_t)grid * slots * rows * attn_row(dim) * sizeof(float);
 }
 template <int D>
 __device__ inline float* attn_part(uint8_t* ws, int64_t grid, int64_t row) {
   return (float*)(ws + (grid * (int64_t)sizeof(AttnPiece) + 255) / 256 * 256) + row * attn_row(D);
+}
+
+__device__ inline int64_t shift_up(int64_t x, int by, int lane) {   // the value of the lane `by` below, 0 at the start
+  const int lo = __shfl_up((int)x, by), hi = __shfl_up((int)(x >> 32), by);
+  return lane >= by ? (int64_t)hi << 32 | (uint32_t)lo : 0;
+}
+__device__ inline int64_t of_lane(int64_t x, int l) {
+  return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+}
+__device__ inline int64_t scan64(int64_t x, int lane) {             // sum of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) x += shift_up(x, o, lane);
+  return x;
+}
+
+// A product that stays one when something is added to it: the largest score less the maximum is 0 only if both were
+// rounded alike, and where scores pass 2^24 nothing else keeps p in range.
+__device__ inline float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// 2^e for the largest magnitude of a bf16 row (as bits), and `down` = 2^-e, which brings the row to [1, 2) (e = 127: to [2, 4), 2^-127
+// is no normal number); 1 for a row of zeros and one with an infinity or a NaN.
+__device__ inline float row_factor(uint32_t big, float& down) {
+  int e = max((int)(big >> 23), 1) - 127;
+  if (big == 0 || big >= 0x7f800000u) e = 0;
+  e = min(e, 126);
+  down = __uint_as_float((uint32_t)(127 - e) << 23);
+  return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
 // four channels of a row: sums over the sum of p, 0 where the row saw nothing
@@ -44,5 +77,12 @@ __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, c
   }
   *(uint2*)p = v;
 }
+
+// cbk_cache_prompt.hip: many rows a sequence
+struct PromptPlan { int parts; int64_t grid; size_t bytes; };
+PromptPlan plan_prompt(const DCache&, const DRows&, int ratio);
+int launch_cache_prompt(const PromptPlan&, const DCache&, const DRows&, const AttnArgs&, hipStream_t);
+// Joins what the `grid` workgroups of a launch left; tiles of `rows` rows begin in every `every`th of them (cbk_cache_attn.hip)
+void launch_cache_join(int dim, const AttnArgs&, int grid, int every, int rows, int slots, hipStream_t);
 
 }  // namespace cbk

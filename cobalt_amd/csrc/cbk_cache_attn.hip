@@ -27,8 +27,6 @@
 namespace cbk {
 
 constexpr int UNIT = 128;                   // tokens: 32 a wavefront
-constexpr float FLOOR = -3.0e38f;           // running maximum before the first token: below every score that is one
-constexpr float P_BITS = 8.f, P_SLACK = 6.f;   // p = 2^(t - M + P_BITS) with t <= M + P_SLACK: at most 2^14
 
 struct Range { int units, head, skip; };    // units of a sequence; the first `head` from token 0, the others `skip` units on
 __device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
@@ -50,19 +48,6 @@ __device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads,
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
   return tiles * heads * range_of(s, a).units;
 }
-__device__ inline int64_t shift_up(int64_t x, int by, int lane) {   // the value of the lane `by` below, 0 at the start
-  const int lo = __shfl_up((int)x, by), hi = __shfl_up((int)(x >> 32), by);
-  return lane >= by ? (int64_t)hi << 32 | (uint32_t)lo : 0;
-}
-__device__ inline int64_t of_lane(int64_t x, int l) {
-  return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
-}
-__device__ inline int64_t scan64(int64_t x, int lane) {             // sum of the lanes up to this one
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) x += shift_up(x, o, lane);
-  return x;
-}
-
 __device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -70,13 +55,6 @@ __device__ inline float across_max(float x) {                       // over the 
 __device__ inline float across_sum(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
-}
-
-// A product that stays one when something is added to it: the largest score less the maximum is 0 only if both were
-// rounded alike, and where scores pass 2^24 nothing else keeps p in range.
-__device__ inline float rounded_product(float a, float b) {
-#pragma clang fp contract(off)
-  return a * b;
 }
 
 template <int D, int G>
@@ -159,10 +137,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
           for (int i = 0; i < 4; ++i) big = max(big, max(raw[k][i] << 16 & 0x7fff0000u, raw[k][i] & 0x7fff0000u));
         big = max(big, (uint32_t)__shfl_xor((int)big, 16));
         big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-        int e = max((int)(big >> 23), 1) - 127;
-        if (big == 0 || big >= 0x7f800000u) e = 0;
-        const float down = __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);   // 2^-e, e = 127: 2^-126 leaves [2, 4)
-        cs[n] = a.scale * __uint_as_float((uint32_t)(min(e, 126) + 127) << 23);
+        float down;
+        cs[n] *= row_factor(big, down);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -454,17 +430,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
 }
 
 // One row of a tile that several workgroups have parts of: 256 threads, D/4 of them a part, a part after another.
-template <int D, int R>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid) {
+template <int D>
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int every, int rows, int slots) {
   constexpr int C = D / 4, P = 256 / C;
   __shared__ float sh[P][D + 4];
-  const int64_t w = blockIdx.x;
+  const int64_t w = (int64_t)blockIdx.x * every;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
   const int row = blockIdx.y, tid = threadIdx.x, d = 4 * (tid % C), p = tid / C;
   if (e.count == 0 || row >= e.valid) return;
   float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
   for (int i = p; i < e.count; i += P) {
-    const float* const part = attn_part<D>(a.ws, grid, ((w + i) * 2 + (i ? 0 : e.slot)) * R + row);
+    const float* const part = attn_part<D>(a.ws, grid, ((w + i) * slots + (i ? 0 : e.slot)) * rows + row);
     const float4 o = *(const float4*)(part + d);
     const float mm = part[D], ll = part[D + 1], up = fmaxf(top, mm);
     const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
@@ -502,10 +478,22 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   const int64_t most = tiles * units;
   p.grid = (int)(most < 1024 ? most : 1024);
   p.split = units > 1;
-  p.bytes = p.split ? attn_bytes(p.grid, p.rows, c.dim) : 0;
+  p.bytes = p.split ? attn_bytes(p.grid, p.rows, 2, c.dim) : 0;
   return p;
 }
-size_t cache_attn_workspace(const DCache& c, const DRows& r, int ratio) { return plan_attn(c, r, ratio).bytes; }
+void launch_cache_join(int dim, const AttnArgs& a, int grid, int every, int rows, int slots, hipStream_t st) {
+  const dim3 blocks(grid / every, rows);
+  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
+  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
+  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
+}
+
+// More rows a sequence than this, on average, go to the kernel of cbk_cache_prompt.hip.
+constexpr int FEW = 32;
+static bool many_rows(const DRows& r, int ratio) { return (int64_t)r.tokens * ratio > (int64_t)FEW * r.seqs; }
+size_t cache_attn_workspace(const DCache& c, const DRows& r, int ratio) {
+  return many_rows(r, ratio) ? plan_prompt(c, r, ratio).bytes : plan_attn(c, r, ratio).bytes;
+}
 
 template <int D, int G>
 static void attn2(const AttnPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
@@ -517,16 +505,18 @@ static void attn1(const AttnPlan& p, const DCache& c, const DRows& r, const Attn
   if (c.group == 32) attn2<D, 32>(p, c, r, a, st);
   else if (c.group == 64) attn2<D, 64>(p, c, r, a, st);
   else if constexpr (D > 64) attn2<D, 128>(p, c, r, a, st);
-  if (p.split) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16>), dim3(p.grid, 16), dim3(256), 0, st, a, p.grid);
 }
 int launch_cache_attn(const DCache& c, const DRows& r, AttnArgs a, size_t ws_bytes, hipStream_t st) {
+  const size_t need = cache_attn_workspace(c, r, a.ratio);
+  if (need > ws_bytes || (need && !a.ws)) return CBK_ERR_WORKSPACE;
+  if (!need) a.ws = nullptr;
+  if (many_rows(r, a.ratio)) return launch_cache_prompt(plan_prompt(c, r, a.ratio), c, r, a, st);
   const AttnPlan p = plan_attn(c, r, a.ratio);
-  if (p.bytes > ws_bytes || (p.bytes && !a.ws)) return CBK_ERR_WORKSPACE;
-  if (!p.bytes) a.ws = nullptr;
   a.least = p.split ? p.least : 1;
   if (c.dim == 64) attn1<64>(p, c, r, a, st);
   else if (c.dim == 128) attn1<128>(p, c, r, a, st);
   else attn1<256>(p, c, r, a, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, 1, p.rows, 2, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

@@ -1,0 +1,426 @@
+// Attention over the 4-bit cache for many rows a sequence: prompts, and chunks of them behind what the cache holds.
+//
+// The formulas are those of cbk_cache_attn.hip; here the products bound the time, so the cache's tiles are widened to fp16 once
+// per workgroup and read from LDS by all of its wavefronts.  A workgroup has 256 rows (tokens times the query heads on one cache
+// head), 32 a wavefront, as the columns of 32 x 32 x 16 products: S^T = K Q^T and O^T = V^T P^T.  The sums of S^T lie in
+// the lanes that P^T wants them in, eight registers a product, if its tokens are numbered 4h + r of the first and of the second
+// eight; values are stored to LDS in that order, and keys and values both as whole operands (lane after lane, 16 bytes), so that every
+// LDS read is a run of 1 KB without bank conflicts.
+//
+// While the products of a tile run, the next one, whose codes were loaded a tile before, is widened into the other half of
+// LDS: four wavefronts take the keys, four the values, 16 tokens of (at most) 128 channels each.  One barrier a tile.
+//
+// bf16 results: keys m + c s rounded once to fp16, p rounded to fp16 (both far below the result's own step).  fp16 results: keys
+// as their codes with one product a group, multiplied by the token's scale in float32, the minima in a product of their own, and p
+// with its rest as a second operand.
+//
+// Tiles of rows are dealt out the longest first.  Where they are too few to fill the chip, the tokens of each are cut into `parts`,
+// joined by the second launch of cbk_cache_attn.hip.
+#include "cbk_cache.h"
+#include "cbk_cache_attn.h"
+
+namespace cbk {
+
+constexpr int WAVES = 8, ROWS = 32 * WAVES;
+
+template <int D, int G, bool BF>
+struct Tile {
+  static constexpr int KEYS = D == 256 ? 32 : 64;                   // tokens of a tile
+  static constexpr int KT = KEYS / 32, KS = D / 16, GS = D / G, GP = G / 16;   // 32-token blocks, products of a row, groups, products of a group
+  static constexpr int VS = KEYS / 16, VT = D / 32;                 // products along the tokens, 32-channel blocks
+  static constexpr int UG = (D < 128 ? D : 128) / G;                // groups of a wavefront's share of the keys
+  static constexpr int K_BYTES = KEYS * D * 2, V_BYTES = KEYS * D * 2;
+  static constexpr int M_BYTES = BF ? 0 : KT * 1024, S_BYTES = BF ? 0 : GS * KEYS * 2;   // minima as an operand, scales
+  static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES;
+};
+
+template <int D, int G, bool BF>
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, DRows r, AttnArgs a, int parts) {
+  using T = Tile<D, G, BF>;
+  __shared__ v4u lds4[2 * T::BYTES / 16];
+  uint8_t* const lds = (uint8_t*)lds4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+
+  // ---- this workgroup's rows: heads fastest (an XCD then meets few heads), the last tiles of a sequence first
+  const int h = blockIdx.x % c.heads, part = blockIdx.x / c.heads % parts;
+  const int64_t item = blockIdx.x / c.heads / parts;
+  const int64_t place = (item * c.heads + h) * parts + part;         // in the workspace: the parts of a tile side by side
+  AttnPiece* const desc = (AttnPiece*)a.ws + place;
+  int64_t base = 0;
+  int b = -1;
+  auto tiles_of = [&](int q) { return q < r.seqs ? (int64_t)((int64_t)seq_of(r, q).n * a.ratio + ROWS - 1) / ROWS : (int64_t)0; };
+  for (int j = 0; j < r.seqs; j += 64) {
+    const int64_t sum = scan64(tiles_of(j + lane), lane), here = of_lane(sum, 63);
+    if (item < base + here) {
+      const int l = __popcll(__ballot(base + sum <= item));
+      b = j + l;
+      if (l) base += of_lane(sum, l - 1);
+      break;
+    }
+    base += here;
+  }
+  if (b < 0) {
+    if (parts > 1 && tid == 0) desc->count = 0;
+    return;
+  }
+  const Seq s = seq_of(r, b);
+  const int rows = s.n * a.ratio, row0 = ((rows + ROWS - 1) / ROWS - 1 - (int)(item - base)) * ROWS, valid = min(ROWS, rows - row0);
+  const int pos_lo = s.pos0 + row0 / a.ratio, pos_hi = s.pos0 + (row0 + valid - 1) / a.ratio;
+
+  // ---- its tiles of tokens: the first `head`, then the others `skip` on
+  int all = max((min(s.held, pos_hi + 1) + T::KEYS - 1) / T::KEYS, 1), head = 0, skip = 0;
+  if (a.window > 0) {
+    const int lo = min(max(pos_lo - a.window + 1, 0) / T::KEYS, all - 1);
+    head = min((a.sinks + T::KEYS - 1) / T::KEYS, lo);
+    skip = lo - head;
+    all -= skip;
+  }
+  const int t0 = (int)((int64_t)all * part / parts), t1 = (int)((int64_t)all * (part + 1) / parts);
+  auto token_of = [&](int t) { return (t < head ? t : t + skip) * T::KEYS; };
+
+  // ---- queries
+  const int wrow0 = row0 + 32 * wave, wvalid = min(32, rows - wrow0);   // (none: not positive)
+  const int wpos_lo = s.pos0 + wrow0 / a.ratio, wpos_hi = s.pos0 + (wrow0 + max(wvalid, 1) - 1) / a.ratio;
+  const bool is = col < wvalid;
+  const int tok_q = is ? (wrow0 + col) / a.ratio : 0, head_q = h * a.ratio + (is ? (wrow0 + col) % a.ratio : 0);
+  const int pos = is ? s.pos0 + tok_q : wpos_hi;
+  const uint16_t* const qp = (const uint16_t*)a.q + (int64_t)(s.first + tok_q) * a.qt + (int64_t)head_q * a.qh;
+  v8h q[T::KS], qm;
+  float cs = a.scale;
+  if constexpr (BF) {
+    v4u raw[T::KS];
+#pragma unroll
+    for (int k = 0; k < T::KS; ++k) raw[k] = is ? *(const v4u*)(qp + 16 * k + 8 * half) : v4u{};
+    uint32_t big = 0;
+#pragma unroll
+    for (int k = 0; k < T::KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) big = max(big, max(raw[k][i] << 16 & 0x7fff0000u, raw[k][i] & 0x7fff0000u));
+    big = max(big, (uint32_t)__shfl_xor((int)big, 32));
+    float down;
+    cs *= row_factor(big, down);
+#pragma unroll
+    for (int k = 0; k < T::KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[k][2 * i] = (_Float16)(__uint_as_float(raw[k][i] << 16) * down);
+        q[k][2 * i + 1] = (_Float16)(__uint_as_float(raw[k][i] & 0xffff0000u) * down);
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < T::KS; ++k) {
+      const v4u raw = is ? *(const v4u*)(qp + 16 * k + 8 * half) : v4u{};
+      q[k] = __builtin_bit_cast(v8h, raw);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qm[i] = (_Float16)0.f;
+#pragma unroll
+    for (int g = 0; g < T::GS; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = g * T::GP; k < (g + 1) * T::GP; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += (float)q[k][i];
+      sum += __shfl_xor(sum, 32);
+      const _Float16 hi = (_Float16)sum;
+      if (half == g / 4) { qm[2 * (g % 4)] = hi; qm[2 * (g % 4) + 1] = (_Float16)(sum - (float)hi); }
+    }
+  }
+  cs = fmaxf(cs, 1e-30f);
+
+  // ---- the share of a tile that this wavefront widens: keys (0 - 3) or values (4 - 7)
+  const Exponents ex = exponents();
+  const bool takes_keys = wave < 4;
+  const int sub = D == 256 ? wave & 1 : wave & 3, chunk = D == 256 ? wave >> 1 & 1 : 0;
+  const int c16 = lane & 15, h4 = lane >> 4, block = (h4 & 1) << 1 | h4 >> 1;   // block: the four tokens of the sixteen whose values the lane takes
+  const uint32_t code_page = (uint32_t)c.heads * c.page * (D / 2), meta_page = (uint32_t)c.heads * c.page * (T::GS * 4);
+  const uint8_t* const codes = (takes_keys ? c.kc : c.vc) + (int64_t)h * c.page * (D / 2);
+  const uint8_t* const metas = (const uint8_t*)(takes_keys ? c.km : c.vm) + (int64_t)h * c.page * (T::GS * 4);
+  const int n8 = D == 64 ? c16 & 7 : c16 + 16 * chunk;             // the dword of a value's eight channels
+  const uint32_t code_at = takes_keys ? c16 * (D / 2) + 64 * chunk + h4 * (D == 64 ? 8 : 16) : block * (2 * D) + n8 * 16;
+  v4u code;
+  uint32_t meta[4];
+  int limit;                                                        // tokens of the sixteen that are there
+  auto fetch = [&](int page, int tok) {
+    const uint32_t in = tok & (c.page - 1), p = max(page, 0);
+    const uint8_t* cp = codes + ((uint64_t)p * code_page + in * (D / 2)) + code_at;
+    const uint8_t* mp = metas + ((uint64_t)p * meta_page + in * 4);
+    limit = page < 0 ? 0 : s.held - tok;
+    if (takes_keys) {
+      if constexpr (D == 64) {
+        const v2u two = *(const v2u*)cp;
+        code = v4u{two.x, two.y, 0, 0};
+      } else {
+        code = *(const v4u*)cp;
+      }
+      if constexpr (BF) {
+#pragma unroll
+        for (int g = 0; g < T::UG; ++g) meta[g] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + g) * c.page + c16));
+      } else {
+        meta[0] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + min(h4, T::UG - 1)) * c.page + c16));
+      }
+    } else {
+      code = *(const v4u*)cp;
+      const v4u four = *(const v4u*)(mp + 4 * ((8 * n8 / G) * c.page + 4 * block));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) meta[i] = four[i];
+    }
+  };
+  auto widen = [&](uint8_t* buf) {
+    if (takes_keys) {
+      uint8_t* const to = buf + (sub >> 1) * (T::KS * 1024) + (h4 & 1) * 512 + (16 * (sub & 1) + c16) * 16 + ((h4 >> 1) + 8 * chunk) * 1024;
+#pragma unroll
+      for (int j = 0; j < (D == 64 ? 2 : 4); ++j) {
+        v8h f = code_octet(code[j], ex);
+        if constexpr (BF) {
+          const v2h sm = __builtin_bit_cast(v2h, meta[j * 32 / G]);
+          const v8h s8 = {sm.x, sm.x, sm.x, sm.x, sm.x, sm.x, sm.x, sm.x}, m8 = {sm.y, sm.y, sm.y, sm.y, sm.y, sm.y, sm.y, sm.y};
+          f = __builtin_elementwise_fma(f, s8, m8);
+        }
+        *(v8h*)(to + 2 * j * 1024) = f;
+      }
+      if constexpr (!BF)
+        if (h4 < T::UG) {
+          const int g = T::UG * chunk + h4, key = 16 * sub + c16;
+          uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
+          *(uint32_t*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = __builtin_amdgcn_perm(meta[0], meta[0], 0x03020302u);
+          *(uint16_t*)(mins + T::M_BYTES + (g * T::KEYS + key) * 2) = (uint16_t)meta[0];
+        }
+    } else {
+      if (limit < 16)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) meta[i] = 4 * block + i < limit ? meta[i] : 0;   // whatever stands there: its value is 0
+      v2h s2[2], m2[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x05040100u));
+        m2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x07060302u));
+      }
+      uint8_t* const to = buf + T::K_BYTES + sub * (T::VT * 1024) + (block & 1) * 512 + (block >> 1) * 8;
+#pragma unroll
+      for (int by = 0; by < 4; ++by) {
+        uint32_t pr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w0 = D == 64 ? code[2 * i] >> (4 * (c16 >> 3)) : code[2 * i], w1 = D == 64 ? code[2 * i + 1] >> (4 * (c16 >> 3)) : code[2 * i + 1];
+          pr[i] = __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + by * 0x00010001u);
+        }
+        auto put = [&](int nibble, v2h x, v2h y) {
+          const int at = n8 + (D / 8) * nibble;                     // row of V^T
+          typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+          *(v4h*)(to + (at >> 5) * 1024 + (at & 31) * 16) = v4h{x.x, x.y, y.x, y.y};
+        };
+        put(D == 64 ? 2 * by + (c16 >> 3) : 2 * by, __builtin_elementwise_fma(codes_of<false>(pr[0], ex), s2[0], m2[0]),
+            __builtin_elementwise_fma(codes_of<false>(pr[1], ex), s2[1], m2[1]));
+        if constexpr (D > 64)
+          put(2 * by + 1, __builtin_elementwise_fma(codes_of<true>(pr[0], ex), s2[0], m2[0]),
+              __builtin_elementwise_fma(codes_of<true>(pr[1], ex), s2[1], m2[1]));
+      }
+    }
+  };
+  auto page_at = [&](int t) {
+    const int tok = token_of(t) + 16 * sub;
+    return tok < s.held ? page_of(c, r, b, tok) : -1;
+  };
+
+  v16f o[T::VT];
+  float m = FLOOR, l = 0.f;
+#pragma unroll
+  for (int t = 0; t < T::VT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+
+  if constexpr (!BF) {                                              // operand slots of groups that are not: 0, not what LDS holds
+    for (int i = tid; i < T::M_BYTES / 4; i += 64 * WAVES) {
+      *(uint32_t*)(lds + T::K_BYTES + T::V_BYTES + 4 * i) = 0;
+      *(uint32_t*)(lds + T::BYTES + T::K_BYTES + T::V_BYTES + 4 * i) = 0;
+    }
+    __syncthreads();
+  }
+  if (t0 < t1) {
+    fetch(page_at(t0), token_of(t0) + 16 * sub);
+    widen(lds);
+    if (t0 + 1 < t1) fetch(page_at(t0 + 1), token_of(t0 + 1) + 16 * sub);
+  }
+  int page_next = page_at(min(t0 + 2, t1 - 1));
+  __syncthreads();
+
+  for (int t = t0; t < t1; ++t) {
+    uint8_t* const buf = lds + ((t - t0) & 1) * T::BYTES;
+    const int tok = token_of(t);
+    const bool mine = wvalid > 0 && tok <= wpos_hi && (a.window <= 0 || tok + T::KEYS > wpos_lo - a.window + 1 || tok < a.sinks);
+    bool there[T::KT * 2];                                          // (looked up early: a scalar load)
+#pragma unroll
+    for (int i = 0; i < T::KT * 2; ++i) there[i] = tok + 16 * i < s.held && page_of(c, r, b, tok + 16 * i) >= 0;
+    v16f sc[T::KT];
+    if (mine) {
+#pragma unroll
+      for (int kt = 0; kt < T::KT; ++kt) {
+        const uint8_t* const from = buf + kt * (T::KS * 1024) + lane * 16;
+        if constexpr (BF) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < T::KS; ++k) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sc[kt], 0, 0, 0);
+        } else {
+          v16f zero;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+          const uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
+          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(mins + kt * 1024 + lane * 16), qm, zero, 0, 0, 0);
+#pragma unroll
+          for (int g = 0; g < T::GS; ++g) {
+            v16f sum = zero;
+#pragma unroll
+            for (int k = g * T::GP; k < (g + 1) * T::GP; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sum, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const v2u four = *(const v2u*)(mins + T::M_BYTES + (g * T::KEYS + 32 * kt + 8 * i + 4 * half) * 2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t two = four[e >> 1];
+                sc[kt][4 * i + e] = fmaf((float)__builtin_bit_cast(v2h, two)[e & 1], sum[4 * i + e], sc[kt][4 * i + e]);
+              }
+            }
+          }
+        }
+      }
+    }
+    if (t + 1 < t1) {
+      widen(lds + ((t + 1 - t0) & 1) * T::BYTES);
+      if (t + 2 < t1) {
+        fetch(page_next, token_of(t + 2) + 16 * sub);
+        page_next = page_at(min(t + 3, t1 - 1));
+      }
+    }
+    if (mine) {
+      // every row of the wavefront sees all tokens of the tile, and all of them are there
+      bool whole = tok + T::KEYS <= s.held && tok + T::KEYS - 1 <= wpos_lo && (a.window <= 0 || tok > wpos_hi - a.window || tok + T::KEYS <= a.sinks);
+#pragma unroll
+      for (int i = 0; i < T::KT * 2; ++i) whole = whole && there[i];
+      if (!whole) {
+#pragma unroll
+        for (int kt = 0; kt < T::KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = tok + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
+            const bool seen = there[2 * kt + (i >> 3)] && key < s.held && key <= pos && (a.window <= 0 || key > pos - a.window || key < a.sinks);
+            sc[kt][i] = seen ? sc[kt][i] : -__builtin_inff();
+          }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int kt = 0; kt < T::KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kt][i]);
+      top = rounded_product(fmaxf(top, __shfl_xor(top, 32)), cs);
+      if (__ballot(top > m + P_SLACK)) {
+        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < T::VT; ++v) o[v] *= f;
+      }
+      const float shift = P_BITS - m;
+#pragma unroll
+      for (int kt = 0; kt < T::KT; ++kt)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          v8h p, rest;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e0 = __builtin_amdgcn_exp2f(rounded_product(sc[kt][8 * st + 2 * i], cs) + shift);
+            const float e1 = __builtin_amdgcn_exp2f(rounded_product(sc[kt][8 * st + 2 * i + 1], cs) + shift);
+            const v2h ph = {(_Float16)e0, (_Float16)e1};
+            p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
+            l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+            if constexpr (!BF) {
+              const v2h pl = {(_Float16)(e0 - (float)ph.x), (_Float16)(e1 - (float)ph.y)};
+              rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
+              l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+            }
+          }
+          const uint8_t* const from = buf + T::K_BYTES + (2 * kt + st) * (T::VT * 1024) + lane * 16;
+#pragma unroll
+          for (int v = 0; v < T::VT; ++v) {
+            const v8h f = *(const v8h*)(from + v * 1024);
+            o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, p, o[v], 0, 0, 0);
+            if constexpr (!BF) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, rest, o[v], 0, 0, 0);
+          }
+        }
+    }
+    __syncthreads();
+  }
+
+  // ---- the ends of the rows
+  l += __shfl_xor(l, 32);
+  if (parts > 1 && tid == 0) {
+    if (part == 0) { desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = 0; }
+    desc->count = part == 0 ? parts : 0;
+  }
+  if (!is) return;
+  float* const out = parts > 1 ? attn_part<D>(a.ws, gridDim.x, place * ROWS + 32 * wave + col) : nullptr;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  constexpr int NS = D / 16;                                        // eights of channels a lane holds
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int rr = i & 3, aa = i >> 2, n = 8 * aa + 4 * half + rr;
+    float x[8];
+#pragma unroll
+    for (int ch = 0; ch < 8; ++ch) {
+      const int j = ch / 2 + 4 * (ch & 1);                          // the nibble of channel 8n + ch
+      x[ch] = D == 64 ? o[j >> 2][4 * (j & 3) + rr] : D == 128 ? o[j >> 1][4 * (aa + 2 * (j & 1)) + rr] : o[j % T::VT][4 * aa + rr];
+    }
+    if (parts > 1) {
+      *(float4*)(out + 8 * n) = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4*)(out + 8 * n + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      uint16_t* const p = (uint16_t*)a.out + (int64_t)(s.first + tok_q) * a.ot + (int64_t)head_q * a.oh + 8 * n;
+      v4u y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        y[j] = BF ? (uint32_t)f2bf(x[2 * j] * f) | (uint32_t)f2bf(x[2 * j + 1] * f) << 16
+                  : (uint32_t)f2h(x[2 * j] * f) | (uint32_t)f2h(x[2 * j + 1] * f) << 16;
+      *(v4u*)p = y;
+    }
+  }
+  if (parts > 1 && half == 0) { out[D] = m; out[D + 1] = l; }
+}
+
+// ------------------------------------------------------------------ launch
+PromptPlan plan_prompt(const DCache& c, const DRows& r, int ratio) {
+  PromptPlan p;
+  const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;
+  const int most = r.cap / 512 > 1 ? r.cap / 512 : 1;               // parts of 512 tokens at least
+  int64_t parts = tiles >= 256 ? 1 : 512 / tiles;
+  p.parts = (int)(parts < most ? parts : most);
+  p.grid = tiles * p.parts;
+  p.bytes = p.parts > 1 ? attn_bytes((int)p.grid, ROWS, 1, c.dim) : 0;
+  return p;
+}
+
+template <int D, int G, bool BF>
+static int prompt3(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((cache_prompt_kernel<D, G, BF>), dim3((unsigned)p.grid), dim3(64 * WAVES), 0, st, c, r, a, p.parts);
+  return CBK_OK;
+}
+template <int D, int G>
+static int prompt2(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  return a.bf ? prompt3<D, G, true>(p, c, r, a, st) : prompt3<D, G, false>(p, c, r, a, st);
+}
+template <int D>
+static int prompt1(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  if (c.group == 32) return prompt2<D, 32>(p, c, r, a, st);
+  if (c.group == 64) return prompt2<D, 64>(p, c, r, a, st);
+  if constexpr (D > 64) return prompt2<D, 128>(p, c, r, a, st);
+  return CBK_ERR_LAYOUT;
+}
+int launch_cache_prompt(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  const int rc = c.dim == 64 ? prompt1<64>(p, c, r, a, st) : c.dim == 128 ? prompt1<128>(p, c, r, a, st) : prompt1<256>(p, c, r, a, st);
+  if (rc) return rc;
+  if (p.parts > 1) launch_cache_join(c.dim, a, (int)p.grid, p.parts, ROWS, 1, st);
+  return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
+}
+
+}  // namespace cbk

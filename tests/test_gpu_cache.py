@@ -231,6 +231,21 @@ def test_whole_prompts(dim, ratio, dtype, window, sinks):
     s.attend([0, 70, 0, 200, 1, 399], ratio, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,group,page", [(64, 32, 16), (64, 64, 64), (128, 32, 16), (128, 64, 32), (128, 128, 256), (256, 32, 16), (256, 64, 64), (256, 128, 32)])
+def test_prompts_of_every_format(dim, group, page, dtype):
+    s = Setup([1, 75, 0, 300, 64], 2, dim, page, group, dtype, seed=dim * group)
+    s.attend(s.lens, 3)
+    s.attend([0, 40, 0, 130, 64], 2, window=48, sinks=5)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (128, torch.float16), (128, torch.bfloat16), (256, torch.float16)])
+def test_chunks_behind_long_histories_are_cut_and_joined(dim, dtype):
+    s = Setup([7000, 40, 2600], 1, dim, 32, 32, dtype, seed=15)
+    s.attend([60, 40, 33], 4)
+    s.attend([70, 1, 100], 2, window=1500, sinks=100)
+
+
 @pytest.mark.parametrize("lens,heads,ratio", [([20011], 1, 4), ([9000, 3, 12345], 2, 2), ([4097], 8, 4)])
 def test_long_histories_are_cut_and_joined(lens, heads, ratio):
     s = Setup(lens, heads, 128, 64, 32, torch.bfloat16, seed=5)
