@@ -1,7 +1,7 @@
 // Writing keys and values into the 4-bit cache and reading them back.
 //
 // Per token, head and group of G channels, in float32:
-//   x' = x clamped to +-CACHE_TOP;  m = fp16(min x');  s = fp16((max x' - m) / 15)
+//   x' = x clamped to +-CACHE_TOP;  m = fp16(min x');  s = fp16((max x' - m) * fp32(1/15))
 //   c  = clamp(rint((x' - m) / s), 0, 15), 0 where s = 0;   held value: m + c s
 // A NaN anywhere in a token's key or value of a head is held as a NaN in the minimum of all its key groups, and the value
 // as zeros: a row of attention that sees the token gets a NaN score, and a row that does not multiplies a
@@ -60,6 +60,12 @@ template <int N> __device__ inline float group_max(float x) {
   return x;
 }
 
+// A float32 result that is rounded again: without the barrier the compiler takes one instruction that rounds the exact value to fp16.
+__device__ inline float as_float32(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 template <int DT>
 __device__ inline void unpack8(const v4u q, float (&x)[8]) {
 #pragma unroll
@@ -81,7 +87,7 @@ __device__ inline uint32_t quantise(const float (&x)[8], uint32_t& meta) {
   hi = group_max<GL>(hi);
   const uint16_t mb = f2h(lo);
   const float m = h2f(mb);
-  const uint16_t sb = f2h((hi - m) / 15.f);
+  const uint16_t sb = f2h(as_float32((hi - m) * (1.f / 15.f)));
   const float s = h2f(sb);
   meta = (uint32_t)sb | (uint32_t)mb << 16;
   const float r = s > 0.f ? 1.f / s : 0.f;
@@ -151,7 +157,7 @@ __device__ inline void store8(void* p, int64_t i, const float (&x)[8]) {
     v4u o;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      o[j] = DT == CBK_F16 ? (uint32_t)f2h(x[2 * j]) | (uint32_t)f2h(x[2 * j + 1]) << 16
+      o[j] = DT == CBK_F16 ? (uint32_t)f2h(as_float32(x[2 * j])) | (uint32_t)f2h(as_float32(x[2 * j + 1])) << 16
                            : (uint32_t)f2bf(x[2 * j]) | (uint32_t)f2bf(x[2 * j + 1]) << 16;
     *(v4u*)((uint16_t*)p + i) = o;
   }

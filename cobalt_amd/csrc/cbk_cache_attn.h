@@ -53,15 +53,38 @@ __device__ inline float rounded_product(float a, float b) {
   return a * b;
 }
 
-// 2^e for the largest magnitude of a bf16 row (as bits), and `down` = 2^-e, which brings the row to [1, 2) (e = 127: to [2, 4), 2^-127
-// is no normal number); 1 for a row of zeros and one with an infinity or a NaN.
-__device__ inline float row_factor(uint32_t big, float& down) {
-  int e = max((int)(big >> 23), 1) - 127;
-  if (big == 0 || big >= 0x7f800000u) e = 0;
-  e = min(e, 126);
+// Power of two that a query row is divided by, and `down`, its reciprocal, for a largest magnitude `top`: 1 if the row (and sums of
+// 128 of its elements) is an ordinary fp16 row without it, else one that leaves [1, 2).  Also 1 for zeros, infinities and NaN.
+__device__ inline float row_factor(float top, float& down) {
+  int e = 0;
+  if (!(top >= 0x1p-6f && top < 0x1p8f) && top > 0.f && top < __builtin_inff())
+    e = min(max((int)(__float_as_uint(top) >> 23), 1) - 127, 126);  // (e = 127 would need 2^-127, which is no normal number: [2, 4) then)
   down = __uint_as_float((uint32_t)(127 - e) << 23);
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
+__device__ inline float bits_top(const v4u& w, bool bf, float top) {  // the largest magnitude of eight numbers and top; a NaN or infinity gives one
+  uint32_t big = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t hi = w[i] & 0x7fff0000u, lo = w[i] << 16 & 0x7fff0000u;
+    big = max(big, max(lo, hi));
+  }
+  const uint16_t b = (uint16_t)(big >> 16);
+  const float t = bf ? bf2f(b) : h2f(b);
+  return t > top || t != t ? t : top;
+}
+
+// The tokens a row sees, of those the table may hold: lo .. lo + n - 1 and those before `first`
+struct Sight { int lo; uint32_t n; int first; };
+__device__ inline Sight sight_of(int pos, int held, const AttnArgs& a) {
+  const int hi = min(pos, held - 1);
+  Sight s;
+  s.lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+  s.n = (uint32_t)max(hi - s.lo + 1, 0);
+  s.first = a.window > 0 ? min(a.sinks, hi + 1) : 0;
+  return s;
+}
+__device__ inline bool sees(const Sight& s, int token) { return (uint32_t)(token - s.lo) < s.n || token < s.first; }
 
 // four channels of a row: sums over the sum of p, 0 where the row saw nothing
 __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, const float (&y)[4], float sum) {

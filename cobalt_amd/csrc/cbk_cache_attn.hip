@@ -12,8 +12,8 @@
 //
 // Scores are exact up to float32: the codes themselves are the operands, one product per group of channels, and its sum is
 // multiplied by the token's scale; the minima, which are fp16 already, meet the sums of q over the groups in a product
-// of their own.  (Keys rounded to fp16 put 5e-4 of error into an fp16 result, which itself rounds by 2e-4.)  fp16 queries are
-// operands as they are, and a bf16 row is brought to [1, 2) by a power of two and is exact in fp16 then.
+// of their own.  (Keys rounded to fp16 put 5e-4 of error into an fp16 result, which itself rounds by 2e-4.)  Query rows are
+// operands as they are (bf16 of ordinary size is exact in fp16), rows of very large or small numbers after division by a power of two.
 // Values m + c s are rounded once to fp16 (2^-11).  p is kept at 2^8 times its size against the running maximum, so that what
 // an fp16 cannot hold lies 2^-32 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
 // bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
@@ -117,39 +117,31 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     // ---- queries: fragments, positions and factors
     v8h q[NT][KS], qm[NT];
     float cs[NT];
-    int pos[NT];
+    Sight sight[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 16 * n + col;
       const bool is = 16 * n + col < valid;
       const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
-      pos[n] = s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio);
+      sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
       const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
       v4u raw[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
-      cs[n] = a.scale;
-      if constexpr (BF) {
-        uint32_t big = 0;                                           // the largest magnitude, as bits
+      float top = 0.f, down;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+      top = across_max(top);
+      cs[n] = a.scale * row_factor(top, down);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) big = max(big, max(raw[k][i] << 16 & 0x7fff0000u, raw[k][i] & 0x7fff0000u));
-        big = max(big, (uint32_t)__shfl_xor((int)big, 16));
-        big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-        float down;
-        cs[n] *= row_factor(big, down);
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            q[n][k][2 * i] = (_Float16)(__uint_as_float(raw[k][i] << 16) * down);
-            q[n][k][2 * i + 1] = (_Float16)(__uint_as_float(raw[k][i] & 0xffff0000u) * down);
-          }
-      } else {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) q[n][k] = __builtin_bit_cast(v8h, raw[k]);
-      }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = raw[k][i];
+          const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+          q[n][k][2 * i] = (_Float16)(x0 * down);
+          q[n][k][2 * i + 1] = (_Float16)(x1 * down);
+        }
       // sums of q over the groups: as two fp16 that meet the minima
 #pragma unroll
       for (int i = 0; i < 8; ++i) qm[n][i] = (_Float16)0.f;
@@ -287,8 +279,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
             const bool there = key < s.held && (t ? p1 : p0);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const bool seen = there && key <= pos[n] && (a.window <= 0 || key > pos[n] - a.window || key < a.sinks);
-              sc[n][t][i] = seen ? sc[n][t][i] : -__builtin_inff();
+              sc[n][t][i] = there && sees(sight[n], key) ? sc[n][t][i] : -__builtin_inff();
             }
             if (!there)
 #pragma unroll

@@ -30,7 +30,7 @@ struct Tile {
   static constexpr int VS = KEYS / 16, VT = D / 32;                 // products along the tokens, 32-channel blocks
   static constexpr int UG = (D < 128 ? D : 128) / G;                // groups of a wavefront's share of the keys
   static constexpr int K_BYTES = KEYS * D * 2, V_BYTES = KEYS * D * 2;
-  static constexpr int M_BYTES = BF ? 0 : KT * 1024, S_BYTES = BF ? 0 : GS * KEYS * 2;   // minima as an operand, scales
+  static constexpr int M_BYTES = BF ? 0 : KT * 1024, S_BYTES = BF ? 0 : GS * KEYS * 4;   // minima as an operand, scales (float)
   static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES;
 };
 
@@ -86,33 +86,34 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   const int tok_q = is ? (wrow0 + col) / a.ratio : 0, head_q = h * a.ratio + (is ? (wrow0 + col) % a.ratio : 0);
   const int pos = is ? s.pos0 + tok_q : wpos_hi;
   const uint16_t* const qp = (const uint16_t*)a.q + (int64_t)(s.first + tok_q) * a.qt + (int64_t)head_q * a.qh;
+  const Sight sight = sight_of(pos, s.held, a);
+  // The scale of the scores is in the queries (bf16) or in the scales and sums that meet them (fp16, unless it would take those
+  // out of range); `grow` is what is left to multiply with.
+  const float fold = BF || a.scale <= 2.f ? a.scale : 1.f;
   v8h q[T::KS], qm;
-  float cs = a.scale;
-  if constexpr (BF) {
+  float grow;
+  {
     v4u raw[T::KS];
+    float top = 0.f, down;
 #pragma unroll
-    for (int k = 0; k < T::KS; ++k) raw[k] = is ? *(const v4u*)(qp + 16 * k + 8 * half) : v4u{};
-    uint32_t big = 0;
-#pragma unroll
-    for (int k = 0; k < T::KS; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) big = max(big, max(raw[k][i] << 16 & 0x7fff0000u, raw[k][i] & 0x7fff0000u));
-    big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-    float down;
-    cs *= row_factor(big, down);
+    for (int k = 0; k < T::KS; ++k) {
+      raw[k] = is ? *(const v4u*)(qp + 16 * k + 8 * half) : v4u{};
+      top = bits_top(raw[k], BF, top);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32));
+    grow = row_factor(BF ? top * fold : top, down) * (a.scale / fold);
+    const float times = BF ? fold : 1.f;
 #pragma unroll
     for (int k = 0; k < T::KS; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        q[k][2 * i] = (_Float16)(__uint_as_float(raw[k][i] << 16) * down);
-        q[k][2 * i + 1] = (_Float16)(__uint_as_float(raw[k][i] & 0xffff0000u) * down);
+        const uint32_t two = raw[k][i];
+        const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+        q[k][2 * i] = (_Float16)(x0 * down * times);
+        q[k][2 * i + 1] = (_Float16)(x1 * down * times);
       }
-  } else {
-#pragma unroll
-    for (int k = 0; k < T::KS; ++k) {
-      const v4u raw = is ? *(const v4u*)(qp + 16 * k + 8 * half) : v4u{};
-      q[k] = __builtin_bit_cast(v8h, raw);
-    }
+  }
+  if constexpr (!BF) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) qm[i] = (_Float16)0.f;
 #pragma unroll
@@ -122,12 +123,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       for (int k = g * T::GP; k < (g + 1) * T::GP; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += (float)q[k][i];
-      sum += __shfl_xor(sum, 32);
+      sum = (sum + __shfl_xor(sum, 32)) * fold;
       const _Float16 hi = (_Float16)sum;
       if (half == g / 4) { qm[2 * (g % 4)] = hi; qm[2 * (g % 4) + 1] = (_Float16)(sum - (float)hi); }
     }
   }
-  cs = fmaxf(cs, 1e-30f);
+  // Scores start from `start`, P_BITS less the running maximum, so that a sum is p's exponent as it leaves the product.  Rows with
+  // something left to multiply with, maxima so large that adding to them rounds, and rows that have seen nothing take the steps one by one.
+  const bool plain = __ballot(grow != 1.f) == 0;
+  bool ready = false;
+  float start = 0.f;
 
   // ---- the share of a tile that this wavefront widens: keys (0 - 3) or values (4 - 7)
   const Exponents ex = exponents();
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
           const int g = T::UG * chunk + h4, key = 16 * sub + c16;
           uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
           *(uint32_t*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = __builtin_amdgcn_perm(meta[0], meta[0], 0x03020302u);
-          *(uint16_t*)(mins + T::M_BYTES + (g * T::KEYS + key) * 2) = (uint16_t)meta[0];
+          *(float*)(mins + T::M_BYTES + (g * T::KEYS + key) * 4) = h2f((uint16_t)meta[0]) * fold;
         }
     } else {
       if (limit < 16)
@@ -260,28 +265,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         const uint8_t* const from = buf + kt * (T::KS * 1024) + lane * 16;
         if constexpr (BF) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
+          for (int i = 0; i < 16; ++i) sc[kt][i] = start;
 #pragma unroll
           for (int k = 0; k < T::KS; ++k) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sc[kt], 0, 0, 0);
         } else {
-          v16f zero;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) zero[i] = 0.f;
           const uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
-          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(mins + kt * 1024 + lane * 16), qm, zero, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kt][i] = start;
+          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(mins + kt * 1024 + lane * 16), qm, sc[kt], 0, 0, 0);
 #pragma unroll
           for (int g = 0; g < T::GS; ++g) {
-            v16f sum = zero;
+            v16f sum;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 #pragma unroll
             for (int k = g * T::GP; k < (g + 1) * T::GP; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sum, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const v2u four = *(const v2u*)(mins + T::M_BYTES + (g * T::KEYS + 32 * kt + 8 * i + 4 * half) * 2);
+              const v4f four = *(const v4f*)(mins + T::M_BYTES + (g * T::KEYS + 32 * kt + 8 * i + 4 * half) * 4);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t two = four[e >> 1];
-                sc[kt][4 * i + e] = fmaf((float)__builtin_bit_cast(v2h, two)[e & 1], sum[4 * i + e], sc[kt][4 * i + e]);
-              }
+              for (int e = 0; e < 4; ++e) sc[kt][4 * i + e] = fmaf(four[e], sum[4 * i + e], sc[kt][4 * i + e]);
             }
           }
         }
@@ -303,10 +306,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 #pragma unroll
         for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = tok + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
-            const bool seen = there[2 * kt + (i >> 3)] && key < s.held && key <= pos && (a.window <= 0 || key > pos - a.window || key < a.sinks);
-            sc[kt][i] = seen ? sc[kt][i] : -__builtin_inff();
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t n = there[2 * kt + j] ? sight.n : 0;
+            const int first = there[2 * kt + j] ? sight.first : 0;
+#pragma unroll
+            for (int i = 8 * j; i < 8 * j + 8; ++i) {
+              const int key = tok + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
+              sc[kt][i] = sees(Sight{sight.lo, n, first}, key) ? sc[kt][i] : -__builtin_inff();
+            }
           }
       }
       float top = -__builtin_inff();
@@ -314,15 +321,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kt][i]);
-      top = rounded_product(fmaxf(top, __shfl_xor(top, 32)), cs);
-      if (__ballot(top > m + P_SLACK)) {
-        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (!ready || __ballot(top > P_BITS + P_SLACK)) {             // the maximum follows when p would leave its range
+        const float g = ready ? 1.f : grow;
+        const float up = fmaxf(m, rounded_product(top, g) - start), f = __builtin_amdgcn_exp2f(m - up);
         m = up;
         l *= f;
 #pragma unroll
         for (int v = 0; v < T::VT; ++v) o[v] *= f;
+        const float by = (P_BITS - m) - start;
+#pragma unroll
+        for (int kt = 0; kt < T::KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kt][i] = rounded_product(sc[kt][i], g) + by;
+        ready = plain && __ballot(!(fabsf(m) < 0x1p15f)) == 0;
+        start = ready ? P_BITS - m : 0.f;
       }
-      const float shift = P_BITS - m;
 #pragma unroll
       for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
@@ -330,8 +344,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
           v8h p, rest;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e0 = __builtin_amdgcn_exp2f(rounded_product(sc[kt][8 * st + 2 * i], cs) + shift);
-            const float e1 = __builtin_amdgcn_exp2f(rounded_product(sc[kt][8 * st + 2 * i + 1], cs) + shift);
+            const float e0 = __builtin_amdgcn_exp2f(sc[kt][8 * st + 2 * i]);
+            const float e1 = __builtin_amdgcn_exp2f(sc[kt][8 * st + 2 * i + 1]);
             const v2h ph = {(_Float16)e0, (_Float16)e1};
             p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
             l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);

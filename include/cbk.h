@@ -269,7 +269,7 @@ int cbk_linear_act(const cbk_desc* d, const void* x, int x_dtype, int M, int64_t
  * Keys and values of attention in the framework's own terms: groups of `group` consecutive channels of one token and head,
  * 4-bit codes rounded to nearest, an fp16 scale and an fp16 minimum per group (4 + 32 / group bits a value):
  *
- *     x' = x clamped to +-65280,  m = fp16(min x'),  s = fp16((max x' - m) / 15),
+ *     x' = x clamped to +-65280,  m = fp16(min x'),  s = fp16((max x' - m) * fp32(1/15)),
  *     c = clamp(rint((x' - m) / s), 0, 15)  (0 where s = 0),     held value m + c s,
  *
  * in float32 steps.  A NaN anywhere in a token's key or value of a head makes that token's key and value of the head

@@ -14,7 +14,7 @@ def held(k, v, group):
             f = np.where(np.isnan(x), np.float32(0), np.clip(x, -TOP, TOP)).astype(np.float32)
             g = f.reshape(*f.shape[:-1], -1, group)
             m = g.min(-1, keepdims=True).astype(np.float16).astype(np.float32)
-            s = ((g.max(-1, keepdims=True) - m) / np.float32(15)).astype(np.float16).astype(np.float32)
+            s = ((g.max(-1, keepdims=True) - m) * (np.float32(1) / np.float32(15))).astype(np.float16).astype(np.float32)
             c = np.where(s == 0, np.float32(0), np.clip(np.rint((g - m) / np.where(s == 0, np.float32(1), s)), 0, 15))
         y = (m.astype(np.float64) + c.astype(np.float64) * s.astype(np.float64)).reshape(f.shape)
         out.append(np.where(bad, np.nan, y))

@@ -142,6 +142,25 @@ def test_values_at_the_ends_of_the_range():
         np.testing.assert_array_equal(k16.float().cpu().numpy(), torch.from_numpy(s.hk).float().to(t).float().numpy())
 
 
+def test_scales_and_values_at_the_borders_of_rounding():
+    """Ranges whose fifteenth lies exactly between two fp16 numbers, or a float32 step beside, and values between two codes."""
+    g = torch.Generator().manual_seed(1)
+    n = 20000
+    lo = -torch.randint(1, 1 << 11, (n, 1, 1), generator=g) * 2.0 ** -5
+    step = torch.randint(1 << 11, 1 << 12, (n, 1, 1), generator=g) * 2.0 ** -12     # 12 bits: every second one a tie
+
+    def fill(s):
+        s.k[:] = (lo + 15 * step * torch.rand(n, 1, 64, generator=g)).half()
+        s.k[:, :, 0:1], s.k[:, :, 63:] = lo.half(), (lo + 15 * step).half()
+        s.v[:] = (lo + step * (torch.randint(0, 31, (n, 1, 64), generator=g) / 2)).half()
+        s.v[:, :, 0:1], s.v[:, :, 63:] = lo.half(), (lo + 15 * step).half()
+    s = Setup([n], 1, 64, 256, 64, torch.float16, fill=fill)
+    for t in (torch.float32, torch.float16):
+        k, v = ops.cache_read(s.cache, s.rows([n]), n, t)
+        assert torch.equal(k.cpu(), torch.from_numpy(s.hk).float().to(t))
+        assert torch.equal(v.cpu(), torch.from_numpy(s.hv).float().to(t))
+
+
 def test_a_write_touches_its_own_tokens_only():
     s = Setup([37, 20], 3, 128, 16, 64, torch.float16, spare=3)
     n = [2, 1]
@@ -345,6 +364,43 @@ def test_large_and_small_queries():
     for scale in (1e-4, 0.5):
         out = ops.cache_attention(s.cache, q[2:], s.rows([2]), scale=scale)
         s.check(q[2:], out, [2], scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [4, 64])
+def test_rows_of_all_sizes_side_by_side(n, dtype):
+    """Rows from the smallest to the largest numbers of their type, in one product with ordinary ones; scales from 1e-6 to 30."""
+    s = Setup([300], 1, 128, 32, 32, dtype, outliers=False, seed=3)
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(n, 2, 128, generator=g)
+    low, high = (-22, 13) if dtype == torch.float16 else (-120, 60)
+    size = torch.linspace(low, high, 2 * n).view(2, n).t().round()
+    q = (base * 2.0 ** size[..., None]).to(dtype).to(DEV)
+    out = ops.cache_attention(s.cache, q, s.rows([n]))
+    small = (size.amax(1) < 2).to(DEV)                              # (scores below 64, as the bound wants them)
+    qd = q.double().cpu().numpy()
+    for i in range(n):
+        pos = 300 - n + i
+        for h in range(2):
+            sc = s.hk[:pos + 1, 0] @ qd[i, h] * 128 ** -0.5
+            if np.abs(sc).max() < 40:
+                o, spread, sz, reach = R.attention(qd[i:i + 1, h], s.hk[:, 0], s.hv[:, 0], np.array([pos]), np.ones(300, bool), 128 ** -0.5)
+                e = U * reach[0] + U + 2.0 ** -16
+                tol = e / (1 - e) * spread + U * sz
+                tol = tol + HALF[dtype] * (np.abs(o) + tol) + 2.0 ** -25
+                assert (np.abs(out[i, h].double().cpu().numpy() - o[0]) <= tol[0]).all(), (i, h)
+            elif np.sort(sc)[-1] - np.sort(sc)[-2] > 200 + 0.002 * np.abs(sc).max():   # one token takes all
+                want = s.hv[sc.argmax(), 0]
+                assert (np.abs(out[i, h].double().cpu().numpy() - want) <= (HALF[dtype] + U + 2.0 ** -16) * np.abs(want) + 1e-6).all(), (i, h)
+            else:
+                assert bool(torch.isfinite(out[i, h]).all())
+    assert bool(small.any())
+    ones = torch.full((n, 2, 128), 2.0 ** 13, device=DEV).to(dtype)    # all of one sign: their sum leaves fp16's range
+    out = ops.cache_attention(s.cache, ones, s.rows([n]))
+    assert bool(torch.isfinite(out).all())
+    for scale in (1e-6, 0.02, 3.0, 30.0):
+        q = (torch.randn(n, 2, 128, generator=g) * min(1.0, 0.05 / scale)).to(dtype).to(DEV)
+        s.check(q, ops.cache_attention(s.cache, q, s.rows([n]), scale=scale), [n], scale=scale)
 
 
 def test_one_token_outweighs_a_long_history():
