@@ -5,7 +5,9 @@
 namespace cbk {
 
 constexpr float FLOOR = -3.0e38f;           // running maximum before the first token: below every score that is one
-constexpr float P_BITS = 8.f, P_SLACK = 6.f;   // p = 2^(t - M + P_BITS) with t <= M + P_SLACK: at most 2^14
+// p = 2^((t - M) + P_BITS) with t <= M + P_SLACK.  Where scores are so large that float32 holds multiples of 2, 4, 8 ... only, P_BITS rounds to
+// 8 at most and P_SLACK to 4, never both up in steps of 8 and 16: p stays below 2^13 whatever the size of M.
+constexpr float P_BITS = 7.5f, P_SLACK = 3.5f;
 
 struct AttnArgs {
   const void* q;                            // [tokens, ratio * heads, D] fp16 or bf16
@@ -102,10 +104,10 @@ __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, c
 }
 
 // cbk_cache_prompt.hip: many rows a sequence
-struct PromptPlan { int parts; int64_t grid; size_t bytes; };
+struct PromptPlan { bool cut; int64_t grid; size_t bytes; };
 PromptPlan plan_prompt(const DCache&, const DRows&, int ratio);
 int launch_cache_prompt(const PromptPlan&, const DCache&, const DRows&, const AttnArgs&, hipStream_t);
-// Joins what the `grid` workgroups of a launch left; tiles of `rows` rows begin in every `every`th of them (cbk_cache_attn.hip)
-void launch_cache_join(int dim, const AttnArgs&, int grid, int every, int rows, int slots, hipStream_t);
+// Joins what the `grid` workgroups of a launch left; each in `slots` parts of `rows` rows at most (cbk_cache_attn.hip)
+void launch_cache_join(int dim, const AttnArgs&, int grid, int rows, int slots, hipStream_t);
 
 }  // namespace cbk

@@ -14,8 +14,8 @@
 // multiplied by the token's scale; the minima, which are fp16 already, meet the sums of q over the groups in a product
 // of their own.  (Keys rounded to fp16 put 5e-4 of error into an fp16 result, which itself rounds by 2e-4.)  Query rows are
 // operands as they are (bf16 of ordinary size is exact in fp16), rows of very large or small numbers after division by a power of two.
-// Values m + c s are rounded once to fp16 (2^-11).  p is kept at 2^8 times its size against the running maximum, so that what
-// an fp16 cannot hold lies 2^-32 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
+// Values m + c s are rounded once to fp16 (2^-11).  p is kept at 2^7.5 times its size against the running maximum, so that what
+// an fp16 cannot hold lies 2^-31 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
 // bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
 //
 // The tokens of all sequences and heads are one list of units of 128 tokens, cut into equal pieces, one a workgroup;
@@ -422,10 +422,10 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
 
 // One row of a tile that several workgroups have parts of: 256 threads, D/4 of them a part, a part after another.
 template <int D>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int every, int rows, int slots) {
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int rows, int slots) {
   constexpr int C = D / 4, P = 256 / C;
   __shared__ float sh[P][D + 4];
-  const int64_t w = (int64_t)blockIdx.x * every;
+  const int64_t w = blockIdx.x;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
   const int row = blockIdx.y, tid = threadIdx.x, d = 4 * (tid % C), p = tid / C;
   if (e.count == 0 || row >= e.valid) return;
@@ -472,11 +472,11 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   p.bytes = p.split ? attn_bytes(p.grid, p.rows, 2, c.dim) : 0;
   return p;
 }
-void launch_cache_join(int dim, const AttnArgs& a, int grid, int every, int rows, int slots, hipStream_t st) {
-  const dim3 blocks(grid / every, rows);
-  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
-  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
-  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, every, rows, slots);
+void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, int slots, hipStream_t st) {
+  const dim3 blocks(grid, rows);
+  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, rows, slots);
+  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, rows, slots);
+  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, rows, slots);
 }
 
 // More rows a sequence than this, on average, go to the kernel of cbk_cache_prompt.hip.
@@ -507,7 +507,7 @@ int launch_cache_attn(const DCache& c, const DRows& r, AttnArgs a, size_t ws_byt
   if (c.dim == 64) attn1<64>(p, c, r, a, st);
   else if (c.dim == 128) attn1<128>(p, c, r, a, st);
   else attn1<256>(p, c, r, a, st);
-  if (p.split) launch_cache_join(c.dim, a, p.grid, 1, p.rows, 2, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, p.rows, 2, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

@@ -14,61 +14,113 @@
 // as their codes with one product a group, multiplied by the token's scale in float32, the minima in a product of their own, and p
 // with its rest as a second operand.
 //
-// Tiles of rows are dealt out the longest first.  Where they are too few to fill the chip, the tokens of each are cut into `parts`,
-// joined by the second launch of cbk_cache_attn.hip.
+// Work is dealt out in one of two ways (plan_prompt).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
+// workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
+// of a tile that it does not finish is joined by the second launch of cbk_cache_attn.hip.
 #include "cbk_cache.h"
 #include "cbk_cache_attn.h"
 
 namespace cbk {
 
 constexpr int WAVES = 8, ROWS = 32 * WAVES;
+constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
 
 template <int D, int G, bool BF>
 struct Tile {
-  static constexpr int KEYS = D == 256 ? 32 : 64;                   // tokens of a tile
+  static constexpr int KEYS = D == 256 ? 32 : D == 128 ? 64 : 128;  // tokens of a tile
+  static constexpr int NU = D == 64 ? 2 : 1;                        // sixteens of tokens a wavefront widens
   static constexpr int KT = KEYS / 32, KS = D / 16, GS = D / G, GP = G / 16;   // 32-token blocks, products of a row, groups, products of a group
   static constexpr int VS = KEYS / 16, VT = D / 32;                 // products along the tokens, 32-channel blocks
   static constexpr int UG = (D < 128 ? D : 128) / G;                // groups of a wavefront's share of the keys
   static constexpr int K_BYTES = KEYS * D * 2, V_BYTES = KEYS * D * 2;
   static constexpr int M_BYTES = BF ? 0 : KT * 1024, S_BYTES = BF ? 0 : GS * KEYS * 4;   // minima as an operand, scales (float)
-  static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES;
+  static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES + 16;   // and a byte for each sixteen: its page is there
+};
+
+__device__ inline int row_tiles(const Seq& s, int ratio) { return (int)(((int64_t)s.n * ratio + ROWS - 1) / ROWS); }
+
+// What tiles of rows weigh when the list is cut: the tokens they see, times the query heads of a cache head so that no fraction is lost.  Only
+// the balance rests on it, not what is computed: a piece of a tile's weight is that piece of its tokens, rounded to tiles.
+struct Weights {
+  int ratio, window, sinks;
+  __device__ int64_t first(const Seq& s) const { return (int64_t)max(s.pos0, 0) * ratio; }
+  __device__ int64_t flat() const { return (int64_t)ROWS + (int64_t)ratio * ((int64_t)window + sinks); }
+  __device__ int64_t of(const Seq& s, int i) const { return window > 0 ? flat() : first(s) + (int64_t)(i + 1) * ROWS; }
+  __device__ int64_t before(const Seq& s, int i) const { return window > 0 ? i * flat() : i * first(s) + (int64_t)i * (i + 1) / 2 * ROWS; }
+  __device__ int64_t all(const Seq& s) const { return s.n > 0 ? before(s, row_tiles(s, ratio)) : 0; }
 };
 
 template <int D, int G, bool BF>
-__global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, DRows r, AttnArgs a, int parts) {
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, DRows r, AttnArgs a, int cut) {
   using T = Tile<D, G, BF>;
   __shared__ v4u lds4[2 * T::BYTES / 16];
   uint8_t* const lds = (uint8_t*)lds4;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
+  const Exponents ex = exponents();
 
-  // ---- this workgroup's rows: heads fastest (an XCD then meets few heads), the last tiles of a sequence first
-  const int h = blockIdx.x % c.heads, part = blockIdx.x / c.heads % parts;
-  const int64_t item = blockIdx.x / c.heads / parts;
-  const int64_t place = (item * c.heads + h) * parts + part;         // in the workspace: the parts of a tile side by side
-  AttnPiece* const desc = (AttnPiece*)a.ws + place;
-  int64_t base = 0;
-  int b = -1;
-  auto tiles_of = [&](int q) { return q < r.seqs ? (int64_t)((int64_t)seq_of(r, q).n * a.ratio + ROWS - 1) / ROWS : (int64_t)0; };
-  for (int j = 0; j < r.seqs; j += 64) {
-    const int64_t sum = scan64(tiles_of(j + lane), lane), here = of_lane(sum, 63);
-    if (item < base + here) {
-      const int l = __popcll(__ballot(base + sum <= item));
-      b = j + l;
-      if (l) base += of_lane(sum, l - 1);
-      break;
+  // ---- this workgroup's share: tile `tile` of head h of sequence b, or units [at, end) of the list
+  const Weights wt{a.ratio, a.window, a.sinks};
+  AttnPiece* desc = nullptr;
+  int64_t base = 0, at = 0, end = 0, begin = 0, total = 0, pieces = 0, place = 0;
+  int h, b = -1, tile = 0;
+  bool joined = false;
+  if (!cut) {                                                       // heads fastest: an XCD meets few of them; a sequence's last tiles first
+    h = blockIdx.x % c.heads;
+    const int64_t item = blockIdx.x / c.heads;
+    for (int j = 0; j < r.seqs; j += 64) {
+      const int64_t n = j + lane < r.seqs ? row_tiles(seq_of(r, j + lane), a.ratio) : 0, sum = scan64(n, lane), here = of_lane(sum, 63);
+      if (item < base + here) {
+        const int q = __popcll(__ballot(base + sum <= item));
+        b = j + q;
+        if (q) base += of_lane(sum, q - 1);
+        break;
+      }
+      base += here;
     }
-    base += here;
+    if (b < 0) return;
+    tile = row_tiles(seq_of(r, b), a.ratio) - 1 - (int)(item - base);
+  } else {                                                          // workgroups of an XCD are neighbours in the list: a head's tokens stay in its L2
+    place = gridDim.x % 8 ? blockIdx.x : (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    desc = (AttnPiece*)a.ws + place;
+    int64_t one = 0;                                                // units of a head
+    for (int j = 0; j < r.seqs; j += 64) one += of_lane(scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), 63);
+    total = one * c.heads;
+    pieces = min((int64_t)gridDim.x, total);
+    if (place >= pieces) {
+      if (tid == 0) desc->count = 0;
+      return;
+    }
+    const int64_t each = total / pieces, more = total % pieces;     // (no product of a place and the total: it could pass 64 bits)
+    begin = at = place * each + min(place, more);
+    end = at + each + (place < more);
+    h = (int)(begin / one);
+    base = h * one;
+    for (int j = 0;; j += 64) {
+      const int64_t sum = scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), here = of_lane(sum, 63);
+      if (begin < base + here) {
+        const int q = __popcll(__ballot(base + sum <= begin));
+        b = j + q;
+        if (q) base += of_lane(sum, q - 1);
+        break;
+      }
+      base += here;
+    }
+    const Seq s = seq_of(r, b);                                     // its tile: the last that begins at or before
+    int lo = 0, hi = row_tiles(s, a.ratio) - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (base + wt.before(s, mid) <= begin) lo = mid; else hi = mid - 1;
+    }
+    tile = lo;
   }
-  if (b < 0) {
-    if (parts > 1 && tid == 0) desc->count = 0;
-    return;
-  }
+
+  for (;;) {
   const Seq s = seq_of(r, b);
-  const int rows = s.n * a.ratio, row0 = ((rows + ROWS - 1) / ROWS - 1 - (int)(item - base)) * ROWS, valid = min(ROWS, rows - row0);
+  const int rows = s.n * a.ratio, row0 = tile * ROWS, valid = min(ROWS, rows - row0);
   const int pos_lo = s.pos0 + row0 / a.ratio, pos_hi = s.pos0 + (row0 + valid - 1) / a.ratio;
 
-  // ---- its tiles of tokens: the first `head`, then the others `skip` on
+  // ---- its tiles of tokens: the first `head`, then the others `skip` on; of them t0 .. t1 - 1
   int all = max((min(s.held, pos_hi + 1) + T::KEYS - 1) / T::KEYS, 1), head = 0, skip = 0;
   if (a.window > 0) {
     const int lo = min(max(pos_lo - a.window + 1, 0) / T::KEYS, all - 1);
@@ -76,7 +128,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     skip = lo - head;
     all -= skip;
   }
-  const int t0 = (int)((int64_t)all * part / parts), t1 = (int)((int64_t)all * (part + 1) / parts);
+  int t0 = 0, t1 = all;
+  bool whole_tile = true;
+  int64_t first_unit = 0, units = 0;
+  if (cut) {
+    first_unit = base + wt.before(s, tile);
+    units = wt.of(s, tile);
+    const int64_t x0 = at - first_unit, x1 = min(units, end - first_unit);
+    auto tiles_before = [&](int64_t x) { return x == units ? all : min((int)((double)x / (double)units * all), all); };
+    t0 = tiles_before(x0);
+    t1 = tiles_before(x1);
+    whole_tile = x0 == 0 && x1 == units;
+  }
   auto token_of = [&](int t) { return (t < head ? t : t + skip) * T::KEYS; };
 
   // ---- queries
@@ -135,7 +198,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   float start = 0.f;
 
   // ---- the share of a tile that this wavefront widens: keys (0 - 3) or values (4 - 7)
-  const Exponents ex = exponents();
   const bool takes_keys = wave < 4;
   const int sub = D == 256 ? wave & 1 : wave & 3, chunk = D == 256 ? wave >> 1 & 1 : 0;
   const int c16 = lane & 15, h4 = lane >> 4, block = (h4 & 1) << 1 | h4 >> 1;   // block: the four tokens of the sixteen whose values the lane takes
@@ -144,42 +206,57 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   const uint8_t* const metas = (const uint8_t*)(takes_keys ? c.km : c.vm) + (int64_t)h * c.page * (T::GS * 4);
   const int n8 = D == 64 ? c16 & 7 : c16 + 16 * chunk;             // the dword of a value's eight channels
   const uint32_t code_at = takes_keys ? c16 * (D / 2) + 64 * chunk + h4 * (D == 64 ? 8 : 16) : block * (2 * D) + n8 * 16;
-  v4u code;
-  uint32_t meta[4];
-  int limit;                                                        // tokens of the sixteen that are there
-  auto fetch = [&](int page, int tok) {
-    const uint32_t in = tok & (c.page - 1), p = max(page, 0);
-    const uint8_t* cp = codes + ((uint64_t)p * code_page + in * (D / 2)) + code_at;
-    const uint8_t* mp = metas + ((uint64_t)p * meta_page + in * 4);
-    limit = page < 0 ? 0 : s.held - tok;
-    if (takes_keys) {
-      if constexpr (D == 64) {
-        const v2u two = *(const v2u*)cp;
-        code = v4u{two.x, two.y, 0, 0};
-      } else {
-        code = *(const v4u*)cp;
-      }
-      if constexpr (BF) {
+  v4u code[T::NU];
+  uint32_t meta[T::NU][4];
+  int limit[T::NU], page_next[T::NU];                               // limit: tokens of the sixteen that are there
+  auto pages_at = [&](int t) {
 #pragma unroll
-        for (int g = 0; g < T::UG; ++g) meta[g] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + g) * c.page + c16));
-      } else {
-        meta[0] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + min(h4, T::UG - 1)) * c.page + c16));
-      }
-    } else {
-      code = *(const v4u*)cp;
-      const v4u four = *(const v4u*)(mp + 4 * ((8 * n8 / G) * c.page + 4 * block));
+    for (int u = 0; u < T::NU; ++u) {
+      const int tok = token_of(t) + 16 * (sub + 4 * u);
+      page_next[u] = tok < s.held ? page_of(c, r, b, tok) : -1;
+    }
+  };
+  auto fetch = [&](int t) {                                         // the pages of t are in page_next
 #pragma unroll
-      for (int i = 0; i < 4; ++i) meta[i] = four[i];
+    for (int u = 0; u < T::NU; ++u) {
+      const int tok = token_of(t) + 16 * (sub + 4 * u);
+      const uint32_t in = tok & (c.page - 1), p = max(page_next[u], 0);
+      const uint8_t* cp = codes + ((uint64_t)p * code_page + in * (D / 2)) + code_at;
+      const uint8_t* mp = metas + ((uint64_t)p * meta_page + in * 4);
+      limit[u] = page_next[u] < 0 ? 0 : s.held - tok;
+      if (takes_keys) {
+        if constexpr (D == 64) {
+          const v2u two = *(const v2u*)cp;
+          code[u] = v4u{two.x, two.y, 0, 0};
+        } else {
+          code[u] = *(const v4u*)cp;
+        }
+        if constexpr (BF) {
+#pragma unroll
+          for (int g = 0; g < T::UG; ++g) meta[u][g] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + g) * c.page + c16));
+        } else {
+          meta[u][0] = *(const uint32_t*)(mp + 4 * ((T::UG * chunk + min(h4, T::UG - 1)) * c.page + c16));
+        }
+      } else {
+        code[u] = *(const v4u*)cp;
+        const v4u four = *(const v4u*)(mp + 4 * ((8 * n8 / G) * c.page + 4 * block));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) meta[u][i] = four[i];
+      }
     }
   };
   auto widen = [&](uint8_t* buf) {
+#pragma unroll
+    for (int u = 0; u < T::NU; ++u) {
+    const int sb = sub + 4 * u;
     if (takes_keys) {
-      uint8_t* const to = buf + (sub >> 1) * (T::KS * 1024) + (h4 & 1) * 512 + (16 * (sub & 1) + c16) * 16 + ((h4 >> 1) + 8 * chunk) * 1024;
+      if (lane == 0) *(uint8_t*)(buf + T::BYTES - 16 + sb) = limit[u] > 0;
+      uint8_t* const to = buf + (sb >> 1) * (T::KS * 1024) + (h4 & 1) * 512 + (16 * (sb & 1) + c16) * 16 + ((h4 >> 1) + 8 * chunk) * 1024;
 #pragma unroll
       for (int j = 0; j < (D == 64 ? 2 : 4); ++j) {
-        v8h f = code_octet(code[j], ex);
+        v8h f = code_octet(code[u][j], ex);
         if constexpr (BF) {
-          const v2h sm = __builtin_bit_cast(v2h, meta[j * 32 / G]);
+          const v2h sm = __builtin_bit_cast(v2h, meta[u][j * 32 / G]);
           const v8h s8 = {sm.x, sm.x, sm.x, sm.x, sm.x, sm.x, sm.x, sm.x}, m8 = {sm.y, sm.y, sm.y, sm.y, sm.y, sm.y, sm.y, sm.y};
           f = __builtin_elementwise_fma(f, s8, m8);
         }
@@ -187,28 +264,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       }
       if constexpr (!BF)
         if (h4 < T::UG) {
-          const int g = T::UG * chunk + h4, key = 16 * sub + c16;
+          const int g = T::UG * chunk + h4, key = 16 * sb + c16;
           uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
-          *(uint32_t*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = __builtin_amdgcn_perm(meta[0], meta[0], 0x03020302u);
-          *(float*)(mins + T::M_BYTES + (g * T::KEYS + key) * 4) = h2f((uint16_t)meta[0]) * fold;
+          *(uint32_t*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = __builtin_amdgcn_perm(meta[u][0], meta[u][0], 0x03020302u);
+          *(float*)(mins + T::M_BYTES + (g * T::KEYS + key) * 4) = h2f((uint16_t)meta[u][0]) * fold;
         }
     } else {
-      if (limit < 16)
+      if (limit[u] < 16)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) meta[i] = 4 * block + i < limit ? meta[i] : 0;   // whatever stands there: its value is 0
+        for (int i = 0; i < 4; ++i) meta[u][i] = 4 * block + i < limit[u] ? meta[u][i] : 0;   // whatever stands there: its value is 0
       v2h s2[2], m2[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        s2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x05040100u));
-        m2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x07060302u));
+        s2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[u][2 * i + 1], meta[u][2 * i], 0x05040100u));
+        m2[i] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(meta[u][2 * i + 1], meta[u][2 * i], 0x07060302u));
       }
-      uint8_t* const to = buf + T::K_BYTES + sub * (T::VT * 1024) + (block & 1) * 512 + (block >> 1) * 8;
+      uint8_t* const to = buf + T::K_BYTES + sb * (T::VT * 1024) + (block & 1) * 512 + (block >> 1) * 8;
 #pragma unroll
       for (int by = 0; by < 4; ++by) {
         uint32_t pr[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t w0 = D == 64 ? code[2 * i] >> (4 * (c16 >> 3)) : code[2 * i], w1 = D == 64 ? code[2 * i + 1] >> (4 * (c16 >> 3)) : code[2 * i + 1];
+          const uint32_t w0 = D == 64 ? code[u][2 * i] >> (4 * (c16 >> 3)) : code[u][2 * i], w1 = D == 64 ? code[u][2 * i + 1] >> (4 * (c16 >> 3)) : code[u][2 * i + 1];
           pr[i] = __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + by * 0x00010001u);
         }
         auto put = [&](int nibble, v2h x, v2h y) {
@@ -223,12 +300,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
               __builtin_elementwise_fma(codes_of<true>(pr[1], ex), s2[1], m2[1]));
       }
     }
+    }
   };
-  auto page_at = [&](int t) {
-    const int tok = token_of(t) + 16 * sub;
-    return tok < s.held ? page_of(c, r, b, tok) : -1;
-  };
-
   v16f o[T::VT];
   float m = FLOOR, l = 0.f;
 #pragma unroll
@@ -236,6 +309,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
 
+  __syncthreads();                                                  // (the reads of the last tile of rows)
   if constexpr (!BF) {                                              // operand slots of groups that are not: 0, not what LDS holds
     for (int i = tid; i < T::M_BYTES / 4; i += 64 * WAVES) {
       *(uint32_t*)(lds + T::K_BYTES + T::V_BYTES + 4 * i) = 0;
@@ -244,20 +318,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     __syncthreads();
   }
   if (t0 < t1) {
-    fetch(page_at(t0), token_of(t0) + 16 * sub);
+    pages_at(t0);
+    fetch(t0);
     widen(lds);
-    if (t0 + 1 < t1) fetch(page_at(t0 + 1), token_of(t0 + 1) + 16 * sub);
+    if (t0 + 1 < t1) {
+      pages_at(t0 + 1);
+      fetch(t0 + 1);
+      pages_at(min(t0 + 2, t1 - 1));
+    }
   }
-  int page_next = page_at(min(t0 + 2, t1 - 1));
   __syncthreads();
 
   for (int t = t0; t < t1; ++t) {
     uint8_t* const buf = lds + ((t - t0) & 1) * T::BYTES;
     const int tok = token_of(t);
     const bool mine = wvalid > 0 && tok <= wpos_hi && (a.window <= 0 || tok + T::KEYS > wpos_lo - a.window + 1 || tok < a.sinks);
-    bool there[T::KT * 2];                                          // (looked up early: a scalar load)
-#pragma unroll
-    for (int i = 0; i < T::KT * 2; ++i) there[i] = tok + 16 * i < s.held && page_of(c, r, b, tok + 16 * i) >= 0;
+    const v2u flags = *(const v2u*)(buf + T::BYTES - 16);
     v16f sc[T::KT];
     if (mine) {
 #pragma unroll
@@ -293,22 +369,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     if (t + 1 < t1) {
       widen(lds + ((t + 1 - t0) & 1) * T::BYTES);
       if (t + 2 < t1) {
-        fetch(page_next, token_of(t + 2) + 16 * sub);
-        page_next = page_at(min(t + 3, t1 - 1));
+        fetch(t + 2);
+        pages_at(min(t + 3, t1 - 1));
       }
     }
     if (mine) {
       // every row of the wavefront sees all tokens of the tile, and all of them are there
       bool whole = tok + T::KEYS <= s.held && tok + T::KEYS - 1 <= wpos_lo && (a.window <= 0 || tok > wpos_hi - a.window || tok + T::KEYS <= a.sinks);
-#pragma unroll
-      for (int i = 0; i < T::KT * 2; ++i) whole = whole && there[i];
+      uint32_t there[2] = {(uint32_t)__builtin_amdgcn_readfirstlane((int)flags.x), (uint32_t)__builtin_amdgcn_readfirstlane((int)flags.y)};
+      if (T::KEYS == 32) there[0] |= 0x01010000u;
+      whole = whole && there[0] == 0x01010101u && (T::KEYS < 128 || there[1] == 0x01010101u);
       if (!whole) {
 #pragma unroll
         for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t n = there[2 * kt + j] ? sight.n : 0;
-            const int first = there[2 * kt + j] ? sight.first : 0;
+            const bool held = there[kt >> 1] >> (8 * (2 * (kt & 1) + j)) & 1;
+            const uint32_t n = held ? sight.n : 0;
+            const int first = held ? sight.first : 0;
 #pragma unroll
             for (int i = 8 * j; i < 8 * j + 8; ++i) {
               const int key = tok + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
@@ -329,11 +407,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         l *= f;
 #pragma unroll
         for (int v = 0; v < T::VT; ++v) o[v] *= f;
-        const float by = (P_BITS - m) - start;
+        const float less = ready ? (m + start) - P_BITS : m, more = ready ? 0.f : P_BITS;   // (less the maximum first: it may dwarf P_BITS)
 #pragma unroll
         for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = rounded_product(sc[kt][i], g) + by;
+          for (int i = 0; i < 16; ++i) sc[kt][i] = (rounded_product(sc[kt][i], g) - less) + more;
         ready = plain && __ballot(!(fabsf(m) < 0x1p15f)) == 0;
         start = ready ? P_BITS - m : 0.f;
       }
@@ -369,54 +447,76 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 
   // ---- the ends of the rows
   l += __shfl_xor(l, 32);
-  if (parts > 1 && tid == 0) {
-    if (part == 0) { desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = 0; }
-    desc->count = part == 0 ? parts : 0;
-  }
-  if (!is) return;
-  float* const out = parts > 1 ? attn_part<D>(a.ws, gridDim.x, place * ROWS + 32 * wave + col) : nullptr;
-  const float f = l == 0.f ? 0.f : 1.f / l;
-  constexpr int NS = D / 16;                                        // eights of channels a lane holds
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const int rr = i & 3, aa = i >> 2, n = 8 * aa + 4 * half + rr;
-    float x[8];
-#pragma unroll
-    for (int ch = 0; ch < 8; ++ch) {
-      const int j = ch / 2 + 4 * (ch & 1);                          // the nibble of channel 8n + ch
-      x[ch] = D == 64 ? o[j >> 2][4 * (j & 3) + rr] : D == 128 ? o[j >> 1][4 * (aa + 2 * (j & 1)) + rr] : o[j % T::VT][4 * aa + rr];
-    }
-    if (parts > 1) {
-      *(float4*)(out + 8 * n) = make_float4(x[0], x[1], x[2], x[3]);
-      *(float4*)(out + 8 * n + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-      uint16_t* const p = (uint16_t*)a.out + (int64_t)(s.first + tok_q) * a.ot + (int64_t)head_q * a.oh + 8 * n;
-      v4u y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        y[j] = BF ? (uint32_t)f2bf(x[2 * j] * f) | (uint32_t)f2bf(x[2 * j + 1] * f) << 16
-                  : (uint32_t)f2h(x[2 * j] * f) | (uint32_t)f2h(x[2 * j + 1] * f) << 16;
-      *(v4u*)p = y;
+  const int slot = at == begin ? 0 : 1;
+  if (!whole_tile && at == first_unit) {                            // this workgroup begins the tile: it is joined from here
+    joined = true;
+    if (tid == 0) {
+      const int64_t last = first_unit + units - 1, each = total / pieces, more = total % pieces;
+      const int64_t e = last < more * (each + 1) ? last / (each + 1) : more + (last - more * (each + 1)) / each;
+      desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = slot;
+      desc->count = (int)(e - place + 1);
     }
   }
-  if (parts > 1 && half == 0) { out[D] = m; out[D + 1] = l; }
+  if (is) {
+    float* const out = whole_tile ? nullptr : attn_part<D>(a.ws, gridDim.x, (place * 2 + slot) * ROWS + 32 * wave + col);
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    constexpr int NS = D / 16;                                      // eights of channels a lane holds
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int rr = i & 3, aa = i >> 2, n = 8 * aa + 4 * half + rr;
+      float x[8];
+#pragma unroll
+      for (int ch = 0; ch < 8; ++ch) {
+        const int j = ch / 2 + 4 * (ch & 1);                        // the nibble of channel 8n + ch
+        x[ch] = D == 64 ? o[j >> 2][4 * (j & 3) + rr] : D == 128 ? o[j >> 1][4 * (aa + 2 * (j & 1)) + rr] : o[j % T::VT][4 * aa + rr];
+      }
+      if (!whole_tile) {
+        *(float4*)(out + 8 * n) = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(out + 8 * n + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        uint16_t* const p = (uint16_t*)a.out + (int64_t)(s.first + tok_q) * a.ot + (int64_t)head_q * a.oh + 8 * n;
+        v4u y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          y[j] = BF ? (uint32_t)f2bf(x[2 * j] * f) | (uint32_t)f2bf(x[2 * j + 1] * f) << 16
+                    : (uint32_t)f2h(x[2 * j] * f) | (uint32_t)f2h(x[2 * j + 1] * f) << 16;
+        *(v4u*)p = y;
+      }
+    }
+    if (!whole_tile && half == 0) { out[D] = m; out[D + 1] = l; }
+  }
+  if (!cut) return;
+
+  // ---- the next tile of the list
+  at = min(end, first_unit + units);
+  if (at >= end) break;
+  if (tile + 1 < row_tiles(s, a.ratio)) {
+    ++tile;
+  } else {
+    base += wt.all(s);
+    tile = 0;
+    do {                                                            // (there is one: at < total)
+      if (++b == r.seqs) { b = 0; ++h; }
+    } while (seq_of(r, b).n <= 0);
+  }
+  }
+  if (!joined && tid == 0) desc->count = 0;
 }
 
 // ------------------------------------------------------------------ launch
 PromptPlan plan_prompt(const DCache& c, const DRows& r, int ratio) {
   PromptPlan p;
-  const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;
-  const int most = r.cap / 512 > 1 ? r.cap / 512 : 1;               // parts of 512 tokens at least
-  int64_t parts = tiles >= 256 ? 1 : 512 / tiles;
-  p.parts = (int)(parts < most ? parts : most);
-  p.grid = tiles * p.parts;
-  p.bytes = p.parts > 1 ? attn_bytes((int)p.grid, ROWS, 1, c.dim) : 0;
+  const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;   // at most
+  const bool prompts = 2 * (int64_t)r.tokens > (int64_t)r.cap * r.seqs;          // most of what the table can hold is new
+  p.cut = tiles < (prompts ? 2 : 4) * CHIP;
+  p.grid = p.cut ? CHIP : tiles;
+  p.bytes = p.cut ? attn_bytes((int)p.grid, ROWS, 2, c.dim) : 0;
   return p;
 }
 
 template <int D, int G, bool BF>
 static int prompt3(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((cache_prompt_kernel<D, G, BF>), dim3((unsigned)p.grid), dim3(64 * WAVES), 0, st, c, r, a, p.parts);
+  hipLaunchKernelGGL((cache_prompt_kernel<D, G, BF>), dim3((unsigned)p.grid), dim3(64 * WAVES), 0, st, c, r, a, (int)p.cut);
   return CBK_OK;
 }
 template <int D, int G>
@@ -433,7 +533,7 @@ static int prompt1(const PromptPlan& p, const DCache& c, const DRows& r, const A
 int launch_cache_prompt(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
   const int rc = c.dim == 64 ? prompt1<64>(p, c, r, a, st) : c.dim == 128 ? prompt1<128>(p, c, r, a, st) : prompt1<256>(p, c, r, a, st);
   if (rc) return rc;
-  if (p.parts > 1) launch_cache_join(c.dim, a, (int)p.grid, p.parts, ROWS, 1, st);
+  if (p.cut) launch_cache_join(c.dim, a, (int)p.grid, ROWS, 2, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 
