@@ -114,60 +114,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     const int h = (int)(item / tiles), row0 = (int)(item % tiles) * R;
     const int valid = min(R, rows - row0);
 
-    // ---- queries: fragments, positions and factors
-    v8h q[NT][KS], qm[NT];
-    float cs[NT];
-    Sight sight[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 16 * n + col;
-      const bool is = 16 * n + col < valid;
-      const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
-      sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
-      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
-      v4u raw[KS];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
-      float top = 0.f, down;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
-      top = across_max(top);
-      cs[n] = a.scale * row_factor(top, down);
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = raw[k][i];
-          const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
-          q[n][k][2 * i] = (_Float16)(x0 * down);
-          q[n][k][2 * i + 1] = (_Float16)(x1 * down);
-        }
-      // sums of q over the groups: as two fp16 that meet the minima
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qm[n][i] = (_Float16)0.f;
-#pragma unroll
-      for (int g = 0; g < GS; ++g) {
-        float sum = 0.f;
-#pragma unroll
-        for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum += (float)q[n][k][i];
-        sum = across_sum(sum);
-        const _Float16 hi = (_Float16)sum;
-        if (h4 == g % 4) { qm[n][2 * (g / 4)] = hi; qm[n][2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
-      }
-      cs[n] = fmaxf(cs[n], 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
-    }
     const int pos_lo = s.pos0 + row0 / a.ratio, pos_hi = s.pos0 + (row0 + valid - 1) / a.ratio;
-
-    v4f o[NT][TILES];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m[n] = FLOOR; l[n] = 0.f;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) o[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    }
 
     // where the cache head's part of page 0 is, and what a page takes; offsets of the lane from a sixteen's first token
     const uint32_t code_page = (uint32_t)c.heads * c.page * (D / 2), meta_page = (uint32_t)c.heads * c.page * (GS * 4);
@@ -224,8 +171,63 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     fetch_keys(token_of(u0), pg);
     fetch_values(token_of(u0), pg);
     pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
+
+    // ---- queries: fragments, positions and factors
+    v8h q[NT][KS], qm[NT];
+    float cs[NT];
+    Sight sight[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + 16 * n + col;
+      const bool is = 16 * n + col < valid;
+      const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
+      sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
+      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
+      v4u raw[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
+      float top = 0.f, down;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+      top = across_max(top);
+      cs[n] = a.scale * row_factor(top, down);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = raw[k][i];
+          const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+          q[n][k][2 * i] = (_Float16)(x0 * down);
+          q[n][k][2 * i + 1] = (_Float16)(x1 * down);
+        }
+      // sums of q over the groups: as two fp16 that meet the minima
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qm[n][i] = (_Float16)0.f;
+#pragma unroll
+      for (int g = 0; g < GS; ++g) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum += (float)q[n][k][i];
+        sum = across_sum(sum);
+        const _Float16 hi = (_Float16)sum;
+        if (h4 == g % 4) { qm[n][2 * (g / 4)] = hi; qm[n][2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
+      }
+      cs[n] = fmaxf(cs[n], 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
+    }
+    v4f o[NT][TILES];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = FLOOR; l[n] = 0.f;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
     for (int u = u0; u < u1; ++u) {
       const int tok = token_of(u), tok_next = token_of(min(u + 1, u1 - 1));
+      if (tok >= s.held) break;                                     // (of the last unit: nothing follows)
       const bool p0 = pg[0] >= 0, p1 = pg[1] >= 0;
       // every row sees all 32 tokens, and all of them are there
       const bool whole = p0 && p1 && tok + 32 <= s.held && tok + 31 <= pos_lo &&
@@ -467,7 +469,9 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   // every tile of rows in units, if all sequences were as long as the table allows
   const int64_t tiles = ((int64_t)r.tokens * ratio / p.rows + r.seqs) * c.heads, units = r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1;
   const int64_t most = tiles * units;
-  p.grid = (int)(most < 1024 ? most : 1024);
+  // as many as run at once: four, three or two a CU, by the registers and the LDS they take
+  const int chip = 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2);
+  p.grid = (int)(most < chip ? most : chip);
   p.split = units > 1;
   p.bytes = p.split ? attn_bytes(p.grid, p.rows, 2, c.dim) : 0;
   return p;
