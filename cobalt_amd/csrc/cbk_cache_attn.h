@@ -17,7 +17,7 @@ struct AttnArgs {
   int ratio;                                // query heads on a cache head
   float scale;                              // times log2 e
   int window, sinks;                        // window 0: none
-  int least;                                // units a workgroup takes at least
+  int whole;                                // 1: a tile of rows is one workgroup's
   uint8_t* ws;                              // nullptr: nothing is cut
 };
 

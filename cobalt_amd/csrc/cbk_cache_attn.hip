@@ -27,6 +27,7 @@
 namespace cbk {
 
 constexpr int UNIT = 128;                   // tokens: 32 a wavefront
+constexpr int EXTRA = 2;                    // units that a tile of rows counts for by itself: its queries, its end
 
 struct Range { int units, head, skip; };    // units of a sequence; the first `head` from token 0, the others `skip` units on
 __device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
@@ -46,7 +47,7 @@ __device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads,
   if (b >= r.seqs) return 0;
   const Seq s = seq_of(r, b);
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
-  return tiles * heads * range_of(s, a).units;
+  return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
 }
 __device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
   // ---- this workgroup's piece of the list; every wavefront looks for itself, 64 sequences at a time
   int64_t sum = scan64(units_of(r, a, c.heads, lane, R), lane), total = of_lane(sum, 63);
   for (int j = 64; j < r.seqs; j += 64) total += of_lane(scan64(units_of(r, a, c.heads, j + lane, R), lane), 63);
-  const int64_t pieces = min((int64_t)gridDim.x, (total + a.least - 1) / a.least);
+  const int64_t pieces = min((int64_t)gridDim.x, total);
   const int64_t w = blockIdx.x;
   AttnPiece* const desc = (AttnPiece*)a.ws + w;
   if (w >= pieces) {
@@ -106,11 +107,15 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     const Seq s = seq_of(r, b);
     const Range g = range_of(s, a);
     const int rows = s.n * a.ratio, tiles = (rows + R - 1) / R;
-    const int64_t all = (int64_t)tiles * c.heads * g.units;
+    const int weight = a.whole ? 1 : g.units + EXTRA;
+    const int64_t all = (int64_t)tiles * c.heads * weight;
     if (at >= base + all) { base += all; ++b; continue; }
-    const int64_t item = (at - base) / g.units;
-    const int u0 = (int)((at - base) - item * g.units);
-    const int u1 = (int)min((int64_t)g.units, u0 + (end - at));
+    const int64_t item = (at - base) / weight, start = base + item * weight;
+    const int64_t until = min(end, start + weight);
+    const int u0 = a.whole ? 0 : max((int)(at - start) - EXTRA, 0), u1 = a.whole ? g.units : (int)(until - start) - EXTRA;
+    const bool is_first = at == begin;
+    at = until;
+    if (u1 <= u0) continue;                                         // nothing but what the tile counts for by itself
     const int h = (int)(item / tiles), row0 = (int)(item % tiles) * R;
     const int valid = min(R, rows - row0);
 
@@ -384,10 +389,10 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     }
     __syncthreads();
     const bool direct = u0 == 0 && u1 == g.units;
-    const int slot = at == begin ? 0 : 1;
+    const int slot = is_first ? 0 : 1;
     if (!direct && u0 == 0 && tid == 0) {                           // this workgroup begins the tile: it is joined from here
       // the last piece with a unit of it: pieces are cut at floor(i total / pieces)
-      const int64_t last = base + (item + 1) * g.units - 1;
+      const int64_t last = start + weight - 1;
       int64_t e = last * pieces / total;
       while (e + 1 < pieces && (e + 1) * total / pieces <= last) ++e;
       while (e > w && e * total / pieces > last) --e;
@@ -417,7 +422,6 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
         if (d == 0) { part[D] = top; part[D + 1] = sum; }
       }
     }
-    at += u1 - u0;
   }
   if (a.ws && !joined && tid == 0) desc->count = 0;
 }
@@ -461,18 +465,19 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int gr
 }
 
 // ------------------------------------------------------------------ launch
-struct AttnPlan { int grid, least, rows; bool split; size_t bytes; };
+struct AttnPlan { int grid, rows; bool split; size_t bytes; };
 static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   AttnPlan p;
   p.rows = 16;
-  p.least = 1;
-  // every tile of rows in units, if all sequences were as long as the table allows
+  // every tile of rows, in units as if all sequences were as long as the table allows
   const int64_t tiles = ((int64_t)r.tokens * ratio / p.rows + r.seqs) * c.heads, units = r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1;
-  const int64_t most = tiles * units;
-  // as many as run at once: four, three or two a CU, by the registers and the LDS they take
+  // as many workgroups as run at once: four, three or two a CU, by the registers and the LDS they take
   const int chip = 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2);
+  // Tiles of few units stay in one piece, which saves the second launch: up to 4 units (300 tokens of one sequence 10.2 against 11.4 us,
+  // 500 alike, 700 14.5 against 11.6), up to 8 where the tiles fill half the chip (64 sequences of 1000 tokens 24.4 against 32.5 us).
+  p.split = units > 8 || (units > 4 && 2 * tiles < chip);
+  const int64_t most = p.split ? tiles * (units + EXTRA) : tiles;
   p.grid = (int)(most < chip ? most : chip);
-  p.split = units > 1;
   p.bytes = p.split ? attn_bytes(p.grid, p.rows, 2, c.dim) : 0;
   return p;
 }
@@ -507,7 +512,7 @@ int launch_cache_attn(const DCache& c, const DRows& r, AttnArgs a, size_t ws_byt
   if (!need) a.ws = nullptr;
   if (many_rows(r, a.ratio)) return launch_cache_prompt(plan_prompt(c, r, a.ratio), c, r, a, st);
   const AttnPlan p = plan_attn(c, r, a.ratio);
-  a.least = p.split ? p.least : 1;
+  a.whole = !p.split;
   if (c.dim == 64) attn1<64>(p, c, r, a, st);
   else if (c.dim == 128) attn1<128>(p, c, r, a, st);
   else attn1<256>(p, c, r, a, st);

@@ -17,6 +17,7 @@
 // Work is dealt out in one of two ways (plan_prompt).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
 // workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
 // of a tile that it does not finish is joined by the second launch of cbk_cache_attn.hip.
+#include <type_traits>
 #include "cbk_cache.h"
 #include "cbk_cache_attn.h"
 
@@ -27,13 +28,13 @@ constexpr int CHIP = 256;                   // workgroups that run at once: one 
 
 template <int D, int G, bool BF>
 struct Tile {
-  static constexpr int KEYS = D == 256 ? 32 : D == 128 ? 64 : 128;  // tokens of a tile
-  static constexpr int NU = D == 64 ? 2 : 1;                        // sixteens of tokens a wavefront widens
-  static constexpr int KT = KEYS / 32, KS = D / 16, GS = D / G, GP = G / 16;   // 32-token blocks, products of a row, groups, products of a group
-  static constexpr int VS = KEYS / 16, VT = D / 32;                 // products along the tokens, 32-channel blocks
+  static constexpr int BLOCK = D == 256 ? 32 : 64, NU = 2;          // tokens whose scores are in registers at a time; of those a tile has NU
+  static constexpr int KEYS = NU * BLOCK;                           // tokens of a tile
+  static constexpr int KT = BLOCK / 32, KS = D / 16, GS = D / G, GP = G / 16;   // 32-token products of a block, products of a row, groups, products of a group
+  static constexpr int VS = BLOCK / 16, VT = D / 32;                // products along a block's tokens, 32-channel blocks
   static constexpr int UG = (D < 128 ? D : 128) / G;                // groups of a wavefront's share of the keys
   static constexpr int K_BYTES = KEYS * D * 2, V_BYTES = KEYS * D * 2;
-  static constexpr int M_BYTES = BF ? 0 : KT * 1024, S_BYTES = BF ? 0 : GS * KEYS * 4;   // minima as an operand, scales (float)
+  static constexpr int M_BYTES = BF ? 0 : KEYS / 32 * 1024, S_BYTES = BF ? 0 : GS * KEYS * 4;   // minima as an operand, scales (float)
   static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES + 16;   // and a byte for each sixteen: its page is there
 };
 
@@ -212,14 +213,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   auto pages_at = [&](int t) {
 #pragma unroll
     for (int u = 0; u < T::NU; ++u) {
-      const int tok = token_of(t) + 16 * (sub + 4 * u);
+      const int tok = token_of(t) + 16 * (sub + T::VS * u);
       page_next[u] = tok < s.held ? page_of(c, r, b, tok) : -1;
     }
   };
   auto fetch = [&](int t) {                                         // the pages of t are in page_next
 #pragma unroll
     for (int u = 0; u < T::NU; ++u) {
-      const int tok = token_of(t) + 16 * (sub + 4 * u);
+      const int tok = token_of(t) + 16 * (sub + T::VS * u);
       const uint32_t in = tok & (c.page - 1), p = max(page_next[u], 0);
       const uint8_t* cp = codes + ((uint64_t)p * code_page + in * (D / 2)) + code_at;
       const uint8_t* mp = metas + ((uint64_t)p * meta_page + in * 4);
@@ -245,10 +246,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       }
     }
   };
-  auto widen = [&](uint8_t* buf) {
-#pragma unroll
-    for (int u = 0; u < T::NU; ++u) {
-    const int sb = sub + 4 * u;
+  auto widen = [&](uint8_t* buf, auto unit) {
+    constexpr int u = decltype(unit)::value;
+    const int sb = sub + T::VS * u;
     if (takes_keys) {
       if (lane == 0) *(uint8_t*)(buf + T::BYTES - 16 + sb) = limit[u] > 0;
       uint8_t* const to = buf + (sb >> 1) * (T::KS * 1024) + (h4 & 1) * 512 + (16 * (sb & 1) + c16) * 16 + ((h4 >> 1) + 8 * chunk) * 1024;
@@ -300,8 +300,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
               __builtin_elementwise_fma(codes_of<true>(pr[1], ex), s2[1], m2[1]));
       }
     }
-    }
   };
+
   v16f o[T::VT];
   float m = FLOOR, l = 0.f;
 #pragma unroll
@@ -320,7 +320,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   if (t0 < t1) {
     pages_at(t0);
     fetch(t0);
-    widen(lds);
+    widen(lds, std::integral_constant<int, 0>{});
+    widen(lds, std::integral_constant<int, 1>{});
     if (t0 + 1 < t1) {
       pages_at(t0 + 1);
       fetch(t0 + 1);
@@ -331,34 +332,40 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 
   for (int t = t0; t < t1; ++t) {
     uint8_t* const buf = lds + ((t - t0) & 1) * T::BYTES;
-    const int tok = token_of(t);
-    const bool mine = wvalid > 0 && tok <= wpos_hi && (a.window <= 0 || tok + T::KEYS > wpos_lo - a.window + 1 || tok < a.sinks);
     const v2u flags = *(const v2u*)(buf + T::BYTES - 16);
+    auto block = [&](auto which) {
+    constexpr int hb = decltype(which)::value;
+    const int tok = token_of(t) + hb * T::BLOCK;
+    const bool mine = wvalid > 0 && tok <= wpos_hi && (a.window <= 0 || tok + T::BLOCK > wpos_lo - a.window + 1 || tok < a.sinks);
     v16f sc[T::KT];
     if (mine) {
+      const uint8_t* const from = buf + lane * 16;
 #pragma unroll
-      for (int kt = 0; kt < T::KT; ++kt) {
-        const uint8_t* const from = buf + kt * (T::KS * 1024) + lane * 16;
-        if constexpr (BF) {
+      for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = start;
+        for (int i = 0; i < 16; ++i) sc[kt][i] = start;
+      if constexpr (BF) {
 #pragma unroll
-          for (int k = 0; k < T::KS; ++k) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sc[kt], 0, 0, 0);
-        } else {
-          const uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
+        for (int k = 0; k < T::KS; ++k)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kt][i] = start;
-          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(mins + kt * 1024 + lane * 16), qm, sc[kt], 0, 0, 0);
+          for (int kt = 0; kt < T::KT; ++kt)
+            sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + ((hb * T::KT + kt) * T::KS + k) * 1024), q[k], sc[kt], 0, 0, 0);
+      } else {
+        const uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
+#pragma unroll
+        for (int kt = 0; kt < T::KT; ++kt) {
+          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(mins + (hb * T::KT + kt) * 1024 + lane * 16), qm, sc[kt], 0, 0, 0);
 #pragma unroll
           for (int g = 0; g < T::GS; ++g) {
             v16f sum;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 #pragma unroll
-            for (int k = g * T::GP; k < (g + 1) * T::GP; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + k * 1024), q[k], sum, 0, 0, 0);
+            for (int k = g * T::GP; k < (g + 1) * T::GP; ++k)
+              sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + ((hb * T::KT + kt) * T::KS + k) * 1024), q[k], sum, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const v4f four = *(const v4f*)(mins + T::M_BYTES + (g * T::KEYS + 32 * kt + 8 * i + 4 * half) * 4);
+              const v4f four = *(const v4f*)(mins + T::M_BYTES + (g * T::KEYS + hb * T::BLOCK + 32 * kt + 8 * i + 4 * half) * 4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) sc[kt][4 * i + e] = fmaf(four[e], sum[4 * i + e], sc[kt][4 * i + e]);
             }
@@ -366,25 +373,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         }
       }
     }
-    if (t + 1 < t1) {
-      widen(lds + ((t + 1 - t0) & 1) * T::BYTES);
-      if (t + 2 < t1) {
-        fetch(t + 2);
-        pages_at(min(t + 3, t1 - 1));
-      }
-    }
+    if (t + 1 < t1) widen(lds + ((t + 1 - t0) & 1) * T::BYTES, which);
     if (mine) {
       // every row of the wavefront sees all tokens of the tile, and all of them are there
-      bool whole = tok + T::KEYS <= s.held && tok + T::KEYS - 1 <= wpos_lo && (a.window <= 0 || tok > wpos_hi - a.window || tok + T::KEYS <= a.sinks);
-      uint32_t there[2] = {(uint32_t)__builtin_amdgcn_readfirstlane((int)flags.x), (uint32_t)__builtin_amdgcn_readfirstlane((int)flags.y)};
-      if (T::KEYS == 32) there[0] |= 0x01010000u;
-      whole = whole && there[0] == 0x01010101u && (T::KEYS < 128 || there[1] == 0x01010101u);
+      bool whole = tok + T::BLOCK <= s.held && tok + T::BLOCK - 1 <= wpos_lo && (a.window <= 0 || tok > wpos_hi - a.window || tok + T::BLOCK <= a.sinks);
+      uint32_t there = (uint32_t)__builtin_amdgcn_readfirstlane((int)(T::BLOCK == 64 && hb ? flags.y : flags.x));   // a byte a sixteen
+      if constexpr (T::BLOCK == 32) there = (hb ? there >> 16 : there & 0xffffu) | 0x01010000u;
+      whole = whole && there == 0x01010101u;
       if (!whole) {
 #pragma unroll
         for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const bool held = there[kt >> 1] >> (8 * (2 * (kt & 1) + j)) & 1;
+            const bool held = there >> (8 * (2 * kt + j)) & 1;
             const uint32_t n = held ? sight.n : 0;
             const int first = held ? sight.first : 0;
 #pragma unroll
@@ -415,32 +416,41 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         ready = plain && __ballot(!(fabsf(m) < 0x1p15f)) == 0;
         start = ready ? P_BITS - m : 0.f;
       }
+      // p of sixteen tokens while the products of the sixteen before run
+      v8h p[2], rest[2];
+      auto weights = [&](int st) {
 #pragma unroll
-      for (int kt = 0; kt < T::KT; ++kt)
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          v8h p, rest;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e0 = __builtin_amdgcn_exp2f(sc[kt][8 * st + 2 * i]);
-            const float e1 = __builtin_amdgcn_exp2f(sc[kt][8 * st + 2 * i + 1]);
-            const v2h ph = {(_Float16)e0, (_Float16)e1};
-            p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
-            l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
-            if constexpr (!BF) {
-              const v2h pl = {(_Float16)(e0 - (float)ph.x), (_Float16)(e1 - (float)ph.y)};
-              rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
-              l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
-            }
-          }
-          const uint8_t* const from = buf + T::K_BYTES + (2 * kt + st) * (T::VT * 1024) + lane * 16;
-#pragma unroll
-          for (int v = 0; v < T::VT; ++v) {
-            const v8h f = *(const v8h*)(from + v * 1024);
-            o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, p, o[v], 0, 0, 0);
-            if constexpr (!BF) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, rest, o[v], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const float e0 = __builtin_amdgcn_exp2f(sc[st >> 1][8 * (st & 1) + 2 * i]), e1 = __builtin_amdgcn_exp2f(sc[st >> 1][8 * (st & 1) + 2 * i + 1]);
+          const v2h ph = {(_Float16)e0, (_Float16)e1};
+          p[st & 1][2 * i] = ph.x; p[st & 1][2 * i + 1] = ph.y;
+          l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+          if constexpr (!BF) {
+            const v2h pl = {(_Float16)(e0 - (float)ph.x), (_Float16)(e1 - (float)ph.y)};
+            rest[st & 1][2 * i] = pl.x; rest[st & 1][2 * i + 1] = pl.y;
+            l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
           }
         }
+      };
+      weights(0);
+#pragma unroll
+      for (int st = 0; st < T::VS; ++st) {
+        const uint8_t* const from = buf + T::K_BYTES + (hb * T::VS + st) * (T::VT * 1024) + lane * 16;
+        if (st + 1 < T::VS) weights(st + 1);
+#pragma unroll
+        for (int v = 0; v < T::VT; ++v) {
+          const v8h f = *(const v8h*)(from + v * 1024);
+          o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, p[st & 1], o[v], 0, 0, 0);
+          if constexpr (!BF) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, rest[st & 1], o[v], 0, 0, 0);
+        }
+      }
+    }
+    };
+    block(std::integral_constant<int, 0>{});
+    block(std::integral_constant<int, 1>{});
+    if (t + 2 < t1) {
+      fetch(t + 2);
+      pages_at(min(t + 3, t1 - 1));
     }
     __syncthreads();
   }
