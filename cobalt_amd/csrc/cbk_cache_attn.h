@@ -27,8 +27,8 @@ struct AttnPiece { int count, slot, first, row0, valid, head, pad[2]; };
 
 // rows of a part: D sums, the maximum they stand against, the sum of p, padding to 16 bytes
 constexpr int attn_row(int dim) { return dim + 4; }
-inline size_t attn_bytes(int grid, int rows, int slots, int dim) {   // slots: parts a workgroup may leave
-  return ((size_t)grid * sizeof(AttnPiece) + 255) / 256 * 256 + (size_t)grid * slots * rows * attn_row(dim) * sizeof(float);
+inline size_t attn_bytes(int grid, int rows, int dim) {            // a workgroup may leave two parts
+  return ((size_t)grid * sizeof(AttnPiece) + 255) / 256 * 256 + (size_t)grid * 2 * rows * attn_row(dim) * sizeof(float);
 }
 template <int D>
 __device__ inline float* attn_part(uint8_t* ws, int64_t grid, int64_t row) {
@@ -107,7 +107,7 @@ __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, c
 struct PromptPlan { bool cut; int64_t grid; size_t bytes; };
 PromptPlan plan_prompt(const DCache&, const DRows&, int ratio);
 int launch_cache_prompt(const PromptPlan&, const DCache&, const DRows&, const AttnArgs&, hipStream_t);
-// Joins what the `grid` workgroups of a launch left; each in `slots` parts of `rows` rows at most (cbk_cache_attn.hip)
-void launch_cache_join(int dim, const AttnArgs&, int grid, int rows, int slots, hipStream_t);
+// Joins what the `grid` workgroups of a launch left of tiles of `rows` rows (cbk_cache_attn.hip)
+void launch_cache_join(int dim, const AttnArgs&, int grid, int rows, hipStream_t);
 
 }  // namespace cbk

@@ -65,9 +65,9 @@ struct Held {                               // a wavefront's 32 tokens: two sixt
   v4u v[2][D > 128 ? D / 128 : 1], vm[2][D > 128 ? D / 128 : 1];
 };
 
-template <int D, int G, int NT, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCache c, DRows r, AttnArgs a) {
-  constexpr int R = 16 * NT, KS = D / 32, GS = D / G, GU = (GS + 3) / 4, VU = D > 128 ? D / 128 : 1, TILES = D / 16;
+template <int D, int G, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_attn_kernel(DCache c, DRows r, AttnArgs a) {
+  constexpr int R = 16, KS = D / 32, GS = D / G, GU = (GS + 3) / 4, VU = D > 128 ? D / 128 : 1, TILES = D / 16;
   __shared__ float o_sh[4][R][D + 4];
   __shared__ float m_sh[4][R], l_sh[4][R];
   __shared__ v2u scale_sh[4][2][GS][4];       // a wavefront's own: scales of its 32 keys, by group, four in a piece
@@ -178,57 +178,51 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
     pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
 
     // ---- queries: fragments, positions and factors
-    v8h q[NT][KS], qm[NT];
-    float cs[NT];
-    Sight sight[NT];
+    v8h q[KS], qm;
+    float cs;
+    Sight sight;
+    const int row = row0 + col;
+    const bool is = col < valid;
+    const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
+    sight = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
+    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
+    v4u raw[KS];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 16 * n + col;
-      const bool is = 16 * n + col < valid;
-      const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
-      sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
-      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
-      v4u raw[KS];
+    for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
+    float top = 0.f, down;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 32 * k + 8 * h4) : v4u{};
-      float top = 0.f, down;
+    for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+    top = across_max(top);
+    cs = a.scale * row_factor(top, down);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
-      top = across_max(top);
-      cs[n] = a.scale * row_factor(top, down);
+    for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = raw[k][i];
-          const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
-          q[n][k][2 * i] = (_Float16)(x0 * down);
-          q[n][k][2 * i + 1] = (_Float16)(x1 * down);
-        }
-      // sums of q over the groups: as two fp16 that meet the minima
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qm[n][i] = (_Float16)0.f;
-#pragma unroll
-      for (int g = 0; g < GS; ++g) {
-        float sum = 0.f;
-#pragma unroll
-        for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum += (float)q[n][k][i];
-        sum = across_sum(sum);
-        const _Float16 hi = (_Float16)sum;
-        if (h4 == g % 4) { qm[n][2 * (g / 4)] = hi; qm[n][2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = raw[k][i];
+        const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+        q[k][2 * i] = (_Float16)(x0 * down);
+        q[k][2 * i + 1] = (_Float16)(x1 * down);
       }
-      cs[n] = fmaxf(cs[n], 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
-    }
-    v4f o[NT][TILES];
-    float m[NT], l[NT];
+    // sums of q over the groups: as two fp16 that meet the minima
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m[n] = FLOOR; l[n] = 0.f;
+    for (int i = 0; i < 8; ++i) qm[i] = (_Float16)0.f;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) o[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < GS; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += (float)q[k][i];
+      sum = across_sum(sum);
+      const _Float16 hi = (_Float16)sum;
+      if (h4 == g % 4) { qm[2 * (g / 4)] = hi; qm[2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
     }
+    cs = fmaxf(cs, 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
+    v4f o[TILES];
+    float m, l;
+    m = FLOOR; l = 0.f;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
 
     for (int u = u0; u < u1; ++u) {
       const int tok = token_of(u), tok_next = token_of(min(u + 1, u1 - 1));
@@ -237,7 +231,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
       // every row sees all 32 tokens, and all of them are there
       const bool whole = p0 && p1 && tok + 32 <= s.held && tok + 31 <= pos_lo &&
                          (a.window <= 0 || tok > pos_hi - a.window || tok + 32 <= a.sinks);
-      v4f sc[NT][2];
+      v4f sc[2];
       uint16_t* const mine_sh = (uint16_t*)scale_sh[wave];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -252,26 +246,21 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
         v8h mins;
 #pragma unroll
         for (int i = 0; i < 8; ++i) mins[i] = i < 2 * GU ? __builtin_bit_cast(v2h, x.km[t][i / 2 % GU]).y : (_Float16)0.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mins, qm[n], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mins, qm, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
         for (int g = 0; g < GS; ++g) {
-          v4f part[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) part[n] = v4f{0.f, 0.f, 0.f, 0.f};
+          v4f part;
+          part = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k) {
             const v8h f = code_octet(x.k[t][k], ex);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) part[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[n][k], part[n], 0, 0, 0);
+            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], part, 0, 0, 0);
           }
           const v2u sm = scale_sh[wave][t][g][h4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t two = sm[i >> 1];                      // (a bit cast of a vector's element reads its first)
-              sc[n][t][i] = fmaf((float)__builtin_bit_cast(v2h, two)[i & 1], part[n][i], sc[n][t][i]);
+              sc[t][i] = fmaf((float)__builtin_bit_cast(v2h, two)[i & 1], part[i], sc[t][i]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);                          // (or the second sixteen's operands take registers early)
@@ -284,43 +273,37 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
           for (int i = 0; i < 4; ++i) {
             const int key = tok + 16 * t + 4 * h4 + i;
             const bool there = key < s.held && (t ? p1 : p0);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              sc[n][t][i] = there && sees(sight[n], key) ? sc[n][t][i] : -__builtin_inff();
-            }
+            sc[t][i] = there && sees(sight, key) ? sc[t][i] : -__builtin_inff();
             if (!there)
 #pragma unroll
               for (int v = 0; v < VU; ++v) x.vm[t][v][i] = 0;       // whatever stands there: its value is 0
           }
       }
-      v8h p[NT], rest[NT];
+      v8h p, rest;
+      float e[8], top;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float e[8], top;
+      for (int i = 0; i < 8; ++i) e[i] = rounded_product(sc[i >> 2][i & 3], cs);
+      top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+      top = across_max(top);
+      if (__ballot(top > m + P_SLACK)) {                       // the maximum follows when p would leave its range
+        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = rounded_product(sc[n][i >> 2][i & 3], cs[n]);
-        top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-        top = across_max(top);
-        if (__ballot(top > m[n] + P_SLACK)) {                       // the maximum follows when p would leave its range
-          const float up = fmaxf(m[n], top), f = __builtin_amdgcn_exp2f(m[n] - up);
-          m[n] = up;
-          l[n] *= f;
+        for (int t = 0; t < TILES; ++t) o[t] *= f;
+      }
+      const float shift = P_BITS - m;
 #pragma unroll
-          for (int t = 0; t < TILES; ++t) o[n][t] *= f;
-        }
-        const float shift = P_BITS - m[n];
+      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i] + shift);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i] + shift);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
-          l[n] = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
-          p[n][2 * i] = ph.x; p[n][2 * i + 1] = ph.y;
-          if constexpr (!BF) {
-            const v2h pl = {(_Float16)(e[2 * i] - (float)ph.x), (_Float16)(e[2 * i + 1] - (float)ph.y)};
-            rest[n][2 * i] = pl.x; rest[n][2 * i + 1] = pl.y;
-            l[n] = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
-          }
+      for (int i = 0; i < 4; ++i) {
+        const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
+        l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+        p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
+        if constexpr (!BF) {
+          const v2h pl = {(_Float16)(e[2 * i] - (float)ph.x), (_Float16)(e[2 * i + 1] - (float)ph.y)};
+          rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
+          l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
         }
       }
 #pragma unroll
@@ -348,19 +331,15 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
 #pragma unroll
           for (int i = 0; i < 4; ++i) { const v2h y = __builtin_elementwise_fma(codes_of<false>(pr[i], ex), s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
           const int t0 = D == 64 ? by : 2 * by * VU + v;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) o[n][t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[n], o[n][t0], 0, 0, 0);
+          o[t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[t0], 0, 0, 0);
           if constexpr (!BF)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest[n], o[n][t0], 0, 0, 0);
+            o[t0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest, o[t0], 0, 0, 0);
           if constexpr (D > 64) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) { const v2h y = __builtin_elementwise_fma(codes_of<true>(pr[i], ex), s2[i], m2[i]); f[2 * i] = y.x; f[2 * i + 1] = y.y; }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[n], o[n][t0 + VU], 0, 0, 0);
+            o[t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[t0 + VU], 0, 0, 0);
             if constexpr (!BF)
-#pragma unroll
-              for (int n = 0; n < NT; ++n) o[n][t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest[n], o[n][t0 + VU], 0, 0, 0);
+              o[t0 + VU] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest, o[t0 + VU], 0, 0, 0);
           }
         }
       }
@@ -373,20 +352,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
 
     // ---- the four wavefronts' parts together
     __syncthreads();                                                // (the reads of the last item)
+    l = across_sum(l);
+    if (h4 == 0) { m_sh[wave][col] = m; l_sh[wave][col] = l; }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      l[n] = across_sum(l[n]);
-      if (h4 == 0) { m_sh[wave][16 * n + col] = m[n]; l_sh[wave][16 * n + col] = l[n]; }
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rw = 4 * h4 + i;                                // row of the tile: channel 8 n + that of the nibble
-          const int nd = D == 64 ? rw & 7 : D == 128 ? rw : 16 * (t & 1) + rw;
-          const int nib = D == 64 ? 2 * t + (rw >> 3) : D == 128 ? t : t >> 1;
-          o_sh[wave][16 * n + col][8 * nd + (nib < 4 ? 2 * nib : 2 * nib - 7)] = o[n][t][i];
-        }
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int rw = 4 * h4 + i;                                // row of the tile: channel 8 n + that of the nibble
+        const int nd = D == 64 ? rw & 7 : D == 128 ? rw : 16 * (t & 1) + rw;
+        const int nib = D == 64 ? 2 * t + (rw >> 3) : D == 128 ? t : t >> 1;
+        o_sh[wave][col][8 * nd + (nib < 4 ? 2 * nib : 2 * nib - 7)] = o[t][i];
+      }
     __syncthreads();
     const bool direct = u0 == 0 && u1 == g.units;
     const int slot = is_first ? 0 : 1;
@@ -426,79 +402,95 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void cache_attn_kernel(DCach
   if (a.ws && !joined && tid == 0) desc->count = 0;
 }
 
-// One row of a tile that several workgroups have parts of: 256 threads, D/4 of them a part, a part after another.
+// Rows of a tile that several workgroups have parts of, `share` of them a workgroup: D/4 threads a part, a part after another.
 template <int D>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int rows, int slots) {
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int rows, int share) {
   constexpr int C = D / 4, P = 256 / C;
   __shared__ float sh[P][D + 4];
-  const int64_t w = blockIdx.x;
+  // (turned by y: tiles often begin every so many workgroups, and workgroups go to the XCDs in turn.  512 rows in 16 parts each
+  // took one XCD 68 us.)
+  const int64_t w = (blockIdx.x + blockIdx.y) % gridDim.x;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
-  const int row = blockIdx.y, tid = threadIdx.x, d = 4 * (tid % C), p = tid / C;
-  if (e.count == 0 || row >= e.valid) return;
-  float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = p; i < e.count; i += P) {
-    const float* const part = attn_part<D>(a.ws, grid, ((w + i) * slots + (i ? 0 : e.slot)) * rows + row);
-    const float4 o = *(const float4*)(part + d);
-    const float mm = part[D], ll = part[D + 1], up = fmaxf(top, mm);
-    const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
-    top = up;
-    sum = sum * f + ll * g;
-    y[0] = y[0] * f + o.x * g; y[1] = y[1] * f + o.y * g; y[2] = y[2] * f + o.z * g; y[3] = y[3] * f + o.w * g;
+  if (e.count == 0) return;
+  const int tid = threadIdx.x, d = 4 * (tid % C), p = tid / C, end = min((int)(blockIdx.y + 1) * share, e.valid);
+  for (int row = blockIdx.y * share; row < end; ++row) {
+    float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = p; i < e.count; i += P) {
+      const float* const part = attn_part<D>(a.ws, grid, ((w + i) * 2 + (i ? 0 : e.slot)) * rows + row);
+      const float4 o = *(const float4*)(part + d);
+      const float mm = part[D], ll = part[D + 1], up = fmaxf(top, mm);
+      const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
+      top = up;
+      sum = sum * f + ll * g;
+      y[0] = y[0] * f + o.x * g; y[1] = y[1] * f + o.y * g; y[2] = y[2] * f + o.z * g; y[3] = y[3] * f + o.w * g;
+    }
+    *(float4*)&sh[p][d] = make_float4(y[0], y[1], y[2], y[3]);
+    if (d == 0) { sh[p][D] = top; sh[p][D + 1] = sum; }
+    __syncthreads();
+    if (p == 0) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) top = fmaxf(top, sh[i][D]);
+      sum = 0.f;
+      y[0] = y[1] = y[2] = y[3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float f = __builtin_amdgcn_exp2f(sh[i][D] - top);
+        sum += f * sh[i][D + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] += f * sh[i][d + j];
+      }
+      const int gr = e.row0 + row;
+      store_row4(a, e.first + gr / a.ratio, e.head * a.ratio + gr % a.ratio, d, y, sum);
+    }
+    __syncthreads();
   }
-  *(float4*)&sh[p][d] = make_float4(y[0], y[1], y[2], y[3]);
-  if (d == 0) { sh[p][D] = top; sh[p][D + 1] = sum; }
-  __syncthreads();
-  if (p) return;
-#pragma unroll
-  for (int i = 0; i < P; ++i) top = fmaxf(top, sh[i][D]);
-  sum = 0.f;
-  y[0] = y[1] = y[2] = y[3] = 0.f;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sh[i][D] - top);
-    sum += f * sh[i][D + 1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] += f * sh[i][d + j];
-  }
-  const int gr = e.row0 + row;
-  store_row4(a, e.first + gr / a.ratio, e.head * a.ratio + gr % a.ratio, d, y, sum);
 }
 
 // ------------------------------------------------------------------ launch
-struct AttnPlan { int grid, rows; bool split; size_t bytes; };
+// Every tile of 16 rows, at most; its units, if all sequences were as long as the table allows; the workgroups that run at once:
+// four, three or two a CU, by the registers and the LDS they take.
+struct Load { int64_t tiles, units; int chip; };
+static Load load_of(const DCache& c, const DRows& r, int ratio) {
+  return {((int64_t)r.tokens * ratio / 16 + r.seqs) * c.heads, r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1, 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2)};
+}
+struct AttnPlan { int grid; bool split; size_t bytes; };
 static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
+  const Load w = load_of(c, r, ratio);
   AttnPlan p;
-  p.rows = 16;
-  // every tile of rows, in units as if all sequences were as long as the table allows
-  const int64_t tiles = ((int64_t)r.tokens * ratio / p.rows + r.seqs) * c.heads, units = r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1;
-  // as many workgroups as run at once: four, three or two a CU, by the registers and the LDS they take
-  const int chip = 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2);
   // Tiles of few units stay in one piece, which saves the second launch: up to 4 units (300 tokens of one sequence 10.2 against 11.4 us,
   // 500 alike, 700 14.5 against 11.6), up to 8 where the tiles fill half the chip (64 sequences of 1000 tokens 24.4 against 32.5 us).
-  p.split = units > 8 || (units > 4 && 2 * tiles < chip);
-  const int64_t most = p.split ? tiles * (units + EXTRA) : tiles;
-  p.grid = (int)(most < chip ? most : chip);
-  p.bytes = p.split ? attn_bytes(p.grid, p.rows, 2, c.dim) : 0;
+  p.split = w.units > 8 || (w.units > 4 && 2 * w.tiles < w.chip);
+  const int64_t most = p.split ? w.tiles * (w.units + EXTRA) : w.tiles;
+  p.grid = (int)(most < w.chip ? most : w.chip);
+  p.bytes = p.split ? attn_bytes(p.grid, 16, c.dim) : 0;
   return p;
 }
-void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, int slots, hipStream_t st) {
-  const dim3 blocks(grid, rows);
-  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, rows, slots);
-  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, rows, slots);
-  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, rows, slots);
+void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, hipStream_t st) {
+  const int share = rows > 16 ? 4 : 1;                              // (a workgroup a row would be 65 k of them for tiles of 256 rows, most with nothing to do)
+  const dim3 blocks(grid, rows / share);
+  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, rows, share);
+  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, rows, share);
+  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, rows, share);
 }
 
-// More rows a sequence than this, on average, go to the kernel of cbk_cache_prompt.hip.
-constexpr int FEW = 32;
-static bool many_rows(const DRows& r, int ratio) { return (int64_t)r.tokens * ratio > (int64_t)FEW * r.seqs; }
+// Which of the two kernels.  That of cbk_cache_prompt.hip takes tiles of 256 rows, filled or not, and wins from about 100 rows a sequence
+// (128 channels, 8 cache heads, 16 sequences of 4096 tokens: 96 rows 85 against 89 us here, 256 rows 110 against 235; fp16 128 rows 146
+// against 137, 256 rows 172 against 256), but only where there is work for the chip: it starts and joins more slowly (one sequence of 8192
+// tokens: 256 rows 56 against 41 us here, 512 rows 59 against 66; of 1024 tokens: 1024 rows 56 against 23).
+static bool many_rows(const DCache& c, const DRows& r, int ratio) {
+  const int64_t rows = (int64_t)r.tokens * ratio;
+  if (rows <= (int64_t)112 * r.seqs) return false;
+  const Load w = load_of(c, r, ratio);
+  return w.tiles * (w.units + EXTRA) > (int64_t)16 * w.chip;
+}
 size_t cache_attn_workspace(const DCache& c, const DRows& r, int ratio) {
-  return many_rows(r, ratio) ? plan_prompt(c, r, ratio).bytes : plan_attn(c, r, ratio).bytes;
+  return many_rows(c, r, ratio) ? plan_prompt(c, r, ratio).bytes : plan_attn(c, r, ratio).bytes;
 }
 
 template <int D, int G>
 static void attn2(const AttnPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
-  if (a.bf) hipLaunchKernelGGL((cache_attn_kernel<D, G, 1, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
-  else hipLaunchKernelGGL((cache_attn_kernel<D, G, 1, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  if (a.bf) hipLaunchKernelGGL((cache_attn_kernel<D, G, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  else hipLaunchKernelGGL((cache_attn_kernel<D, G, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
 }
 template <int D>
 static void attn1(const AttnPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
@@ -510,13 +502,13 @@ int launch_cache_attn(const DCache& c, const DRows& r, AttnArgs a, size_t ws_byt
   const size_t need = cache_attn_workspace(c, r, a.ratio);
   if (need > ws_bytes || (need && !a.ws)) return CBK_ERR_WORKSPACE;
   if (!need) a.ws = nullptr;
-  if (many_rows(r, a.ratio)) return launch_cache_prompt(plan_prompt(c, r, a.ratio), c, r, a, st);
+  if (many_rows(c, r, a.ratio)) return launch_cache_prompt(plan_prompt(c, r, a.ratio), c, r, a, st);
   const AttnPlan p = plan_attn(c, r, a.ratio);
   a.whole = !p.split;
   if (c.dim == 64) attn1<64>(p, c, r, a, st);
   else if (c.dim == 128) attn1<128>(p, c, r, a, st);
   else attn1<256>(p, c, r, a, st);
-  if (p.split) launch_cache_join(c.dim, a, p.grid, p.rows, 2, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, 16, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

@@ -24,6 +24,7 @@
 namespace cbk {
 
 constexpr int WAVES = 8, ROWS = 32 * WAVES;
+constexpr int LEAST = 3;                     // tiles of tokens that are worth a share of their own
 constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
 
 template <int D, int G, bool BF>
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     int64_t one = 0;                                                // units of a head
     for (int j = 0; j < r.seqs; j += 64) one += of_lane(scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), 63);
     total = one * c.heads;
-    pieces = min((int64_t)gridDim.x, total);
+    pieces = min((int64_t)gridDim.x, max(total / ((int64_t)LEAST * T::KEYS * a.ratio), (int64_t)1));
     if (place >= pieces) {
       if (tid == 0) desc->count = 0;
       return;
@@ -520,7 +521,7 @@ PromptPlan plan_prompt(const DCache& c, const DRows& r, int ratio) {
   const bool prompts = 2 * (int64_t)r.tokens > (int64_t)r.cap * r.seqs;          // most of what the table can hold is new
   p.cut = tiles < (prompts ? 2 : 4) * CHIP;
   p.grid = p.cut ? CHIP : tiles;
-  p.bytes = p.cut ? attn_bytes((int)p.grid, ROWS, 2, c.dim) : 0;
+  p.bytes = p.cut ? attn_bytes((int)p.grid, ROWS, c.dim) : 0;
   return p;
 }
 
@@ -543,7 +544,7 @@ static int prompt1(const PromptPlan& p, const DCache& c, const DRows& r, const A
 int launch_cache_prompt(const PromptPlan& p, const DCache& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
   const int rc = c.dim == 64 ? prompt1<64>(p, c, r, a, st) : c.dim == 128 ? prompt1<128>(p, c, r, a, st) : prompt1<256>(p, c, r, a, st);
   if (rc) return rc;
-  if (p.cut) launch_cache_join(c.dim, a, (int)p.grid, ROWS, 2, st);
+  if (p.cut) launch_cache_join(c.dim, a, (int)p.grid, ROWS, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 
