@@ -8,7 +8,8 @@ protocol of the reference's src/prod/bench.py: steady-state tokens per second at
 that the number is the GPU work of a step and not the Python dispatch of its ~40 small kernels
 per block.  Prints one JSON line per measurement.  There are no checkpoints or datasets here:
 weights are random-initialised and calibration tokens are random ids, which leaves the timing
-unaffected and says nothing about accuracy.
+unaffected and says nothing about accuracy.  `--cache 4bit` decodes on the 4-bit key/value cache
+(`model.cobalt_cache`) instead of a static fp16 one, `--context` after a longer prompt.
 """
 from __future__ import annotations
 
@@ -19,8 +20,19 @@ import time
 import torch
 
 
-def _decode_tokens_per_s(tr, model, cfg, dev, steps: int, prompt: int, max_len: int) -> float:
-    cache = tr.StaticCache(config=cfg, max_cache_len=max_len)
+def _decode_tokens_per_s(tr, model, cfg, dev, steps: int, prompt: int, max_len: int, kind: str = "fp16") -> float:
+    if kind == "4bit":
+        from .model import cobalt_cache
+        was = model.config._attn_implementation
+        cache = cobalt_cache(model, 1, max_len)
+        try:
+            return _steps_per_s(model, cfg, dev, steps, prompt, cache)
+        finally:
+            model.set_attn_implementation(was)
+    return _steps_per_s(model, cfg, dev, steps, prompt, tr.StaticCache(config=cfg, max_cache_len=max_len))
+
+
+def _steps_per_s(model, cfg, dev, steps: int, prompt: int, cache) -> float:
     ids = torch.randint(0, cfg.vocab_size, (1, prompt), device=dev)
     tok = torch.zeros(1, 1, dtype=torch.long, device=dev)
     pos = torch.zeros(1, dtype=torch.long, device=dev)
@@ -77,6 +89,8 @@ def main(argv=None):
     ap.add_argument("--group", type=int, default=128)
     ap.add_argument("--steps", type=int, default=128)
     ap.add_argument("--prefill", type=int, default=2048)
+    ap.add_argument("--cache", choices=("fp16", "4bit"), default="fp16", help="the key/value cache of the decode steps")
+    ap.add_argument("--context", type=int, default=16, help="tokens of the prompt in front of the decode steps")
     a = ap.parse_args(argv)
     import transformers as tr
     from . import model as Mo
@@ -85,7 +99,7 @@ def main(argv=None):
     dev = "cuda:0"
     cfg = tr.MistralConfig(vocab_size=a.vocab, hidden_size=a.hidden, intermediate_size=a.inter,
                            num_hidden_layers=a.layers, num_attention_heads=a.heads, num_key_value_heads=a.kv_heads,
-                           max_position_embeddings=4096, sliding_window=None)
+                           max_position_embeddings=max(4096, a.context + a.steps + 64), sliding_window=None)
     torch.manual_seed(0)
     model = tr.MistralForCausalLM(cfg).to(dev, torch.float16).eval()
     t0 = time.time()
@@ -99,9 +113,9 @@ def main(argv=None):
             Mo.fuse_model(model)
         elif name != "packed":
             model = Mo.dense_twin(model, torch.float16)
-        tps = _decode_tokens_per_s(tr, model, cfg, dev, a.steps, 16, 512)
+        tps = _decode_tokens_per_s(tr, model, cfg, dev, a.steps, a.context, max(512, a.context + a.steps + 64), a.cache)
         pms = _prefill_ms(model, cfg, dev, a.prefill)
-        print(json.dumps(dict(base, linears=name, decode_tokens_per_s=round(tps, 1),
+        print(json.dumps(dict(base, linears=name, cache=a.cache, context=a.context, decode_tokens_per_s=round(tps, 1),
                               prefill_tokens=a.prefill, prefill_ms=round(pms, 2))), flush=True)
 
 

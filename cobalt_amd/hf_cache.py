@@ -1,0 +1,162 @@
+"""A Hugging Face decoder on the 4-bit key/value cache: `model.cobalt_cache` builds the cache that is passed as
+`past_key_values`; the model's attention layers then call `cobalt_attention`, which writes their keys and values with
+`ops.cache_write` and reads the cache with `ops.cache_attention`, prompts and single tokens alike."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from transformers import AttentionInterface, AttentionMaskInterface
+from transformers.cache_utils import Cache, CacheLayerMixin
+
+from . import ops
+from .cache import KVCache, KVRows
+
+NAME = "cobalt_cache"
+
+
+class _Sequences:
+    """What the layers of one cache share: the pages, the lengths, and the rows of the step under way."""
+
+    def __init__(self, batch: int, max_len: int, page: int, device):
+        if batch < 1 or max_len < 1:
+            raise ValueError(f"batch and max_len must be at least 1, got {batch} and {max_len}")
+        self.batch, self.max_len, self.page = batch, max_len, page
+        per = -(-max_len // page)
+        self.pages = batch * per
+        self.table = torch.arange(self.pages, dtype=torch.int32, device=device).view(batch, per)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)         # real tokens, padding left out
+        self.seen = torch.zeros((), dtype=torch.int64, device=device)            # tokens with the padding
+        self.clear()
+
+    def clear(self):
+        self.lens.zero_()
+        self.seen.zero_()
+        self.steps = 0           # tokens with the padding, as the host has issued them: replays of a graph are not in it
+        self.pads = [0] * self.batch
+        self.rows: Optional[KVRows] = None
+
+    def begin(self, batch: int, tokens: int, mask: Optional[torch.Tensor]):
+        """The rows of a step of `tokens` tokens a sequence, called by the first layer; advances the lengths."""
+        if batch != self.batch:
+            raise ValueError(f"the cache is for {self.batch} sequences, the step has {batch}")
+        if self.steps + tokens > self.max_len:
+            raise ValueError(f"the cache is for {self.max_len} tokens a sequence, the step ends at {self.steps + tokens}")
+        first = self.steps == 0
+        if mask is not None:
+            pads = self._padding(mask, tokens)
+            if first:
+                self.pads = pads
+            elif pads != self.pads:
+                raise ValueError("attention_mask: padding belongs in front of a sequence, in the first call")
+        self.steps += tokens
+        self.seen.add_(tokens)
+        self.lens.add_(tokens)
+        self.rows = KVRows(self.table, self.lens)
+        if first and any(self.pads):
+            # the padding's rows belong to sequences of their own, which are empty and have no pages: not written, and 0 as the answer
+            pads = torch.tensor(self.pads, dtype=torch.int32).to(self.lens.device)
+            self.lens.sub_(pads)
+            ends = torch.arange(batch, dtype=torch.int32, device=pads.device) * tokens
+            starts = torch.stack([ends, ends + pads], 1).flatten()
+            self.rows = KVRows(torch.stack([torch.full_like(self.table, -1), self.table], 1).flatten(0, 1).contiguous(),
+                               torch.stack([torch.zeros_like(self.lens), self.lens], 1).flatten(),
+                               torch.cat([starts, starts.new_full((1,), batch * tokens)]))
+
+    def _padding(self, mask, tokens):
+        if mask.dim() != 2 or mask.shape[0] != self.batch or mask.shape[1] != self.steps + tokens:
+            raise ValueError(f"attention_mask must be [{self.batch}, {self.steps + tokens}], got {list(mask.shape)}")
+        if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise ValueError("attention_mask is read by the host: a step recorded in a graph takes none (padding of the first call stays left out)")
+        real = mask.bool()
+        holes = (real[:, :-1] & ~real[:, 1:]).any(1)
+        pads = torch.where(holes, -1, (~real).sum(1)).tolist()
+        if -1 in pads:
+            raise ValueError("attention_mask: padding belongs in front of a sequence, in the first call")
+        return pads
+
+
+class CobaltCacheLayer(CacheLayerMixin):
+    """One decoder layer's pool.  `update` only hands the step's keys and values on: `cobalt_attention` writes them."""
+    is_compileable = False
+    is_sliding = False
+
+    def __init__(self, sequences: _Sequences, index: int, group: int, sinks: int):
+        super().__init__()
+        self.sequences, self.index, self.group, self.sinks = sequences, index, group, sinks
+        self.pool: Optional[KVCache] = None
+
+    def lazy_initialization(self, key_states, value_states):
+        if key_states.shape != value_states.shape:
+            raise ValueError(f"keys {list(key_states.shape)} and values {list(value_states.shape)} must have the same shape")
+        if key_states.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call with a new cache makes its pages: it cannot be recorded in a graph")
+        self.pool = KVCache(self.sequences.pages, key_states.shape[1], key_states.shape[3], page=self.sequences.page, group=self.group,
+                            device=key_states.device)
+        self.is_initialized = True
+
+    def update(self, key_states, value_states, *args, **kwargs):
+        if self.pool is None:
+            self.lazy_initialization(key_states, value_states)
+        key_states._cobalt_layer = self
+        return key_states, value_states
+
+    def get_seq_length(self):
+        return self.sequences.seen
+
+    def get_mask_sizes(self, query_length):
+        tokens = query_length if isinstance(query_length, int) else query_length.shape[0]
+        return self.sequences.steps + tokens, 0
+
+    def get_max_cache_shape(self):
+        return self.sequences.max_len
+
+    get_max_length = get_max_cache_shape
+
+    def reset(self):
+        self.sequences.clear()
+
+    def _refuse(self, *args, **kwargs):
+        raise NotImplementedError("the 4-bit cache does not reorder, repeat, select or crop its sequences, and is not offloaded")
+
+    reorder_cache = batch_repeat_interleave = batch_select_indices = crop = offload = prefetch = _refuse
+
+
+def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None, **kwargs):
+    """The attention function behind the name "cobalt_cache": query [batch, heads, tokens, head_dim] -> [batch, tokens, heads, head_dim]."""
+    layer = getattr(key, "_cobalt_layer", None)
+    if layer is None:
+        raise ValueError('attention "cobalt_cache" needs a cache of model.cobalt_cache as past_key_values')
+    if dropout or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None or not getattr(module, "is_causal", True) \
+            or kwargs.get("is_causal") is False:
+        raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
+    if query.requires_grad or key.requires_grad or value.requires_grad:
+        raise RuntimeError("the 4-bit cache has no backward pass: call the model under torch.no_grad()")
+    batch, _, tokens, _ = query.shape
+    if layer.index == 0:
+        layer.sequences.begin(batch, tokens, attention_mask)
+    as_rows = lambda x: x.transpose(1, 2).reshape(batch * tokens, x.shape[1], x.shape[3])
+    ops.cache_write(layer.pool, as_rows(key), as_rows(value), layer.sequences.rows)
+    out = ops.cache_attention(layer.pool, as_rows(query), layer.sequences.rows, scale=scaling, window=sliding_window or None,
+                              sinks=layer.sinks if sliding_window else 0)
+    return out.view(batch, tokens, query.shape[1], query.shape[3]), None
+
+
+def _padding_mask(*args, attention_mask=None, **kwargs):
+    """The 2-D mask of the padding as it is; what else a mask says follows from the lengths and the window."""
+    return attention_mask
+
+
+def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) -> Cache:
+    cfg = model.config.get_text_config()
+    kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
+    if kinds - {"full_attention", "sliding_attention"} or getattr(model.config, "is_encoder_decoder", False):
+        raise ValueError(f"the 4-bit cache is for decoders of full and sliding-window attention, not {sorted(kinds)}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    AttentionInterface.register(NAME, cobalt_attention)
+    AttentionMaskInterface.register(NAME, _padding_mask)
+    seqs = _Sequences(batch, max_len, page, next(model.parameters()).device)
+    cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, sinks) for i in range(cfg.num_hidden_layers)])
+    model.set_attn_implementation(NAME)
+    return cache

@@ -396,6 +396,16 @@ def load_compressed_state_dict(model: nn.Module, state_dict: Dict[str, torch.Ten
     return model.load_state_dict(state_dict, strict=strict)
 
 
+def cobalt_cache(model: nn.Module, batch: int, max_len: int, page: int = 64, group: int = 32, sinks: int = 0):
+    """A key/value cache in 4 bits for a Hugging Face decoder: `batch` sequences of up to `max_len` tokens, 4 + 32 / group
+    bits a value.  Pass it as `past_key_values` to the model or to its `generate` (not with beams); the model's attention
+    implementation is switched to it, and `model.set_attn_implementation` switches it back.  Sliding-window layers also see the
+    first `sinks` tokens of a sequence.  A batch may be padded in front (2-D `attention_mask`); a step without a mask can be
+    recorded in a graph, its replays go on from the lengths on the device.  `cache.reset()` empties it."""
+    from . import hf_cache
+    return hf_cache.build(model, batch, max_len, page, group, sinks)
+
+
 def dense_twin(model: nn.Module, dtype: Optional[torch.dtype] = None) -> nn.Module:
     """The same model with every `CobaltLinear` turned back into an `nn.Linear` that holds the
     dequantised weight: what the packed model computes, through the dense library GEMM.  Modifies

@@ -1,0 +1,174 @@
+"""A Hugging Face decoder on `model.cobalt_cache`, without the GPU: the two operators are replaced by exact ones (nothing rounded,
+float64), so the logits must be those of the same float64 model with its own attention and cache: which rows, lengths, windows,
+padding and positions the decoder hands to the operators.  The five norms of the model round to float32 whatever its type, so sums in
+another order may come out half a step apart there, 2^-23 relative: 1e-5 is 80 such steps of values around 1, a wrong row or mask is above 1e-2."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_ref as R
+
+tr = pytest.importorskip("transformers")
+Mo = pytest.importorskip("cobalt_amd.model")
+hf = pytest.importorskip("cobalt_amd.hf_cache")
+ATOL = 1e-5
+
+
+def _model(window=None, layers=2):
+    cfg = tr.MistralConfig(vocab_size=97, hidden_size=128, intermediate_size=128, num_hidden_layers=layers, num_attention_heads=4,
+                           num_key_value_heads=2, head_dim=64, max_position_embeddings=512, sliding_window=window, pad_token_id=0,
+                           bos_token_id=1, eos_token_id=None, attn_implementation="sdpa")
+    torch.manual_seed(3)
+    return tr.MistralForCausalLM(cfg).double().eval().requires_grad_(False)
+
+
+def _tokens(rows, seqs, tokens):
+    """(row, sequence, token) of every row of a call that belongs to a sequence."""
+    starts = (torch.arange(seqs + 1) * (tokens // seqs) if rows.starts is None else rows.starts).tolist()
+    for b, n in enumerate(rows.lens.tolist()):
+        for r in range(starts[b], starts[b + 1]):
+            yield r, b, n - (starts[b + 1] - r)
+
+
+@pytest.fixture
+def exact(monkeypatch):
+    """The operators with a dense float64 pool in place of the 4-bit one."""
+    pools = {}
+
+    def write(cache, k, v, rows):
+        pool = pools.setdefault(id(cache), np.full((2, cache.pages * cache.page, cache.heads, cache.head_dim), np.nan))
+        for r, b, t in _tokens(rows, rows.lens.numel(), k.shape[0]):
+            page = int(rows.table[b, t // cache.page]) if t >= 0 else -1
+            if page >= 0:
+                pool[:, page * cache.page + t % cache.page] = torch.stack([k[r], v[r]]).numpy()
+
+    def attention(cache, q, rows, scale=None, window=None, sinks=0, out=None):
+        out = torch.zeros_like(q)
+        ratio = q.shape[1] // cache.heads
+        for r, b, t in _tokens(rows, rows.lens.numel(), q.shape[0]):
+            pages = rows.table[b].tolist()
+            if t < 0 or pages[0] < 0:
+                continue
+            at = np.array([pages[j // cache.page] * cache.page + j % cache.page for j in range(t + 1)])
+            k, v = pools[id(cache)][:, at]
+            for h in range(q.shape[1]):
+                o = R.attention(q[r:r + 1, h].numpy(), k[:, h // ratio], v[:, h // ratio], np.array([t]), np.ones(t + 1, bool), scale, window, sinks)[0]
+                out[r, h] = torch.from_numpy(o[0])
+        return out
+
+    monkeypatch.setattr(hf.ops, "cache_write", write)
+    monkeypatch.setattr(hf.ops, "cache_attention", attention)
+
+
+def _same_steps(window, steps, batch=2, pads=None, page=16):
+    m = _model(window)
+    g = torch.Generator().manual_seed(5)
+    calls = [torch.randint(2, 97, (batch, n), generator=g) for n in steps]
+    masks = [None] * len(calls)
+    if pads is not None:
+        total = 0
+        for i, ids in enumerate(calls):
+            total += ids.shape[1]
+            masks[i] = torch.stack([(torch.arange(total) >= p).long() for p in pads])
+    want, dense = [], tr.DynamicCache(config=m.config)
+    with torch.no_grad():
+        for ids, mask in zip(calls, masks):
+            want.append(m(ids, past_key_values=dense, attention_mask=mask).logits)
+        cache = Mo.cobalt_cache(m, batch, 128, page=page)
+        assert m.config._attn_implementation == "cobalt_cache"
+        for i, (ids, mask) in enumerate(zip(calls, masks)):
+            got = m(ids, past_key_values=cache, attention_mask=mask).logits
+            for b in range(batch):
+                first = pads[b] if pads is not None and i == 0 else 0
+                assert float((got[b, first:] - want[i][b, first:]).abs().max()) < ATOL, (i, b)
+    assert int(cache.get_seq_length()) == sum(steps)
+    return m, cache
+
+
+@pytest.mark.parametrize("window", [None, 7, 2])
+def test_prompt_steps_and_drafts_answer_as_the_model_does(exact, window):
+    _same_steps(window, [33, 1, 1, 4, 1])
+
+
+def test_a_batch_padded_in_front(exact):
+    _same_steps(None, [20, 1, 1, 3], batch=3, pads=[0, 19, 6])
+
+
+def test_padding_under_a_window(exact):
+    _same_steps(5, [18, 1, 2], batch=2, pads=[11, 0])
+
+
+def test_a_mask_without_padding_changes_nothing(exact):
+    _same_steps(None, [9, 1], batch=2, pads=[0, 0])
+
+
+def test_generate_answers_as_with_the_models_own_cache(exact):
+    m = _model()
+    ids = torch.randint(2, 97, (2, 11), generator=torch.Generator().manual_seed(1))
+    mask = torch.ones_like(ids)
+    mask[1, :4] = 0
+    kw = dict(attention_mask=mask, max_new_tokens=9, do_sample=False)
+    want = m.generate(ids, **kw)
+    cache = Mo.cobalt_cache(m, 2, 64)
+    assert torch.equal(m.generate(ids, past_key_values=cache, **kw), want)
+    cache.reset()                                                      # an emptied cache takes the next batch, padded otherwise
+    mask = torch.ones_like(ids)
+    mask[0, :2] = 0
+    kw["attention_mask"] = mask
+    again = m.generate(ids, past_key_values=cache, **kw)
+    m.set_attn_implementation("sdpa")
+    assert torch.equal(again, m.generate(ids, **kw))
+
+
+def test_sinks_reach_the_layers_with_a_window_only(exact, monkeypatch):
+    seen = []
+    real = hf.ops.cache_attention
+    monkeypatch.setattr(hf.ops, "cache_attention", lambda *a, **k: seen.append((k["window"], k["sinks"])) or real(*a, **k))
+    ids = torch.arange(2, 12)[None]
+    for window, want in ((6, (6, 2)), (None, (None, 0))):
+        m = _model(window)
+        m(ids, past_key_values=Mo.cobalt_cache(m, 1, 32, sinks=2))
+        assert set(seen) == {want}
+        seen.clear()
+
+
+def test_calls_that_do_not_fit_are_refused(exact):
+    m = _model()
+    ids = torch.randint(2, 97, (2, 6), generator=torch.Generator().manual_seed(1))
+    for kw in (dict(batch=0, max_len=8), dict(batch=1, max_len=0), dict(batch=1, max_len=8, sinks=-1)):
+        with pytest.raises(ValueError):
+            Mo.cobalt_cache(m, **kw)
+    with pytest.raises(ValueError, match="pages of"):
+        m(ids, past_key_values=Mo.cobalt_cache(m, 2, 8, page=24))
+    with pytest.raises(ValueError, match="for 8 tokens"):
+        m(torch.cat([ids, ids], 1), past_key_values=Mo.cobalt_cache(m, 2, 8))
+    with pytest.raises(ValueError, match="for 3 sequences"):
+        m(ids, past_key_values=Mo.cobalt_cache(m, 3, 8))
+    with pytest.raises(ValueError, match="past_key_values"):
+        m(ids)
+    for bad in ([1, 1, 1, 1, 1, 0], [1, 0, 1, 1, 1, 1]):                # behind a sequence, inside it
+        with pytest.raises(ValueError, match="in front"):
+            m(ids, past_key_values=Mo.cobalt_cache(m, 2, 16), attention_mask=torch.tensor([[1] * 6, bad]))
+    cache = Mo.cobalt_cache(m, 2, 16)
+    m(ids, past_key_values=cache)
+    with pytest.raises(ValueError, match="first call"):                 # padding that the first call did not have
+        m(ids[:, :1], past_key_values=cache, attention_mask=torch.tensor([[0] + [1] * 6, [1] * 7]))
+    with pytest.raises(NotImplementedError):
+        m.generate(ids, past_key_values=Mo.cobalt_cache(m, 4, 32), num_beams=2, max_new_tokens=2, attention_mask=torch.ones_like(ids))
+    m.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        m(ids, past_key_values=Mo.cobalt_cache(m, 2, 16))
+    m.requires_grad_(False)
+    m.model.layers[0].self_attn.is_causal = False
+    with pytest.raises(ValueError, match="causal"):
+        m(ids, past_key_values=Mo.cobalt_cache(m, 2, 16))
+
+
+def test_a_step_that_is_refused_leaves_the_lengths(exact):
+    m = _model()
+    cache = Mo.cobalt_cache(m, 1, 8)
+    ids = torch.arange(2, 8)[None]
+    m(ids, past_key_values=cache)
+    with pytest.raises(ValueError):
+        m(ids, past_key_values=cache)
+    assert int(cache.get_seq_length()) == 6 and cache.layers[0].sequences.lens.tolist() == [6]
