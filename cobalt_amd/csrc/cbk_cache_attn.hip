@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
   const int64_t begin = w * total / pieces, end = (w + 1) * total / pieces;
   int64_t base = 0;
   int b = 0;
-  for (int j = 0;; j += 64) {                                       // (begin < total: it is found)
+  for (int j = 0; j < r.seqs; j += 64) {                            // (begin < total: it is found)
     if (j) sum = scan64(units_of(r, a, c.heads, j + lane, R), lane);
     const int64_t here = of_lane(sum, 63);
     if (begin < base + here) {
@@ -109,7 +109,11 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
     const int rows = s.n * a.ratio, tiles = (rows + R - 1) / R;
     const int weight = a.whole ? 1 : g.units + EXTRA;
     const int64_t all = (int64_t)tiles * c.heads * weight;
-    if (at >= base + all) { base += all; ++b; continue; }
+    if (at >= base + all) {
+      base += all;
+      if (++b == r.seqs) break;                                     // (there is a next one, unless lengths change under the call)
+      continue;
+    }
     const int64_t item = (at - base) / weight, start = base + item * weight;
     const int64_t until = min(end, start + weight);
     const int u0 = a.whole ? 0 : max((int)(at - start) - EXTRA, 0), u1 = a.whole ? g.units : (int)(until - start) - EXTRA;

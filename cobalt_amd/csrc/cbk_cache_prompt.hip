@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     int64_t one = 0;                                                // units of a head
     for (int j = 0; j < r.seqs; j += 64) one += of_lane(scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), 63);
     total = one * c.heads;
-    pieces = min((int64_t)gridDim.x, max(total / ((int64_t)LEAST * T::KEYS * a.ratio), (int64_t)1));
+    pieces = total ? min((int64_t)gridDim.x, max(total / ((int64_t)LEAST * T::KEYS * a.ratio), (int64_t)1)) : 0;   // (0: no sequence has a row)
     if (place >= pieces) {
       if (tid == 0) desc->count = 0;
       return;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     end = at + each + (place < more);
     h = (int)(begin / one);
     base = h * one;
-    for (int j = 0;; j += 64) {
+    for (int j = 0; j < r.seqs; j += 64) {
       const int64_t sum = scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), here = of_lane(sum, 63);
       if (begin < base + here) {
         const int q = __popcll(__ballot(base + sum <= begin));
@@ -107,6 +107,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         break;
       }
       base += here;
+    }
+    if (b < 0) {                                                    // (lengths or offsets that change under the call)
+      if (tid == 0) desc->count = 0;
+      return;
     }
     const Seq s = seq_of(r, b);                                     // its tile: the last that begins at or before
     int lo = 0, hi = row_tiles(s, a.ratio) - 1;
@@ -506,9 +510,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   } else {
     base += wt.all(s);
     tile = 0;
-    do {                                                            // (there is one: at < total)
+    do {
       if (++b == r.seqs) { b = 0; ++h; }
-    } while (seq_of(r, b).n <= 0);
+    } while (h < c.heads && seq_of(r, b).n <= 0);
+    if (h == c.heads) break;                                        // (there is one, unless lengths change under the call)
   }
   }
   if (!joined && tid == 0) desc->count = 0;

@@ -311,6 +311,24 @@ def test_rows_that_see_nothing_are_zero():
     s.check(q[3:], out[3:], [2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,seqs", [(4096, 1), (70, 1), (3000, 3), (4096, 20)])
+def test_rows_of_no_sequence_at_all(rows, seqs, dtype):
+    """Every sequence of the call is without rows, however many the call has, in front of them, behind them or between none."""
+    s = Setup([2000] * seqs, 2, 128, 64, 32, dtype, seed=3)
+    q = torch.randn(rows, 8, 128, device=DEV).to(dtype)
+    for at in (0, 1000, rows):
+        out = torch.full_like(q, 9)
+        ops.cache_attention(s.cache, q, KVRows(s.table, ints(s.lens), ints([at] * (seqs + 1))), out=out)
+        assert bool((out == 9).all())
+    starts = [0] * (seqs + 1)
+    starts[-1] = 5                                                  # and with five rows of the last one
+    out = torch.full_like(q, 9)
+    ops.cache_attention(s.cache, q, KVRows(s.table, ints(s.lens), ints(starts)), out=out)
+    assert bool((out[5:] == 9).all())
+    s.check(q[:5], out[:5], [0] * (seqs - 1) + [5])
+
+
 def test_missing_pages_are_not_seen():
     s = Setup([200, 90], 1, 128, 16, 32, torch.bfloat16, seed=2)
     there = [np.ones(200, bool), np.ones(90, bool)]
