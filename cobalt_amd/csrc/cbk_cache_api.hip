@@ -30,7 +30,7 @@ static int to_dcache(const cbk_cache* in, DCache* c, bool need_device_ptrs) {
 static int to_drows(const cbk_rows* in, const DCache& c, DRows* r, bool need_device_ptrs) {
   if (!in) return CBK_ERR_NULL;
   if (in->seqs < 0 || in->table_cols < 0 || in->ld_table < in->table_cols || in->tokens < 0 || in->tokens >= 1 << 30) return CBK_ERR_SHAPE;
-  if (in->table_cols > INT32_MAX / c.page) return CBK_ERR_SHAPE;
+  if (in->table_cols > (1 << 30) / c.page) return CBK_ERR_SHAPE;    // token positions are ints, tiles round them up
   if (in->seqs == 0 && in->tokens > 0 && !in->starts) return CBK_ERR_SHAPE;
   if (!in->starts && in->seqs && in->tokens % in->seqs) return CBK_ERR_SHAPE;
   if (need_device_ptrs && in->seqs > 0 && in->tokens > 0) {
@@ -64,13 +64,14 @@ static int cache_io(const cbk_cache* cache, const cbk_rows* rows, const CacheIo&
   rc = check_dense(io.k, io.kt, io.kh, size);
   if (!rc) rc = check_dense(io.v, io.vt, io.vh, size);
   if (rc) return rc;
-  if ((int64_t)r.tokens * c.heads > (int64_t)INT32_MAX * 4) return CBK_ERR_SHAPE;   // workgroups of a launch
+  if ((int64_t)r.tokens * c.heads * c.dim >= (int64_t)1 << 36) return CBK_ERR_SHAPE;   // 2^32 threads of a launch: 16 numbers each
   return write ? launch_cache_write(c, r, io, dt, (hipStream_t)stream) : launch_cache_read(c, r, io, dt, (hipStream_t)stream);
 }
 
 static int attn_ratio(const DCache& c, const DRows& r, int q_heads, int* ratio) {
   if (q_heads < 1 || q_heads % c.heads || (int64_t)r.tokens * q_heads >= (int64_t)1 << 30) return CBK_ERR_SHAPE;
   *ratio = q_heads / c.heads;
+  if (*ratio > 256) return CBK_ERR_SHAPE;                           // (weights of tiles are rows times tokens in 64 bits)
   return CBK_OK;
 }
 
@@ -118,7 +119,7 @@ int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void
   if (!rc) rc = attn_ratio(c, r, q_heads, &a.ratio);
   if (rc) return rc;
   if (dtype != CBK_F16 && dtype != CBK_BF16T) return CBK_ERR_DTYPE;
-  if (!(scale > 0.f) || scale > 1e30f || window < 0 || sinks < 0) return CBK_ERR_SHAPE;
+  if (!(scale >= 1e-30f) || scale > 1e30f || window < 0 || sinks < 0) return CBK_ERR_SHAPE;
   if (r.tokens == 0 || r.seqs == 0) return CBK_OK;
   rc = check_dense(q, q_row, q_head, 2);
   if (!rc) rc = check_dense(out, out_row, out_head, 2);

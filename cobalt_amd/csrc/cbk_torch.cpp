@@ -582,6 +582,8 @@ Cache as_cache(PyObject* o) {
   for (int i = 0; i < 4; ++i) {
     r.t[i] = as_tensor(PyTuple_GET_ITEM(o, i), "an array of the cache");
     if (!r.t[i].defined()) fail(PyExc_TypeError, "a KVCache is expected");
+    if (!r.t[i].is_contiguous() || r.t[i].device() != r.t[0].device())
+      fail(PyExc_ValueError, "the arrays of the cache must be contiguous and on one device");
     p[i] = r.t[i].mutable_data_ptr();
   }
   long long v[5];
@@ -697,6 +699,8 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         same_device(c, o);
         check_out(o, rows, c.c.heads, c.c.head_dim, t, "the output");
       }
+    if (rows && out[0].defined() && out[1].defined() && out[0].const_data_ptr() == out[1].const_data_ptr())
+      fail(PyExc_ValueError, "keys and values need an output each");
     int rc = CBK_OK;
     {
       const GilRelease other_threads_run;
@@ -727,6 +731,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (heads % c.c.heads)
       fail(PyExc_ValueError, std::to_string(heads) + " query heads are no multiple of the cache's " + std::to_string(c.c.heads));
     if (out.defined()) check_out(out, q.size(0), heads, c.c.head_dim, q.scalar_type(), "out");
+    if (out.defined() && q.size(0) && out.const_data_ptr() == q.const_data_ptr()) fail(PyExc_ValueError, "out must not overlap q");
     const RowMap m = as_rows(c, a[2], a[3], a[4], q.size(0));
     const double scale = PyFloat_AsDouble(a[5]);
     const long long window = PyLong_AsLongLong(a[6]), sinks = PyLong_AsLongLong(a[7]);

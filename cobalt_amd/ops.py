@@ -211,12 +211,12 @@ def cache_attention(cache, q, rows, scale: Optional[float] = None, window: Optio
     """Causal attention of the rows' queries ([rows, query heads, head_dim], float16 or bfloat16) over the cache, which
     holds their own tokens already (`cache_write` first).  `scale`: of the scores, head_dim ** -0.5 by default.  `window`: a row
     sees the last `window` tokens up to its own only, and the first `sinks` tokens of its sequence.  Query
-    heads share the cache's heads in groups, consecutive ones the same.  Returns a tensor like q (or `out`, which must
+    heads share the cache's heads in groups of up to 256, consecutive ones the same.  Returns a tensor like q (or `out`, which must
     not overlap q); a row that sees nothing is 0, and rows that belong to no sequence are not written."""
     if scale is None:
         scale = cache.head_dim ** -0.5
-    if not 0.0 < scale <= 1e30:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale must be positive, between 1e-30 and 1e30, got {scale}")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, or None for all tokens, got {window}")
     if sinks < 0:

@@ -299,7 +299,7 @@ typedef struct cbk_rows {
   int64_t ld_table;
   const void* lens;
   const void* starts;
-  int32_t seqs, table_cols;
+  int32_t seqs, table_cols;   /* table_cols * page at most 2^30                         */
   int64_t tokens;      /* rows of the dense tensors, below 2^30                       */
 } cbk_rows;
 
@@ -319,8 +319,9 @@ int cbk_cache_read(const cbk_cache* cache, const cbk_rows* rows, void* k, int64_
  *   out[t, hq] = sum_j softmax_j(scale q[t, hq] . k_j) v_j,   head hq reads cache head hq / (q_heads / heads),
  * over the tokens j <= i that the cache holds, i the row's own position, and with window > 0 only those with j > i - window
  * or j < sinks.  A row that sees no token is 0.  fp16 or bf16 in and out; scores, their maximum and all sums
- * in float32, operands of the products in fp16 (a key or value is rounded once to fp16, a bf16 query is
- * scaled by a power of two and stays exact).  scale > 0.  The result is the same from call to call, also on
+ * in float32, operands of the products in fp16.  fp16: exact codes and queries, values rounded once, softmax weights as two
+ * fp16.  bf16: keys, values, softmax weights and queries (with the scale in them) may each be rounded once to fp16, an eighth of
+ * the result's own step.  scale in [1e-30, 1e30], scores in the range of float32, q_heads at most 256 heads; out must not overlap q.  The result is the same from call to call, also on
  * another workspace.  The workspace holds nothing between calls and needs no clearing:
  * cbk_cache_attention_workspace_bytes(), 256-byte aligned, one per call in flight. */
 size_t cbk_cache_attention_workspace_bytes(const cbk_cache* cache, const cbk_rows* rows, int q_heads);

@@ -105,6 +105,22 @@ def test_entry_points_refuse_bad_tensors_before_any_launch():
     assert _attend(_cache(), big, ws=None, room=0) == -6
 
 
+def test_entry_points_refuse_what_would_pass_their_integers():
+    most = (1 << 30) // 16
+    for call in (_write, _read, _attend):
+        assert call(_cache(), _rows(table_cols=most + 1, ld_table=most + 1)) == -3
+    assert _lib.lib().cbk_cache_attention_workspace_bytes(ctypes.byref(_cache()), ctypes.byref(_rows(table_cols=most, ld_table=most)), 4) > 0
+    for call in (_write, _read):
+        assert call(_cache(heads=4096), _rows(tokens=1 << 17, seqs=1)) == -3          # 2^36 numbers
+    assert _attend(_cache(), _rows(), heads=2 * 257) == -3
+    assert _attend(_cache(), _rows(), scale=1e-31) == -3 and _attend(_cache(), _rows(), scale=1e31) == -3
+    x = torch.zeros(2, 2, 64, dtype=torch.float16)
+    c = KVCache(3, 2, 64, page=32, device="cpu")
+    for scale in (1e-31, 1e31, -1.0, float("nan")):
+        with pytest.raises(ValueError):
+            ops.cache_attention(c, x, c.rows([[0, 1], [2, -1]], [40, 7]), scale=scale)
+
+
 def test_sizes():
     L = _lib.lib()
     c = _cache(pages=7, page=64, heads=3, head_dim=256, group=64)

@@ -592,3 +592,38 @@ def test_operators_refuse_what_does_not_fit():
         rd(s.cache, r, 2, torch.int8)
     with pytest.raises(ValueError):
         rd(s.cache, r, 2, torch.float16, out=(k, k[:1]))
+
+
+def test_operators_refuse_outputs_that_are_inputs():
+    s = Setup([20, 30], 2, 128, 16, 32, torch.float16)
+    r = s.rows([1, 1])
+    q, k = torch.zeros(2, 4, 128, device=DEV).half(), torch.zeros(2, 2, 128, device=DEV).half()
+    with pytest.raises(ValueError, match="overlap"):
+        ops.cache_attention(s.cache, q, r, out=q)
+    with pytest.raises(ValueError, match="output each"):
+        ops.cache_read(s.cache, r, 2, torch.float16, out=(k, k))
+    s.cache.v_meta = s.cache.v_meta.cpu()
+    with pytest.raises(ValueError, match="one device"):
+        ops.cache_write(s.cache, k, k, r)
+
+
+@pytest.mark.parametrize("dim,ratio,dtype", [(64, 256, torch.float16), (128, 100, torch.bfloat16), (128, 256, torch.float16)])
+def test_many_query_heads_on_one(dim, ratio, dtype):
+    Setup([700, 30], 1, dim, 32, 32, dtype, seed=ratio).attend([3, 30], ratio)
+    Setup([5000], 2, dim, 32, 64, dtype, seed=ratio).attend([9], ratio, window=300, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 300])
+def test_the_smallest_and_largest_scales(n, dtype):
+    """Scores of nothing: the mean.  Scores of 2^20 and more: the tokens of the largest alone, since keys of one value a token are held
+    and multiplied exactly, equal ones alike, and the others lie 2^21 lower: the error is that of the rounded values and result."""
+    s = Setup([700], 2, 128, 64, 32, dtype, seed=n, fill=lambda s: s.k.copy_((torch.arange(700) % 128 / 16).to(dtype)[:, None, None].expand_as(s.k)))
+    q = torch.ones(n, 4, 128, device=DEV).to(dtype)
+    s.check(q, ops.cache_attention(s.cache, q, s.rows([n]), scale=1e-30), [n], scale=1e-30)
+    out = ops.cache_attention(s.cache, q, s.rows([n]), scale=2.0 ** 20).double().cpu().numpy()
+    for h in range(4):
+        o, _, size, _ = R.attention(q[:, h].double().cpu().numpy(), s.hk[:, h // 2], s.hv[:, h // 2], np.arange(700 - n, 700), np.ones(700, bool), 2.0 ** 20)
+        tol = (U + 2.0 ** -16) * size
+        tol = tol + HALF[dtype] * (np.abs(o) + tol) + 2.0 ** -25
+        assert (np.abs(out[:, h] - o) <= tol).all()
