@@ -107,7 +107,7 @@ __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, c
 struct PromptPlan { bool cut; int64_t grid; size_t bytes; };
 PromptPlan plan_prompt(const DCache&, const DRows&, int ratio);
 int launch_cache_prompt(const PromptPlan&, const DCache&, const DRows&, const AttnArgs&, hipStream_t);
-// Joins what the `grid` workgroups of a launch left of tiles of `rows` rows (cbk_cache_attn.hip)
+// Joins what the `grid` workgroups of a launch left of tiles of `rows` rows, 16 or 256 (cbk_cache_attn.hip)
 void launch_cache_join(int dim, const AttnArgs&, int grid, int rows, hipStream_t);
 
 }  // namespace cbk

@@ -406,47 +406,76 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
   if (a.ws && !joined && tid == 0) desc->count = 0;
 }
 
-// Rows of a tile that several workgroups have parts of, `share` of them a workgroup: D/4 threads a part, a part after another.
+// One more part of a row: four channels of it, against the maximum so far
 template <int D>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid, int rows, int share) {
-  constexpr int C = D / 4, P = 256 / C;
+__device__ inline void add_part(const AttnArgs& a, int grid, int64_t part, int rows, int row, int d, float& top, float& sum, float (&y)[4]) {
+  const float* const x = attn_part<D>(a.ws, grid, part * rows + row);
+  const float4 o = *(const float4*)(x + d);
+  const float mm = x[D], ll = x[D + 1], up = fmaxf(top, mm);
+  const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
+  top = up;
+  sum = sum * f + ll * g;
+  y[0] = y[0] * f + o.x * g; y[1] = y[1] * f + o.y * g; y[2] = y[2] * f + o.z * g; y[3] = y[3] * f + o.w * g;
+}
+
+// Rows of a tile that several workgroups have parts of.  Workgroup (x, y) takes row y of the tile that begins in workgroup x: D/4 threads a
+// part, 1024/D parts side by side, there may be hundreds.  (x is turned by y: tiles often begin every so many workgroups, and workgroups go to
+// the XCDs in turn.  512 rows in 16 parts each took one XCD 68 us.)
+template <int D>
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid) {
+  constexpr int C = D / 4, P = 256 / C, R = 16;
   __shared__ float sh[P][D + 4];
-  // (turned by y: tiles often begin every so many workgroups, and workgroups go to the XCDs in turn.  512 rows in 16 parts each
-  // took one XCD 68 us.)
+  const int64_t w = (blockIdx.x + blockIdx.y) % gridDim.x;
+  const AttnPiece e = ((const AttnPiece*)a.ws)[w];
+  const int tid = threadIdx.x, d = 4 * (tid % C), p = tid / C, row = blockIdx.y;
+  if (e.count == 0 || row >= e.valid) return;
+  float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = p; i < e.count; i += P) add_part<D>(a, grid, (w + i) * 2 + (i ? 0 : e.slot), R, row, d, top, sum, y);
+  *(float4*)&sh[p][d] = make_float4(y[0], y[1], y[2], y[3]);
+  if (d == 0) { sh[p][D] = top; sh[p][D + 1] = sum; }
+  __syncthreads();
+  if (p) return;
+#pragma unroll
+  for (int i = 0; i < P; ++i) top = fmaxf(top, sh[i][D]);
+  sum = 0.f;
+  y[0] = y[1] = y[2] = y[3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sh[i][D] - top);
+    sum += f * sh[i][D + 1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] += f * sh[i][d + j];
+  }
+  const int gr = e.row0 + row;
+  store_row4(a, e.first + gr / a.ratio, e.head * a.ratio + gr % a.ratio, d, y, sum);
+}
+
+// The same for tiles of 256 rows, most of them in two or three parts: a wavefront a row, 256/D parts side by side.
+template <int D>
+__global__ __launch_bounds__(256) void cache_prompt_join_kernel(AttnArgs a, int grid) {
+  constexpr int C = D / 4, P = 64 / C, R = 256, SHARE = 16;
   const int64_t w = (blockIdx.x + blockIdx.y) % gridDim.x;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
   if (e.count == 0) return;
-  const int tid = threadIdx.x, d = 4 * (tid % C), p = tid / C, end = min((int)(blockIdx.y + 1) * share, e.valid);
-  for (int row = blockIdx.y * share; row < end; ++row) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = 4 * (lane % C), p = lane / C;
+  const int end = min(((int)blockIdx.y + 1) * SHARE, e.valid);
+  for (int row = blockIdx.y * SHARE + wave; row < end; row += 4) {
     float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = p; i < e.count; i += P) {
-      const float* const part = attn_part<D>(a.ws, grid, ((w + i) * 2 + (i ? 0 : e.slot)) * rows + row);
-      const float4 o = *(const float4*)(part + d);
-      const float mm = part[D], ll = part[D + 1], up = fmaxf(top, mm);
-      const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
+    for (int i = p; i < e.count; i += P) add_part<D>(a, grid, (w + i) * 2 + (i ? 0 : e.slot), R, row, d, top, sum, y);
+#pragma unroll
+    for (int by = C; by < 64; by *= 2) {
+      const float up = fmaxf(top, __shfl_xor(top, by)), f = __builtin_amdgcn_exp2f(top - up);
       top = up;
-      sum = sum * f + ll * g;
-      y[0] = y[0] * f + o.x * g; y[1] = y[1] * f + o.y * g; y[2] = y[2] * f + o.z * g; y[3] = y[3] * f + o.w * g;
-    }
-    *(float4*)&sh[p][d] = make_float4(y[0], y[1], y[2], y[3]);
-    if (d == 0) { sh[p][D] = top; sh[p][D + 1] = sum; }
-    __syncthreads();
-    if (p == 0) {
+      sum *= f;
+      sum += __shfl_xor(sum, by);
 #pragma unroll
-      for (int i = 0; i < P; ++i) top = fmaxf(top, sh[i][D]);
-      sum = 0.f;
-      y[0] = y[1] = y[2] = y[3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float f = __builtin_amdgcn_exp2f(sh[i][D] - top);
-        sum += f * sh[i][D + 1];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] += f * sh[i][d + j];
+      for (int j = 0; j < 4; ++j) {
+        y[j] *= f;
+        y[j] += __shfl_xor(y[j], by);
       }
-      const int gr = e.row0 + row;
-      store_row4(a, e.first + gr / a.ratio, e.head * a.ratio + gr % a.ratio, d, y, sum);
     }
-    __syncthreads();
+    const int gr = e.row0 + row;
+    if (p == 0) store_row4(a, e.first + gr / a.ratio, e.head * a.ratio + gr % a.ratio, d, y, sum);
   }
 }
 
@@ -469,12 +498,15 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   p.bytes = p.split ? attn_bytes(p.grid, 16, c.dim) : 0;
   return p;
 }
+template <int D>
+static void join1(const AttnArgs& a, int grid, int rows, hipStream_t st) {
+  if (rows == 16) hipLaunchKernelGGL((cache_attn_join_kernel<D>), dim3(grid, 16), dim3(256), 0, st, a, grid);
+  else hipLaunchKernelGGL((cache_prompt_join_kernel<D>), dim3(grid, 16), dim3(256), 0, st, a, grid);
+}
 void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, hipStream_t st) {
-  const int share = rows > 16 ? 4 : 1;                              // (a workgroup a row would be 65 k of them for tiles of 256 rows, most with nothing to do)
-  const dim3 blocks(grid, rows / share);
-  if (dim == 64) hipLaunchKernelGGL((cache_attn_join_kernel<64>), blocks, dim3(256), 0, st, a, grid, rows, share);
-  else if (dim == 128) hipLaunchKernelGGL((cache_attn_join_kernel<128>), blocks, dim3(256), 0, st, a, grid, rows, share);
-  else hipLaunchKernelGGL((cache_attn_join_kernel<256>), blocks, dim3(256), 0, st, a, grid, rows, share);
+  if (dim == 64) join1<64>(a, grid, rows, st);
+  else if (dim == 128) join1<128>(a, grid, rows, st);
+  else join1<256>(a, grid, rows, st);
 }
 
 // Which of the two kernels.  That of cbk_cache_prompt.hip takes tiles of 256 rows, filled or not, and wins from about 100 rows a sequence
