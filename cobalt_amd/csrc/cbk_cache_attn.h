@@ -48,6 +48,40 @@ __device__ inline int64_t scan64(int64_t x, int lane) {             // sum of th
   return x;
 }
 
+// The sequences one behind the other, units(b) units of work each.  Every wavefront looks for its place by itself: a lane adds up `each`
+// consecutive sequences, one scan gives where they begin, and a second one, among the sequences of the lane that has the place, the sequence.
+// (1024 sequences of 300 tokens 140 us; with a scan for every 64 of them 152.)
+struct Index {
+  int seqs, each, lane;
+  int64_t sum, total;                       // units up to the end of this lane's sequences, of all
+  template <class F>
+  __device__ Index(int seqs_, int lane_, F units) : seqs(seqs_), each((seqs_ + 63) / 64), lane(lane_), sum(0) {
+    const int first = lane * each, last = min(first + each, seqs);
+#pragma unroll 4
+    for (int b = first; b < last; ++b) sum += units(b);
+    sum = scan64(sum, lane);
+    total = of_lane(sum, 63);
+  }
+  // the sequence that unit `at` < total is of, and the unit it begins with
+  template <class F>
+  __device__ int find(int64_t at, int64_t& base, F units) const {
+    const int q = __popcll(__ballot(sum <= at));
+    base = q ? of_lane(sum, min(q, 64) - 1) : 0;
+    if (each == 1 || q == 64) return min(q, seqs - 1);              // (64: lengths or offsets that change under the call)
+    const int last = min((q + 1) * each, seqs);
+    for (int j = q * each; j < last; j += 64) {
+      const int64_t to = scan64(j + lane < last ? units(j + lane) : 0, lane), here = of_lane(to, 63);
+      if (at < base + here) {
+        const int l = __popcll(__ballot(base + to <= at));
+        if (l) base += of_lane(to, l - 1);
+        return j + l;
+      }
+      base += here;
+    }
+    return seqs - 1;
+  }
+};
+
 // A product that stays one when something is added to it: the largest score less the maximum is 0 only if both were
 // rounded alike, and where scores pass 2^24 nothing else keeps p in range.
 __device__ inline float rounded_product(float a, float b) {

@@ -44,7 +44,6 @@ __device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
 }
 
 __device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads, int b, int rows) {
-  if (b >= r.seqs) return 0;
   const Seq s = seq_of(r, b);
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
   return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
@@ -70,14 +69,16 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
   constexpr int R = 16, KS = D / 32, GS = D / G, GU = (GS + 3) / 4, VU = D > 128 ? D / 128 : 1, TILES = D / 16;
   __shared__ float o_sh[4][R][D + 4];
   __shared__ float m_sh[4][R], l_sh[4][R];
+  constexpr bool Q_LDS = G == 32 && D > 64;   // queries in LDS, not in registers, of which groups of 32 leave too few (32 sequences of 8192 tokens: 128 channels 80 -> 70 us, 256 channels 138 -> 90)
+  __shared__ v8h q_sh[Q_LDS ? KS * 64 : 1];
   __shared__ v2u scale_sh[4][2][GS][4];       // a wavefront's own: scales of its 32 keys, by group, four in a piece
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, h4 = lane >> 4;
 
-  // ---- this workgroup's piece of the list; every wavefront looks for itself, 64 sequences at a time
-  int64_t sum = scan64(units_of(r, a, c.heads, lane, R), lane), total = of_lane(sum, 63);
-  for (int j = 64; j < r.seqs; j += 64) total += of_lane(scan64(units_of(r, a, c.heads, j + lane, R), lane), 63);
-  const int64_t pieces = min((int64_t)gridDim.x, total);
+  // ---- this workgroup's piece of the list
+  auto units = [&](int b) { return units_of(r, a, c.heads, b, R); };
+  const Index list(r.seqs, lane, units);
+  const int64_t total = list.total, pieces = min((int64_t)gridDim.x, total);
   const int64_t w = blockIdx.x;
   AttnPiece* const desc = (AttnPiece*)a.ws + w;
   if (w >= pieces) {
@@ -85,19 +86,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
     return;
   }
   const int64_t begin = w * total / pieces, end = (w + 1) * total / pieces;
-  int64_t base = 0;
-  int b = 0;
-  for (int j = 0; j < r.seqs; j += 64) {                            // (begin < total: it is found)
-    if (j) sum = scan64(units_of(r, a, c.heads, j + lane, R), lane);
-    const int64_t here = of_lane(sum, 63);
-    if (begin < base + here) {
-      const int l = __popcll(__ballot(base + sum <= begin));        // sequences that end before it
-      b = j + l;
-      if (l) base += of_lane(sum, l - 1);
-      break;
-    }
-    base += here;
-  }
+  int64_t base;
+  int b = list.find(begin, base, units);
   int64_t at = begin;
   int joined = 0;
   const Exponents ex = exponents();
@@ -134,45 +124,49 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
     const uint32_t v_at = h4 * (2 * D) + (D == 64 ? col & 7 : col) * 16;
     const uint32_t km_at = 4 * (min(h4, GS - 1) * c.page + col), vm_at = 4 * ((8 * (D == 64 ? col & 7 : col) / G) * c.page + 4 * h4);
     auto token_of = [&](int u) { return ((u < g.head ? u : u + g.skip) * 4 + wave) * 32; };
-    auto pages_of = [&](int tok, int (&pg)[2]) {                    // pages of the two sixteens of a step
-#pragma unroll
-      for (int t = 0; t < 2; ++t) pg[t] = tok + 16 * t < s.held ? page_of(c, r, b, tok + 16 * t) : -1;
+    // Pages of the two sixteens of a step.  Pages of 32 tokens and more hold both, so that one address serves them (2 to 4 % of the time at 64 and 128
+    // channels)
+    const bool one_page = c.page >= 32;
+    auto pages_of = [&](int tok, int (&pg)[2]) {
+      pg[0] = tok < s.held ? page_of(c, r, b, tok) : -1;
+      pg[1] = one_page ? pg[0] : tok + 16 < s.held ? page_of(c, r, b, tok + 16) : -1;
     };
     Held<D, G> x;
-    auto fetch_keys = [&](int tok, const int (&pg)[2]) {            // (a page that is not there: page 0, and masked)
+    auto key_of = [&](int t, const uint8_t* kp, const uint8_t* mp) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t in = (tok + 16 * t) & (c.page - 1), page = max(pg[t], 0);
-        const uint8_t* kp = kc + ((uint64_t)page * code_page + in * (D / 2));
-        const uint8_t* mp = km + ((uint64_t)page * meta_page + in * 4);
-#pragma unroll
-        for (int i = 0; i < GU; ++i) x.km[t][i] = *(const uint32_t*)(mp + (uint32_t)(i * 16) * c.page + km_at);
-        if constexpr (D == 64) {
-          const uint2 d = *(const uint2*)(kp + k_at);
-          x.k[t][0] = d.x; x.k[t][1] = d.y;
-        } else {
-#pragma unroll
-          for (int i = 0; i < VU; ++i) {
-            const v4u d = *(const v4u*)(kp + 64 * i + k_at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = d[j];
-          }
-        }
-      }
-    };
-    auto fetch_values = [&](int tok, const int (&pg)[2]) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t in = (tok + 16 * t) & (c.page - 1), page = max(pg[t], 0);
-        const uint8_t* vp = vc + ((uint64_t)page * code_page + in * (D / 2));
-        const uint8_t* mp = vm + ((uint64_t)page * meta_page + in * 4);
+      for (int i = 0; i < GU; ++i) x.km[t][i] = *(const uint32_t*)(mp + (uint32_t)(i * 16) * c.page + km_at);
+      if constexpr (D == 64) {
+        const uint2 d = *(const uint2*)(kp + k_at);
+        x.k[t][0] = d.x; x.k[t][1] = d.y;
+      } else {
 #pragma unroll
         for (int i = 0; i < VU; ++i) {
-          x.v[t][i] = *(const v4u*)(vp + 256 * i + v_at);
-          x.vm[t][i] = *(const v4u*)(mp + (uint32_t)(i * (128 / G) * 4) * c.page + vm_at);
+          const v4u d = *(const v4u*)(kp + 64 * i + k_at);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.k[t][4 * i + j] = d[j];
         }
       }
     };
+    auto value_of = [&](int t, const uint8_t* vp, const uint8_t* mp) {
+#pragma unroll
+      for (int i = 0; i < VU; ++i) {
+        x.v[t][i] = *(const v4u*)(vp + 256 * i + v_at);
+        x.vm[t][i] = *(const v4u*)(mp + (uint32_t)(i * (128 / G) * 4) * c.page + vm_at);
+      }
+    };
+    auto fetch = [&](auto of, const uint8_t* codes, const uint8_t* metas, int tok, const int (&pg)[2]) {   // (a page that is not there: page 0, and masked)
+      const uint32_t in = tok & (c.page - 1), page = max(pg[0], 0);
+      const uint8_t *cp = codes + ((uint64_t)page * code_page + in * (D / 2)), *mp = metas + ((uint64_t)page * meta_page + in * 4);
+      of(0, cp, mp);
+      if (one_page) {
+        of(1, cp + 16 * (D / 2), mp + 16 * 4);
+      } else {
+        const uint32_t in = (tok + 16) & (c.page - 1), page = max(pg[1], 0);
+        of(1, codes + ((uint64_t)page * code_page + in * (D / 2)), metas + ((uint64_t)page * meta_page + in * 4));
+      }
+    };
+    auto fetch_keys = [&](int tok, const int (&pg)[2]) { fetch(key_of, kc, km, tok, pg); };
+    auto fetch_values = [&](int tok, const int (&pg)[2]) { fetch(value_of, vc, vm, tok, pg); };
 
     // keys of the next step are under way while this one's values are worked on, and the other way round
     int pg[2], pg_next[2];
@@ -221,6 +215,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
       const _Float16 hi = (_Float16)sum;
       if (h4 == g % 4) { qm[2 * (g / 4)] = hi; qm[2 * (g / 4) + 1] = (_Float16)(sum - (float)hi); }
     }
+    if constexpr (Q_LDS) {                                          // (the last item's are read: two barriers ago)
+      if (wave == 0)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q_sh[k * 64 + lane] = q[k];
+      __syncthreads();
+    }
     cs = fmaxf(cs, 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
     v4f o[TILES];
     float m, l;
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
 #pragma unroll
           for (int k = g * (G / 32); k < (g + 1) * (G / 32); ++k) {
             const v8h f = code_octet(x.k[t][k], ex);
-            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], part, 0, 0, 0);
+            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, Q_LDS ? q_sh[k * 64 + lane] : q[k], part, 0, 0, 0);
           }
           const v2u sm = scale_sh[wave][t][g][h4];
 #pragma unroll

@@ -65,28 +65,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   const Weights wt{a.ratio, a.window, a.sinks};
   AttnPiece* desc = nullptr;
   int64_t base = 0, at = 0, end = 0, begin = 0, total = 0, pieces = 0, place = 0;
-  int h, b = -1, tile = 0;
+  int h, b, tile = 0;
   bool joined = false;
   if (!cut) {                                                       // heads fastest: an XCD meets few of them; a sequence's last tiles first
     h = blockIdx.x % c.heads;
     const int64_t item = blockIdx.x / c.heads;
-    for (int j = 0; j < r.seqs; j += 64) {
-      const int64_t n = j + lane < r.seqs ? row_tiles(seq_of(r, j + lane), a.ratio) : 0, sum = scan64(n, lane), here = of_lane(sum, 63);
-      if (item < base + here) {
-        const int q = __popcll(__ballot(base + sum <= item));
-        b = j + q;
-        if (q) base += of_lane(sum, q - 1);
-        break;
-      }
-      base += here;
-    }
-    if (b < 0) return;
+    auto units = [&](int b) { return (int64_t)row_tiles(seq_of(r, b), a.ratio); };
+    const Index list(r.seqs, lane, units);
+    if (item >= list.total) return;
+    b = list.find(item, base, units);
     tile = row_tiles(seq_of(r, b), a.ratio) - 1 - (int)(item - base);
   } else {                                                          // workgroups of an XCD are neighbours in the list: a head's tokens stay in its L2
     place = gridDim.x % 8 ? blockIdx.x : (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
     desc = (AttnPiece*)a.ws + place;
-    int64_t one = 0;                                                // units of a head
-    for (int j = 0; j < r.seqs; j += 64) one += of_lane(scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), 63);
+    auto units = [&](int b) { return wt.all(seq_of(r, b)); };
+    const Index list(r.seqs, lane, units);
+    const int64_t one = list.total;                                 // units of a head
     total = one * c.heads;
     pieces = total ? min((int64_t)gridDim.x, max(total / ((int64_t)LEAST * T::KEYS * a.ratio), (int64_t)1)) : 0;   // (0: no sequence has a row)
     if (place >= pieces) {
@@ -97,21 +91,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     begin = at = place * each + min(place, more);
     end = at + each + (place < more);
     h = (int)(begin / one);
-    base = h * one;
-    for (int j = 0; j < r.seqs; j += 64) {
-      const int64_t sum = scan64(j + lane < r.seqs ? wt.all(seq_of(r, j + lane)) : 0, lane), here = of_lane(sum, 63);
-      if (begin < base + here) {
-        const int q = __popcll(__ballot(base + sum <= begin));
-        b = j + q;
-        if (q) base += of_lane(sum, q - 1);
-        break;
-      }
-      base += here;
-    }
-    if (b < 0) {                                                    // (lengths or offsets that change under the call)
-      if (tid == 0) desc->count = 0;
-      return;
-    }
+    b = list.find(begin - h * one, base, units);
+    base += h * one;
     const Seq s = seq_of(r, b);                                     // its tile: the last that begins at or before
     int lo = 0, hi = row_tiles(s, a.ratio) - 1;
     while (lo < hi) {
