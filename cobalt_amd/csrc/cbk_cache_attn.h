@@ -89,6 +89,15 @@ __device__ inline float rounded_product(float a, float b) {
   return a * b;
 }
 
+// What two rounded numbers leave of e0 and e1, exactly: one instruction each, which the compiler makes three of
+__device__ inline v2h rest_of(v2h rounded, float e0, float e1) {
+  const uint32_t two = __builtin_bit_cast(uint32_t, rounded);
+  float r0, r1;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(two), "v"(e0));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(two), "v"(e1));
+  return v2h{(_Float16)r0, (_Float16)r1};
+}
+
 // Power of two that a query row is divided by, and `down`, its reciprocal, for a largest magnitude `top`: 1 if the row (and sums of
 // 128 of its elements) is an ordinary fp16 row without it, else one that leaves [1, 2).  Also 1 for zeros, infinities and NaN.
 __device__ inline float row_factor(float top, float& down) {

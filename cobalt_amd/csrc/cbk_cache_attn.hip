@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
         l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
         p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
         if constexpr (!BF) {
-          const v2h pl = {(_Float16)(e[2 * i] - (float)ph.x), (_Float16)(e[2 * i + 1] - (float)ph.y)};
+          const v2h pl = rest_of(ph, e[2 * i], e[2 * i + 1]);
           rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
           l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
         }

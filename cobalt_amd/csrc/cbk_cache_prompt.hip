@@ -412,7 +412,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
           p[st & 1][2 * i] = ph.x; p[st & 1][2 * i + 1] = ph.y;
           l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
           if constexpr (!BF) {
-            const v2h pl = {(_Float16)(e0 - (float)ph.x), (_Float16)(e1 - (float)ph.y)};
+            const v2h pl = rest_of(ph, e0, e1);
             rest[st & 1][2 * i] = pl.x; rest[st & 1][2 * i + 1] = pl.y;
             l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
           }
