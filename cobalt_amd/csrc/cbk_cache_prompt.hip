@@ -8,7 +8,7 @@
 // LDS read is a run of 1 KB without bank conflicts.
 //
 // While the products of a tile run, the next one, whose codes were loaded a tile before, is widened into the other half of
-// LDS: four wavefronts take the keys, four the values, 16 tokens of (at most) 128 channels each.  One barrier a tile.
+// LDS: four wavefronts take the keys, four the values, 16 tokens of (at most) 128 channels each.  One barrier for a tile's two blocks.
 //
 // bf16 results: keys m + c s rounded once to fp16, p rounded to fp16 (both far below the result's own step).  fp16 results: keys
 // as their codes with one product a group, multiplied by the token's scale in float32, the minima in a product of their own, and p
@@ -17,6 +17,13 @@
 // Work is dealt out in one of two ways (plan_prompt).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
 // workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
 // of a tile that it does not finish is joined by the second launch of cbk_cache_attn.hip.
+//
+// A 4096-token prompt of 32 query heads on 8, 128 channels, bf16: 170 us, 810 TFLOP/s; 8192 tokens 590 us, 930 (a large library product
+// reaches 1210); fp16, with its half more of products, 850 to 1045 us by the group.  64 channels 815 us (bf16) and 1180 (fp16) for twice the heads, whose bound
+// is the vector unit: an exponential and five instructions a score.  Matrix unit busy 36 %, vector unit 46 %; the bare loop
+// of products would take 104 of the 170 us, widening 13 to 35 of them, reads from LDS 31 to 35, exponentials 6 to 9.  256 rows
+// a workgroup, because widening is shared by all rows; two blocks of 64 tokens a barrier (one: 180 us).  Built and not kept: the two
+// halves of the wavefronts a phase apart (200 against 178 us), two workgroups a CU for 64 channels, which spills (1035 against 745).
 #include <type_traits>
 #include "cbk_cache.h"
 #include "cbk_cache_attn.h"
@@ -24,7 +31,8 @@
 namespace cbk {
 
 constexpr int WAVES = 8, ROWS = 32 * WAVES;
-constexpr int LEAST = 3;                     // tiles of tokens that are worth a share of their own
+constexpr int OWN = 2;                      // tiles of tokens that a tile of rows counts for by itself: its queries, its start and end (six ragged
+                                            // chunks: none 470 us, 1: 445, 2: 433, 4: 431; a prompt of 8192 tokens, cut: 774, 669, 631, 631)
 constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
 
 template <int D, int G, bool BF>
@@ -45,10 +53,11 @@ __device__ inline int row_tiles(const Seq& s, int ratio) { return (int)(((int64_
 // the balance rests on it, not what is computed: a piece of a tile's weight is that piece of its tokens, rounded to tiles.
 struct Weights {
   int ratio, window, sinks;
+  int64_t own;                               // what a tile of rows weighs by itself
   __device__ int64_t first(const Seq& s) const { return (int64_t)max(s.pos0, 0) * ratio; }
-  __device__ int64_t flat() const { return (int64_t)ROWS + (int64_t)ratio * ((int64_t)window + sinks); }
-  __device__ int64_t of(const Seq& s, int i) const { return window > 0 ? flat() : first(s) + (int64_t)(i + 1) * ROWS; }
-  __device__ int64_t before(const Seq& s, int i) const { return window > 0 ? i * flat() : i * first(s) + (int64_t)i * (i + 1) / 2 * ROWS; }
+  __device__ int64_t flat() const { return own + ROWS + (int64_t)ratio * ((int64_t)window + sinks); }
+  __device__ int64_t of(const Seq& s, int i) const { return window > 0 ? flat() : own + first(s) + (int64_t)(i + 1) * ROWS; }
+  __device__ int64_t before(const Seq& s, int i) const { return window > 0 ? i * flat() : i * (own + first(s)) + (int64_t)i * (i + 1) / 2 * ROWS; }
   __device__ int64_t all(const Seq& s) const { return s.n > 0 ? before(s, row_tiles(s, ratio)) : 0; }
 };
 
@@ -62,7 +71,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   const Exponents ex = exponents();
 
   // ---- this workgroup's share: tile `tile` of head h of sequence b, or units [at, end) of the list
-  const Weights wt{a.ratio, a.window, a.sinks};
+  const Weights wt{a.ratio, a.window, a.sinks, (int64_t)OWN * T::KEYS * a.ratio};
   AttnPiece* desc = nullptr;
   int64_t base = 0, at = 0, end = 0, begin = 0, total = 0, pieces = 0, place = 0;
   int h, b, tile = 0;
@@ -82,7 +91,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
     const Index list(r.seqs, lane, units);
     const int64_t one = list.total;                                 // units of a head
     total = one * c.heads;
-    pieces = total ? min((int64_t)gridDim.x, max(total / ((int64_t)LEAST * T::KEYS * a.ratio), (int64_t)1)) : 0;   // (0: no sequence has a row)
+    pieces = total ? min((int64_t)gridDim.x, max(total / ((int64_t)T::KEYS * a.ratio), (int64_t)1)) : 0;   // (0: no sequence has a row)
     if (place >= pieces) {
       if (tid == 0) desc->count = 0;
       return;
@@ -503,9 +512,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 // ------------------------------------------------------------------ launch
 PromptPlan plan_prompt(const DCache& c, const DRows& r, int ratio) {
   PromptPlan p;
+  // Whole tiles where there are enough of them or where they are prompts, whose tiles are of all lengths and fill the chip one behind the
+  // other; equal shares where a few tiles stand behind long histories.  128 channels, 8 cache heads of 4 query heads, whole against cut: prompts
+  // of 1024 tokens 45 and 56 us, of 2048 80 and 92, of 4096 187 and 206; the last 512 of 2048 tokens 72 and 55, of 16384 504 and 168; the
+  // last 1024 of 4096 136 and 102; six ragged chunks (630 tiles) 469 and 432; 8 x 1000 of 6000 (1090 tiles) 784 and 797.
   const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;   // at most
   const bool prompts = 2 * (int64_t)r.tokens > (int64_t)r.cap * r.seqs;          // most of what the table can hold is new
-  p.cut = tiles < (prompts ? 2 : 4) * CHIP;
+  p.cut = !prompts && tiles < 3 * CHIP;
   p.grid = p.cut ? CHIP : tiles;
   p.bytes = p.cut ? attn_bytes((int)p.grid, ROWS, c.dim) : 0;
   return p;
