@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(DCache c, DRows r, Cach
 }
 
 // Rows a lane takes: four where wavefronts that take one would fill the chip more than four times over (65536 tokens of 8 heads of 128
-// channels: written in 83 us, 93 with one row; read in 63, 71; 8192 tokens alike)
+// channels: written in 83 us, 93 with one row; read in 63, 71; 16384 tokens alike, 2048 tokens 4.9 with one row and 5.4, read 5.1 and 7.3)
 constexpr int MANY = 4;                     // (to write: two, which a chip-wide call has enough wavefronts for)
 static bool many_io(const DCache& c, const DRows& r) { return (int64_t)r.tokens * c.heads * c.dim >= (int64_t)MANY * 8192 * 512; }
 static dim3 io_grid(const DCache& c, const DRows& r, int u) {
