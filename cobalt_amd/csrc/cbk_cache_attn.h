@@ -48,6 +48,22 @@ __device__ inline int64_t scan64(int64_t x, int lane) {             // sum of th
   return x;
 }
 
+// A quotient of numbers that are not negative and nearly always short: a division of 64-bit numbers takes some 150 instructions
+// (256 sequences of 300 tokens 33 us, 37 with 64-bit divisions)
+__device__ inline int64_t quotient(int64_t a, int64_t b) { return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
+
+// `total` units in `pieces` shares that differ by one at most, the longer ones first
+struct Shares {
+  int64_t each, more;
+  __device__ Shares(int64_t total, int64_t pieces) : each(quotient(total, pieces)), more(total - each * pieces) {}
+  __device__ int64_t begin(int64_t place) const { return place * each + min(place, more); }
+  __device__ int64_t end(int64_t place) const { return begin(place) + each + (place < more); }
+  __device__ int64_t of(int64_t unit) const {                       // the share that has the unit
+    const int64_t longer = more * (each + 1);
+    return unit < longer ? quotient(unit, each + 1) : more + quotient(unit - longer, each);
+  }
+};
+
 // The sequences one behind the other, units(b) units of work each.  Every wavefront looks for its place by itself: a lane adds up `each`
 // consecutive sequences, one scan gives where they begin, and a second one, among the sequences of the lane that has the place, the sequence.
 // (1024 sequences of 300 tokens 140 us; with a scan for every 64 of them 152.)

@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
     if (a.ws && tid == 0) desc->count = 0;
     return;
   }
-  const int64_t begin = w * total / pieces, end = (w + 1) * total / pieces;
+  const Shares shares(total, pieces);
+  const int64_t begin = shares.begin(w), end = shares.end(w);
   int64_t base;
   int b = list.find(begin, base, units);
   int64_t at = begin;
@@ -110,13 +111,13 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
       if (++b == r.seqs) break;                                     // (there is a next one, unless lengths change under the call)
       continue;
     }
-    const int64_t item = (at - base) / weight, start = base + item * weight;
+    const int64_t item = quotient(at - base, weight), start = base + item * weight;
     const int64_t until = min(end, start + weight);
     const int u0 = a.whole ? 0 : max((int)(at - start) - EXTRA, 0), u1 = a.whole ? g.units : (int)(until - start) - EXTRA;
     const bool is_first = at == begin;
     at = until;
     if (u1 <= u0) continue;                                         // nothing but what the tile counts for by itself
-    const int h = (int)(item / tiles), row0 = (int)(item % tiles) * R;
+    const int h = (int)quotient(item, tiles), row0 = (int)(item - (int64_t)h * tiles) * R;
     const int valid = min(R, rows - row0);
 
     const int pos_lo = s.pos0 + row0 / a.ratio, pos_hi = s.pos0 + (row0 + valid - 1) / a.ratio;
@@ -377,13 +378,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
     const bool direct = u0 == 0 && u1 == g.units;
     const int slot = is_first ? 0 : 1;
     if (!direct && u0 == 0 && tid == 0) {                           // this workgroup begins the tile: it is joined from here
-      // the last piece with a unit of it: pieces are cut at floor(i total / pieces)
-      const int64_t last = start + weight - 1;
-      int64_t e = last * pieces / total;
-      while (e + 1 < pieces && (e + 1) * total / pieces <= last) ++e;
-      while (e > w && e * total / pieces > last) --e;
       desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = slot;
-      desc->count = (int)(e - w + 1);
+      desc->count = (int)(shares.of(start + weight - 1) - w + 1);
     }
     if (!direct && u0 == 0) joined = 1;
     for (int x = tid; x < valid * (D / 4); x += 256) {

@@ -96,9 +96,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       if (tid == 0) desc->count = 0;
       return;
     }
-    const int64_t each = total / pieces, more = total % pieces;     // (no product of a place and the total: it could pass 64 bits)
-    begin = at = place * each + min(place, more);
-    end = at + each + (place < more);
+    const Shares shares(total, pieces);
+    begin = at = shares.begin(place);
+    end = shares.end(place);
     h = (int)(begin / one);
     b = list.find(begin - h * one, base, units);
     base += h * one;
@@ -456,10 +456,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
   if (!whole_tile && at == first_unit) {                            // this workgroup begins the tile: it is joined from here
     joined = true;
     if (tid == 0) {
-      const int64_t last = first_unit + units - 1, each = total / pieces, more = total % pieces;
-      const int64_t e = last < more * (each + 1) ? last / (each + 1) : more + (last - more * (each + 1)) / each;
       desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = slot;
-      desc->count = (int)(e - place + 1);
+      desc->count = (int)(Shares(total, pieces).of(first_unit + units - 1) - place + 1);
     }
   }
   if (is) {
