@@ -627,3 +627,64 @@ def test_the_smallest_and_largest_scales(n, dtype):
         tol = (U + 2.0 ** -16) * size
         tol = tol + HALF[dtype] * (np.abs(o) + tol) + 2.0 ** -25
         assert (np.abs(out[:, h] - o) <= tol).all()
+
+
+@pytest.mark.parametrize("seed,large", [(i, False) for i in range(12)] + [(i, True) for i in range(13, 18)])
+def test_calls_of_all_kinds(seed, large):
+    """Drawn calls: sequences without tokens or rows, more rows than tokens, tables that end before the sequence does or name pages that are
+    not there, rows in front of the first sequence and behind the last, windows, sinks, strides, both kernels."""
+    g = torch.Generator().manual_seed(1000 + seed)
+    draw = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))
+    pick = lambda *x: x[draw(0, len(x) - 1)]
+    dim, dtype, page, heads, ratio = pick(64, 128, 256), pick(torch.float16, torch.bfloat16), pick(16, 32, 64, 256), draw(1, 3), pick(1, 2, 3, 4, 7)
+    group = pick(32, 64, 128) if dim > 64 else pick(32, 64)
+    seqs = draw(1, 70) if seed % 4 == 0 else draw(1, 5)
+    lens = [draw(0, 40) if seqs > 5 or draw(0, 3) == 0 else draw(100, 2500) for _ in range(seqs)]
+    s = Setup(lens, heads, dim, page, group, dtype, seed=seed)
+    most = pick(3, 70, 700)
+    new = [draw(0, min(n + 5, most)) for n in lens]
+    if large:                                                       # enough rows and heads for the kernel of many rows
+        heads, ratio, lens = 4, pick(4, 5), [draw(1000, 1600) for _ in range(2)] + [draw(0, 60), draw(1000, 2500)]
+        s = Setup(lens, heads, dim, page, group, dtype, seed=seed)
+        new = [draw(400, 600), draw(400, 1005), draw(0, 60), draw(400, 600)]
+    table = s.table.cpu()
+    cols = draw(max(1, table.shape[1] // 2), table.shape[1])
+    there = []
+    for b, n in enumerate(lens):
+        for i in range(table.shape[1]):
+            if draw(0, 9) == 0:
+                table[b, i] = pick(-1, -7, s.pages, 2 ** 31 - 1)
+        pages = torch.where((table[b] >= 0) & (table[b] < s.pages), 1, 0).bool()
+        pages[cols:] = False
+        there.append(pages.repeat_interleave(page)[:n].numpy())
+    front, behind = draw(0, 3), draw(0, 3)
+    starts = ints((np.concatenate([[0], np.cumsum(new)]) + front).tolist())
+    wide = torch.full((table.shape[0], table.shape[1] + 2), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    rows = KVRows(wide.to(DEV)[:, :cols], ints(lens), starts)
+    window, sinks = pick((None, 0), (None, 0), (1, 0), (17, 3), (200, 40), (1000, 0))
+    total = sum(new)
+    q = torch.randn(total + front + behind, heads * ratio, dim, generator=g).to(dtype).to(DEV)
+    out = torch.full((heads * ratio, total + front + behind, dim), 9.0, device=DEV, dtype=dtype).transpose(0, 1)
+    ops.cache_attention(s.cache, q, rows, window=window, sinks=sinks, out=out)
+    assert bool((out[:front] == 9).all()) and bool((out[front + total:] == 9).all())
+    s.check(q[front:front + total], out[front:front + total], new, window=window, sinks=sinks, there=there)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [4, 300])
+def test_a_query_that_is_no_number_stays_alone(n, dtype):
+    s = Setup([3000, 2000], 2, 128, 64, 32, dtype, seed=n)
+    q = torch.randn(2 * n, 8, 128, generator=torch.Generator().manual_seed(2)).to(dtype)
+    q[1, 3, 7], q[2, 5, 100], q[n, 0, 0] = float("nan"), float("inf"), float("-inf")
+    out = ops.cache_attention(s.cache, q.to(DEV), s.rows([n, n]))
+    for r, h in ((1, 3), (2, 5), (n, 0)):
+        assert bool(out[r, h].isnan().all())
+        q[r, h], out[r, h] = 0, s_mean(s, r, h, n).to(out)         # (a query of zeros: the mean of the values it sees)
+    s.check(q, out, [n, n])
+
+
+def s_mean(s, r, h, n):
+    b = r // n
+    v = s.hv[s.cut[b]:s.cut[b + 1] - n + r % n + 1, h // 4]
+    return torch.from_numpy(v.mean(0)).to(s.dtype)
