@@ -13,6 +13,7 @@ from . import ops
 from .cache import KVCache, KVRows
 
 NAME = "cobalt_cache"
+DTYPES = (torch.float16, torch.bfloat16)
 
 
 class _Sequences:
@@ -81,9 +82,9 @@ class CobaltCacheLayer(CacheLayerMixin):
     is_compileable = False
     is_sliding = False
 
-    def __init__(self, sequences: _Sequences, index: int, group: int, sinks: int):
+    def __init__(self, sequences: _Sequences, index: int, group: int, window: Optional[int], sinks: int):
         super().__init__()
-        self.sequences, self.index, self.group, self.sinks = sequences, index, group, sinks
+        self.sequences, self.index, self.group, self.window, self.sinks = sequences, index, group, window, sinks
         self.pool: Optional[KVCache] = None
 
     def lazy_initialization(self, key_states, value_states):
@@ -132,13 +133,16 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
         raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
     if query.requires_grad or key.requires_grad or value.requires_grad:
         raise RuntimeError("the 4-bit cache has no backward pass: call the model under torch.no_grad()")
+    if query.dtype not in DTYPES:                                    # (before the lengths advance)
+        raise TypeError(f"the 4-bit cache is for float16 and bfloat16 models, not {query.dtype}")
     batch, _, tokens, _ = query.shape
+    window = sliding_window or layer.window                          # (models that leave it to their mask do not pass one)
     if layer.index == 0:
         layer.sequences.begin(batch, tokens, attention_mask)
     as_rows = lambda x: x.transpose(1, 2).reshape(batch * tokens, x.shape[1], x.shape[3])
     ops.cache_write(layer.pool, as_rows(key), as_rows(value), layer.sequences.rows)
-    out = ops.cache_attention(layer.pool, as_rows(query), layer.sequences.rows, scale=scaling, window=sliding_window or None,
-                              sinks=layer.sinks if sliding_window else 0)
+    out = ops.cache_attention(layer.pool, as_rows(query), layer.sequences.rows, scale=scaling, window=window,
+                              sinks=layer.sinks if window else 0)
     return out.view(batch, tokens, query.shape[1], query.shape[3]), None
 
 
@@ -149,7 +153,8 @@ def _padding_mask(*args, attention_mask=None, **kwargs):
 
 def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) -> Cache:
     cfg = model.config.get_text_config()
-    kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
+    types = getattr(cfg, "layer_types", None) or ["full_attention"] * cfg.num_hidden_layers
+    kinds = set(types)
     if kinds - {"full_attention", "sliding_attention"} or getattr(model.config, "is_encoder_decoder", False):
         raise ValueError(f"the 4-bit cache is for decoders of full and sliding-window attention, not {sorted(kinds)}")
     if sinks < 0:
@@ -157,6 +162,7 @@ def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) ->
     AttentionInterface.register(NAME, cobalt_attention)
     AttentionMaskInterface.register(NAME, _padding_mask)
     seqs = _Sequences(batch, max_len, page, next(model.parameters()).device)
-    cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, sinks) for i in range(cfg.num_hidden_layers)])
+    window = lambda kind: getattr(cfg, "sliding_window", None) if kind == "sliding_attention" else None
+    cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, window(kind), sinks) for i, kind in enumerate(types)])
     model.set_attn_implementation(NAME)
     return cache

@@ -56,6 +56,7 @@ def exact(monkeypatch):
                 out[r, h] = torch.from_numpy(o[0])
         return out
 
+    monkeypatch.setattr(hf, "DTYPES", (torch.float64,))
     monkeypatch.setattr(hf.ops, "cache_write", write)
     monkeypatch.setattr(hf.ops, "cache_attention", attention)
 
@@ -172,3 +173,26 @@ def test_a_step_that_is_refused_leaves_the_lengths(exact):
     with pytest.raises(ValueError):
         m(ids, past_key_values=cache)
     assert int(cache.get_seq_length()) == 6 and cache.layers[0].sequences.lens.tolist() == [6]
+
+
+def test_windows_of_the_configuration_hold_where_a_model_passes_none(exact, monkeypatch):
+    cfg = tr.Qwen2Config(vocab_size=97, hidden_size=128, intermediate_size=128, num_hidden_layers=3, num_attention_heads=2, num_key_value_heads=1,
+                         use_sliding_window=True, sliding_window=6, max_window_layers=1)
+    m = tr.Qwen2ForCausalLM(cfg).double().eval().requires_grad_(False)
+    seen = []
+    real = hf.cobalt_attention
+    monkeypatch.setattr(hf, "cobalt_attention", lambda mod, q, k, v, mask, **kw: real(mod, q, k, v, mask, **{**kw, "sliding_window": None}))
+    attend = hf.ops.cache_attention
+    monkeypatch.setattr(hf.ops, "cache_attention", lambda *a, **k: seen.append(k["window"]) or attend(*a, **k))
+    ids = torch.arange(2, 22)[None]
+    want = m(ids).logits
+    got = m(ids, past_key_values=Mo.cobalt_cache(m, 1, 32)).logits
+    assert seen == [None, 6, 6] and float((got - want).abs().max()) < ATOL
+
+
+def test_a_model_of_another_type_is_refused_before_the_lengths_advance():
+    m = _model().float()
+    cache = Mo.cobalt_cache(m, 1, 8)
+    with pytest.raises(TypeError, match="float16"):
+        m(torch.arange(2, 8)[None], past_key_values=cache)
+    assert int(cache.get_seq_length()) == 0 and cache.layers[0].sequences.steps == 0
