@@ -536,6 +536,33 @@ def test_steps_in_a_graph_follow_the_lengths():
             assert torch.equal(t, x)
 
 
+def test_two_graphs_of_one_memory_pool():
+    """Their workspaces are the same memory: replayed in turn, with eager calls between, both answer as eager calls do."""
+    s = Setup([5000, 2600], 4, 128, 64, 32, torch.float16, seed=21)
+    calls = []
+    for new, window in (([1, 1], None), ([700, 500], None), ([3, 2], 300)):
+        q = torch.randn(sum(new), 16, 128, device=DEV).half()
+        rows = s.rows(new)
+        calls.append((q, rows, window, ops.cache_attention(s.cache, q, rows, window=window)))
+        if sum(new) < 10:
+            s.check(q, calls[-1][3], new, window=window)
+    torch.cuda.synchronize()
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for q, rows, window, want in calls:
+        out, graph = torch.zeros_like(q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            ops.cache_attention(s.cache, q, rows, window=window, out=out)
+        graphs.append((graph, out, want))
+    for i in range(4):
+        for graph, out, want in graphs if i % 2 else graphs[::-1]:
+            out.fill_(5)
+            graph.replay()
+            torch.empty(16 << 20, dtype=torch.uint8, device=DEV).fill_(255)
+            assert torch.equal(out, want)
+        q, rows, window, want = calls[i % 3]
+        assert torch.equal(ops.cache_attention(s.cache, q, rows, window=window), want)
+
+
 def test_two_streams_at_once():
     a, b = (Setup([3000, 200], 2, 128, 64, 32, torch.float16, seed=i) for i in (20, 21))
     q = [torch.randn(2, 8, 128, device=DEV).half() for _ in range(2)]
