@@ -3,11 +3,13 @@
 `ops.cache_write` and reads the cache with `ops.cache_attention`, prompts and single tokens alike."""
 from __future__ import annotations
 
+from types import FunctionType
 from typing import Optional
 
 import torch
 from transformers import AttentionInterface, AttentionMaskInterface
 from transformers.cache_utils import Cache, CacheLayerMixin
+from transformers.masking_utils import causal_mask_function, sliding_window_causal_mask_function
 
 from . import ops
 from .cache import KVCache, KVRows
@@ -146,8 +148,46 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
     return out.view(batch, tokens, query.shape[1], query.shape[3]), None
 
 
-def _padding_mask(*args, attention_mask=None, **kwargs):
-    """The 2-D mask of the padding as it is; what else a mask says follows from the lengths and the window."""
+def _same(a, b) -> bool:
+    """Whether two mask functions are of the same code over the same values (the library builds new closures for every step)."""
+    if isinstance(a, (tuple, list)) and isinstance(b, (tuple, list)):
+        return len(a) == len(b) and all(map(_same, a, b))
+    if isinstance(a, FunctionType) and isinstance(b, FunctionType):
+        inner = lambda f: [c.cell_contents for c in f.__closure__ or ()]
+        return a.__code__ is b.__code__ and _same(inner(a), inner(b))
+    return type(a) is type(b) and isinstance(a, (int, float, str, type(None))) and a == b
+
+
+def _answers_alike(f, plain, batch, heads, q_length, kv_length, q_offset, kv_offset, device) -> bool:
+    """Whether a mask function hides and shows what the plain one does, over the rows and tokens of a step; read by the host."""
+    at = lambda first, n, dim: (first + torch.arange(n, device=device)).view([n if d == dim else 1 for d in range(4)])
+    b, h, kv = at(0, batch, 0), at(0, heads, 1), at(kv_offset, kv_length, 3)
+    rows = max(1, (1 << 24) // (batch * kv_length))                     # at a time: 16 MB of truth values (a head)
+    for i in range(0, q_length, rows):
+        q = at(q_offset + i, min(rows, q_length - i), 2)
+        if not bool((f(b, h, q, kv) == plain(b, h, q, kv)).all()):
+            return False
+    return True
+
+
+def _padding_mask(batch_size=1, q_length=1, kv_length=1, q_offset=0, kv_offset=0, mask_function=causal_mask_function, attention_mask=None,
+                  local_size=None, config=None, device=None, **kwargs):
+    """The 2-D mask of the padding as it is.  What else the mask function says follows from the lengths and the window, if it is the
+    plain causal or sliding one, or answers as that does (an image's tokens see one another, in a step without an image); any other is
+    refused."""
+    if local_size is not None:
+        plain = [sliding_window_causal_mask_function(local_size)]
+    else:                                                               # (with something added to it, the window is not told)
+        size = getattr(config, "sliding_window", None)
+        plain = [causal_mask_function] + ([sliding_window_causal_mask_function(size)] if size else [])
+    if any(_same(mask_function, f) for f in plain):
+        return attention_mask
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise ValueError("a mask that a model adds to the causal one is read by the host: such a step cannot be recorded in a graph")
+    heads = getattr(config, "num_attention_heads", 1)
+    if not any(_answers_alike(mask_function, f, batch_size, heads, q_length, kv_length, q_offset, kv_offset, device) for f in plain):
+        raise ValueError("attention over the 4-bit cache is causal, under a sliding window at most: this step's mask says otherwise "
+                         "(tokens that see later ones, or blocks that are kept apart)")
     return attention_mask
 
 

@@ -196,3 +196,52 @@ def test_a_model_of_another_type_is_refused_before_the_lengths_advance():
     with pytest.raises(TypeError, match="float16"):
         m(torch.arange(2, 8)[None], past_key_values=cache)
     assert int(cache.get_seq_length()) == 0 and cache.layers[0].sequences.steps == 0
+
+
+def _mixed(images="gemma3"):
+    """Small decoders with a vision tower: Gemma 3, whose image tokens see one another, and Llava, which is causal throughout."""
+    text = dict(vocab_size=97, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                head_dim=64, max_position_embeddings=512)
+    vision = dict(hidden_size=32, intermediate_size=32, num_hidden_layers=2, num_attention_heads=2, image_size=28, patch_size=14)
+    torch.manual_seed(3)
+    if images == "gemma3":
+        cfg = tr.Gemma3Config(text_config=tr.Gemma3TextConfig(**text, sliding_window=6, layer_types=["sliding_attention", "full_attention"]).to_dict(),
+                              vision_config=tr.SiglipVisionConfig(**vision).to_dict(), mm_tokens_per_image=4, image_token_index=90,
+                              boi_token_index=91, eoi_token_index=92)
+        m = tr.Gemma3ForConditionalGeneration(cfg)
+    else:
+        cfg = tr.LlavaConfig(text_config=tr.MistralConfig(**text, sliding_window=None), vision_config=tr.CLIPVisionConfig(**vision), image_token_index=90)
+        m = tr.LlavaForConditionalGeneration(cfg)
+    return m.double().eval().requires_grad_(False)
+
+
+def test_a_mask_that_says_more_than_causal_is_refused(exact):
+    m = _mixed()
+    ids = torch.arange(2, 22)[None]
+    types = torch.zeros_like(ids)
+    want = m(ids, token_type_ids=types).logits
+    got = m(ids, token_type_ids=types, past_key_values=Mo.cobalt_cache(m, 1, 32)).logits
+    assert float((got - want).abs().max()) < ATOL                       # text alone
+    types[0, 4:8] = 1                                                   # an image: its tokens see one another
+    cache = Mo.cobalt_cache(m, 1, 32)
+    with pytest.raises(ValueError, match="causal"):
+        m(ids, token_type_ids=types, past_key_values=cache)
+    assert int(cache.get_seq_length()) == 0 and cache.layers[0].sequences.steps == 0
+
+
+def test_masks_are_told_apart():
+    mu = pytest.importorskip("transformers.masking_utils")
+    causal, sliding = mu.causal_mask_function, mu.sliding_window_causal_mask_function
+    mask = torch.ones(2, 9)
+    hook = lambda f, size=None, n=9: hf._padding_mask(batch_size=2, q_length=n, kv_length=9, q_offset=9 - n, attention_mask=mask, mask_function=f, local_size=size)
+    types = torch.tensor([[0, 0, 0, 0, 0, 0, 0, 0, 0], [0, 0, 1, 1, 0, 0, 0, 0, 0]])
+    image = lambda b, h, q, k: (types[b, q] == 1) & (types[b, k] == 1)
+    none = lambda b, h, q, k: (types[b, q] == 2) & (types[b, k] == 2)
+    head = lambda b, h, q, k: (h == 0) & (q >= 0)
+    for f, size in ((causal, None), (sliding(7), 7), (mu.or_masks(causal, none), None), (mu.or_masks(sliding(3), none), 3)):
+        assert hook(f, size) is mask
+    assert hook(mu.or_masks(causal, image), None, 3) is mask            # the image lies before the step's tokens
+    for f, size in ((sliding(7), None), (sliding(6), 7), (causal, 7), (mu.or_masks(causal, image), None), (mu.or_masks(sliding(7), image), 7),
+                    (mu.bidirectional_mask_function, None), (mu.and_masks(mu.packed_sequence_mask_function(types), causal), None), (mu.or_masks(causal, head), None)):
+        with pytest.raises(ValueError, match="causal"):
+            hook(f, size)
