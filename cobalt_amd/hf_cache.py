@@ -38,6 +38,8 @@ class _Sequences:
         self.steps = 0           # tokens with the padding, as the host has issued them: replays of a graph are not in it
         self.pads = [0] * self.batch
         self.rows: Optional[KVRows] = None
+        self.mask: Optional[torch.Tensor] = None     # of the step under way, as the first layer got it
+        self.first = True                            # that step is the first
 
     def begin(self, batch: int, tokens: int, mask: Optional[torch.Tensor]):
         """The rows of a step of `tokens` tokens a sequence, called by the first layer; advances the lengths."""
@@ -52,6 +54,7 @@ class _Sequences:
                 self.pads = pads
             elif pads != self.pads:
                 raise ValueError("attention_mask: padding belongs in front of a sequence, in the first call")
+        self.mask, self.first = mask, first
         self.steps += tokens
         self.seen.add_(tokens)
         self.lens.add_(tokens)
@@ -66,9 +69,27 @@ class _Sequences:
                                torch.stack([torch.zeros_like(self.lens), self.lens], 1).flatten(),
                                torch.cat([starts, starts.new_full((1,), batch * tokens)]))
 
+    def same_mask(self, mask: Optional[torch.Tensor]):
+        """The mask of a further layer: a dictionary of masks by kinds of layers reaches them as it is, and all must say the same."""
+        if mask is self.mask:
+            return
+        if mask is not None:
+            self._shape(mask, self.steps)
+        if getattr(mask, "_cobalt_hook", False) and getattr(self.mask, "_cobalt_hook", False):
+            return                                                              # both of the one mask the model was called with
+        pads = self._pads(mask) if mask is not None else [0] * self.batch if self.first else self.pads
+        if pads != self.pads:
+            raise ValueError("attention_mask: all layers must have the same padding")
+
+    def _shape(self, mask, total):
+        if mask.dim() != 2 or mask.shape[0] != self.batch or mask.shape[1] != total:
+            raise ValueError(f"attention_mask must be [{self.batch}, {total}], got {list(mask.shape)}")
+
     def _padding(self, mask, tokens):
-        if mask.dim() != 2 or mask.shape[0] != self.batch or mask.shape[1] != self.steps + tokens:
-            raise ValueError(f"attention_mask must be [{self.batch}, {self.steps + tokens}], got {list(mask.shape)}")
+        self._shape(mask, self.steps + tokens)
+        return self._pads(mask)
+
+    def _pads(self, mask):
         if mask.is_cuda and torch.cuda.is_current_stream_capturing():
             raise ValueError("attention_mask is read by the host: a step recorded in a graph takes none (padding of the first call stays left out)")
         real = mask.bool()
@@ -141,6 +162,8 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
     window = sliding_window or layer.window                          # (models that leave it to their mask do not pass one)
     if layer.index == 0:
         layer.sequences.begin(batch, tokens, attention_mask)
+    else:
+        layer.sequences.same_mask(attention_mask)
     as_rows = lambda x: x.transpose(1, 2).reshape(batch * tokens, x.shape[1], x.shape[3])
     ops.cache_write(layer.pool, as_rows(key), as_rows(value), layer.sequences.rows)
     out = ops.cache_attention(layer.pool, as_rows(query), layer.sequences.rows, scale=scaling, window=window,
@@ -180,15 +203,19 @@ def _padding_mask(batch_size=1, q_length=1, kv_length=1, q_offset=0, kv_offset=0
     else:                                                               # (with something added to it, the window is not told)
         size = getattr(config, "sliding_window", None)
         plain = [causal_mask_function] + ([sliding_window_causal_mask_function(size)] if size else [])
+    mask = None
+    if attention_mask is not None:
+        mask = attention_mask.view(attention_mask.shape)                # one of its own, which the layers know to come from here
+        mask._cobalt_hook = True
     if any(_same(mask_function, f) for f in plain):
-        return attention_mask
+        return mask
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise ValueError("a mask that a model adds to the causal one is read by the host: such a step cannot be recorded in a graph")
     heads = getattr(config, "num_attention_heads", 1)
     if not any(_answers_alike(mask_function, f, batch_size, heads, q_length, kv_length, q_offset, kv_offset, device) for f in plain):
         raise ValueError("attention over the 4-bit cache is causal, under a sliding window at most: this step's mask says otherwise "
                          "(tokens that see later ones, or blocks that are kept apart)")
-    return attention_mask
+    return mask
 
 
 def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) -> Cache:

@@ -239,9 +239,37 @@ def test_masks_are_told_apart():
     none = lambda b, h, q, k: (types[b, q] == 2) & (types[b, k] == 2)
     head = lambda b, h, q, k: (h == 0) & (q >= 0)
     for f, size in ((causal, None), (sliding(7), 7), (mu.or_masks(causal, none), None), (mu.or_masks(sliding(3), none), 3)):
-        assert hook(f, size) is mask
-    assert hook(mu.or_masks(causal, image), None, 3) is mask            # the image lies before the step's tokens
+        assert hook(f, size).data_ptr() == mask.data_ptr()
+    assert hook(mu.or_masks(causal, image), None, 3).data_ptr() == mask.data_ptr()           # the image lies before the step's tokens
     for f, size in ((sliding(7), None), (sliding(6), 7), (causal, 7), (mu.or_masks(causal, image), None), (mu.or_masks(sliding(7), image), 7),
                     (mu.bidirectional_mask_function, None), (mu.and_masks(mu.packed_sequence_mask_function(types), causal), None), (mu.or_masks(causal, head), None)):
         with pytest.raises(ValueError, match="causal"):
             hook(f, size)
+
+
+def test_masks_given_for_each_kind_of_layer_are_looked_at(exact):
+    """A dictionary of masks reaches the layers as it is: none but the padding's own 2-D mask may be in it."""
+    cfg = tr.Gemma3TextConfig(vocab_size=97, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
+                              num_key_value_heads=2, head_dim=64, sliding_window=6, layer_types=["sliding_attention", "full_attention"])
+    torch.manual_seed(3)
+    m = tr.Gemma3ForCausalLM(cfg).double().eval().requires_grad_(False)
+    ids = torch.arange(2, 12)[None]
+    want = m(ids, attention_mask=torch.ones_like(ids)).logits
+    real = torch.ones(1, 10)
+    got = m(ids, attention_mask=dict(sliding_attention=real, full_attention=real.bool()), past_key_values=Mo.cobalt_cache(m, 1, 16)).logits
+    assert float((got - want).abs().max()) < ATOL
+    four, less = torch.zeros(1, 1, 10, 10), torch.ones(1, 7)
+    for full in (four, less):
+        with pytest.raises(ValueError, match="attention_mask must be"):
+            m(ids, attention_mask=dict(sliding_attention=None, full_attention=full), past_key_values=Mo.cobalt_cache(m, 1, 16))
+        with pytest.raises(ValueError, match="attention_mask must be"):
+            m(ids, attention_mask=dict(sliding_attention=full, full_attention=None), past_key_values=Mo.cobalt_cache(m, 1, 16))
+    pad = real.clone()
+    pad[0, :3] = 0
+    for masks in (dict(sliding_attention=real, full_attention=pad), dict(sliding_attention=None, full_attention=pad)):
+        with pytest.raises(ValueError, match="the same padding"):
+            m(ids, attention_mask=masks, past_key_values=Mo.cobalt_cache(m, 1, 16))
+    cache = Mo.cobalt_cache(m, 1, 16)
+    m(ids, attention_mask=dict(sliding_attention=pad, full_attention=pad.bool()), past_key_values=cache)
+    m(ids[:, :1], attention_mask=dict(sliding_attention=torch.cat([pad, real[:, :1]], 1), full_attention=None), past_key_values=cache)
+    assert cache.layers[0].sequences.lens.tolist() == [8]
