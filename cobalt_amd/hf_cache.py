@@ -231,5 +231,5 @@ def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) ->
     seqs = _Sequences(batch, max_len, page, next(model.parameters()).device)
     window = lambda kind: getattr(cfg, "sliding_window", None) if kind == "sliding_attention" else None
     cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, window(kind), sinks) for i, kind in enumerate(types)])
-    model.set_attn_implementation(NAME)
+    (model.get_decoder() or model).set_attn_implementation(NAME)       # (a vision tower of the same model keeps its own)
     return cache

@@ -273,3 +273,26 @@ def test_masks_given_for_each_kind_of_layer_are_looked_at(exact):
     m(ids, attention_mask=dict(sliding_attention=pad, full_attention=pad.bool()), past_key_values=cache)
     m(ids[:, :1], attention_mask=dict(sliding_attention=torch.cat([pad, real[:, :1]], 1), full_attention=None), past_key_values=cache)
     assert cache.layers[0].sequences.lens.tolist() == [8]
+
+
+def test_only_the_decoder_of_a_mixed_model_is_switched(exact):
+    g = torch.Generator().manual_seed(2)
+    m = _mixed("llava")
+    ids = torch.randint(2, 90, (1, 12), generator=g)
+    ids[0, 3:7] = 90                                                    # four patches of an image
+    kw = dict(pixel_values=torch.randn(1, 3, 28, 28, dtype=torch.float64, generator=g))
+    want = m(ids, **kw).logits
+    dense = tr.DynamicCache(config=m.config.get_text_config())
+    m(ids, past_key_values=dense, **kw)
+    step = m(ids[:, :1], past_key_values=dense).logits
+    cache = Mo.cobalt_cache(m, 1, 32)
+    assert m.model.vision_tower.config._attn_implementation == "sdpa"
+    assert float((m(ids, past_key_values=cache, **kw).logits - want).abs().max()) < ATOL
+    assert float((m(ids[:, :1], past_key_values=cache).logits - step).abs().max()) < ATOL
+    m.set_attn_implementation("sdpa")
+    assert torch.equal(m(ids, **kw).logits, want)
+    m = _mixed()                                                        # Gemma 3: its vision tower runs, its image is refused
+    Mo.cobalt_cache(m, 1, 32)
+    types = (ids == 90).long()
+    with pytest.raises(ValueError, match="this step's mask"):
+        m(ids, token_type_ids=types, past_key_values=Mo.cobalt_cache(m, 1, 32), **kw)
