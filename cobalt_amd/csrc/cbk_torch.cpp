@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/InlineDeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <memory>
@@ -652,13 +653,22 @@ void check_out(const at::Tensor& o, int64_t rows, int64_t heads, int64_t dim, at
     fail(PyExc_ValueError, std::string(what) + " must have unit stride along head_dim, rows that do not overlap and 16-byte aligned heads");
 }
 
+// Nothing here has a backward pass: a gradient that would be lost is an error, as it is for torch's own operators with an output given.
+void no_gradient(std::initializer_list<const at::Tensor*> ts, const char* what) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad())
+      fail(PyExc_RuntimeError, std::string(what) + " has no backward pass: call it under torch.no_grad(), or on detached tensors");
+}
+
 // cache_write(cache, k, v, table, lens, starts or None)
 PyObject* py_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 6)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const Cache c = as_cache(a[0]);
     at::Tensor k = as_tensor(a[1], "k"), v = as_tensor(a[2], "v");
     if (!k.defined() || !v.defined()) fail(PyExc_TypeError, "k and v must be tensors");
+    no_gradient({&k, &v}, "cache_write");
+    const Cache c = as_cache(a[0]);
     same_device(c, k);
     same_device(c, v);
     check_heads(k, c.c.heads, c.c.head_dim, "k");
@@ -685,6 +695,8 @@ PyObject* py_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 8)) return nullptr;
   return guarded([&]() -> PyObject* {
+    at::Tensor out[2] = {as_tensor(a[6], "k"), as_tensor(a[7], "v")};
+    no_gradient({&out[0], &out[1]}, "cache_read");
     const Cache c = as_cache(a[0]);
     const long long rows = PyLong_AsLongLong(a[4]);
     if (PyErr_Occurred()) throw Fail{};
@@ -693,7 +705,6 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!THPDtype_Check(a[5])) fail(PyExc_TypeError, "dtype must be a torch.dtype");
     const at::ScalarType t = ((THPDtype*)a[5])->scalar_type;
     const int dt = dtype_code(t);
-    at::Tensor out[2] = {as_tensor(a[6], "k"), as_tensor(a[7], "v")};
     for (at::Tensor& o : out)
       if (o.defined()) {
         same_device(c, o);
@@ -720,9 +731,10 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 9)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const Cache c = as_cache(a[0]);
     at::Tensor q = as_tensor(a[1], "q"), out = as_tensor(a[8], "out");
     if (!q.defined()) fail(PyExc_TypeError, "q must be a tensor");
+    no_gradient({&q, &out}, "cache_attention");
+    const Cache c = as_cache(a[0]);
     same_device(c, q);
     same_device(c, out);
     check_heads(q, 0, c.c.head_dim, "q");

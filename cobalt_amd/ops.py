@@ -191,6 +191,7 @@ def transcode(pm: PackedMatrix, layout: int, bits=None, group=None, keep=None, t
 
 
 # ------------------------------------------------------------------ the key/value cache held in 4 bits (cache.py)
+# Without a backward pass: a tensor that requires a gradient is refused, except under torch.no_grad().
 def cache_write(cache, k, v, rows) -> None:
     """The rows' keys and values (float16 or bfloat16, [rows, heads, head_dim]) into the cache, rounded to 4 bits per
     group: codes c = rint((x - m) / s) with the fp16 minimum m and scale s of the group, held value m + c s.  Magnitudes above

@@ -144,3 +144,16 @@ def test_ops_refuse_a_cache_on_the_cpu():
     for call in (lambda: ops.cache_write(c, x, x, r), lambda: ops.cache_read(c, r, 2), lambda: ops.cache_attention(c, x, r)):
         with pytest.raises(_lib.CbkError):
             call()
+
+
+def test_ops_refuse_tensors_that_require_a_gradient():
+    c = KVCache(3, 2, 64, page=32, device="cpu")
+    r = c.rows([[0, 1], [2, -1]], [40, 7])
+    x, y = torch.zeros(2, 2, 64, dtype=torch.float16), torch.zeros(2, 2, 64, dtype=torch.float16, requires_grad=True)
+    calls = (lambda: ops.cache_attention(c, y, r), lambda: ops.cache_attention(c, x, r, out=y), lambda: ops.cache_write(c, y, x, r),
+             lambda: ops.cache_write(c, x, y, r), lambda: ops.cache_read(c, r, 2, out=(x, y)))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(_lib.CbkError):             # as any other call: the cache is not on the GPU
+            call()
