@@ -18,6 +18,10 @@ NAME = "cobalt_cache"
 DTYPES = (torch.float16, torch.bfloat16)
 
 
+def _recording() -> bool:
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
 class _Sequences:
     """What the layers of one cache share: the pages, the lengths, and the rows of the step under way."""
 
@@ -30,32 +34,45 @@ class _Sequences:
         self.table = torch.arange(self.pages, dtype=torch.int32, device=device).view(batch, per)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)         # real tokens, padding left out
         self.seen = torch.zeros((), dtype=torch.int64, device=device)            # tokens with the padding
+        self.recorded = False    # a step has been: its replays advance the lengths on the device alone
         self.clear()
 
     def clear(self):
         self.lens.zero_()
         self.seen.zero_()
-        self.steps = 0           # tokens with the padding, as the host has issued them: replays of a graph are not in it
+        self.steps = 0           # `seen` as the host knows it (issued())
         self.pads = [0] * self.batch
         self.rows: Optional[KVRows] = None
         self.mask: Optional[torch.Tensor] = None     # of the step under way, as the first layer got it
         self.first = True                            # that step is the first
 
+    def issued(self) -> int:
+        """Tokens with the padding so far.  Once a step has been recorded an eager one reads them back, which waits for the device;
+        while a step is recorded they are what they were before it."""
+        if self.recorded and not _recording():
+            self.steps = int(self.seen)
+        return self.steps
+
     def begin(self, batch: int, tokens: int, mask: Optional[torch.Tensor]):
         """The rows of a step of `tokens` tokens a sequence, called by the first layer; advances the lengths."""
         if batch != self.batch:
             raise ValueError(f"the cache is for {self.batch} sequences, the step has {batch}")
-        if self.steps + tokens > self.max_len:
-            raise ValueError(f"the cache is for {self.max_len} tokens a sequence, the step ends at {self.steps + tokens}")
-        first = self.steps == 0
+        steps = self.issued()
+        if steps + tokens > self.max_len:
+            raise ValueError(f"the cache is for {self.max_len} tokens a sequence, the step ends at {steps + tokens}")
+        first = steps == 0
         if mask is not None:
-            pads = self._padding(mask, tokens)
+            self._shape(mask, steps + tokens)
+            pads = self._pads(mask)
             if first:
                 self.pads = pads
             elif pads != self.pads:
                 raise ValueError("attention_mask: padding belongs in front of a sequence, in the first call")
         self.mask, self.first = mask, first
-        self.steps += tokens
+        if _recording():
+            self.recorded = True
+        else:
+            self.steps += tokens
         self.seen.add_(tokens)
         self.lens.add_(tokens)
         self.rows = KVRows(self.table, self.lens)
@@ -73,8 +90,8 @@ class _Sequences:
         """The mask of a further layer: a dictionary of masks by kinds of layers reaches them as it is, and all must say the same."""
         if mask is self.mask:
             return
-        if mask is not None:
-            self._shape(mask, self.steps)
+        if mask is not None and (self.mask is None or mask.shape != self.mask.shape):
+            self._shape(mask, self.issued())
         if getattr(mask, "_cobalt_hook", False) and getattr(self.mask, "_cobalt_hook", False):
             return                                                              # both of the one mask the model was called with
         pads = self._pads(mask) if mask is not None else [0] * self.batch if self.first else self.pads
@@ -85,12 +102,8 @@ class _Sequences:
         if mask.dim() != 2 or mask.shape[0] != self.batch or mask.shape[1] != total:
             raise ValueError(f"attention_mask must be [{self.batch}, {total}], got {list(mask.shape)}")
 
-    def _padding(self, mask, tokens):
-        self._shape(mask, self.steps + tokens)
-        return self._pads(mask)
-
     def _pads(self, mask):
-        if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        if mask.is_cuda and _recording():
             raise ValueError("attention_mask is read by the host: a step recorded in a graph takes none (padding of the first call stays left out)")
         real = mask.bool()
         holes = (real[:, :-1] & ~real[:, 1:]).any(1)
@@ -113,7 +126,7 @@ class CobaltCacheLayer(CacheLayerMixin):
     def lazy_initialization(self, key_states, value_states):
         if key_states.shape != value_states.shape:
             raise ValueError(f"keys {list(key_states.shape)} and values {list(value_states.shape)} must have the same shape")
-        if key_states.is_cuda and torch.cuda.is_current_stream_capturing():
+        if key_states.is_cuda and _recording():
             raise RuntimeError("the first call with a new cache makes its pages: it cannot be recorded in a graph")
         self.pool = KVCache(self.sequences.pages, key_states.shape[1], key_states.shape[3], page=self.sequences.page, group=self.group,
                             device=key_states.device)
@@ -130,7 +143,7 @@ class CobaltCacheLayer(CacheLayerMixin):
 
     def get_mask_sizes(self, query_length):
         tokens = query_length if isinstance(query_length, int) else query_length.shape[0]
-        return self.sequences.steps + tokens, 0
+        return self.sequences.issued() + tokens, 0
 
     def get_max_cache_shape(self):
         return self.sequences.max_len
@@ -209,7 +222,7 @@ def _padding_mask(batch_size=1, q_length=1, kv_length=1, q_offset=0, kv_offset=0
         mask._cobalt_hook = True
     if any(_same(mask_function, f) for f in plain):
         return mask
-    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+    if _recording():
         raise ValueError("a mask that a model adds to the causal one is read by the host: such a step cannot be recorded in a graph")
     heads = getattr(config, "num_attention_heads", 1)
     if not any(_answers_alike(mask_function, f, batch_size, heads, q_length, kv_length, q_offset, kv_offset, device) for f in plain):

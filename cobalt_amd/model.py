@@ -401,7 +401,8 @@ def cobalt_cache(model: nn.Module, batch: int, max_len: int, page: int = 64, gro
     bits a value.  Pass it as `past_key_values` to the model or to its `generate` (not with beams); the model's attention
     implementation is switched to it, and `model.set_attn_implementation` switches it back.  Sliding-window layers also see the
     first `sinks` tokens of a sequence.  A batch may be padded in front (2-D `attention_mask`); a step without a mask can be
-    recorded in a graph; its replays go on from the lengths on the device, and past `max_len` write nothing.  `cache.reset()` empties it."""
+    recorded in a graph; its replays go on from the lengths on the device, and past the pages of `max_len` write nothing.  Eager steps may
+    follow them (each then waits for the device to tell the lengths).  `cache.reset()` empties it."""
     from . import hf_cache
     return hf_cache.build(model, batch, max_len, page, group, sinks)
 

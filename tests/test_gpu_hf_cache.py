@@ -133,3 +133,42 @@ def test_generate_runs_and_the_cache_is_reused():
     first = m.generate(ids, past_key_values=cache, **kw)
     cache.reset()
     assert first.shape == (2, 60) and torch.equal(m.generate(ids, past_key_values=cache, **kw), first)
+
+
+def test_eager_steps_after_replays():
+    from cobalt_amd import model as Mo
+    m = _model(torch.float16)
+    ids = torch.randint(0, 512, (2, 60), generator=torch.Generator().manual_seed(4)).to(DEV)
+    mask = lambda n: torch.stack([(torch.arange(n) >= p).long() for p in (0, 9)]).to(DEV)
+    runs = []
+    for recorded in (False, True):
+        cache = Mo.cobalt_cache(m, 2, 64)
+        got = [m(ids[:, :40], past_key_values=cache, attention_mask=mask(40)).logits]
+        tok = ids[:, 40:41].clone()
+        if recorded:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                got.append(m(tok, past_key_values=cache).logits.clone())
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = m(tok, past_key_values=cache).logits
+        else:
+            got.append(m(tok, past_key_values=cache).logits)
+        for i in range(41, 50):
+            tok.copy_(ids[:, i:i + 1])
+            if recorded:
+                graph.replay()
+                got.append(out.clone())
+            else:
+                got.append(m(tok, past_key_values=cache).logits)
+        got.append(m(ids[:, 50:51], past_key_values=cache, attention_mask=mask(51)).logits)     # as generate passes it
+        got.append(m(ids[:, 51:60], past_key_values=cache).logits)
+        assert int(cache.get_seq_length()) == 60 and cache.layers[0].sequences.lens.tolist() == [60, 51]
+        with pytest.raises(ValueError, match="for 64 tokens"):
+            m(ids[:, :5], past_key_values=cache)
+        runs.append(got)
+    for i, (a, b) in enumerate(zip(*runs)):
+        assert torch.equal(a, b), i

@@ -296,3 +296,33 @@ def test_only_the_decoder_of_a_mixed_model_is_switched(exact):
     types = (ids == 90).long()
     with pytest.raises(ValueError, match="this step's mask"):
         m(ids, token_type_ids=types, past_key_values=Mo.cobalt_cache(m, 1, 32), **kw)
+
+
+def test_an_eager_step_after_replays_goes_on_from_the_device(exact, monkeypatch):
+    """A recorded step and its replays advance the lengths on the device, and no count on the host."""
+    m = _model()
+    ids = torch.randint(2, 97, (2, 17), generator=torch.Generator().manual_seed(4))
+    mask = lambda n: torch.stack([(torch.arange(n) >= p).long() for p in (0, 3)])
+    want = m(ids, attention_mask=mask(17)).logits
+    recording = [False]
+    monkeypatch.setattr(hf, "_recording", lambda: recording[0], raising=False)
+    cache = Mo.cobalt_cache(m, 2, 18, page=16)
+    seqs = cache.layers[0].sequences
+    for _ in range(2):
+        m(ids[:, :10], past_key_values=cache, attention_mask=mask(10))
+        recording[0] = True
+        for i in range(10, 14):                                         # what four replays do
+            m(ids[:, i:i + 1], past_key_values=cache)
+            seqs.steps = 10
+        recording[0] = False
+        got = m(ids[:, 14:17], past_key_values=cache, attention_mask=mask(17)).logits
+        assert int(cache.get_seq_length()) == 17 and seqs.lens.tolist() == [17, 14]
+        assert float((got - want[:, 14:]).abs().max()) < ATOL
+        with pytest.raises(ValueError, match="for 18 tokens"):
+            m(ids[:, :2], past_key_values=cache)
+        recording[0] = True
+        m(ids[:, :1], past_key_values=cache)                            # one more replay: no room is left
+        recording[0] = False
+        with pytest.raises(ValueError, match="for 18 tokens"):
+            m(ids[:, :1], past_key_values=cache)
+        cache.reset()                                                   # and anew: replays may follow a reset as well
