@@ -20,6 +20,7 @@
 #include <c10/core/impl/InlineDeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <memory>
+#include <numeric>
 #include "cbk_internal.h"
 
 namespace {
@@ -653,6 +654,29 @@ void check_out(const at::Tensor& o, int64_t rows, int64_t heads, int64_t dim, at
     fail(PyExc_ValueError, std::string(what) + " must have unit stride along head_dim, rows that do not overlap and 16-byte aligned heads");
 }
 
+// Whether two [rows, heads, dim] tensors of one type, unit stride along dim, can be seen to share no byte: their extents are apart, or what
+// repeats every so many bytes in both lies side by side: whole rows (columns of one wider tensor), whole heads, or single heads of a row.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.numel() || !b.numel()) return true;
+  const int64_t size = a.element_size();
+  const uintptr_t pa = (uintptr_t)a.const_data_ptr(), pb = (uintptr_t)b.const_data_ptr();
+  auto span = [&](const at::Tensor& x, bool rows, bool heads) {
+    return size * ((rows ? (x.size(0) - 1) * row_stride(x) : 0) + (heads ? (x.size(1) - 1) * head_stride(x) : 0) + x.size(2));
+  };
+  if (pa + span(a, true, true) <= pb || pb + span(b, true, true) <= pa) return true;
+  auto beside = [&](int64_t every, int64_t in_a, int64_t in_b) {     // (every: in elements, 0 where nothing repeats)
+    every *= size;
+    if (in_a > every || in_b > every) return false;
+    int64_t at = (int64_t)(pb - pa) % every;                        // where b begins behind a piece of a
+    if (at < 0) at += every;
+    return at >= in_a && at + in_b <= every;
+  };
+  const int64_t ra = row_stride(a), rb = row_stride(b), ha = head_stride(a), hb = head_stride(b);
+  return beside(std::gcd(ra, rb), span(a, false, true), span(b, false, true)) ||
+         beside(std::gcd(ha, hb), span(a, true, false), span(b, true, false)) ||
+         beside(std::gcd(std::gcd(ra, rb), std::gcd(ha, hb)), span(a, false, false), span(b, false, false));
+}
+
 // Nothing here has a backward pass: a gradient that would be lost is an error, as it is for torch's own operators with an output given.
 void no_gradient(std::initializer_list<const at::Tensor*> ts, const char* what) {
   if (!c10::GradMode::is_enabled()) return;
@@ -710,8 +734,8 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         same_device(c, o);
         check_out(o, rows, c.c.heads, c.c.head_dim, t, "the output");
       }
-    if (rows && out[0].defined() && out[1].defined() && out[0].const_data_ptr() == out[1].const_data_ptr())
-      fail(PyExc_ValueError, "keys and values need an output each");
+    if (out[0].defined() && out[1].defined() && !apart(out[0], out[1]))
+      fail(PyExc_ValueError, "keys and values need an output each: these overlap");
     int rc = CBK_OK;
     {
       const GilRelease other_threads_run;
@@ -743,7 +767,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (heads % c.c.heads)
       fail(PyExc_ValueError, std::to_string(heads) + " query heads are no multiple of the cache's " + std::to_string(c.c.heads));
     if (out.defined()) check_out(out, q.size(0), heads, c.c.head_dim, q.scalar_type(), "out");
-    if (out.defined() && q.size(0) && out.const_data_ptr() == q.const_data_ptr()) fail(PyExc_ValueError, "out must not overlap q");
+    if (out.defined() && readable16(q) && !apart(out, q)) fail(PyExc_ValueError, "out must not overlap q");   // (any other q is copied first)
     const RowMap m = as_rows(c, a[2], a[3], a[4], q.size(0));
     const double scale = PyFloat_AsDouble(a[5]);
     const long long window = PyLong_AsLongLong(a[6]), sinks = PyLong_AsLongLong(a[7]);

@@ -715,3 +715,62 @@ def s_mean(s, r, h, n):
     b = r // n
     v = s.hv[s.cut[b]:s.cut[b + 1] - n + r % n + 1, h // 4]
     return torch.from_numpy(v.mean(0)).to(s.dtype)
+
+
+def _bytes_of(x):
+    """The addresses of a tensor's elements, in elements of its storage."""
+    at = x.storage_offset()
+    for n, step in zip(x.shape, x.stride()):
+        at = (np.asarray(at)[..., None] + np.arange(n) * step)
+    return set(at.reshape(-1).tolist())
+
+
+def test_outputs_that_overlap_in_part_are_refused():
+    """Views of one buffer as query and output, and as the two outputs of a read: wherever they share a byte the call is refused, and
+    columns, planes and pieces of one tensor that do not are taken."""
+    s = Setup([20, 30], 2, 64, 16, 32, torch.float16)
+    n, r = 6, s.rows([3, 3])
+    buf = torch.zeros(8 * n * 2 * 64, device=DEV).half()
+    view = lambda at, rs, hs: buf[at:].as_strided((n, 2, 64), (rs, hs, 1), at)
+    want = ops.cache_read(s.cache, r, n)
+
+    def both(a, b):
+        share = bool(_bytes_of(a) & _bytes_of(b))
+        try:
+            ops.cache_read(s.cache, r, n, out=(a, b))
+            taken = True
+            assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+        except ValueError as e:
+            assert "overlap" in str(e)
+            taken = False
+        x = torch.randn(n, 2, 64, device=DEV).half()
+        a.copy_(x)
+        try:
+            ops.cache_attention(s.cache, a, r, out=b)
+            assert torch.equal(b, ops.cache_attention(s.cache, x, r))
+            assert taken
+        except ValueError as e:
+            assert "overlap" in str(e) and not taken
+        assert not (share and taken)
+        return taken
+
+    for a, b, ok in (((0, 128, 64), (128, 128, 64), False),             # a row further on
+                     ((0, 128, 64), (64, 128, 64), False), ((128, 128, 64), (0, 128, 64), False), ((0, 128, 64), (0, 128, 64), False),
+                     ((0, 128, 64), (n * 128, 128, 64), True), ((n * 128, 128, 64), (0, 128, 64), True),      # one behind the other
+                     ((0, 256, 64), (128, 256, 64), True), ((128, 256, 64), (0, 256, 64), True),              # columns of one row
+                     ((0, 256, 64), (64, 256, 64), False), ((0, 256, 128), (64, 256, 128), True),             # heads in turn
+                     ((0, 256, 64), (3 * 256 + 128, 256, 64), True), ((3 * 256, 256, 64), (0, 256, 64), False),
+                     ((0, 64, n * 64), (2 * n * 64, 64, n * 64), True), ((0, 64, 2 * n * 64), (n * 64, 64, 2 * n * 64), True),   # planes
+                     ((0, 64, 2 * n * 64), (n * 64 - 64, 64, 2 * n * 64), False), ((0, 128, 64), (64, 64, n * 64), False)):
+        assert both(view(*a), view(*b)) == ok, (a, b)
+    g = np.random.default_rng(3)
+    taken = 0
+    for _ in range(60):                                                 # and drawn ones
+        def one():
+            if g.random() < 0.5:
+                hs = int(g.choice([64, 72, 128]))
+                return view(int(g.integers(0, 60)) * 8, int(g.choice([hs + 64, 256, 384])), hs)
+            rs = int(g.choice([64, 72, 128]))
+            return view(int(g.integers(0, 60)) * 8, rs, int(g.choice([(n - 1) * rs + 64, 1024])))
+        taken += both(one(), one())
+    assert taken
