@@ -52,5 +52,14 @@ class KVCache:
 
     def rows(self, table, lens, starts=None) -> KVRows:
         """KVRows of lists or tensors of any integer type, on this cache's device."""
-        as_ints = lambda t: None if t is None else torch.as_tensor(t).to(self.device, torch.int32).contiguous()
-        return KVRows(as_ints(table), as_ints(lens), as_ints(starts))
+        def as_ints(t, name):
+            if t is None:
+                return None
+            t = torch.as_tensor(t)
+            if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+                if t.numel():                                       # (an empty list makes a float tensor)
+                    raise TypeError(f"{name} must be integers, not {t.dtype}")
+            elif t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+                t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)      # a larger one stays large: no page, no row
+            return t.to(self.device, torch.int32).contiguous()
+        return KVRows(as_ints(table, "table"), as_ints(lens, "lens"), as_ints(starts, "starts"))

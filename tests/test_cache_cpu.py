@@ -157,3 +157,20 @@ def test_ops_refuse_tensors_that_require_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(_lib.CbkError):             # as any other call: the cache is not on the GPU
             call()
+
+
+def test_rows_of_integers_that_int32_does_not_hold():
+    c = KVCache(3, 2, 64, page=32, device="cpu")
+    for table in ([[0, 1 << 32], [-(1 << 33), 1]], torch.tensor([[0, 1 << 32], [-(1 << 33), 1]])):
+        r = c.rows(table, [(1 << 32) + 5, 7], torch.tensor([0, 1, 1 << 40]))
+        assert r.table.tolist() == [[0, (1 << 31) - 1], [-(1 << 31), 1]]        # neither is a page of the pool
+        assert r.lens.tolist() == [(1 << 31) - 1, 7] and r.starts.tolist() == [0, 1, (1 << 31) - 1]
+    for t in (torch.int8, torch.int16, torch.uint8, torch.uint16, torch.uint32, torch.int64):
+        assert c.rows(torch.tensor([[0, 2]], dtype=t), torch.tensor([100], dtype=t)).table.tolist() == [[0, 2]]
+    for bad in ([[0.5, 1.0]], torch.zeros(1, 2), torch.zeros(1, 2, dtype=torch.bool)):
+        with pytest.raises(TypeError, match="table must be integers"):
+            c.rows(bad, [3])
+    with pytest.raises(TypeError, match="lens must be integers"):
+        c.rows([[0, 1]], [3.7])
+    r = c.rows(torch.zeros(0, 2, dtype=torch.int32), [], [0])
+    assert r.lens.dtype == torch.int32 and r.lens.shape == (0,)
