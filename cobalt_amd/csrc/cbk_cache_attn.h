@@ -115,12 +115,13 @@ __device__ inline v2h rest_of(v2h rounded, float e0, float e1) {
 }
 
 // Power of two that a query row is divided by, and `down`, its reciprocal, for a largest magnitude `top`: 1 if the row (and sums of
-// 128 of its elements) is an ordinary fp16 row without it, else one that leaves [1, 2).  Also 1 for zeros, infinities and NaN.
+// 128 of its elements) is an ordinary fp16 row without it, else one that leaves [1, 2).  Also 1 for zeros and NaN.  An infinity makes the whole
+// row NaN (`down` is): products that are -inf alone would leave a row without weights, which is a row that saw nothing.
 __device__ inline float row_factor(float top, float& down) {
   int e = 0;
   if (!(top >= 0x1p-6f && top < 0x1p8f) && top > 0.f && top < __builtin_inff())
     e = min(max((int)(__float_as_uint(top) >> 23), 1) - 127, 126);  // (e = 127 would need 2^-127, which is no normal number: [2, 4) then)
-  down = __uint_as_float((uint32_t)(127 - e) << 23);
+  down = top < __builtin_inff() ? __uint_as_float((uint32_t)(127 - e) << 23) : __builtin_nanf("");
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 __device__ inline float bits_top(const v4u& w, bool bf, float top) {  // the largest magnitude of eight numbers and top; a NaN or infinity gives one

@@ -206,6 +206,47 @@ def test_what_stands_behind_the_last_token_does_not_matter(dim, dtype, plan):
     assert torch.equal(a, ops.cache_attention(s.cache, q, rows))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("plan", ["whole", "cut"])
+def test_queries_that_are_no_numbers_stay_alone(dtype, plan):
+    s = Setup([1300, 1200], 4, 128, 64, 32, dtype, seed=3)
+    new = [1300, 1200] if plan == "whole" else [400, 500]
+    q = torch.randn(sum(new), 16, 128, generator=torch.Generator().manual_seed(2)).to(dtype)
+    bad = [(1, 3), (2, 5), (new[0], 0), (300, 15), (350, 15)]
+    for (r, h), x in zip(bad, (float("nan"), float("inf"), float("-inf"), float("inf"), float("-inf"))):
+        q[r, h, 7 * h] = x
+    q = q.to(DEV)
+    rows = rows_of(s, new, 1300 if plan == "whole" else 8000)
+    assert plan_of(s, rows, sum(new), 16) == plan
+    out = ops.cache_attention(s.cache, q, rows)
+    for r, h in bad:
+        assert bool(out[r, h].isnan().all())
+    clean = q.clone()
+    for r, h in bad:
+        clean[r, h] = 0
+    check(s, clean, out, new, skip=bad)
+    assert not bool(ops.cache_attention(s.cache, q, rows._replace(lens=torch.zeros_like(rows.lens))).any())      # and nothing is seen: 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("plan", ["few", "whole"])
+def test_an_infinite_query_over_keys_of_one_sign(dtype, plan):
+    """Scores that are all infinite have no softmax, whatever their sign."""
+    s = Setup([1290], 4, 128, 64, 32, dtype, seed=3, fill=lambda s: s.k[:, :, 5].abs_().add_(1))
+    n = 4 if plan == "few" else 1290
+    q = torch.randn(n, 16, 128, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    bad = [(0, 0), (1, 3), (3, 14)]
+    for (r, h), x in zip(bad, (float("-inf"), float("inf"), float("-inf"))):
+        q[r, h, 5] = x
+    rows = rows_of(s, [n], 1290)
+    assert plan_of(s, rows, n, 16) == plan
+    out = ops.cache_attention(s.cache, q, rows)
+    for r, h in bad:
+        assert bool(out[r, h].isnan().all())
+        q[r, h] = 0
+    check(s, q, out, [n], skip=bad)
+
+
 # ------------------------------------------------------------------ scores
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("dim,group", [(64, 32), (128, 64), (256, 128)])
