@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
         for (int k = 0; k < KS; ++k) q_sh[k * 64 + lane] = q[k];
       __syncthreads();
     }
-    cs = fmaxf(cs, 1e-30f);         // (a smaller one has every score at 0; a masked one stays -inf)
+    cs = fminf(fmaxf(cs, 1e-30f), 0x1.fffffep127f);                 // (a smaller one has every score at 0, a larger one every difference past any weight; a masked one stays -inf)
     v4f o[TILES];
     float m, l;
     m = FLOOR; l = 0.f;

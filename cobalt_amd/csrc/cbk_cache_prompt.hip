@@ -160,7 +160,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       top = bits_top(raw[k], BF, top);
     }
     top = fmaxf(top, __shfl_xor(top, 32));
-    grow = row_factor(BF ? top * fold : top, down) * (a.scale / fold);
+    const float size = BF && top < __builtin_inff() ? fminf(top * fold, 0x1.fffffep127f) : top;   // (of what `times` leaves)
+    grow = row_factor(size, down) * (a.scale / fold);
     const float times = BF ? fold : 1.f;
 #pragma unroll
     for (int k = 0; k < T::KS; ++k)

@@ -319,6 +319,29 @@ def test_large_scores_that_rise_and_fall(dim, dtype):
             assert bool(torch.isfinite(out[:, h]).all())
 
 
+@pytest.mark.parametrize("plan", ["few", "cut"])
+@pytest.mark.parametrize("size,scale,unit", [(30, 1e30, -14), (100, 1.0, -14), (-30, 1e30, 0), (126, 1e-30, 0), (127, 1.0, -14)])
+def test_large_queries_times_large_scales(size, scale, unit, plan):
+    """bf16 queries of 2^size whose product with the scale may pass float32, over keys that bring the scores back into it."""
+    s = Setup([1300], 4, 128, 64, 32, BF16, fill=lambda s: s.k.copy_((torch.arange(1300) % 16 * 2.0 ** unit).to(BF16)[:, None, None].expand_as(s.k)))
+    n = 4 if plan == "few" else 600
+    q = torch.zeros(n, 16, 128)
+    q[:, :, 40] = 2.0 ** size
+    rows = rows_of(s, [n], 1300 if plan == "few" else 8000)
+    assert plan_of(s, rows, n, 16) == plan
+    out = ops.cache_attention(s.cache, q.bfloat16().to(DEV), rows, scale=scale)
+    key = torch.arange(1300, device=DEV) % 16
+    seen = torch.arange(1300, device=DEV)[None, :] <= torch.arange(1300 - n, 1300, device=DEV)[:, None]
+    w = (seen & (key[None, :] == 15)).double()                      # the largest alone: the others lie far below
+    w = w / w.sum(1, keepdim=True)
+    for h in range(16):
+        v = torch.from_numpy(s.hv[:, h // 4].copy()).to(DEV)
+        o = w @ v
+        tol = (U + 2.0 ** -16 + 1400 * 2.0 ** -23) * (w @ v.abs())
+        tol = tol + HALF[BF16] * (o.abs() + tol) + 2.0 ** -25
+        assert bool(((out[:, h].double() - o).abs() <= tol).all())
+
+
 # ------------------------------------------------------------------ what fp16 calls promise
 def _whole_numbers(s):
     """Values from -8 to 7, which are held as they are."""
