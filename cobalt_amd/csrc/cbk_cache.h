@@ -71,6 +71,12 @@ __device__ inline int page_of(const DCache& c, const DRows& r, int b, int pos) {
   return p >= 0 && p < c.pages ? p : -1;
 }
 
+// A float32 result that is rounded again: without the barrier the compiler takes one instruction that rounds the exact value to fp16.
+__device__ inline float as_float32(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // ------------------------------------------------------------------ codes to fp16
 // The low four bits of each half of a dword (hi: the next four) under the exponent of 2^10 (2^6) are the numbers 1024 + c
 // (64 + c), and the difference is c, exactly.  One instruction masks and sets the exponent if the exponent is in a vector register: a

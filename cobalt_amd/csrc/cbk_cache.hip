@@ -84,12 +84,6 @@ __device__ inline float over_lanes(float x, F f) {
   return x;
 }
 
-// A float32 result that is rounded again: without the barrier the compiler takes one instruction that rounds the exact value to fp16.
-__device__ inline float as_float32(float x) {
-  asm("" : "+v"(x));
-  return x;
-}
-
 template <int DT>
 __device__ inline void unpack8(const v4u q, float (&x)[8]) {
 #pragma unroll

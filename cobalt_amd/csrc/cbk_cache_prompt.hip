@@ -33,6 +33,8 @@ namespace cbk {
 constexpr int WAVES = 8, ROWS = 32 * WAVES;
 constexpr int OWN = 2;                      // tiles of tokens that a tile of rows counts for by itself: its queries, its start and end (six ragged
                                             // chunks: none 470 us, 1: 445, 2: 433, 4: 431; a prompt of 8192 tokens, cut: 774, 669, 631, 631)
+constexpr float REST = 2048.f;              // What the first fp16 leaves of a sum of q is kept this many times as large, and meets minima that many times smaller: with a small
+                                            // scale in it the rest has no digits as an fp16 (2^-25 of a minimum of 60000 is 2e-3 of a score; now 2^-36, and 2^-25 of the sum)
 constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
 
 template <int D, int G, bool BF>
@@ -183,9 +185,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
       for (int k = g * T::GP; k < (g + 1) * T::GP; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += (float)q[k][i];
-      sum = (sum + __shfl_xor(sum, 32)) * fold;
+      sum = as_float32((sum + __shfl_xor(sum, 32)) * fold);         // (rounded one way for both: their first halves have to be the same)
       const _Float16 hi = (_Float16)sum;
-      if (half == g / 4) { qm[2 * (g % 4)] = hi; qm[2 * (g % 4) + 1] = (_Float16)(sum - (float)hi); }
+      if (half == g / 4) { qm[2 * (g % 4)] = hi; qm[2 * (g % 4) + 1] = (_Float16)((sum - (float)hi) * REST); }
     }
   }
   // Scores start from `start`, P_BITS less the running maximum, so that a sum is p's exponent as it leaves the product.  Rows with
@@ -262,7 +264,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
         if (h4 < T::UG) {
           const int g = T::UG * chunk + h4, key = 16 * sb + c16;
           uint8_t* const mins = buf + T::K_BYTES + T::V_BYTES;
-          *(uint32_t*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = __builtin_amdgcn_perm(meta[u][0], meta[u][0], 0x03020302u);
+          const _Float16 least = __builtin_bit_cast(v2h, meta[u][0]).y;
+          *(v2h*)(mins + (key >> 5) * 1024 + (g >> 2) * 512 + (key & 31) * 16 + (g & 3) * 4) = v2h{least, least * (_Float16)(1.f / REST)};
           *(float*)(mins + T::M_BYTES + (g * T::KEYS + key) * 4) = h2f((uint16_t)meta[u][0]) * fold;
         }
     } else {

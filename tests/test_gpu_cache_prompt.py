@@ -373,6 +373,60 @@ def test_codes_queries_and_weights_are_not_rounded(dim, group, plan):
         attend(s, [n], 4, span, plan, q=q.half().to(DEV), exact_values=True)
 
 
+def _tie(near):
+    """A scale near the given one and an fp16 number whose product, with log2 e in it, is a tie of fp16 once rounded to float32, and rounds the other way
+    where it is exact."""
+    log2e, f = np.float32(1.44269504088896341), np.float32
+    for i in range(1025, 2048):
+        x = np.float16(2 * i / 1024)
+        for t in range(3, 400, 2):
+            tie = f(near * float(x) * float(log2e)) * (1 + t / 4096)
+            step = 2.0 ** (np.floor(np.log2(tie)) - 10)
+            tie = f((np.floor(tie / step) + 0.5) * step)
+            for scale in (f(float(tie) / float(x) / float(log2e)) * (1 + f(2) ** -23 * f(k)) for k in (-1, 0, 1)):
+                fold = scale * log2e
+                exact = float(fold) * float(x)                      # (24 and 11 bits: exact in float64)
+                if f(exact) == tie and exact != float(tie) and np.float16(f(exact)) != np.float16(exact):
+                    return float(scale), float(x)
+    raise AssertionError
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 32), (256, 128)])
+@pytest.mark.parametrize("plan", ["few", "whole", "cut"])
+def test_a_sum_of_queries_that_is_a_tie(dim, group, plan):
+    """The sum of a query over a group times the scale goes into two fp16: the second has to be the rest of the very first, also where that could be
+    rounded either way.  Keys whose minima are large and whose product with the query is small show a step of it."""
+    scale, x = _tie(dim ** -0.5)
+
+    def fill(s):
+        low = -200 * torch.rand(s.k.shape[0], s.heads, 1, generator=torch.Generator().manual_seed(4))
+        s.k[:] = (low * torch.rand(s.k.shape, generator=torch.Generator().manual_seed(5))).half()
+        s.k.view(s.k.shape[0], s.heads, -1, s.group)[..., 3:4] = low.half()[..., None]
+        s.k.view(s.k.shape[0], s.heads, -1, s.group)[..., 9] = 0
+        _whole_numbers(s)
+    n = {"few": 24, "whole": 1290, "cut": 300}[plan]
+    s = Setup([n], 4, dim, 64, group, F16, fill=fill)
+    q = torch.zeros(n, 16, dim)
+    q.view(n, 16, -1, group)[..., 9] = x
+    q[:, ::3, 9] = -x
+    attend(s, [n], 4, {"few": 1100, "whole": n, "cut": 16384}[plan], plan, q=q.half().to(DEV), scale=scale, exact_values=True)
+
+
+@pytest.mark.parametrize("scale", [1e-8, 1e-6, 1e-4, 0.01, 0.1, 1.3])
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 32), (128, 128), (256, 32)])
+@pytest.mark.parametrize("plan", ["few", "cut"])
+def test_small_scales_over_large_keys(dim, group, scale, plan):
+    """Scores that a small scale brings down from large keys: the minima are as large as the keys, and the scale must not cost their sums a digit."""
+    def fill(s):
+        g = torch.Generator().manual_seed(1)
+        s.k[:] = (torch.randn(s.k.shape, generator=g) * 20000 * torch.rand(s.k.shape[0], s.heads, 1, generator=g)).clamp(-60000, 60000).half()
+        _whole_numbers(s)
+    s = Setup([300], 4, dim, 64, group, F16, fill=fill)
+    n = 24 if plan == "few" else 300
+    q = (torch.randn(n, 16, dim, generator=torch.Generator().manual_seed(2)) * min(0.02, 1e-4 / scale)).half().to(DEV)
+    attend(s, [n], 4, 1100 if plan == "few" else 16384, plan, q=q, scale=scale, exact_values=True)
+
+
 def test_a_call_of_many_rows_among_recorded_ones():
     """As it is against the definition, and the same from a graph whose pool a call of few rows shares."""
     s = Setup([5000, 2600], 4, 128, 64, 32, F16, seed=21)
