@@ -169,8 +169,9 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
         raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
     if query.requires_grad or key.requires_grad or value.requires_grad:
         raise RuntimeError("the 4-bit cache has no backward pass: call the model under torch.no_grad()")
-    if query.dtype not in DTYPES:                                    # (before the lengths advance)
-        raise TypeError(f"the 4-bit cache is for float16 and bfloat16 models, not {query.dtype}")
+    types = {x.dtype for x in (query, key, value)}
+    if len(types) > 1 or not types <= set(DTYPES):                   # (before the lengths advance)
+        raise TypeError(f"the 4-bit cache is for float16 and bfloat16 models, not {', '.join(sorted(map(str, types)))}")
     batch, _, tokens, _ = query.shape
     window = sliding_window or layer.window                          # (models that leave it to their mask do not pass one)
     if layer.index == 0:

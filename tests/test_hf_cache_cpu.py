@@ -326,3 +326,14 @@ def test_an_eager_step_after_replays_goes_on_from_the_device(exact, monkeypatch)
         with pytest.raises(ValueError, match="for 18 tokens"):
             m(ids[:, :1], past_key_values=cache)
         cache.reset()                                                   # and anew: replays may follow a reset as well
+
+
+def test_values_of_another_type_are_refused_before_the_lengths_advance(exact):
+    m = _model()
+    cache = Mo.cobalt_cache(m, 1, 16)
+    ids = torch.arange(2, 8)[None]
+    m(ids, past_key_values=cache)
+    m.model.layers[0].self_attn.v_proj.register_forward_hook(lambda mod, args, out: out.float())
+    with pytest.raises(TypeError, match="float16"):
+        m(ids[:, :1], past_key_values=cache)
+    assert int(cache.get_seq_length()) == 6 and cache.layers[0].sequences.lens.tolist() == [6]
