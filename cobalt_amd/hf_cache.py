@@ -34,17 +34,26 @@ class _Sequences:
         self.table = torch.arange(self.pages, dtype=torch.int32, device=device).view(batch, per)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)         # real tokens, padding left out
         self.seen = torch.zeros((), dtype=torch.int64, device=device)            # tokens with the padding
+        self.waiting = False     # a layer has handed on its keys and values, which its attention has not taken yet
         self.recorded = False    # a step has been: its replays advance the lengths on the device alone
         self.clear()
 
     def clear(self):
         self.lens.zero_()
         self.seen.zero_()
+        self.waiting = False
         self.steps = 0           # `seen` as the host knows it (issued())
         self.pads = [0] * self.batch
         self.rows: Optional[KVRows] = None
         self.mask: Optional[torch.Tensor] = None     # of the step under way, as the first layer got it
         self.first = True                            # that step is the first
+
+    def attended(self):
+        """Refuses a model some of whose layers attend by themselves, over what `update` gives them: the step's own keys and values."""
+        if self.waiting:
+            self.waiting = False
+            raise RuntimeError('a layer that uses the 4-bit cache has not called the attention "cobalt_cache": the model does not take it, or its '
+                               "attention was switched back while the cache is in use")
 
     def issued(self) -> int:
         """Tokens with the padding so far.  Once a step has been recorded an eager one reads them back, which waits for the device;
@@ -135,6 +144,8 @@ class CobaltCacheLayer(CacheLayerMixin):
     def update(self, key_states, value_states, *args, **kwargs):
         if self.pool is None:
             self.lazy_initialization(key_states, value_states)
+        self.sequences.attended()
+        self.sequences.waiting = True
         key_states._cobalt_layer = self
         return key_states, value_states
 
@@ -164,6 +175,7 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
     layer = getattr(key, "_cobalt_layer", None)
     if layer is None:
         raise ValueError('attention "cobalt_cache" needs a cache of model.cobalt_cache as past_key_values')
+    layer.sequences.waiting = False
     if dropout or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None or not getattr(module, "is_causal", True) \
             or kwargs.get("is_causal") is False:
         raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
@@ -245,5 +257,8 @@ def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) ->
     seqs = _Sequences(batch, max_len, page, next(model.parameters()).device)
     window = lambda kind: getattr(cfg, "sliding_window", None) if kind == "sliding_attention" else None
     cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, window(kind), sinks) for i, kind in enumerate(types)])
-    (model.get_decoder() or model).set_attn_implementation(NAME)       # (a vision tower of the same model keeps its own)
+    decoder = model.get_decoder() or model                              # (a vision tower of the same model keeps its own)
+    decoder.set_attn_implementation(NAME)
+    if decoder.config._attn_implementation != NAME:
+        raise ValueError(f"{type(decoder).__name__} has an attention of its own that cannot be switched: no 4-bit cache for it")
     return cache

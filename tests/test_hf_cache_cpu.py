@@ -337,3 +337,30 @@ def test_values_of_another_type_are_refused_before_the_lengths_advance(exact):
     with pytest.raises(TypeError, match="float16"):
         m(ids[:, :1], past_key_values=cache)
     assert int(cache.get_seq_length()) == 6 and cache.layers[0].sequences.lens.tolist() == [6]
+
+
+def test_models_with_an_attention_of_their_own_are_refused(exact):
+    """GPT-J's layers take no other attention function: they would attend over the step's own keys alone."""
+    m = tr.GPTJForCausalLM(tr.GPTJConfig(vocab_size=97, n_embd=128, n_layer=2, n_head=2, rotary_dim=32)).double().eval().requires_grad_(False)
+    with pytest.raises(ValueError, match="cannot be switched"):
+        Mo.cobalt_cache(m, 1, 16)
+
+
+def test_a_step_whose_layers_attend_otherwise_is_refused(exact):
+    m = _model()
+    ids = torch.arange(2, 8)[None]
+    cache = Mo.cobalt_cache(m, 1, 32)
+    m(ids, past_key_values=cache)
+    m.set_attn_implementation("sdpa")                                   # switched back, and the cache passed on all the same
+    with pytest.raises(RuntimeError, match="switched back"):
+        m(ids[:, :1], past_key_values=cache)
+    one = _model(layers=1)                                              # with a single layer the next call tells
+    cache = Mo.cobalt_cache(one, 1, 32)
+    one.set_attn_implementation("sdpa")
+    one(ids, past_key_values=cache)
+    with pytest.raises(RuntimeError, match="switched back"):
+        one(ids, past_key_values=cache)
+    cache.reset()
+    one.set_attn_implementation("cobalt_cache")
+    one(ids, past_key_values=cache)
+    assert int(cache.get_seq_length()) == 6
