@@ -16,7 +16,8 @@ class KVRows(NamedTuple):
     last of them is its token lens[b] - 1.  Token j of sequence b is on page table[b, j // page].
 
     All three are int32 tensors on the cache's device and are read when the kernels run: nothing here is copied to the host,
-    and a call recorded in a graph follows them.  A table entry outside the pool (-1) is a page that is not there."""
+    and a call recorded in a graph follows them; they must not change while it runs.  A table entry outside the pool (-1) is a page
+    that is not there."""
     table: torch.Tensor
     lens: torch.Tensor
     starts: Optional[torch.Tensor] = None

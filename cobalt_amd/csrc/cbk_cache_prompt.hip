@@ -19,8 +19,8 @@
 // of a tile that it does not finish is joined by the second launch of cbk_cache_attn.hip.
 //
 // A 4096-token prompt of 32 query heads on 8, 128 channels, bf16: 170 us, 810 TFLOP/s; 8192 tokens 590 us, 930 (a large library product
-// reaches 1210); fp16, with its half more of products, 850 to 1045 us by the group.  64 channels 815 us (bf16) and 1180 (fp16) for twice the heads, whose bound
-// is the vector unit: an exponential and five instructions a score.  Matrix unit busy 36 %, vector unit 46 %; the bare loop
+// reaches 1210); fp16, with its half more of products, 860 to 1040 us by the group.  64 channels 815 us (bf16) and 1190 (fp16; groups of 32: 1350) for twice the
+// heads, whose bound is the vector unit: an exponential and five instructions a score.  Matrix unit busy 36 %, vector unit 46 %; the bare loop
 // of products would take 104 of the 170 us, widening 13 to 35 of them, reads from LDS 31 to 35, exponentials 6 to 9.  256 rows
 // a workgroup, because widening is shared by all rows; two blocks of 64 tokens a barrier (one: 180 us).  Built and not kept: the two
 // halves of the wavefronts a phase apart (200 against 178 us), two workgroups a CU for 64 channels, which spills (1035 against 745).
@@ -515,9 +515,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_prompt_kernel(DCache c, D
 PromptPlan plan_prompt(const DCache& c, const DRows& r, int ratio) {
   PromptPlan p;
   // Whole tiles where there are enough of them or where they are prompts, whose tiles are of all lengths and fill the chip one behind the
-  // other; equal shares where a few tiles stand behind long histories.  128 channels, 8 cache heads of 4 query heads, whole against cut: prompts
-  // of 1024 tokens 45 and 56 us, of 2048 80 and 92, of 4096 187 and 206; the last 512 of 2048 tokens 72 and 55, of 16384 504 and 168; the
-  // last 1024 of 4096 136 and 102; six ragged chunks (630 tiles) 469 and 432; 8 x 1000 of 6000 (1090 tiles) 784 and 797.
+  // other; equal shares where a few tiles stand behind long histories.  128 channels, 8 cache heads of 4 query heads, bf16, whole against cut:
+  // prompts of 1024 tokens 45 and 56 us, of 2048 80 and 88, of 4096 172 and 199; the last 512 of 2048 tokens 73 and 55, of 16384 512 and 173;
+  // the last 1024 of 4096 139 and 103; six ragged chunks (590 tiles) 515 and 507 (64 channels, fp16, 3 query heads: 444 and 380); 8 x 1000 of
+  // 6000 (1060 tiles) 825 and 833.
   const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;   // at most
   const bool prompts = 2 * (int64_t)r.tokens > (int64_t)r.cap * r.seqs;          // most of what the table can hold is new
   p.cut = !prompts && tiles < 3 * CHIP;

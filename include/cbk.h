@@ -291,8 +291,8 @@ typedef struct cbk_cache {
  * sequences packed one behind the other: sequence b owns rows starts[b] .. starts[b+1]-1 (starts NULL: tokens / seqs
  * rows each), and the last of them is its token lens[b] - 1, so lens counts them.  Token j is on page
  * table[b * ld_table + j / page] of the pool.  All of these are DEVICE arrays of int32, read when the kernels
- * run: a recorded call follows them.  Nothing in them can lead outside the arrays: a table entry outside
- * [0, pages), or a token behind the table's last column, is a token the cache does not hold.  A row before
+ * run: a recorded call follows them, and they must not change while it runs.  Nothing in them can lead outside the arrays: a table
+ * entry outside [0, pages), or a token behind the table's last column, is a token the cache does not hold.  A row before
  * starts[0] or behind starts[seqs] belongs to no sequence and stays as it was. */
 typedef struct cbk_rows {
   const void* table;
@@ -321,7 +321,7 @@ int cbk_cache_read(const cbk_cache* cache, const cbk_rows* rows, void* k, int64_
  * or j < sinks.  A row that sees no token is 0.  fp16 or bf16 in and out; scores, their maximum and all sums
  * in float32, operands of the products in fp16.  fp16: exact codes and queries, values rounded once, softmax weights as two
  * fp16.  bf16: keys, values, softmax weights and queries (with the scale in them) may each be rounded once to fp16, an eighth of
- * the result's own step.  scale in [1e-30, 1e30], scores in the range of float32, q_heads at most 256 heads; out must not overlap q.  The result is the same from call to call, also on
+ * the result's own step.  A query with an infinity or a NaN gives NaN where it sees a token.  scale in [1e-30, 1e30], scores in the range of float32, q_heads at most 256 heads; out must not overlap q.  The result is the same from call to call, also on
  * another workspace.  The workspace holds nothing between calls and needs no clearing:
  * cbk_cache_attention_workspace_bytes(), 256-byte aligned, one per call in flight. */
 size_t cbk_cache_attention_workspace_bytes(const cbk_cache* cache, const cbk_rows* rows, int q_heads);
