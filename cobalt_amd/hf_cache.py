@@ -175,7 +175,7 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
     layer = getattr(key, "_cobalt_layer", None)
     if layer is None:
         raise ValueError('attention "cobalt_cache" needs a cache of model.cobalt_cache as past_key_values')
-    layer.sequences.waiting = False
+    fresh, layer.sequences.waiting = layer.sequences.waiting, False    # (not fresh: a layer that shares the keys and values of an earlier one)
     if dropout or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None or not getattr(module, "is_causal", True) \
             or kwargs.get("is_causal") is False:
         raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
@@ -186,12 +186,13 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
         raise TypeError(f"the 4-bit cache is for float16 and bfloat16 models, not {', '.join(sorted(map(str, types)))}")
     batch, _, tokens, _ = query.shape
     window = sliding_window or layer.window                          # (models that leave it to their mask do not pass one)
-    if layer.index == 0:
+    if layer.index == 0 and fresh:
         layer.sequences.begin(batch, tokens, attention_mask)
     else:
         layer.sequences.same_mask(attention_mask)
     as_rows = lambda x: x.transpose(1, 2).reshape(batch * tokens, x.shape[1], x.shape[3])
-    ops.cache_write(layer.pool, as_rows(key), as_rows(value), layer.sequences.rows)
+    if fresh:
+        ops.cache_write(layer.pool, as_rows(key), as_rows(value), layer.sequences.rows)
     out = ops.cache_attention(layer.pool, as_rows(query), layer.sequences.rows, scale=scaling, window=window,
                               sinks=layer.sinks if window else 0)
     return out.view(batch, tokens, query.shape[1], query.shape[3]), None

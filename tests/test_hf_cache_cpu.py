@@ -364,3 +364,21 @@ def test_a_step_whose_layers_attend_otherwise_is_refused(exact):
     one.set_attn_implementation("cobalt_cache")
     one(ids, past_key_values=cache)
     assert int(cache.get_seq_length()) == 6
+
+
+@pytest.mark.parametrize("types,shared", [(["full_attention"] * 2, 1), (["sliding_attention", "full_attention"] * 2, 2)])
+def test_layers_that_share_keys_and_values(exact, types, shared):
+    """The last layers of Gemma 3n attend over what an earlier one has written, the very first among them."""
+    cfg = tr.Gemma3nTextConfig(vocab_size=97, vocab_size_per_layer_input=97, hidden_size=128, intermediate_size=128, hidden_size_per_layer_input=32,
+                               num_hidden_layers=len(types), num_attention_heads=2, num_key_value_heads=1, head_dim=64, max_position_embeddings=512,
+                               sliding_window=6, layer_types=types, num_kv_shared_layers=shared, laurel_rank=8,
+                               activation_sparsity_pattern=[0.0] * len(types), pad_token_id=0)
+    torch.manual_seed(0)
+    m = tr.Gemma3nForCausalLM(cfg).double().eval().requires_grad_(False)
+    ids = torch.randint(2, 97, (2, 20), generator=torch.Generator().manual_seed(0))
+    dense = tr.DynamicCache(config=m.config)
+    want = [m(x, past_key_values=dense).logits for x in (ids[:, :15], ids[:, 15:16], ids[:, 16:])]
+    cache = Mo.cobalt_cache(m, 2, 32)
+    for i, x in enumerate((ids[:, :15], ids[:, 15:16], ids[:, 16:])):
+        assert float((m(x, past_key_values=cache).logits - want[i]).abs().max()) < ATOL, i
+    assert cache.layers[0].sequences.lens.tolist() == [20, 20]
