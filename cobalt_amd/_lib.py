@@ -18,6 +18,20 @@ class CbkCache(ctypes.Structure):
                 ("head_dim", ctypes.c_int32), ("group", ctypes.c_int32)]
 
 
+class CbkCache8(ctypes.Structure):
+    """struct cbk_cache8 (include/cbk.h)"""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("page", ctypes.c_int32), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("block", ctypes.c_int32)]
+
+
+class CbkPages(ctypes.Structure):
+    """struct cbk_pages (include/cbk.h)"""
+    _fields_ = [("table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("lens", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p), ("pages", ctypes.c_int64), ("seqs", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+                ("page", ctypes.c_int32)]
+
+
 class CbkRows(ctypes.Structure):
     """struct cbk_rows (include/cbk.h)"""
     _fields_ = [("table", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("lens", ctypes.c_void_p),
@@ -34,6 +48,7 @@ _DP = ctypes.POINTER(CbkDesc)
 _MM = [_DP, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64, _P, _P,
        ctypes.c_size_t, _P]
 _CP, _RP = ctypes.POINTER(CbkCache), ctypes.POINTER(CbkRows)
+_C8P, _PP = ctypes.POINTER(CbkCache8), ctypes.POINTER(CbkPages)
 _ROWS = [_P, ctypes.c_int64, ctypes.c_int64]                        # a dense tensor: address, strides of rows and heads
 SIGNATURES = {
     "cbk_abi_version": (ctypes.c_int, []),
@@ -63,6 +78,16 @@ SIGNATURES = {
     "cbk_cache_attention_workspace_bytes": (ctypes.c_size_t, [_CP, _RP, ctypes.c_int]),
     "cbk_cache_attention": (ctypes.c_int, [_CP, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                                                       ctypes.c_int, _P, ctypes.c_size_t, _P]),
+    "cbk_cache8_code_bytes": (ctypes.c_size_t, [_C8P]),
+    "cbk_cache8_scale_bytes": (ctypes.c_size_t, [_C8P]),
+    "cbk_cache8_write": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache8_read": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache8_attention_workspace_bytes": (ctypes.c_size_t, [_C8P, _RP, ctypes.c_int]),
+    "cbk_cache8_attention": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                                                       ctypes.c_int, _P, ctypes.c_size_t, _P]),
+    "cbk_cache_pages_workspace_bytes": (ctypes.c_size_t, [_PP]),
+    "cbk_cache_pages": (ctypes.c_int, [_PP, _P, _P, _P, ctypes.c_size_t, _P]),
+    "cbk_cache_slots": (ctypes.c_int, [_RP, ctypes.c_int64, ctypes.c_int, _P, _P, _P]),
 }
 ACT_CODE = {"gelu_tanh": 0, "silu": 1}
 

@@ -15,7 +15,7 @@ SOURCES = ["cbk_api.hip", "cbk_dequant.hip", "cbk_gemv_generic.hip", "cbk_gemv.h
            "cbk_gemm_big_b2.hip", "cbk_gemm_big_b3.hip", "cbk_gemm_big_b4.hip", "cbk_gemm_big_b6.hip"] + [
            f"cbk_gemm_big_b{b}_t{t}.hip" for b in (2, 3, 4) for t in (1, 2, 4)] + ["cbk_act.hip", "cbk_pack.hip", "cbk_gemm_skinny.hip", "cbk_gemm_skinny_b2.hip",
            "cbk_gemm_skinny_b3.hip", "cbk_gemm_skinny_b4.hip", "cbk_gemm_skinny_b68.hip", "cbk_cache.hip", "cbk_cache_attn.hip", "cbk_cache_prompt.hip",
-           "cbk_cache_api.hip"]
+           "cbk_cache_api.hip", "cbk_cache8.hip", "cbk_cache8_attn.hip", "cbk_cache8_prompt.hip", "cbk_cache8_api.hip", "cbk_pages.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-std=c++17",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wno-unused-command-line-argument", "-Wno-inline-asm"]
@@ -84,7 +84,7 @@ VALU_TO_MFMA = 2                                                       # a vecto
 VALU_TO_VMEM = 5                                                       # a scalar register written by a vector instruction -> a memory instruction reads it
 # Kernels whose products the compiler has placed among its own instructions: it also adds to sums that stand in other registers than the
 # result, or reuses those of sums that the next product takes over, which the hardware keeps in order.  Operands still have to wait.
-COMPILED = ("cache_attn_kernel", "cache_prompt_kernel")
+COMPILED = ("cache_attn_kernel", "cache_prompt_kernel", "cache8_attn_kernel", "cache8_prompt_kernel")
 _REG = re.compile(r"(?<![\w])([vas])(?:(\d+)\b|\[(\d+):(\d+)\])")
 _TARGET = re.compile(r"<(\S+?)(?:\+0x([0-9a-f]+))?>$")
 

@@ -1,5 +1,7 @@
-"""The key/value cache held in 4 bits: a pool of pages (`KVCache`) and the description of whose tokens the rows of a
-call are (`KVRows`).  Written, read and attended over by `ops.cache_write`, `ops.cache_read` and `ops.cache_attention`."""
+"""The key/value cache held in 4 or in 8 bits: pools of pages (`KVCache`, `KVCache8`), the description of whose tokens the rows of a
+call are (`KVRows`), and the tables of which page belongs to which sequence (`KVPages`).  Pools are written, read and attended over by
+`ops.cache_write`, `ops.cache_read` and `ops.cache_attention`; tables follow the lengths that requests ask for with `ops.cache_pages`,
+and `ops.cache_slots` tells where the rows of a step go."""
 from __future__ import annotations
 
 import ctypes
@@ -23,33 +25,10 @@ class KVRows(NamedTuple):
     starts: Optional[torch.Tensor] = None
 
 
-class KVCache:
-    """A pool of `pages` pages of `page` tokens for `heads` key/value heads of `head_dim` channels, in groups of `group`
-    channels with an fp16 scale and minimum each: 4 + 32 / group bits a value.
-
-    page: 16, 32, 64, 128 or 256 tokens; head_dim: 64, 128 or 256; group: 32, 64 or 128, at most head_dim.  Which
-    page belongs to which sequence is the caller's business (`KVRows.table`)."""
-
-    def __init__(self, pages: int, heads: int, head_dim: int, page: int = 64, group: int = 32, device="cuda"):
-        self.pages, self.page, self.heads, self.head_dim, self.group = int(pages), int(page), int(heads), int(head_dim), int(group)
-        d = _lib.CbkCache(pages=self.pages, page=self.page, heads=self.heads, head_dim=self.head_dim, group=self.group)
-        codes = _lib.lib().cbk_cache_code_bytes(ctypes.byref(d))
-        meta = _lib.lib().cbk_cache_meta_bytes(ctypes.byref(d))
-        if not codes:
-            raise ValueError(f"no cache of {pages} pages of {page} tokens, {heads} heads of {head_dim} channels in groups of {group}: "
-                             "pages >= 1; page 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; group 32, 64 or 128, at most head_dim")
-        self.k_codes, self.v_codes = (torch.zeros(codes, dtype=torch.uint8, device=device) for _ in range(2))
-        self.k_meta, self.v_meta = (torch.zeros(meta, dtype=torch.uint8, device=device) for _ in range(2))
-
+class _Pool:
     @property
     def device(self):
         return self.k_codes.device
-
-    def native(self):
-        return (self.k_codes, self.v_codes, self.k_meta, self.v_meta, self.pages, self.page, self.heads, self.head_dim, self.group)
-
-    def nbytes(self) -> int:
-        return 2 * (self.k_codes.numel() + self.k_meta.numel())
 
     def rows(self, table, lens, starts=None) -> KVRows:
         """KVRows of lists or tensors of any integer type, on this cache's device."""
@@ -64,3 +43,75 @@ class KVCache:
                 t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)      # a larger one stays large: no page, no row
             return t.to(self.device, torch.int32).contiguous()
         return KVRows(as_ints(table, "table"), as_ints(lens, "lens"), as_ints(starts, "starts"))
+
+
+class KVCache(_Pool):
+    """A pool of `pages` pages of `page` tokens for `heads` key/value heads of `head_dim` channels, in groups of `group`
+    channels with an fp16 scale and minimum each: 4 + 32 / group bits a value.
+
+    page: 16, 32, 64, 128 or 256 tokens; head_dim: 64, 128 or 256; group: 32, 64 or 128, at most head_dim.  Which
+    page belongs to which sequence is the caller's business (`KVRows.table`, or a `KVPages` that keeps it)."""
+
+    def __init__(self, pages: int, heads: int, head_dim: int, page: int = 64, group: int = 32, device="cuda"):
+        self.pages, self.page, self.heads, self.head_dim, self.group = int(pages), int(page), int(heads), int(head_dim), int(group)
+        d = _lib.CbkCache(pages=self.pages, page=self.page, heads=self.heads, head_dim=self.head_dim, group=self.group)
+        codes = _lib.lib().cbk_cache_code_bytes(ctypes.byref(d))
+        meta = _lib.lib().cbk_cache_meta_bytes(ctypes.byref(d))
+        if not codes:
+            raise ValueError(f"no cache of {pages} pages of {page} tokens, {heads} heads of {head_dim} channels in groups of {group}: "
+                             "pages >= 1; page 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; group 32, 64 or 128, at most head_dim")
+        self.k_codes, self.v_codes = (torch.zeros(codes, dtype=torch.uint8, device=device) for _ in range(2))
+        self.k_meta, self.v_meta = (torch.zeros(meta, dtype=torch.uint8, device=device) for _ in range(2))
+
+    def native(self):
+        return (self.k_codes, self.v_codes, self.k_meta, self.v_meta, self.pages, self.page, self.heads, self.head_dim, self.group)
+
+    def nbytes(self) -> int:
+        return 2 * (self.k_codes.numel() + self.k_meta.numel())
+
+
+class KVCache8(_Pool):
+    """The same pool in 8 bits: e4m3 codes, and for each `block` consecutive tokens of a head a power of two that scales its keys and one
+    that scales its values: 8 + 32 / (block * head_dim) bits a value.  A block's scale grows with the largest magnitude written to it; the codes
+    of its older tokens follow (a move of the exponent).  With its first token a block begins anew: what it held behind the rows of that call is lost.
+
+    page: 16, 32, 64, 128 or 256 tokens; head_dim: 64, 128 or 256; block: 16, 32, 64, 128 or 256 tokens, at most page."""
+
+    def __init__(self, pages: int, heads: int, head_dim: int, page: int = 64, block: int = 16, device="cuda"):
+        self.pages, self.page, self.heads, self.head_dim, self.block = int(pages), int(page), int(heads), int(head_dim), int(block)
+        d = _lib.CbkCache8(pages=self.pages, page=self.page, heads=self.heads, head_dim=self.head_dim, block=self.block)
+        codes = _lib.lib().cbk_cache8_code_bytes(ctypes.byref(d))
+        if not codes:
+            raise ValueError(f"no cache of {pages} pages of {page} tokens, {heads} heads of {head_dim} channels in blocks of {block} tokens: "
+                             "pages >= 1; page 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; block 16, 32, 64, 128 or 256, at most page")
+        self.k_codes, self.v_codes = (torch.zeros(codes, dtype=torch.uint8, device=device) for _ in range(2))
+        self.scales = torch.zeros(_lib.lib().cbk_cache8_scale_bytes(ctypes.byref(d)), dtype=torch.uint8, device=device)
+
+    def native(self):
+        return (self.k_codes, self.v_codes, self.scales, self.pages, self.page, self.heads, self.head_dim, self.block)
+
+    def nbytes(self) -> int:
+        return 2 * self.k_codes.numel() + self.scales.numel()
+
+
+class KVPages:
+    """Which of a pool's `pages` pages belong to which of `seqs` sequences of up to `max_len` tokens, on the device: `table` [seqs,
+    ceil(max_len / page)] (-1: no page), `lens` [seqs], and the pages that belong to nobody as a stack, free[:count].  All int32; they
+    are written by `ops.cache_pages` only.  One set of tables serves every layer's pool of the same number of pages and tokens a page."""
+
+    def __init__(self, pages: int, seqs: int, max_len: int, page: int = 64, device="cuda"):
+        self.pages, self.page, self.seqs, self.max_len = int(pages), int(page), int(seqs), int(max_len)
+        if self.page not in (16, 32, 64, 128, 256) or not 1 <= self.pages < 1 << 31 or not 1 <= self.seqs < 1 << 24 or not 1 <= self.max_len <= 1 << 30:
+            raise ValueError(f"no tables for {seqs} sequences of {max_len} tokens on {pages} pages of {page}: pages, seqs and max_len are at "
+                             "least 1, page is 16, 32, 64, 128 or 256")
+        self.table = torch.full((self.seqs, -(-self.max_len // self.page)), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(self.seqs, dtype=torch.int32, device=device)
+        self.free = torch.arange(self.pages - 1, -1, -1, dtype=torch.int32, device=device)      # handed out from the end: 0, 1, 2 ...
+        self.count = torch.full((1,), self.pages, dtype=torch.int32, device=device)
+
+    @property
+    def device(self):
+        return self.table.device
+
+    def native(self):
+        return (self.table, self.lens, self.free, self.count, self.pages, self.page)

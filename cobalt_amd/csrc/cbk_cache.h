@@ -64,7 +64,8 @@ __device__ inline Seq seq_of(const DRows& r, int b) {
 }
 
 // page of token `pos` (not negative) of sequence b; -1: the table has none
-__device__ inline int page_of(const DCache& c, const DRows& r, int b, int pos) {
+template <class Pool>
+__device__ inline int page_of(const Pool& c, const DRows& r, int b, int pos) {
   const int i = pos >> c.shift;
   if (i >= r.cols) return -1;
   const int p = ((const __attribute__((address_space(4))) int32_t*)r.table)[(int64_t)b * r.ld + i];   // (never written by a kernel that reads it)

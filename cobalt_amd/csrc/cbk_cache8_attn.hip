@@ -1,0 +1,327 @@
+// Attention over the 8-bit cache for few rows a sequence: single tokens, drafts, the ends of prompts.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c q_i . k_j - M_i),  c = scale log2 e
+//
+// over the tokens j that row i sees, in one pass with running M and sum (float32; the products of p and v are
+// of 16 bits each, see below).  The rows of a sequence that read one cache head (its tokens times the query heads on
+// that head) are the columns of the matrix instructions, 16 at a time: S^T = K Q^T and O^T = V^T P^T.  In both the
+// cache is the left operand and comes straight out of the loads: a lane holds 16 channels a load of one token's key, or four
+// channels of four tokens' values.  The sums of S^T lie in the lanes that P^T wants them in when the tokens of a
+// step are numbered 4h + r of the first and of the second 16, so nothing passes through LDS until a wavefront has done
+// its share.
+//
+// Held values are fp16 numbers, so keys and values are exact as operands: one instruction widens two codes and multiplies them
+// with their block's scale.  Query rows are operands as they are (bf16 of ordinary size is exact in fp16), rows of very large or small
+// numbers after division by a power of two; scores are exact up to float32.  p is kept at 2^7.5 times its size against the running
+// maximum, so that what an fp16 cannot hold lies 2^-31 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
+// bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
+//
+// The tokens of all sequences and heads are one list of units of 128 tokens, cut into equal pieces, one a workgroup;
+// what a workgroup has of a head it does not finish goes to the workspace with its maximum and sum, and a second
+// launch joins the pieces.  Lengths are read on the device: the host knows none of them.
+//
+// Bound by the bytes of the cache where histories are long.
+#include "cbk_cache8.h"
+#include "cbk_cache_attn.h"
+#include "cbk_cache8_attn.h"
+
+namespace cbk {
+
+template <int D>
+struct Held8 {                              // a wavefront's 32 tokens: two sixteens
+  v4u k[2][D / 64], v[2][D / 64];
+  float2 s[2];                              // scales of their keys and values
+};
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_attn_kernel(DCache8 c, DRows r, AttnArgs a) {
+  constexpr int R = 16, KS = D / 32, VU = D / 64, TILES = D / 16;
+  __shared__ float o_sh[4][R][D + 4];
+  __shared__ float m_sh[4][R], l_sh[4][R];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, h4 = lane >> 4;
+
+  // ---- this workgroup's piece of the list
+  auto units = [&](int b) { return units_of(r, a, c.heads, b, R); };
+  const Index list(r.seqs, lane, units);
+  const int64_t total = list.total, pieces = min((int64_t)gridDim.x, total);
+  const int64_t w = blockIdx.x;
+  AttnPiece* const desc = (AttnPiece*)a.ws + w;
+  if (w >= pieces) {
+    if (a.ws && tid == 0) desc->count = 0;
+    return;
+  }
+  const Shares shares(total, pieces);
+  const int64_t begin = shares.begin(w), end = shares.end(w);
+  int64_t base;
+  int b = list.find(begin, base, units);
+  int64_t at = begin;
+  int joined = 0;
+
+  while (at < end) {
+    // ---- one head's tile of rows and the units of it that are this workgroup's
+    const Seq s = seq_of(r, b);
+    const Range g = range_of(s, a);
+    const int rows = s.n * a.ratio, tiles = (rows + R - 1) / R;
+    const int weight = a.whole ? 1 : g.units + EXTRA;
+    const int64_t all = (int64_t)tiles * c.heads * weight;
+    if (at >= base + all) {
+      base += all;
+      if (++b == r.seqs) break;                                     // (there is a next one, unless lengths change under the call)
+      continue;
+    }
+    const int64_t item = quotient(at - base, weight), start = base + item * weight;
+    const int64_t until = min(end, start + weight);
+    const int u0 = a.whole ? 0 : max((int)(at - start) - EXTRA, 0), u1 = a.whole ? g.units : (int)(until - start) - EXTRA;
+    const bool is_first = at == begin;
+    at = until;
+    if (u1 <= u0) continue;                                         // nothing but what the tile counts for by itself
+    const int h = (int)quotient(item, tiles), row0 = (int)(item - (int64_t)h * tiles) * R;
+    const int valid = min(R, rows - row0);
+
+    const int pos_lo = s.pos0 + row0 / a.ratio, pos_hi = s.pos0 + (row0 + valid - 1) / a.ratio;
+
+    const Parts8 part(c, h, D);
+    const uint32_t k_at = col * D + h4 * 16, v_at = h4 * (4 * D) + col * 16;   // of the lane, from a sixteen's first token
+    auto token_of = [&](int u) { return ((u < g.head ? u : u + g.skip) * 4 + wave) * 32; };
+    // Pages of the two sixteens of a step.  Pages of 32 tokens and more hold both
+    const bool one_page = c.page >= 32;
+    auto pages_of = [&](int tok, int (&pg)[2]) {
+      pg[0] = tok < s.held ? page_of(c, r, b, tok) : -1;
+      pg[1] = one_page ? pg[0] : tok + 16 < s.held ? page_of(c, r, b, tok + 16) : -1;
+    };
+    Held8<D> x;
+    // (a page that is not there: page 0, and masked)
+    auto fetch_keys = [&](int tok, const int (&pg)[2]) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t in = (tok + 16 * t) & (c.page - 1);
+        const int page = max(pg[t], 0);
+        const uint8_t* const p = c.kc + (part.code(page) + in * D) + k_at;
+        x.s[t].x = scales8(c, part.scale(page), in).x;
+#pragma unroll
+        for (int j = 0; j < VU; ++j) x.k[t][j] = *(const v4u*)(p + 64 * j);
+      }
+    };
+    auto fetch_values = [&](int tok, const int (&pg)[2]) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t in = (tok + 16 * t) & (c.page - 1);
+        const int page = max(pg[t], 0);
+        const uint8_t* const p = c.vc + (part.code(page) + in * D) + v_at;
+        x.s[t].y = scales8(c, part.scale(page), in).y;
+#pragma unroll
+        for (int j = 0; j < VU; ++j) x.v[t][j] = *(const v4u*)(p + 256 * j);
+      }
+    };
+
+    // keys of the next step are under way while this one's values are worked on, and the other way round
+    int pg[2], pg_next[2];
+    pages_of(token_of(u0), pg);
+    fetch_keys(token_of(u0), pg);
+    fetch_values(token_of(u0), pg);
+    pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
+
+    // ---- queries: fragments, positions and factors
+    v8h q[KS];
+    float cs;
+    Sight sight;
+    const int row = row0 + col;
+    const bool is = col < valid;
+    const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
+    sight = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
+    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
+    v4u raw[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 64 * (k >> 1) + 16 * h4 + 8 * (k & 1)) : v4u{};
+    float top = 0.f, down;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+    top = across_max(top);
+    cs = a.scale * row_factor(top, down);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = raw[k][i];
+        const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+        q[k][2 * i] = (_Float16)(x0 * down);
+        q[k][2 * i + 1] = (_Float16)(x1 * down);
+      }
+    cs = fminf(fmaxf(cs, 1e-30f), 0x1.fffffep127f);                 // (a smaller one has every score at 0, a larger one every difference past any weight; a masked one stays -inf)
+    v4f o[TILES];
+    float m, l;
+    m = FLOOR; l = 0.f;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    for (int u = u0; u < u1; ++u) {
+      const int tok = token_of(u), tok_next = token_of(min(u + 1, u1 - 1));
+      if (tok >= s.held) break;                                     // (of the last unit: nothing follows)
+      const bool p0 = pg[0] >= 0, p1 = pg[1] >= 0;
+      // every row sees all 32 tokens, and all of them are there
+      const bool whole = p0 && p1 && tok + 32 <= s.held && tok + 31 <= pos_lo &&
+                         (a.window <= 0 || tok > pos_hi - a.window || tok + 32 <= a.sinks);
+      v4f sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const v4u w4 = x.k[t][k >> 1];
+          const v8h f = octet8(w4[2 * (k & 1)], w4[2 * (k & 1) + 1], x.s[t].x, x.s[t].x);
+          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], sc[t], 0, 0, 0);
+        }
+      }
+      if (u + 1 < u1) fetch_keys(tok_next, pg_next);
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = tok + 16 * t + 4 * h4 + i;
+            sc[t][i] = key < s.held && (t ? p1 : p0) && sees(sight, key) ? sc[t][i] : -__builtin_inff();
+          }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {                               // whatever stands where no token is: its value is 0
+          const uint32_t keep = bytes_below((t ? p1 : p0) ? s.held - (tok + 16 * t + 4 * h4) : 0);
+#pragma unroll
+          for (int v = 0; v < VU; ++v) x.v[t][v] &= keep;
+        }
+      }
+      v8h p, rest;
+      float e[8], top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = rounded_product(sc[i >> 2][i & 3], cs);
+      top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+      top = across_max(top);
+      if (__ballot(top > m + P_SLACK)) {                       // the maximum follows when p would leave its range
+        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) o[t] *= f;
+      }
+      const float shift = P_BITS - m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i] + shift);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
+        l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+        p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
+        if constexpr (!BF) {
+          const v2h pl = rest_of(ph, e[2 * i], e[2 * i + 1]);
+          rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
+          l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < VU; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                               // channels 64 v + 4 n + i
+          const v8h f = octet8(x.v[0][v][i], x.v[1][v][i], x.s[0].y, x.s[1].y);
+          o[4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[4 * v + i], 0, 0, 0);
+          if constexpr (!BF)
+            o[4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest, o[4 * v + i], 0, 0, 0);
+        }
+      if (u + 1 < u1) {
+        fetch_values(tok_next, pg_next);
+        pg[0] = pg_next[0]; pg[1] = pg_next[1];
+        pages_of(token_of(min(u + 2, u1 - 1)), pg_next);
+      }
+    }
+
+    // ---- the four wavefronts' parts together
+    __syncthreads();                                                // (the reads of the last item)
+    l = across_sum(l);
+    if (h4 == 0) { m_sh[wave][col] = m; l_sh[wave][col] = l; }
+#pragma unroll
+    for (int v = 0; v < VU; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)                                   // row n = 4 h4 + i of four tiles: channels 64 v + 4 n ..
+        *(v4f*)&o_sh[wave][col][64 * v + 16 * h4 + 4 * i] = v4f{o[4 * v][i], o[4 * v + 1][i], o[4 * v + 2][i], o[4 * v + 3][i]};
+    __syncthreads();
+    const bool direct = u0 == 0 && u1 == g.units;
+    const int slot = is_first ? 0 : 1;
+    if (!direct && u0 == 0 && tid == 0) {                           // this workgroup begins the tile: it is joined from here
+      desc->first = s.first; desc->row0 = row0; desc->valid = valid; desc->head = h; desc->slot = slot;
+      desc->count = (int)(shares.of(start + weight - 1) - w + 1);
+    }
+    if (!direct && u0 == 0) joined = 1;
+    for (int x = tid; x < valid * (D / 4); x += 256) {
+      const int row = x / (D / 4), d = 4 * (x % (D / 4));
+      float top = m_sh[0][row];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) top = fmaxf(top, m_sh[i][row]);
+      float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = __builtin_amdgcn_exp2f(m_sh[i][row] - top);
+        sum += f * l_sh[i][row];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] += f * o_sh[i][row][d + j];
+      }
+      if (direct) {
+        const int gr = row0 + row;
+        store_row4(a, s.first + gr / a.ratio, h * a.ratio + gr % a.ratio, d, y, sum);
+      } else {
+        float* const part = attn_part<D>(a.ws, gridDim.x, (w * 2 + slot) * R + row);
+        *(float4*)(part + d) = make_float4(y[0], y[1], y[2], y[3]);
+        if (d == 0) { part[D] = top; part[D + 1] = sum; }
+      }
+    }
+  }
+  if (a.ws && !joined && tid == 0) desc->count = 0;
+}
+
+// ------------------------------------------------------------------ launch
+// Every tile of 16 rows, at most; its units, if all sequences were as long as the table allows; the workgroups that run at once:
+// four, three or two a CU, by the registers and the LDS they take.
+struct Load8 { int64_t tiles, units; int chip; };
+static Load8 load_of(const DCache8& c, const DRows& r, int ratio) {
+  return {((int64_t)r.tokens * ratio / 16 + r.seqs) * c.heads, r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1, 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2)};
+}
+struct Plan8 { int grid; bool split; size_t bytes; };
+static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
+  const Load8 w = load_of(c, r, ratio);
+  Plan8 p;
+  // Tiles of few units stay in one piece, which saves the second launch
+  p.split = w.units > 8 || (w.units > 4 && 2 * w.tiles < w.chip);
+  const int64_t most = p.split ? w.tiles * (w.units + EXTRA) : w.tiles;
+  p.grid = (int)(most < w.chip ? most : w.chip);
+  p.bytes = p.split ? attn_bytes(p.grid, 16, c.dim) : 0;
+  return p;
+}
+
+// Which of the two kernels: that of cbk_cache8_prompt.hip takes tiles of 256 rows, filled or not
+static bool many_rows(const DCache8& c, const DRows& r, int ratio) {
+  const int64_t rows = (int64_t)r.tokens * ratio;
+  if (rows <= (int64_t)112 * r.seqs) return false;
+  const Load8 w = load_of(c, r, ratio);
+  return w.tiles * (w.units + EXTRA) > (int64_t)16 * w.chip;
+}
+size_t cache8_attn_workspace(const DCache8& c, const DRows& r, int ratio) {
+  return many_rows(c, r, ratio) ? plan_prompt8(c, r, ratio).bytes : plan_few(c, r, ratio).bytes;
+}
+
+template <int D>
+static void few(const Plan8& p, const DCache8& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  if (a.bf) hipLaunchKernelGGL((cache8_attn_kernel<D, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  else hipLaunchKernelGGL((cache8_attn_kernel<D, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+}
+int launch_cache8_attn(const DCache8& c, const DRows& r, AttnArgs a, size_t ws_bytes, hipStream_t st) {
+  const size_t need = cache8_attn_workspace(c, r, a.ratio);
+  if (need > ws_bytes || (need && !a.ws)) return CBK_ERR_WORKSPACE;
+  if (!need) a.ws = nullptr;
+  if (many_rows(c, r, a.ratio)) return launch_cache8_prompt(plan_prompt8(c, r, a.ratio), c, r, a, st);
+  const Plan8 p = plan_few(c, r, a.ratio);
+  a.whole = !p.split;
+  if (c.dim == 64) few<64>(p, c, r, a, st);
+  else if (c.dim == 128) few<128>(p, c, r, a, st);
+  else few<256>(p, c, r, a, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, 16, st);
+  return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
+}
+
+}  // namespace cbk

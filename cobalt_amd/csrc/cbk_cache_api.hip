@@ -2,6 +2,7 @@
 // synchronisation, no global state.
 #include "cbk_cache.h"
 #include "cbk_cache_attn.h"
+#include "cbk_cache_check.h"
 
 namespace cbk {
 
@@ -27,36 +28,11 @@ static int to_dcache(const cbk_cache* in, DCache* c, bool need_device_ptrs) {
   return CBK_OK;
 }
 
-static int to_drows(const cbk_rows* in, const DCache& c, DRows* r, bool need_device_ptrs) {
-  if (!in) return CBK_ERR_NULL;
-  if (in->seqs < 0 || in->table_cols < 0 || in->ld_table < in->table_cols || in->tokens < 0 || in->tokens >= 1 << 30) return CBK_ERR_SHAPE;
-  if (in->table_cols > (1 << 30) / c.page) return CBK_ERR_SHAPE;    // token positions are ints, tiles round them up
-  if (in->seqs == 0 && in->tokens > 0 && !in->starts) return CBK_ERR_SHAPE;
-  if (!in->starts && in->seqs && in->tokens % in->seqs) return CBK_ERR_SHAPE;
-  if (need_device_ptrs && in->seqs > 0 && in->tokens > 0) {
-    if (!in->lens || (in->table_cols && !in->table)) return CBK_ERR_NULL;
-    if (((uintptr_t)in->lens | (uintptr_t)in->table | (uintptr_t)in->starts) & 3) return CBK_ERR_ALIGN;
-  }
-  r->table = (const int32_t*)in->table; r->lens = (const int32_t*)in->lens; r->starts = (const int32_t*)in->starts;
-  r->ld = in->ld_table; r->seqs = in->seqs; r->cols = in->table_cols; r->tokens = (int)in->tokens;
-  r->per = in->starts || !in->seqs ? 0 : (int)(in->tokens / in->seqs);
-  r->cap = in->table_cols * c.page;
-  return CBK_OK;
-}
-
-// Rows of `heads` heads of D elements: unit stride along D, 16-byte pieces
-static int check_dense(const void* p, int64_t rs, int64_t hs, int size) {
-  if (!p) return CBK_ERR_NULL;
-  if (rs < 0 || hs < 0) return CBK_ERR_SHAPE;
-  if (((uintptr_t)p & 15) || (rs * size & 15) || (hs * size & 15)) return CBK_ERR_ALIGN;
-  return CBK_OK;
-}
-
 static int cache_io(const cbk_cache* cache, const cbk_rows* rows, const CacheIo& io, int dt, bool write, void* stream) {
   DCache c;
   DRows r;
   int rc = to_dcache(cache, &c, true);
-  if (!rc) rc = to_drows(rows, c, &r, true);
+  if (!rc) rc = to_drows(rows, c.page, &r, true);
   if (rc) return rc;
   if (dt != CBK_F16 && dt != CBK_BF16T && (write || dt != CBK_F32)) return CBK_ERR_DTYPE;
   if (r.tokens == 0 || r.seqs == 0) return CBK_OK;
@@ -66,13 +42,6 @@ static int cache_io(const cbk_cache* cache, const cbk_rows* rows, const CacheIo&
   if (rc) return rc;
   if ((int64_t)r.tokens * c.heads * c.dim >= (int64_t)1 << 36) return CBK_ERR_SHAPE;   // 2^32 threads of a launch: 16 numbers each
   return write ? launch_cache_write(c, r, io, dt, (hipStream_t)stream) : launch_cache_read(c, r, io, dt, (hipStream_t)stream);
-}
-
-static int attn_ratio(const DCache& c, const DRows& r, int q_heads, int* ratio) {
-  if (q_heads < 1 || q_heads % c.heads || (int64_t)r.tokens * q_heads >= (int64_t)1 << 30) return CBK_ERR_SHAPE;
-  *ratio = q_heads / c.heads;
-  if (*ratio > 256) return CBK_ERR_SHAPE;                           // (weights of tiles are rows times tokens in 64 bits)
-  return CBK_OK;
 }
 
 }  // namespace cbk
@@ -104,7 +73,7 @@ size_t cbk_cache_attention_workspace_bytes(const cbk_cache* cache, const cbk_row
   DCache c;
   DRows r;
   int ratio;
-  if (to_dcache(cache, &c, false) || to_drows(rows, c, &r, false) || attn_ratio(c, r, q_heads, &ratio)) return 0;
+  if (to_dcache(cache, &c, false) || to_drows(rows, c.page, &r, false) || attn_ratio(c.heads, r, q_heads, &ratio)) return 0;
   return r.tokens && r.seqs ? cache_attn_workspace(c, r, ratio) : 0;
 }
 
@@ -115,8 +84,8 @@ int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void
   DRows r;
   AttnArgs a{};
   int rc = to_dcache(cache, &c, true);
-  if (!rc) rc = to_drows(rows, c, &r, true);
-  if (!rc) rc = attn_ratio(c, r, q_heads, &a.ratio);
+  if (!rc) rc = to_drows(rows, c.page, &r, true);
+  if (!rc) rc = attn_ratio(c.heads, r, q_heads, &a.ratio);
   if (rc) return rc;
   if (dtype != CBK_F16 && dtype != CBK_BF16T) return CBK_ERR_DTYPE;
   if (!(scale >= 1e-30f) || scale > 1e30f || window < 0 || sinks < 0) return CBK_ERR_SHAPE;
@@ -125,13 +94,7 @@ int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void
   if (!rc) rc = check_dense(out, out_row, out_head, 2);
   if (rc) return rc;
   if (((uintptr_t)workspace & 255)) return CBK_ERR_ALIGN;
-  a.q = q; a.out = out;
-  a.qt = q_row; a.qh = q_head; a.ot = out_row; a.oh = out_head;
-  a.bf = dtype == CBK_BF16T;
-  a.scale = scale * 1.44269504088896341f;
-  a.window = window >= 1 << 30 ? 0 : window;                        // (positions end below 2^31: such a window hides nothing a table holds)
-  a.sinks = sinks < 1 << 30 ? sinks : 1 << 30;
-  a.ws = (uint8_t*)workspace;
+  set_attn(&a, q, q_row, q_head, out, out_row, out_head, dtype, scale, window, sinks, workspace);
   return launch_cache_attn(c, r, a, workspace_bytes, (hipStream_t)stream);
 }
 

@@ -163,6 +163,56 @@ __device__ inline void store_row4(const AttnArgs& a, int row, int head, int d, c
   *(uint2*)p = v;
 }
 
+// ------------------------------------------------------------------ few rows: tiles of 16, units of tokens
+constexpr int UNIT = 128;                   // tokens: 32 a wavefront
+constexpr int EXTRA = 2;                    // units that a tile of rows counts for by itself: its queries, its end (32 ragged sequences: 0: 53 us, 2: 42.5, 4: 42)
+
+struct Range { int units, head, skip; };    // units of a sequence; the first `head` from token 0, the others `skip` units on
+__device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
+  Range g{0, 0, 0};
+  if (s.n <= 0) return g;
+  const int all = max((s.held + UNIT - 1) / UNIT, 1);
+  if (a.window > 0) {
+    const int lo = min(max(s.pos0 - a.window + 1, 0) / UNIT, all - 1);
+    g.head = min((a.sinks + UNIT - 1) / UNIT, lo);
+    g.skip = lo - g.head;
+  }
+  g.units = all - g.skip;
+  return g;
+}
+
+__device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads, int b, int rows) {
+  const Seq s = seq_of(r, b);
+  const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
+  return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
+}
+__device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float across_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// ------------------------------------------------------------------ many rows: tiles of 256
+constexpr int WAVES = 8, ROWS = 32 * WAVES;
+constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
+
+__device__ inline int row_tiles(const Seq& s, int ratio) { return (int)(((int64_t)s.n * ratio + ROWS - 1) / ROWS); }
+
+// What tiles of rows weigh when the list is cut: the tokens they see, times the query heads of a cache head so that no fraction is lost.  Only
+// the balance rests on it, not what is computed: a piece of a tile's weight is that piece of its tokens, rounded to tiles.
+struct Weights {
+  int ratio, window, sinks;
+  int64_t own;                               // what a tile of rows weighs by itself
+  __device__ int64_t first(const Seq& s) const { return (int64_t)max(s.pos0, 0) * ratio; }
+  __device__ int64_t flat() const { return own + ROWS + (int64_t)ratio * ((int64_t)window + sinks); }
+  __device__ int64_t of(const Seq& s, int i) const { return window > 0 ? flat() : own + first(s) + (int64_t)(i + 1) * ROWS; }
+  __device__ int64_t before(const Seq& s, int i) const { return window > 0 ? i * flat() : i * (own + first(s)) + (int64_t)i * (i + 1) / 2 * ROWS; }
+  __device__ int64_t all(const Seq& s) const { return s.n > 0 ? before(s, row_tiles(s, ratio)) : 0; }
+};
+
 // cbk_cache_prompt.hip: many rows a sequence
 struct PromptPlan { bool cut; int64_t grid; size_t bytes; };
 PromptPlan plan_prompt(const DCache&, const DRows&, int ratio);

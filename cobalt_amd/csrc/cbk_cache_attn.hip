@@ -32,37 +32,6 @@
 
 namespace cbk {
 
-constexpr int UNIT = 128;                   // tokens: 32 a wavefront
-constexpr int EXTRA = 2;                    // units that a tile of rows counts for by itself: its queries, its end (32 ragged sequences: 0: 53 us, 2: 42.5, 4: 42)
-
-struct Range { int units, head, skip; };    // units of a sequence; the first `head` from token 0, the others `skip` units on
-__device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
-  Range g{0, 0, 0};
-  if (s.n <= 0) return g;
-  const int all = max((s.held + UNIT - 1) / UNIT, 1);
-  if (a.window > 0) {
-    const int lo = min(max(s.pos0 - a.window + 1, 0) / UNIT, all - 1);
-    g.head = min((a.sinks + UNIT - 1) / UNIT, lo);
-    g.skip = lo - g.head;
-  }
-  g.units = all - g.skip;
-  return g;
-}
-
-__device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads, int b, int rows) {
-  const Seq s = seq_of(r, b);
-  const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
-  return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
-}
-__device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ inline float across_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-
 template <int D, int G>
 struct Held {                               // a wavefront's 32 tokens: two sixteens
   uint32_t k[2][D / 32];

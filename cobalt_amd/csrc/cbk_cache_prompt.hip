@@ -30,12 +30,10 @@
 
 namespace cbk {
 
-constexpr int WAVES = 8, ROWS = 32 * WAVES;
 constexpr int OWN = 2;                      // tiles of tokens that a tile of rows counts for by itself: its queries, its start and end (six ragged
                                             // chunks: none 470 us, 1: 445, 2: 433, 4: 431; a prompt of 8192 tokens, cut: 774, 669, 631, 631)
 constexpr float REST = 2048.f;              // What the first fp16 leaves of a sum of q is kept this many times as large, and meets minima that many times smaller: with a small
                                             // scale in it the rest has no digits as an fp16 (2^-25 of a minimum of 60000 is 2e-3 of a score; now 2^-36, and 2^-25 of the sum)
-constexpr int CHIP = 256;                   // workgroups that run at once: one a CU
 
 template <int D, int G, bool BF>
 struct Tile {
@@ -47,20 +45,6 @@ struct Tile {
   static constexpr int K_BYTES = KEYS * D * 2, V_BYTES = KEYS * D * 2;
   static constexpr int M_BYTES = BF ? 0 : KEYS / 32 * 1024, S_BYTES = BF ? 0 : GS * KEYS * 4;   // minima as an operand, scales (float)
   static constexpr int BYTES = K_BYTES + V_BYTES + M_BYTES + S_BYTES + 16;   // and a byte for each sixteen: its page is there
-};
-
-__device__ inline int row_tiles(const Seq& s, int ratio) { return (int)(((int64_t)s.n * ratio + ROWS - 1) / ROWS); }
-
-// What tiles of rows weigh when the list is cut: the tokens they see, times the query heads of a cache head so that no fraction is lost.  Only
-// the balance rests on it, not what is computed: a piece of a tile's weight is that piece of its tokens, rounded to tiles.
-struct Weights {
-  int ratio, window, sinks;
-  int64_t own;                               // what a tile of rows weighs by itself
-  __device__ int64_t first(const Seq& s) const { return (int64_t)max(s.pos0, 0) * ratio; }
-  __device__ int64_t flat() const { return own + ROWS + (int64_t)ratio * ((int64_t)window + sinks); }
-  __device__ int64_t of(const Seq& s, int i) const { return window > 0 ? flat() : own + first(s) + (int64_t)(i + 1) * ROWS; }
-  __device__ int64_t before(const Seq& s, int i) const { return window > 0 ? i * flat() : i * (own + first(s)) + (int64_t)i * (i + 1) / 2 * ROWS; }
-  __device__ int64_t all(const Seq& s) const { return s.n > 0 ? before(s, row_tiles(s, ratio)) : 0; }
 };
 
 template <int D, int G, bool BF>

@@ -574,14 +574,38 @@ PyObject* py_pack_end(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// ------------------------------------------------------------------ the 4-bit key/value cache
-// The pool as Python holds it: (k_codes, v_codes, k_meta, v_meta, pages, page, heads, head_dim, group).
-struct Cache { at::Tensor t[4]; cbk_cache c; };
+// ------------------------------------------------------------------ the key/value caches
+// A pool as Python holds it: (k_codes, v_codes, k_meta, v_meta, pages, page, heads, head_dim, group) in 4 bits, or
+// (k_codes, v_codes, scales, pages, page, heads, head_dim, block) in 8.
+struct Cache {
+  at::Tensor t[4];
+  int bits;
+  cbk_cache c;
+  cbk_cache8 c8;
+  int64_t pages;
+  int32_t page, heads, head_dim;
+  int write(const cbk_rows* r, const void* k, int64_t kr, int64_t kh, const void* v, int64_t vr, int64_t vh, int dt, void* st) const {
+    return bits == 8 ? cbk_cache8_write(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_write(&c, r, k, kr, kh, v, vr, vh, dt, st);
+  }
+  int read(const cbk_rows* r, void* k, int64_t kr, int64_t kh, void* v, int64_t vr, int64_t vh, int dt, void* st) const {
+    return bits == 8 ? cbk_cache8_read(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_read(&c, r, k, kr, kh, v, vr, vh, dt, st);
+  }
+  size_t attention_workspace(const cbk_rows* r, int heads) const {
+    return bits == 8 ? cbk_cache8_attention_workspace_bytes(&c8, r, heads) : cbk_cache_attention_workspace_bytes(&c, r, heads);
+  }
+  int attention(const cbk_rows* r, const void* q, int64_t qr, int64_t qh, void* out, int64_t orow, int64_t oh, int dt, int heads, float scale,
+                int window, int sinks, void* ws, size_t bytes, void* st) const {
+    return bits == 8 ? cbk_cache8_attention(&c8, r, q, qr, qh, out, orow, oh, dt, heads, scale, window, sinks, ws, bytes, st)
+                     : cbk_cache_attention(&c, r, q, qr, qh, out, orow, oh, dt, heads, scale, window, sinks, ws, bytes, st);
+  }
+};
 Cache as_cache(PyObject* o) {
-  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 9) fail(PyExc_TypeError, "a KVCache is expected");
-  Cache r;
+  if (!PyTuple_Check(o) || (PyTuple_GET_SIZE(o) != 9 && PyTuple_GET_SIZE(o) != 8)) fail(PyExc_TypeError, "a KVCache is expected");
+  Cache r{};
+  r.bits = PyTuple_GET_SIZE(o) == 9 ? 4 : 8;
+  const int arrays = r.bits == 4 ? 4 : 3;
   void* p[4];
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < arrays; ++i) {
     r.t[i] = as_tensor(PyTuple_GET_ITEM(o, i), "an array of the cache");
     if (!r.t[i].defined()) fail(PyExc_TypeError, "a KVCache is expected");
     if (!r.t[i].is_contiguous() || r.t[i].device() != r.t[0].device())
@@ -589,12 +613,22 @@ Cache as_cache(PyObject* o) {
     p[i] = r.t[i].mutable_data_ptr();
   }
   long long v[5];
-  for (int i = 0; i < 5; ++i) v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, 4 + i));
+  for (int i = 0; i < 5; ++i) v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, arrays + i));
   if (PyErr_Occurred()) throw Fail{};
-  r.c = cbk_cache{p[0], p[1], p[2], p[3], (int64_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4]};
-  const size_t codes = cbk_cache_code_bytes(&r.c), meta = cbk_cache_meta_bytes(&r.c);
-  if (!codes || r.t[0].nbytes() < codes || r.t[1].nbytes() < codes || r.t[2].nbytes() < meta || r.t[3].nbytes() < meta)
-    fail(PyExc_ValueError, "the arrays of the cache do not hold what its description says");
+  r.pages = v[0]; r.page = (int32_t)v[1]; r.heads = (int32_t)v[2]; r.head_dim = (int32_t)v[3];
+  size_t need[4];
+  if (r.bits == 4) {
+    r.c = cbk_cache{p[0], p[1], p[2], p[3], (int64_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4]};
+    need[0] = need[1] = cbk_cache_code_bytes(&r.c);
+    need[2] = need[3] = cbk_cache_meta_bytes(&r.c);
+  } else {
+    r.c8 = cbk_cache8{p[0], p[1], p[2], (int64_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4]};
+    need[0] = need[1] = cbk_cache8_code_bytes(&r.c8);
+    need[2] = cbk_cache8_scale_bytes(&r.c8);
+  }
+  bool enough = need[0] != 0;
+  for (int i = 0; i < arrays; ++i) enough = enough && r.t[i].nbytes() >= need[i];
+  if (!enough) fail(PyExc_ValueError, "the arrays of the cache do not hold what its description says");
   if (!r.t[0].is_cuda()) fail(g_error, "the cache must live on the GPU; this package has no CPU execution path");
   return r;
 }
@@ -695,8 +729,8 @@ PyObject* py_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Cache c = as_cache(a[0]);
     same_device(c, k);
     same_device(c, v);
-    check_heads(k, c.c.heads, c.c.head_dim, "k");
-    check_heads(v, c.c.heads, c.c.head_dim, "v");
+    check_heads(k, c.heads, c.head_dim, "k");
+    check_heads(v, c.heads, c.head_dim, "v");
     if (k.size(0) != v.size(0) || k.scalar_type() != v.scalar_type() || !half_type(k.scalar_type()))
       fail(PyExc_ValueError, "k and v have the same number of rows and are both float16 or both bfloat16");
     const RowMap m = as_rows(c, a[3], a[4], a[5], k.size(0));
@@ -707,7 +741,7 @@ PyObject* py_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const c10::DeviceGuard guard(k.device());
       k = dense_in(k);
       v = dense_in(v);
-      rc = cbk_cache_write(&c.c, &m.r, k.const_data_ptr(), row_stride(k), head_stride(k), v.const_data_ptr(), row_stride(v),
+      rc = c.write(&m.r, k.const_data_ptr(), row_stride(k), head_stride(k), v.const_data_ptr(), row_stride(v),
                            head_stride(v), dt, stream_of(k));
     }
     check(rc, "cbk_cache_write");
@@ -732,7 +766,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (at::Tensor& o : out)
       if (o.defined()) {
         same_device(c, o);
-        check_out(o, rows, c.c.heads, c.c.head_dim, t, "the output");
+        check_out(o, rows, c.heads, c.head_dim, t, "the output");
       }
     if (out[0].defined() && out[1].defined() && !apart(out[0], out[1]))
       fail(PyExc_ValueError, "keys and values need an output each: these overlap");
@@ -741,9 +775,9 @@ PyObject* py_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const GilRelease other_threads_run;
       const c10::DeviceGuard guard(c.t[0].device());
       for (at::Tensor& o : out)
-        if (!o.defined()) o = at::empty({(int64_t)rows, c.c.heads, c.c.head_dim}, c.t[0].options().dtype(t));
+        if (!o.defined()) o = at::empty({(int64_t)rows, c.heads, c.head_dim}, c.t[0].options().dtype(t));
       if (rows)
-        rc = cbk_cache_read(&c.c, &m.r, out[0].mutable_data_ptr(), row_stride(out[0]), head_stride(out[0]), out[1].mutable_data_ptr(),
+        rc = c.read(&m.r, out[0].mutable_data_ptr(), row_stride(out[0]), head_stride(out[0]), out[1].mutable_data_ptr(),
                             row_stride(out[1]), head_stride(out[1]), dt, stream_of(c.t[0]));
     }
     check(rc, "cbk_cache_read");
@@ -761,12 +795,12 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Cache c = as_cache(a[0]);
     same_device(c, q);
     same_device(c, out);
-    check_heads(q, 0, c.c.head_dim, "q");
+    check_heads(q, 0, c.head_dim, "q");
     if (!half_type(q.scalar_type())) fail(PyExc_TypeError, "q is float16 or bfloat16");
     const int64_t heads = q.size(1);
-    if (heads % c.c.heads)
-      fail(PyExc_ValueError, std::to_string(heads) + " query heads are no multiple of the cache's " + std::to_string(c.c.heads));
-    if (out.defined()) check_out(out, q.size(0), heads, c.c.head_dim, q.scalar_type(), "out");
+    if (heads % c.heads)
+      fail(PyExc_ValueError, std::to_string(heads) + " query heads are no multiple of the cache's " + std::to_string(c.heads));
+    if (out.defined()) check_out(out, q.size(0), heads, c.head_dim, q.scalar_type(), "out");
     if (out.defined() && readable16(q) && !apart(out, q)) fail(PyExc_ValueError, "out must not overlap q");   // (any other q is copied first)
     const RowMap m = as_rows(c, a[2], a[3], a[4], q.size(0));
     const double scale = PyFloat_AsDouble(a[5]);
@@ -778,11 +812,11 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
       const GilRelease other_threads_run;
       const c10::DeviceGuard guard(q.device());
-      if (!out.defined()) out = at::empty({q.size(0), heads, (int64_t)c.c.head_dim}, q.options().requires_grad(false));
+      if (!out.defined()) out = at::empty({q.size(0), heads, (int64_t)c.head_dim}, q.options().requires_grad(false));
       if (q.size(0)) {
         q = dense_in(q);
-        const at::Tensor ws = scratch(q, cbk_cache_attention_workspace_bytes(&c.c, &m.r, (int)heads));
-        rc = cbk_cache_attention(&c.c, &m.r, q.const_data_ptr(), row_stride(q), head_stride(q), out.mutable_data_ptr(),
+        const at::Tensor ws = scratch(q, c.attention_workspace(&m.r, (int)heads));
+        rc = c.attention(&m.r, q.const_data_ptr(), row_stride(q), head_stride(q), out.mutable_data_ptr(),
                                  row_stride(out), head_stride(out), dt, (int)heads, (float)scale,
                                  (int)(window < INT32_MAX ? window : INT32_MAX), (int)(sinks < INT32_MAX ? sinks : INT32_MAX),
                                  ws.defined() ? ws.mutable_data_ptr() : nullptr, ws.defined() ? ws.nbytes() : 0, stream_of(q));
@@ -790,6 +824,99 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     check(rc, "cbk_cache_attention");
     return THPVariable_Wrap(out);
+  });
+}
+
+// ------------------------------------------------------------------ tables of pages
+// A pool's tables as Python holds them: (table, lens, free, count, pages, page).
+struct Pages { at::Tensor t[4]; cbk_pages p; };
+Pages as_pages(PyObject* o) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 6) fail(PyExc_TypeError, "a KVPages is expected");
+  Pages r;
+  static const char* const names[4] = {"table", "lens", "free", "count"};
+  for (int i = 0; i < 4; ++i) {
+    r.t[i] = as_tensor(PyTuple_GET_ITEM(o, i), names[i]);
+    if (!r.t[i].defined()) fail(PyExc_TypeError, "a KVPages is expected");
+    if (!r.t[i].is_contiguous() || r.t[i].device() != r.t[0].device() || r.t[i].scalar_type() != at::kInt || r.t[i].dim() != (i ? 1 : 2))
+      fail(PyExc_ValueError, "the arrays of a KVPages are contiguous int32 tensors on one device");
+  }
+  const long long pages = PyLong_AsLongLong(PyTuple_GET_ITEM(o, 4)), page = PyLong_AsLongLong(PyTuple_GET_ITEM(o, 5));
+  if (PyErr_Occurred()) throw Fail{};
+  const int64_t seqs = r.t[0].size(0), cols = r.t[0].size(1);
+  if (r.t[1].size(0) != seqs || r.t[2].size(0) != pages || r.t[3].size(0) != 1)
+    fail(PyExc_ValueError, "the arrays of a KVPages do not hold what its description says");
+  if (!r.t[0].is_cuda()) fail(g_error, "the tables must live on the GPU; this package has no CPU execution path");
+  if (seqs > INT32_MAX || cols > INT32_MAX || page > INT32_MAX) check(CBK_ERR_SHAPE, "cbk_pages");
+  r.p = cbk_pages{r.t[0].mutable_data_ptr(), cols, r.t[1].mutable_data_ptr(), r.t[2].mutable_data_ptr(), r.t[3].mutable_data_ptr(),
+                  (int64_t)pages, (int32_t)seqs, (int32_t)cols, (int32_t)page};
+  return r;
+}
+
+// cache_pages(pages, want, starts or None) -> starts
+PyObject* py_cache_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 3)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Pages p = as_pages(a[0]);
+    const at::Tensor want = as_tensor(a[1], "lens");
+    at::Tensor starts = as_tensor(a[2], "starts");
+    if (!want.defined()) fail(PyExc_TypeError, "lens must be a tensor");
+    for (const at::Tensor* t : {&want, (const at::Tensor*)&starts})
+      if (t->defined()) {
+        if (t->device() != p.t[0].device())
+          fail(g_error, "tensor on " + t->device().str() + ", tables on " + p.t[0].device().str());
+        if (t->scalar_type() != at::kInt) fail(PyExc_TypeError, "lens and starts are int32 tensors");
+        if (t->dim() != 1 || t->size(0) != p.p.seqs + (t == &starts)) fail(PyExc_ValueError, "lens is [sequences], starts has one entry more");
+        if (t->size(0) > 1 && t->stride(0) != 1) fail(PyExc_ValueError, "lens and starts have unit stride");
+      }
+    if (starts.defined())
+      for (const at::Tensor* t : {&want, &p.t[0], &p.t[1], &p.t[2], &p.t[3]}) {
+        const uintptr_t x = (uintptr_t)starts.const_data_ptr(), y = (uintptr_t)t->const_data_ptr();
+        if (t->numel() && x < y + 4 * t->numel() && y < x + 4 * starts.numel()) fail(PyExc_ValueError, "starts must not overlap lens or the pool's arrays");
+      }
+    for (int i : {0, 2, 3}) {                                       // (lens themselves may be asked for)
+      const uintptr_t x = (uintptr_t)want.const_data_ptr(), y = (uintptr_t)p.t[i].const_data_ptr();
+      if (want.numel() && p.t[i].numel() && x < y + 4 * p.t[i].numel() && y < x + 4 * want.numel())
+        fail(PyExc_ValueError, "lens must not overlap the pool's table or stack");
+    }
+    int rc = CBK_OK;
+    {
+      const GilRelease other_threads_run;
+      const c10::DeviceGuard guard(p.t[0].device());
+      if (!starts.defined()) starts = p.p.seqs ? at::empty({p.p.seqs + 1}, p.t[0].options()) : at::zeros({1}, p.t[0].options());
+      const at::Tensor ws = scratch(p.t[0], cbk_cache_pages_workspace_bytes(&p.p));
+      rc = cbk_cache_pages(&p.p, want.const_data_ptr(), starts.mutable_data_ptr(), ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                           ws.defined() ? ws.nbytes() : 0, stream_of(p.t[0]));
+    }
+    check(rc, "cbk_cache_pages");
+    return THPVariable_Wrap(starts);
+  });
+}
+
+// cache_slots(pages, page, table, lens, starts or None, rows) -> (slots, positions)
+PyObject* py_cache_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 6)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const long long pages = PyLong_AsLongLong(a[0]), page = PyLong_AsLongLong(a[1]), rows = PyLong_AsLongLong(a[5]);
+    if (PyErr_Occurred()) throw Fail{};
+    if (rows < 0) fail(PyExc_ValueError, "the number of rows is negative");
+    const at::Tensor table = as_tensor(a[2], "table");
+    if (!table.defined()) fail(PyExc_TypeError, "table and lens must be tensors");
+    if (!table.is_cuda()) fail(g_error, "the table must live on the GPU; this package has no CPU execution path");
+    Cache like{};                                                   // (the device that all must be on)
+    like.t[0] = table;
+    const RowMap m = as_rows(like, a[2], a[3], a[4], rows);
+    if (page > INT32_MAX) check(CBK_ERR_LAYOUT, "cbk_cache_slots");
+    at::Tensor slots, positions;
+    int rc = CBK_OK;
+    {
+      const GilRelease other_threads_run;
+      const c10::DeviceGuard guard(table.device());
+      slots = at::empty({(int64_t)rows}, table.options().dtype(at::kLong));
+      positions = at::empty({(int64_t)rows}, table.options().dtype(at::kInt));
+      rc = cbk_cache_slots(&m.r, pages, (int)page, slots.mutable_data_ptr(), positions.mutable_data_ptr(), stream_of(table));
+    }
+    check(rc, "cbk_cache_slots");
+    return Py_BuildValue("NN", THPVariable_Wrap(slots), THPVariable_Wrap(positions));
   });
 }
 
@@ -815,6 +942,8 @@ PyMethodDef methods[] = {
     {"cache_write", (PyCFunction)(void (*)())py_cache_write, METH_FASTCALL, nullptr},
     {"cache_read", (PyCFunction)(void (*)())py_cache_read, METH_FASTCALL, nullptr},
     {"cache_attention", (PyCFunction)(void (*)())py_cache_attention, METH_FASTCALL, nullptr},
+    {"cache_pages", (PyCFunction)(void (*)())py_cache_pages, METH_FASTCALL, nullptr},
+    {"cache_slots", (PyCFunction)(void (*)())py_cache_slots, METH_FASTCALL, nullptr},
     {"set_error", py_set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -9,6 +9,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .cache import KVRows
 from .format import PackedMatrix
 
 def _stream_ptr(device) -> int:
@@ -190,13 +191,14 @@ def transcode(pm: PackedMatrix, layout: int, bits=None, group=None, keep=None, t
     return out
 
 
-# ------------------------------------------------------------------ the key/value cache held in 4 bits (cache.py)
+# ------------------------------------------------------------------ the key/value caches, KVCache in 4 bits and KVCache8 in 8 (cache.py)
 # Without a backward pass: a tensor that requires a gradient is refused, except under torch.no_grad().
 def cache_write(cache, k, v, rows) -> None:
-    """The rows' keys and values (float16 or bfloat16, [rows, heads, head_dim]) into the cache, rounded to 4 bits per
-    group: codes c = rint((x - m) / s) with the fp16 minimum m and scale s of the group, held value m + c s.  Magnitudes above
-    65280 are held as 65280; a NaN makes its token's key and value of that head NaN.  Rows whose token has no page are
-    left out.  Two rows of a call must not be the same token of the same page."""
+    """The rows' keys and values (float16 or bfloat16, [rows, heads, head_dim]) into the cache.
+    KVCache: rounded to 4 bits per group, codes c = rint((x - m) / s) with the fp16 minimum m and scale s of the group, held value m + c s.
+    KVCache8: c = e4m3(x / s) with the power of two s of the token's block, which grows with what is written, held value c s.  Magnitudes above
+    65280 (KVCache8: 57344) are held as that; a NaN makes its token's key and value of that head NaN.  Rows whose token has no page are
+    left out.  Two rows of a call must not be the same token of the same page (KVCache8: rows of two sequences not of one block)."""
     _lib.native().cache_write(cache.native(), k, v, rows.table, rows.lens, rows.starts)
 
 
@@ -223,3 +225,19 @@ def cache_attention(cache, q, rows, scale: Optional[float] = None, window: Optio
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     return _lib.native().cache_attention(cache.native(), q, rows.table, rows.lens, rows.starts, scale, window or 0, sinks, out)
+
+
+def cache_pages(pool, lens, starts=None):
+    """Makes the sequences of a KVPages `lens` tokens long (int32 [seqs] on the pool's device, read when the kernel runs; negative: as long as
+    it is).  Pages that are no longer needed go back to the pool, then sequences take what they lack in their order.  Once the pages
+    do not last for one, it and those behind it that lack pages keep their lengths; one that asks for more than the table holds does so alone: `pool.lens`
+    tells.  Returns KVRows of the tokens that the sequences gained, packed one behind the other (`starts`: int32 [seqs + 1] to put
+    their offsets into); its table and lens are the pool's own, which the next call changes."""
+    return KVRows(pool.table, pool.lens, _lib.native().cache_pages(pool.native(), lens, starts))
+
+
+def cache_slots(pool, rows, count: int):
+    """(slots int64, positions int32) of the `count` rows of a call over a pool (a KVCache, KVCache8 or KVPages): page * pool.page + place in
+    the page, -1 for a token that no page holds and for rows of no sequence; and the token's position in its sequence, 0 for rows of none.
+    `rows.starts` must ascend."""
+    return _lib.native().cache_slots(pool.pages, pool.page, rows.table, rows.lens, rows.starts, count)

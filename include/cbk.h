@@ -329,6 +329,73 @@ int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void
                         void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
                         int sinks, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- key/value cache held in 8 bits
+ * The same pool of pages with e4m3 codes and, for each block of `block` consecutive tokens of a page and head, a power of two as the
+ * scale of its keys and one of its values (8 + 32 / (block * head_dim) bits a value).  With x' = x clamped to +-57344, and the rows
+ * of a call that stand in one block:
+ *
+ *     need = the smallest power of two s >= 2^-15 with max |x'| <= 448 s,
+ *     s    = need if the block's first token is among them (the block begins anew), else max(need, s so far),
+ *     c    = e4m3(x' / s), to nearest with ties to even,     held value c s (fp16 and bf16 hold it exactly);
+ *
+ * where s has grown the codes of the block's other tokens become e4m3(c s_old / s).  A NaN anywhere in a token's key or value of a
+ * head makes that token's key and value of the head NaN and counts nothing for the scales; infinities are held as +-57344.
+ * Writing a block's first token again loses what the block held behind the rows of that call.
+ *
+ * k_codes and v_codes have cbk_cache8_code_bytes() each, scales cbk_cache8_scale_bytes(), all 16-byte aligned and cleared to zero
+ * once before their first use; what stands where is the library's own (cbk_cache8.h). */
+typedef struct cbk_cache8 {
+  void *k_codes, *v_codes, *scales;
+  int64_t pages;
+  int32_t page;        /* tokens a page: 16, 32, 64, 128 or 256                       */
+  int32_t heads;       /* key/value heads                                             */
+  int32_t head_dim;    /* 64, 128 or 256                                              */
+  int32_t block;       /* tokens a scale: 16, 32, 64, 128 or 256, at most page        */
+} cbk_cache8;
+
+size_t cbk_cache8_code_bytes(const cbk_cache8* cache);    /* 0: not a valid description */
+size_t cbk_cache8_scale_bytes(const cbk_cache8* cache);
+
+/* As cbk_cache_write, cbk_cache_read and cbk_cache_attention, with the same cbk_rows.  Two sequences of a call must not write into
+ * the same block, and tokens * heads is below 2^29 to write or read.  Attention: keys and values are exact as operands; fp16: queries are too, and
+ * softmax weights are two fp16; bf16: softmax weights and queries (with the scale in them) may each be rounded once to fp16. */
+int cbk_cache8_write(const cbk_cache8* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
+                     const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+int cbk_cache8_read(const cbk_cache8* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
+                    void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+size_t cbk_cache8_attention_workspace_bytes(const cbk_cache8* cache, const cbk_rows* rows, int q_heads);
+int cbk_cache8_attention(const cbk_cache8* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
+                         void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
+                         int sinks, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- which pages belong to which sequence
+ * A pool's tables on the device: `table` (seqs rows of table_cols entries, ld_table apart, -1: no page), `lens`, and the pages that belong to
+ * nobody as a stack, free_pages[0 .. free_count[0]) with its top at the end.  All int32, all written by the call below only; before
+ * the first call table is -1, lens 0, free_pages the numbers of all pages in any order and free_count[0] = pages. */
+typedef struct cbk_pages {
+  void* table;
+  int64_t ld_table;
+  void *lens, *free_pages, *free_count;
+  int64_t pages;
+  int32_t seqs, table_cols;   /* seqs below 2^24, table_cols * page at most 2^30        */
+  int32_t page;
+} cbk_pages;
+
+/* Sequence b is to have want[b] tokens (a DEVICE array of int32; negative: as many as it has): it keeps ceil(want[b] / page) pages or takes
+ * what it lacks.  Pages that are no longer needed go back first, and lie on the stack in the order of sequences and
+ * entries, the first on top; then the sequences take pages from the top in their order.  Once the pages do not last for a sequence, it and
+ * all behind it that lack pages keep their lengths; a length that the table has no entries for is refused in the same way, alone.  lens
+ * is what came of it.  starts (seqs + 1, or NULL): where the new rows of each sequence begin, when what they gained is packed one
+ * behind the other, for a cbk_rows of table, lens and starts.  Nothing is waited for and nothing read by the host; calls on one pool
+ * follow one another on a stream.  The workspace holds nothing between calls: cbk_cache_pages_workspace_bytes(), 256-byte aligned. */
+size_t cbk_cache_pages_workspace_bytes(const cbk_pages* pages);
+int cbk_cache_pages(const cbk_pages* pages, const void* want, void* starts, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Of each of the rows->tokens rows of a call: slots[t] = page number * page + place in the page (int64; -1: no sequence, or no page of
+ * the pool's `pages`), positions[t] = the token's position in its sequence (int32; 0 for rows of no sequence and rows in front of the
+ * first token).  Either may be NULL.  starts must ascend. */
+int cbk_cache_slots(const cbk_rows* rows, int64_t pages, int page, void* slots, void* positions, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
