@@ -21,141 +21,212 @@ struct DPages {
   int64_t ld, pages;
   int seqs, cols, page, shift;
 };
-struct PagePlan { int64_t count, gone, taken, moves; };             // pages on the stack before, given back, taken; the larger of the two
+// Pages on the stack before, given back, taken (and the larger of the two); all below 2^31, as the table's entries are
+struct PagePlan { int64_t count, gone, taken, moves; };
+// Behind the plan in the workspace, or in LDS: running sums over the sequences, and the entry that a sequence's pages leave from or go to
+struct PageEnds { int32_t *gone, *more, *first; };
 
-constexpr int PLAN_THREADS = 1024;
-constexpr int64_t INLINE_MOVES = 8192;      // entries of a table whose pages the first launch moves
+constexpr int INLINE_ENTRIES = 8192, INLINE_SEQS = 1024;            // entries and rows of a table whose pages the first launch moves
 
-struct Change { int have, need, now; };     // pages before and asked for; the length asked for
-__device__ inline Change change_of(const DPages& p, const int32_t* want, int len, int b) {
-  const int cap = p.cols * p.page;
-  len = min(max(len, 0), cap);
+struct Change { int len, now, have, need; };                        // tokens before and asked for, and their pages
+__device__ inline Change change_of(const DPages& p, const int32_t* want, int b) {
+  const int cap = p.cols * p.page, w = want[b];
   Change c;
-  const int w = want[b];
-  c.now = w < 0 || w > cap ? len : w;                               // (negative: stays; more than the table holds: refused)
-  c.have = (len + p.page - 1) >> p.shift;
+  c.len = min(max(p.lens[b], 0), cap);
+  c.now = w < 0 || w > cap ? c.len : w;                             // (negative: stays; more than the table holds: refused)
+  c.have = (c.len + p.page - 1) >> p.shift;
   c.need = (c.now + p.page - 1) >> p.shift;
   return c;
 }
 
-// Sum of a workgroup's threads up to and with this one, and of all (sh: a word a wavefront and one more)
-__device__ inline int64_t block_scan(int64_t x, int64_t* sh, int64_t& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  x = scan64(x, lane);
-  __syncthreads();
-  if (lane == 63) sh[wave] = x;
-  __syncthreads();
-  int64_t before = 0;
-  all = 0;
+template <class X>
+__device__ inline X wave_scan(X x, int lane) {                      // sum of the lanes up to and with this one
 #pragma unroll
-  for (int i = 0; i < PLAN_THREADS / 64; ++i) {
-    const int64_t y = sh[i];
-    before += i < wave ? y : 0;
-    all += y;
+  for (int o = 1; o < 64; o *= 2) {
+    const X y = __shfl_up(x, o);
+    x += lane >= o ? y : 0;
   }
-  return x + before;
+  return x;
+}
+// Two such sums over a workgroup's T threads, and of all
+template <int T, class X>
+__device__ inline void block_scan(X& x, int& y, X& all_x, int& all_y, X* shx, int* shy) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x = wave_scan(x, lane);
+  y = wave_scan(y, lane);
+  if (lane == 63) { shx[wave] = x; shy[wave] = y; }
+  __syncthreads();
+  X bx = 0;
+  int by = 0;
+  all_x = 0; all_y = 0;
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) {
+    if (i < wave) { bx += shx[i]; by += shy[i]; }
+    all_x += shx[i]; all_y += shy[i];
+  }
+  x += bx; y += by;
 }
 
-// The sequence whose share of a running sum `ends` has x, and the sum before it
-__device__ inline int share_of(const int64_t* ends, int n, int64_t x, int64_t& before) {
-  int lo = 0, hi = n - 1;                                           // the first b with ends[b] > x
+// The first b in [lo, hi] with ends[b] > x (there is one)
+__device__ inline int share_of(const int32_t* ends, int lo, int hi, int x) {
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (ends[mid] > x) hi = mid; else lo = mid + 1;
   }
-  before = lo ? ends[lo - 1] : 0;
   return lo;
 }
-
-// The x-th page: from where it is given back, or from the stack, to where it is taken, or to the stack
-__device__ inline void move_page(const DPages& p, const PagePlan& plan, const int64_t* gone_ends, const int64_t* more_ends, const int32_t* firsts, int64_t x) {
-  const int64_t place = plan.count + plan.gone - 1 - x;             // from the top of the stack, with what is given back on it
-  if (place < 0 || place >= p.pages) return;                        // (more given back than the pool has pages: not a table of this pool)
-  int32_t id;
-  if (x < plan.gone) {
-    int64_t before;
-    const int b = share_of(gone_ends, p.seqs, x, before);
-    int32_t* const from = p.table + (int64_t)b * p.ld + firsts[b] + (x - before);
-    id = *from;
-    *from = -1;
-    p.free[place] = id;
-  } else {
-    id = p.free[place];
-  }
-  if (x < plan.taken) {
-    int64_t before;
-    const int b = share_of(more_ends, p.seqs, x, before);
-    p.table[(int64_t)b * p.ld + firsts[b] + (x - before)] = id;
-  }
+// The entry of the table that the x-th page of a list leaves or goes to, if sequence b has it
+__device__ inline int32_t* entry_of(const DPages& p, const int32_t* ends, const int32_t* first, int b, int x) {
+  return p.table + (int64_t)b * p.ld + first[b] + (x - (b ? ends[b - 1] : 0));
 }
 
-__global__ __launch_bounds__(PLAN_THREADS) void pages_plan_kernel(DPages p, const int32_t* want, int32_t* starts, uint8_t* ws, int inline_moves) {
-  __shared__ int64_t sh[PLAN_THREADS / 64];
-  PagePlan* const out = (PagePlan*)ws;
-  int64_t* const gone_ends = (int64_t*)(ws + 64);
-  int64_t* const more_ends = gone_ends + p.seqs;
-  int32_t* const firsts = (int32_t*)(more_ends + p.seqs);
-  const int tid = threadIdx.x, each = (p.seqs + PLAN_THREADS - 1) / PLAN_THREADS;
-  const int b0 = (int)min((int64_t)tid * each, (int64_t)p.seqs), b1 = min(b0 + each, p.seqs);
+// T threads; ONE: no more sequences than that, one a thread; HERE: the pages are moved too, not by a second launch
+template <int T, bool ONE, bool HERE>
+__global__ __launch_bounds__(T) void pages_plan_kernel(DPages p, const int32_t* want, int32_t* starts, uint8_t* ws) {
+  __shared__ int sha[T / 64], shb[T / 64], shd[T / 64];
+  __shared__ int64_t shc[T / 64];
+  __shared__ int32_t ends_sh[HERE ? 3 * T : 1];
+  int32_t* const of = HERE ? ends_sh : (int32_t*)(ws + sizeof(PagePlan));
+  const int n = HERE ? T : p.seqs;
+  const PageEnds ends{of, of + n, of + 2 * n};
+  const int tid = threadIdx.x, each = ONE ? 1 : (p.seqs + T - 1) / T;
+  const int b0 = ONE ? min(tid, p.seqs) : (int)min((int64_t)tid * each, (int64_t)p.seqs), b1 = min(b0 + each, p.seqs);
   const int64_t count = min(max((int64_t)*p.count, (int64_t)0), p.pages);
-  int64_t gone = 0, more = 0, all_gone, all_more;
+  Change mine{};
+  int gone = 0, more = 0, all_gone, all_more;
   for (int b = b0; b < b1; ++b) {
-    const Change c = change_of(p, want, p.lens[b], b);
-    gone += max(c.have - c.need, 0);
-    more += max(c.need - c.have, 0);
+    mine = change_of(p, want, b);
+    gone += max(mine.have - mine.need, 0);
+    more += max(mine.need - mine.have, 0);
   }
-  int64_t gone_at = block_scan(gone, sh, all_gone) - gone, more_at = block_scan(more, sh, all_more) - more;
+  int gone_at = gone, more_at = more;
+  block_scan<T>(gone_at, more_at, all_gone, all_more, sha, shb);
+  gone_at -= gone; more_at -= more;                                 // before this thread's sequences
   const int64_t there = min(count + all_gone, p.pages);
   // who is served, and what each gains
-  int64_t gained = 0, taken = 0, all_gained, all_taken;
-  int64_t at = more_at;
+  int64_t gained = 0, all_gained;
+  int taken = 0, all_taken, at = more_at;
   for (int b = b0; b < b1; ++b) {
-    const int len = min(max(p.lens[b], 0), p.cols * p.page);
-    const Change c = change_of(p, want, len, b);
+    const Change c = ONE ? mine : change_of(p, want, b);
     const int m = max(c.need - c.have, 0);
     at += m;
-    if (m == 0 || at <= there) {
-      gained += max(c.now - len, 0);
-      taken += m;
-    }
+    if (m == 0 || at <= there) { gained += max(c.now - c.len, 0); taken += m; }
   }
-  int64_t row = block_scan(gained, sh, all_gained) - gained;
-  block_scan(taken, sh, all_taken);
-  if (starts && tid == 0) starts[p.seqs] = (int32_t)min(all_gained, (int64_t)0x7fffffff);
+  int64_t row = gained;
+  int took = taken;
+  block_scan<T>(row, took, all_gained, all_taken, shc, shd);
+  row -= gained; took -= taken;
+  constexpr int64_t most = 0x7fffffff;
+  if (starts && tid == 0) starts[p.seqs] = (int32_t)min(all_gained, most);
   at = more_at;
-  int64_t took = min(more_at, all_taken);
   for (int b = b0; b < b1; ++b) {
-    const int len = min(max(p.lens[b], 0), p.cols * p.page);
-    const Change c = change_of(p, want, len, b);
+    const Change c = ONE ? mine : change_of(p, want, b);
     const int m = max(c.need - c.have, 0);
     at += m;
     const bool served = m == 0 || at <= there;
-    if (starts) starts[b] = (int32_t)min(row, (int64_t)0x7fffffff);
-    row += served ? max(c.now - len, 0) : 0;
+    if (starts) starts[b] = (int32_t)min(row, most);
+    row += served ? max(c.now - c.len, 0) : 0;
     gone_at += max(c.have - c.need, 0);
     took += served ? m : 0;
-    gone_ends[b] = gone_at;
-    more_ends[b] = took;
-    firsts[b] = min(c.have, c.need);
-    p.lens[b] = served ? c.now : len;
+    ends.gone[b] = gone_at;
+    ends.more[b] = took;
+    ends.first[b] = min(c.have, c.need);
+    p.lens[b] = served ? c.now : c.len;
   }
-  PagePlan plan{count, all_gone, all_taken, max(all_gone, all_taken)};
+  const PagePlan plan{count, all_gone, all_taken, max(all_gone, all_taken)};
   if (tid == 0) *p.count = (int32_t)max(there - all_taken, (int64_t)0);
-  if (!inline_moves) {
-    if (tid == 0) *out = plan;
+  if constexpr (!HERE) {
+    if (tid == 0) *(PagePlan*)ws = plan;
     return;
   }
   __syncthreads();
-  for (int64_t x = tid; x < plan.moves; x += PLAN_THREADS) move_page(p, plan, gone_ends, more_ends, firsts, x);
+  for (int x = tid; x < plan.moves; x += T) {                       // (as in pages_move_kernel)
+    const int64_t place = plan.count + plan.gone - 1 - x;
+    if (place < 0 || place >= p.pages) continue;
+    int32_t id;
+    if (x < plan.gone) {
+      int32_t* const from = entry_of(p, ends.gone, ends.first, share_of(ends.gone, 0, p.seqs - 1, x), x);
+      id = *from;
+      *from = -1;
+      p.free[place] = id;
+    } else {
+      id = p.free[place];
+    }
+    if (x < plan.taken) *entry_of(p, ends.more, ends.first, share_of(ends.more, 0, p.seqs - 1, x), x) = id;
+  }
 }
 
+// For two numbers that are the same in all lanes, the first i < n whose entry of an ascending list passes them (n: none does):
+// a 64th of the list a step.  above(i, x): whether entry i passes x.
+template <class F>
+__device__ inline void first_above(int n, int lane, int x0, int x1, int& i0, int& i1, F above) {
+  int lo0 = 0, lo1 = 0, width = n;                                  // the answer is in [lo, lo + width]
+  while (width > 0) {
+    const int step = (width + 63) / 64;
+    const int a = lo0 + (lane + 1) * step - 1, b = lo1 + (lane + 1) * step - 1;
+    const bool pa = a >= n || above(a, x0), pb = b >= n || above(b, x1);
+    const uint64_t ma = __ballot(pa), mb = __ballot(pb);
+    lo0 += (ma ? __ffsll((unsigned long long)ma) - 1 : 64) * step;
+    lo1 += (mb ? __ffsll((unsigned long long)mb) - 1 : 64) * step;
+    width = step - 1;
+  }
+  i0 = min(lo0, n); i1 = min(lo1, n);
+}
+
+constexpr int MOVES = 2;                    // pages a thread at a time
+
+// The x-th page from the place it leaves (the table, or the stack) to the one it goes to (the stack, the table).  A workgroup takes neighbours, of few
+// sequences.  SMALL: at most INLINE_SEQS sequences, whose sums come into LDS at once instead of by loads that wait for one another.
+template <bool SMALL>
 __global__ __launch_bounds__(256) void pages_move_kernel(DPages p, const uint8_t* ws) {
+  __shared__ int32_t of_sh[SMALL ? 3 * INLINE_SEQS : 1];
+  const int32_t* of = (const int32_t*)(ws + sizeof(PagePlan));
+  const int lane = threadIdx.x & 63;
+  constexpr int N = SMALL ? 3 * INLINE_SEQS / 256 : 1;
+  int32_t sums[N];
+  if constexpr (SMALL)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[i] = of[min(i * 256 + (int)threadIdx.x, 3 * p.seqs - 1)];
   const PagePlan plan = *(const PagePlan*)ws;
-  const int64_t* const gone_ends = (const int64_t*)(ws + 64);
-  const int64_t* const more_ends = gone_ends + p.seqs;
-  const int32_t* const firsts = (const int32_t*)(more_ends + p.seqs);
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < plan.moves; x += (int64_t)gridDim.x * 256)
-    move_page(p, plan, gone_ends, more_ends, firsts, x);
+  if ((int64_t)blockIdx.x * (256 * MOVES) >= plan.moves) return;
+  if constexpr (SMALL) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) of_sh[i * 256 + threadIdx.x] = sums[i];
+    __syncthreads();
+  }
+  const int32_t *const gone = SMALL ? of_sh : of, *const more = gone + p.seqs, *const first = gone + 2 * p.seqs;
+  for (int64_t base = (int64_t)blockIdx.x * (256 * MOVES); base < plan.moves; base += (int64_t)gridDim.x * (256 * MOVES)) {
+    const int x0 = (int)base, x1 = (int)min(base + 256 * MOVES, plan.moves) - 1;
+    int g0 = 0, g1 = 0, m0 = 0, m1 = 0;                             // the sequences that they can be of
+    if (x0 < plan.gone) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.gone - 1), g0, g1, [&](int i, int x) { return gone[i] > x; });
+    if (x0 < plan.taken) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.taken - 1), m0, m1, [&](int i, int x) { return more[i] > x; });
+    int32_t id[MOVES];
+    int32_t* from[MOVES];
+#pragma unroll
+    for (int u = 0; u < MOVES; ++u) {
+      const int64_t x = base + u * 256 + threadIdx.x, place = plan.count + plan.gone - 1 - x;   // from the top of the stack, with what is given back on it
+      from[u] = nullptr;
+      if (x >= plan.moves || place < 0 || place >= p.pages) continue;   // (more given back than the pool has pages: not a table of this pool)
+      if (x < plan.gone) from[u] = entry_of(p, gone, first, share_of(gone, g0, g1, (int)x), (int)x);
+      id[u] = *(x < plan.gone ? from[u] : p.free + place);
+    }
+#pragma unroll
+    for (int u = 0; u < MOVES; ++u) {
+      const int64_t x = base + u * 256 + threadIdx.x, place = plan.count + plan.gone - 1 - x;
+      if (x >= plan.moves || place < 0 || place >= p.pages) continue;
+      int32_t* const to = x < plan.taken ? entry_of(p, more, first, share_of(more, m0, m1, (int)x), (int)x) : nullptr;
+      if (x < plan.gone) {
+        *from[u] = -1;
+        p.free[place] = id[u];
+      }
+      if (to) *to = id[u];
+    }
+  }
+}
+
+static size_t pages_workspace(const DPages& p) {                    // 0: the pages are moved by the first launch
+  const bool here = p.seqs <= INLINE_SEQS && (int64_t)p.seqs * p.cols <= INLINE_ENTRIES;
+  return here || p.seqs == 0 ? 0 : sizeof(PagePlan) + (size_t)p.seqs * 12;
 }
 
 static int to_dpages(const cbk_pages* in, DPages* p, bool need_device_ptrs) {
@@ -163,7 +234,7 @@ static int to_dpages(const cbk_pages* in, DPages* p, bool need_device_ptrs) {
   if (in->page < 16 || in->page > 256 || (in->page & (in->page - 1))) return CBK_ERR_LAYOUT;
   if (in->pages < 1 || in->pages > INT32_MAX || in->seqs < 0 || in->seqs >= 1 << 24 || in->table_cols < 0 || in->ld_table < in->table_cols)
     return CBK_ERR_SHAPE;
-  if (in->table_cols > (1 << 30) / in->page) return CBK_ERR_SHAPE;
+  if (in->table_cols > (1 << 30) / in->page || (int64_t)in->seqs * in->table_cols > INT32_MAX) return CBK_ERR_SHAPE;
   if (need_device_ptrs && in->seqs > 0) {
     if (!in->lens || !in->free_pages || !in->free_count || (in->table_cols && !in->table)) return CBK_ERR_NULL;
     if (((uintptr_t)in->lens | (uintptr_t)in->table | (uintptr_t)in->free_pages | (uintptr_t)in->free_count) & 3) return CBK_ERR_ALIGN;
@@ -174,45 +245,61 @@ static int to_dpages(const cbk_pages* in, DPages* p, bool need_device_ptrs) {
 }
 
 // ------------------------------------------------------------------ slots
-constexpr int SLOT_ROWS = 4;                // rows a thread
+constexpr int SLOT_ROWS = 2;                // rows a thread
 
-// The last sequence that begins at or before row t (its offsets ascend); -1: none does
-__device__ inline int begins_before(const DRows& r, int t, int lo, int hi) {
-  while (lo < hi) {                                                 // the answer is in [lo - 1, hi - 1]
-    const int mid = (lo + hi) / 2;
-    if (r.starts[mid] <= t) lo = mid + 1; else hi = mid;
-  }
-  return lo - 1;
-}
-
+// SMALL: at most SLOT_SEQS sequences with offsets, which come into LDS at once
+constexpr int SLOT_SEQS = 768;
+template <bool SMALL>
 __global__ __launch_bounds__(256) void cache_slots_kernel(DRows r, int64_t pages, int shift, int64_t* slots, int32_t* positions) {
+  __shared__ int32_t starts_sh[SMALL ? SLOT_SEQS + 256 : 1], lens_sh[SMALL ? SLOT_SEQS : 1];
   const int64_t first = (int64_t)blockIdx.x * (256 * SLOT_ROWS);
-  int lo = 0, hi = 0;
-  if (r.starts) {                                                   // the sequences that the workgroup's rows can be of
-    lo = begins_before(r, (int)first, 0, r.seqs + 1);
-    hi = begins_before(r, (int)min(first + 256 * SLOT_ROWS, (int64_t)r.tokens) - 1, max(lo, 0), r.seqs + 1);
+  if constexpr (SMALL) {
+    int32_t a[SLOT_SEQS / 256 + 1], b[SLOT_SEQS / 256];
+#pragma unroll
+    for (int i = 0; i <= SLOT_SEQS / 256; ++i) a[i] = r.starts[min(i * 256 + (int)threadIdx.x, r.seqs)];
+#pragma unroll
+    for (int i = 0; i < SLOT_SEQS / 256; ++i) b[i] = r.lens[min(i * 256 + (int)threadIdx.x, r.seqs - 1)];
+#pragma unroll
+    for (int i = 0; i <= SLOT_SEQS / 256; ++i) starts_sh[i * 256 + threadIdx.x] = a[i];
+#pragma unroll
+    for (int i = 0; i < SLOT_SEQS / 256; ++i) lens_sh[i * 256 + threadIdx.x] = b[i];
+    __syncthreads();
+  }
+  const int32_t *const starts = SMALL ? starts_sh : r.starts, *const lens = SMALL ? lens_sh : r.lens;
+  int lo = 0, hi = 0;                                               // offsets that pass the workgroup's first and last row: its rows are of sequences [lo - 1, hi)
+  if (starts)
+    first_above(r.seqs + 1, threadIdx.x & 63, (int)first, (int)min(first + 256 * SLOT_ROWS, (int64_t)r.tokens) - 1, lo, hi,
+                [&](int i, int t) { return starts[i] > t; });
+  int64_t slot[SLOT_ROWS];
+  int pos[SLOT_ROWS];
+  int page[SLOT_ROWS];
+#pragma unroll
+  for (int u = 0; u < SLOT_ROWS; ++u) {
+    const int64_t row = first + u * 256 + threadIdx.x;
+    const int t = (int)min(row, (int64_t)r.tokens - 1);
+    int b = hi;
+    if (SMALL || r.starts) {
+      for (int l = lo; l < b;) {                                    // (starts[hi] passes t if anything does)
+        const int mid = (l + b) / 2;
+        if (starts[mid] > t) b = mid; else l = mid + 1;
+      }
+      --b;
+    } else {
+      b = t / r.per;
+    }
+    const bool is = b >= 0 && b < r.seqs;
+    const int at = is ? b : 0, end = !is ? 0 : r.starts ? starts[b + 1] : (b + 1) * r.per;
+    const int64_t j = is ? (int64_t)max(lens[at], 0) - ((int64_t)end - t) : -1;
+    pos[u] = is && t < end ? (int)max(j, (int64_t)0) : 0;           // (its begin is at or before t)
+    page[u] = is && t < end && j >= 0 && j < r.cap ? r.table[(int64_t)b * r.ld + (j >> shift)] : -1;
+    slot[u] = j & ((1 << shift) - 1);
   }
 #pragma unroll
   for (int u = 0; u < SLOT_ROWS; ++u) {
     const int64_t row = first + u * 256 + threadIdx.x;
     if (row >= r.tokens) return;
-    const int t = (int)row;
-    const int b = r.starts ? (lo == hi ? lo : begins_before(r, t, max(lo, 0), hi + 1)) : t / r.per;
-    int64_t slot = -1;
-    int pos = 0;
-    if (b >= 0 && b < r.seqs) {
-      const int end = r.starts ? r.starts[b + 1] : (b + 1) * r.per;
-      const int64_t j = (int64_t)max(r.lens[b], 0) - ((int64_t)end - t);
-      if (t < end) {                                                // (its begin is at or before t)
-        pos = (int)max(j, (int64_t)0);
-        if (j >= 0 && j < r.cap) {
-          const int page = r.table[(int64_t)b * r.ld + (j >> shift)];
-          if (page >= 0 && page < pages) slot = ((int64_t)page << shift) + (j & ((1 << shift) - 1));
-        }
-      }
-    }
-    if (slots) slots[row] = slot;
-    if (positions) positions[row] = pos;
+    if (slots) slots[row] = page[u] >= 0 && page[u] < pages ? ((int64_t)page[u] << shift) + slot[u] : -1;
+    if (positions) positions[row] = pos[u];
   }
 }
 
@@ -224,8 +311,7 @@ extern "C" {
 
 size_t cbk_cache_pages_workspace_bytes(const cbk_pages* pages) {
   DPages p;
-  if (to_dpages(pages, &p, false) || p.seqs == 0) return 0;
-  return 64 + (size_t)p.seqs * 20;
+  return to_dpages(pages, &p, false) ? 0 : pages_workspace(p);
 }
 
 int cbk_cache_pages(const cbk_pages* pages, const void* want, void* starts, void* workspace, size_t workspace_bytes, void* stream) {
@@ -235,29 +321,38 @@ int cbk_cache_pages(const cbk_pages* pages, const void* want, void* starts, void
   if (p.seqs == 0) return CBK_OK;
   if (!want) return CBK_ERR_NULL;
   if (((uintptr_t)want | (uintptr_t)starts) & 3 || (uintptr_t)workspace & 255) return CBK_ERR_ALIGN;
-  if (!workspace || workspace_bytes < 64 + (size_t)p.seqs * 20) return CBK_ERR_WORKSPACE;
-  const int64_t entries = (int64_t)p.seqs * p.cols;                 // pages moved, at most
-  const bool here = entries <= INLINE_MOVES;
-  hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (hipStream_t)stream, p, (const int32_t*)want, (int32_t*)starts,
-                     (uint8_t*)workspace, (int)here);
-  if (!here) {
-    const int64_t most = (entries + 255) / 256;
-    hipLaunchKernelGGL(pages_move_kernel, dim3((unsigned)(most < 1024 ? most : 1024)), dim3(256), 0, (hipStream_t)stream, p, (const uint8_t*)workspace);
+  const size_t need = pages_workspace(p);
+  if (need > workspace_bytes || (need && !workspace)) return CBK_ERR_WORKSPACE;
+  uint8_t* const ws = need ? (uint8_t*)workspace : nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  auto plan = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, st, p, (const int32_t*)want, (int32_t*)starts, ws); };
+  if (p.seqs <= 256) need ? plan(pages_plan_kernel<256, true, false>, 256) : plan(pages_plan_kernel<256, true, true>, 256);
+  else if (p.seqs <= 1024) need ? plan(pages_plan_kernel<1024, true, false>, 1024) : plan(pages_plan_kernel<1024, true, true>, 1024);
+  else plan(pages_plan_kernel<1024, false, false>, 1024);
+  if (need) {
+    const int64_t most = ((int64_t)p.seqs * p.cols + 256 * MOVES - 1) / (256 * MOVES);   // pages moved, at most
+    const dim3 grid((unsigned)(most < 4096 ? (most ? most : 1) : 4096));
+    if (p.seqs <= INLINE_SEQS) hipLaunchKernelGGL(pages_move_kernel<true>, grid, dim3(256), 0, st, p, (const uint8_t*)ws);
+    else hipLaunchKernelGGL(pages_move_kernel<false>, grid, dim3(256), 0, st, p, (const uint8_t*)ws);
   }
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 
 int cbk_cache_slots(const cbk_rows* rows, int64_t pages, int page, void* slots, void* positions, void* stream) {
   if (page < 16 || page > 256 || (page & (page - 1))) return CBK_ERR_LAYOUT;
-  if (pages < 1 || pages > INT32_MAX) return CBK_ERR_SHAPE;
+  if (pages < 1 || pages > INT32_MAX || (rows && rows->seqs >= 1 << 30)) return CBK_ERR_SHAPE;
   DRows r;
   const int rc = to_drows(rows, page, &r, true);
   if (rc) return rc;
   if (((uintptr_t)slots & 7) || ((uintptr_t)positions & 3)) return CBK_ERR_ALIGN;
   if (r.tokens == 0 || (!slots && !positions)) return CBK_OK;
   const unsigned grid = (unsigned)(((int64_t)r.tokens + 256 * SLOT_ROWS - 1) / (256 * SLOT_ROWS));
-  hipLaunchKernelGGL(cache_slots_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, r, pages, __builtin_ctz((unsigned)page), (int64_t*)slots,
-                     (int32_t*)positions);
+  if (r.starts && r.seqs > 0 && r.seqs <= SLOT_SEQS)
+    hipLaunchKernelGGL(cache_slots_kernel<true>, dim3(grid), dim3(256), 0, (hipStream_t)stream, r, pages, __builtin_ctz((unsigned)page),
+                       (int64_t*)slots, (int32_t*)positions);
+  else
+    hipLaunchKernelGGL(cache_slots_kernel<false>, dim3(grid), dim3(256), 0, (hipStream_t)stream, r, pages, __builtin_ctz((unsigned)page),
+                       (int64_t*)slots, (int32_t*)positions);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

@@ -176,9 +176,12 @@ def test_tables_refuse_bad_descriptions_before_any_launch():
         assert _resize(_pages(**kw)) == want, kw
     assert _resize(_pages(), want=None) == -1
     assert _resize(_pages(), want=0x9002) == -4 and _resize(_pages(), starts=0xa001) == -4 and _resize(_pages(), ws=0x10010) == -4
-    need = _lib.lib().cbk_cache_pages_workspace_bytes(ctypes.byref(_pages()))
-    assert need > 0
-    assert _resize(_pages(), room=need - 1) == -6 and _resize(_pages(), ws=None) == -6
+    assert _lib.lib().cbk_cache_pages_workspace_bytes(ctypes.byref(_pages())) == 0
+    for kw in (dict(seqs=2000), dict(seqs=100, table_cols=100, ld_table=100)):
+        need = _lib.lib().cbk_cache_pages_workspace_bytes(ctypes.byref(_pages(**kw)))
+        assert need > 0
+        assert _resize(_pages(**kw), room=need - 1) == -6 and _resize(_pages(**kw), ws=None) == -6
+    assert _resize(_pages(seqs=1 << 16, table_cols=1 << 15, ld_table=1 << 15)) == -3              # 2^31 entries
     assert _resize(_pages(seqs=0)) == 0                             # nothing to do
     assert _lib.lib().cbk_cache_pages(None, None, None, None, 0, None) == -1
 
