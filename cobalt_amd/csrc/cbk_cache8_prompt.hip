@@ -8,8 +8,10 @@
 // LDS read is a run of 1 KB without bank conflicts.  Which channels a block of V^T has is free: those whose stores by neighbouring lanes lie
 // side by side.
 //
-// While the products of a tile run, the next one, whose codes were loaded a tile before, is widened into the other half of
-// LDS: four wavefronts take the keys, four the values, 16 tokens of (at most) 128 channels each.  One barrier for a tile's two blocks.
+// While the products of a tile run, the next one, whose codes were loaded before, is widened into the other half of LDS: four
+// wavefronts take the keys, four the values, 16 tokens of (at most) 128 channels each, half a tile at a time.  A SIMD has one of either.  Keys
+// are widened in front of a block, values behind it, so that one wavefront multiplies while the other one does not; products go first
+// (s_setprio).  (Both behind the scores' products: 168 us for the 4096-token prompt below, apart 160, with priorities 157.)  One barrier for a tile's two blocks.
 //
 // bf16 results: queries with the scale of the scores in them and p rounded once to fp16 (an eighth of the result's own step).  fp16 results: queries as
 // they are, and p with its rest as a second operand.
@@ -17,6 +19,10 @@
 // Work is dealt out in one of two ways (plan_prompt8).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
 // workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
 // of a tile that it does not finish is joined by the second launch (cbk_cache_attn.hip).
+//
+// A 4096-token prompt of 32 query heads on 8, 128 channels: bf16 158 us, 870 TFLOP/s (a large library product reaches 1200), fp16 230 us with its half more
+// products; of 8192 tokens and 64 channels 366 and 555 us, where an exponential and five instructions a score bound it; 4096 tokens of 16 heads on
+// 4, 256 channels, 242 and 316 us.
 #include <type_traits>
 #include "cbk_cache8.h"
 #include "cbk_cache_attn.h"
@@ -25,6 +31,12 @@
 namespace cbk {
 
 constexpr int OWN8 = 2;                     // tiles of tokens that a tile of rows counts for by itself: its queries, its start and end
+
+// The larger of a lane's number and that of the lane 32 on, without the trip through LDS, which the stores of the next tile keep busy
+__device__ inline float halves_max(float x) {
+  const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+}
 
 template <int D>
 struct Tile8 {
@@ -237,13 +249,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
 
   for (int t = t0; t < t1; ++t) {
     uint8_t* const buf = lds + ((t - t0) & 1) * T::BYTES;
+    uint8_t* const next = lds + ((t + 1 - t0) & 1) * T::BYTES;
     const v2u flags = *(const v2u*)(buf + T::BYTES - 16);
     auto block = [&](auto which) {
     constexpr int hb = decltype(which)::value;
     const int tok = token_of(t) + hb * T::BLOCK;
     const bool mine = wvalid > 0 && tok <= wpos_hi && (a.window <= 0 || tok + T::BLOCK > wpos_lo - a.window + 1 || tok < a.sinks);
     v16f sc[T::KT];
+    if (takes_keys && t + 1 < t1) {                                 // in front of the block: the other wavefront of the SIMD multiplies meanwhile
+      widen(next, which);
+      if (hb == 1 && t + 2 < t1) {
+        fetch(t + 2);
+        pages_at(min(t + 3, t1 - 1));
+      }
+    }
     if (mine) {
+      __builtin_amdgcn_s_setprio(1);
       const uint8_t* const from = buf + lane * 16;
 #pragma unroll
       for (int kt = 0; kt < T::KT; ++kt)
@@ -254,8 +275,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
 #pragma unroll
         for (int kt = 0; kt < T::KT; ++kt)
           sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(from + ((hb * T::KT + kt) * T::KS + k) * 1024), q[k], sc[kt], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(0);
+      asm volatile("s_nop 3");                                      // (the scores are looked at next: on every path as far behind the products as the build wants it)
     }
-    if (t + 1 < t1) widen(lds + ((t + 1 - t0) & 1) * T::BYTES, which);
     if (mine) {
       // every row of the wavefront sees all tokens of the tile, and all of them are there
       bool whole = tok + T::BLOCK <= s.held && tok + T::BLOCK - 1 <= wpos_lo && (a.window <= 0 || tok > wpos_hi - a.window || tok + T::BLOCK <= a.sinks);
@@ -282,7 +305,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
       for (int kt = 0; kt < T::KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kt][i]);
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = halves_max(top);
       if constexpr (BF) {
         if (!ready || __ballot(top > P_BITS + P_SLACK)) {             // the maximum follows when p would leave its range
           const float g = ready ? 1.f : grow;
@@ -331,6 +354,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
           }
         }
       };
+      __builtin_amdgcn_s_setprio(1);
       weights(0);
 #pragma unroll
       for (int st = 0; st < T::VS; ++st) {
@@ -343,14 +367,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
           if constexpr (!BF) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, rest[st & 1], o[v], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
+    }
+    if (!takes_keys && t + 1 < t1) {                                // behind it
+      widen(next, which);
+      if (hb == 1 && t + 2 < t1) {
+        fetch(t + 2);
+        pages_at(min(t + 3, t1 - 1));
+      }
     }
     };
     block(std::integral_constant<int, 0>{});
     block(std::integral_constant<int, 1>{});
-    if (t + 2 < t1) {
-      fetch(t + 2);
-      pages_at(min(t + 3, t1 - 1));
-    }
     __syncthreads();
   }
 
