@@ -8,8 +8,8 @@ protocol of the reference's src/prod/bench.py: steady-state tokens per second at
 that the number is the GPU work of a step and not the Python dispatch of its ~40 small kernels
 per block.  Prints one JSON line per measurement.  There are no checkpoints or datasets here:
 weights are random-initialised and calibration tokens are random ids, which leaves the timing
-unaffected and says nothing about accuracy.  `--cache 4bit` decodes on the 4-bit key/value cache
-(`model.cobalt_cache`) instead of a static fp16 one, `--context` after a longer prompt.
+unaffected and says nothing about accuracy.  `--cache 4bit` and `--cache 8bit` decode on the key/value cache in
+4 or 8 bits (`model.cobalt_cache`) instead of a static fp16 one, `--context` after a longer prompt.
 """
 from __future__ import annotations
 
@@ -21,10 +21,10 @@ import torch
 
 
 def _decode_tokens_per_s(tr, model, cfg, dev, steps: int, prompt: int, max_len: int, kind: str = "fp16") -> float:
-    if kind == "4bit":
+    if kind in ("4bit", "8bit"):
         from .model import cobalt_cache
         was = model.config._attn_implementation
-        cache = cobalt_cache(model, 1, max_len)
+        cache = cobalt_cache(model, 1, max_len, bits=int(kind[0]))
         try:
             return _steps_per_s(model, cfg, dev, steps, prompt, cache)
         finally:
@@ -89,7 +89,7 @@ def main(argv=None):
     ap.add_argument("--group", type=int, default=128)
     ap.add_argument("--steps", type=int, default=128)
     ap.add_argument("--prefill", type=int, default=2048)
-    ap.add_argument("--cache", choices=("fp16", "4bit"), default="fp16", help="the key/value cache of the decode steps")
+    ap.add_argument("--cache", choices=("fp16", "4bit", "8bit"), default="fp16", help="the key/value cache of the decode steps")
     ap.add_argument("--context", type=int, default=16, help="tokens of the prompt in front of the decode steps")
     a = ap.parse_args(argv)
     import transformers as tr

@@ -1,8 +1,9 @@
-"""A Hugging Face decoder on the 4-bit key/value cache: `model.cobalt_cache` builds the cache that is passed as
+"""A Hugging Face decoder on the key/value cache in 4 or 8 bits: `model.cobalt_cache` builds the cache that is passed as
 `past_key_values`; the model's attention layers then call `cobalt_attention`, which writes their keys and values with
 `ops.cache_write` and reads the cache with `ops.cache_attention`, prompts and single tokens alike."""
 from __future__ import annotations
 
+from functools import partial
 from types import FunctionType
 from typing import Optional
 
@@ -12,7 +13,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from transformers.masking_utils import causal_mask_function, sliding_window_causal_mask_function
 
 from . import ops
-from .cache import KVCache, KVRows
+from .cache import KVCache, KVCache8, KVPages, KVRows
 
 NAME = "cobalt_cache"
 DTYPES = (torch.float16, torch.bfloat16)
@@ -25,21 +26,25 @@ def _recording() -> bool:
 class _Sequences:
     """What the layers of one cache share: the pages, the lengths, and the rows of the step under way."""
 
-    def __init__(self, batch: int, max_len: int, page: int, device):
+    def __init__(self, batch: int, max_len: int, page: int, device, pages: Optional[int] = None):
         if batch < 1 or max_len < 1:
             raise ValueError(f"batch and max_len must be at least 1, got {batch} and {max_len}")
         self.batch, self.max_len, self.page = batch, max_len, page
         per = -(-max_len // page)
-        self.pages = batch * per
-        self.table = torch.arange(self.pages, dtype=torch.int32, device=device).view(batch, per)
+        self.pages = batch * per if pages is None else pages
+        # each sequence has pages for all of `max_len`, or they take them as they grow
+        self.tables = None if pages is None else KVPages(pages, batch, max_len, page=page, device=device)
+        self.table = torch.arange(self.pages, dtype=torch.int32, device=device).view(batch, per) if pages is None else self.tables.table
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)         # real tokens, padding left out
         self.seen = torch.zeros((), dtype=torch.int64, device=device)            # tokens with the padding
         self.waiting = False     # a layer has handed on its keys and values, which its attention has not taken yet
         self.recorded = False    # a step has been: its replays advance the lengths on the device alone
-        self.clear()
+        self.clear(first=True)
 
-    def clear(self):
+    def clear(self, first: bool = False):
         self.lens.zero_()
+        if self.tables is not None and not first:
+            ops.cache_pages(self.tables, self.lens)
         self.seen.zero_()
         self.waiting = False
         self.steps = 0           # `seen` as the host knows it (issued())
@@ -52,7 +57,7 @@ class _Sequences:
         """Refuses a model some of whose layers attend by themselves, over what `update` gives them: the step's own keys and values."""
         if self.waiting:
             self.waiting = False
-            raise RuntimeError('a layer that uses the 4-bit cache has not called the attention "cobalt_cache": the model does not take it, or its '
+            raise RuntimeError('a layer that uses the cache has not called the attention "cobalt_cache": the model does not take it, or its '
                                "attention was switched back while the cache is in use")
 
     def issued(self) -> int:
@@ -77,6 +82,12 @@ class _Sequences:
                 self.pads = pads
             elif pads != self.pads:
                 raise ValueError("attention_mask: padding belongs in front of a sequence, in the first call")
+        if self.tables is not None:
+            need = sum(-(-(steps + tokens - p) // self.page) for p in self.pads)
+            if need > self.pages:
+                if first:
+                    self.pads = [0] * self.batch
+                raise ValueError(f"the cache has {self.pages} pages of {self.page} tokens, the step ends with {need}")
         self.mask, self.first = mask, first
         if _recording():
             self.recorded = True
@@ -84,11 +95,15 @@ class _Sequences:
             self.steps += tokens
         self.seen.add_(tokens)
         self.lens.add_(tokens)
-        self.rows = KVRows(self.table, self.lens)
-        if first and any(self.pads):
-            # the padding's rows belong to sequences of their own, which are empty and have no pages: not written, and 0 as the answer
+        padded = first and any(self.pads)
+        if padded:
             pads = torch.tensor(self.pads, dtype=torch.int32).to(self.lens.device)
             self.lens.sub_(pads)
+        if self.tables is not None:                                 # (a replay that they do not last for: tokens without pages, not written)
+            ops.cache_pages(self.tables, self.lens)
+        self.rows = KVRows(self.table, self.lens)
+        if padded:
+            # the padding's rows belong to sequences of their own, which are empty and have no pages: not written, and 0 as the answer
             ends = torch.arange(batch, dtype=torch.int32, device=pads.device) * tokens
             starts = torch.stack([ends, ends + pads], 1).flatten()
             self.rows = KVRows(torch.stack([torch.full_like(self.table, -1), self.table], 1).flatten(0, 1).contiguous(),
@@ -127,18 +142,17 @@ class CobaltCacheLayer(CacheLayerMixin):
     is_compileable = False
     is_sliding = False
 
-    def __init__(self, sequences: _Sequences, index: int, group: int, window: Optional[int], sinks: int):
+    def __init__(self, sequences: _Sequences, index: int, make_pool, window: Optional[int], sinks: int):
         super().__init__()
-        self.sequences, self.index, self.group, self.window, self.sinks = sequences, index, group, window, sinks
-        self.pool: Optional[KVCache] = None
+        self.sequences, self.index, self.make_pool, self.window, self.sinks = sequences, index, make_pool, window, sinks
+        self.pool = None
 
     def lazy_initialization(self, key_states, value_states):
         if key_states.shape != value_states.shape:
             raise ValueError(f"keys {list(key_states.shape)} and values {list(value_states.shape)} must have the same shape")
         if key_states.is_cuda and _recording():
             raise RuntimeError("the first call with a new cache makes its pages: it cannot be recorded in a graph")
-        self.pool = KVCache(self.sequences.pages, key_states.shape[1], key_states.shape[3], page=self.sequences.page, group=self.group,
-                            device=key_states.device)
+        self.pool = self.make_pool(self.sequences.pages, key_states.shape[1], key_states.shape[3], page=self.sequences.page, device=key_states.device)
         self.is_initialized = True
 
     def update(self, key_states, value_states, *args, **kwargs):
@@ -165,7 +179,7 @@ class CobaltCacheLayer(CacheLayerMixin):
         self.sequences.clear()
 
     def _refuse(self, *args, **kwargs):
-        raise NotImplementedError("the 4-bit cache does not reorder, repeat, select or crop its sequences, and is not offloaded")
+        raise NotImplementedError("this cache does not reorder, repeat, select or crop its sequences, and is not offloaded")
 
     reorder_cache = batch_repeat_interleave = batch_select_indices = crop = offload = prefetch = _refuse
 
@@ -178,12 +192,12 @@ def cobalt_attention(module, query, key, value, attention_mask, scaling=None, dr
     fresh, layer.sequences.waiting = layer.sequences.waiting, False    # (not fresh: a layer that shares the keys and values of an earlier one)
     if dropout or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None or not getattr(module, "is_causal", True) \
             or kwargs.get("is_causal") is False:
-        raise ValueError("attention over the 4-bit cache is causal, without dropout, soft caps or learned sinks")
+        raise ValueError("attention over this cache is causal, without dropout, soft caps or learned sinks")
     if query.requires_grad or key.requires_grad or value.requires_grad:
-        raise RuntimeError("the 4-bit cache has no backward pass: call the model under torch.no_grad()")
+        raise RuntimeError("this cache has no backward pass: call the model under torch.no_grad()")
     types = {x.dtype for x in (query, key, value)}
     if len(types) > 1 or not types <= set(DTYPES):                   # (before the lengths advance)
-        raise TypeError(f"the 4-bit cache is for float16 and bfloat16 models, not {', '.join(sorted(map(str, types)))}")
+        raise TypeError(f"this cache is for float16 and bfloat16 models, not {', '.join(sorted(map(str, types)))}")
     batch, _, tokens, _ = query.shape
     window = sliding_window or layer.window                          # (models that leave it to their mask do not pass one)
     if layer.index == 0 and fresh:
@@ -240,26 +254,29 @@ def _padding_mask(batch_size=1, q_length=1, kv_length=1, q_offset=0, kv_offset=0
         raise ValueError("a mask that a model adds to the causal one is read by the host: such a step cannot be recorded in a graph")
     heads = getattr(config, "num_attention_heads", 1)
     if not any(_answers_alike(mask_function, f, batch_size, heads, q_length, kv_length, q_offset, kv_offset, device) for f in plain):
-        raise ValueError("attention over the 4-bit cache is causal, under a sliding window at most: this step's mask says otherwise "
+        raise ValueError("attention over this cache is causal, under a sliding window at most: this step's mask says otherwise "
                          "(tokens that see later ones, or blocks that are kept apart)")
     return mask
 
 
-def build(model, batch: int, max_len: int, page: int, group: int, sinks: int) -> Cache:
+def build(model, batch: int, max_len: int, page: int, group: int, sinks: int, bits: int = 4, block: int = 16, pages: Optional[int] = None) -> Cache:
+    if bits not in (4, 8):
+        raise ValueError(f"the cache holds 4 or 8 bits a value, not {bits}")
+    make_pool = partial(KVCache, group=group) if bits == 4 else partial(KVCache8, block=block)
     cfg = model.config.get_text_config()
     types = getattr(cfg, "layer_types", None) or ["full_attention"] * cfg.num_hidden_layers
     kinds = set(types)
     if kinds - {"full_attention", "sliding_attention"} or getattr(model.config, "is_encoder_decoder", False):
-        raise ValueError(f"the 4-bit cache is for decoders of full and sliding-window attention, not {sorted(kinds)}")
+        raise ValueError(f"this cache is for decoders of full and sliding-window attention, not {sorted(kinds)}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     AttentionInterface.register(NAME, cobalt_attention)
     AttentionMaskInterface.register(NAME, _padding_mask)
-    seqs = _Sequences(batch, max_len, page, next(model.parameters()).device)
+    seqs = _Sequences(batch, max_len, page, next(model.parameters()).device, pages)
     window = lambda kind: getattr(cfg, "sliding_window", None) if kind == "sliding_attention" else None
-    cache = Cache(layers=[CobaltCacheLayer(seqs, i, group, window(kind), sinks) for i, kind in enumerate(types)])
+    cache = Cache(layers=[CobaltCacheLayer(seqs, i, make_pool, window(kind), sinks) for i, kind in enumerate(types)])
     decoder = model.get_decoder() or model                              # (a vision tower of the same model keeps its own)
     decoder.set_attn_implementation(NAME)
     if decoder.config._attn_implementation != NAME:
-        raise ValueError(f"{type(decoder).__name__} has an attention of its own that cannot be switched: no 4-bit cache for it")
+        raise ValueError(f"{type(decoder).__name__} has an attention of its own that cannot be switched: no such cache for it")
     return cache

@@ -396,16 +396,18 @@ def load_compressed_state_dict(model: nn.Module, state_dict: Dict[str, torch.Ten
     return model.load_state_dict(state_dict, strict=strict)
 
 
-def cobalt_cache(model: nn.Module, batch: int, max_len: int, page: int = 64, group: int = 32, sinks: int = 0):
-    """A key/value cache in 4 bits for a Hugging Face decoder: `batch` sequences of up to `max_len` tokens, 4 + 32 / group
-    bits a value.  Pass it as `past_key_values` to the model or to its `generate` (not with beams); the model's attention
+def cobalt_cache(model: nn.Module, batch: int, max_len: int, page: int = 64, group: int = 32, sinks: int = 0, bits: int = 4, block: int = 16,
+                 pages: Optional[int] = None):
+    """A key/value cache in 4 or 8 `bits` for a Hugging Face decoder: `batch` sequences of up to `max_len` tokens, 4 + 32 / group
+    bits a value, or 8 with a scale for each `block` tokens of a head.  `pages`: of each layer's pool, which the sequences then share and take from as
+    they grow (a step that they would not last for is refused); by default each sequence has its own for all of `max_len`.  Pass it as `past_key_values` to the model or to its `generate` (not with beams); the model's attention
     implementation is switched to it (of a mixed-modal model the text decoder's), and `model.set_attn_implementation` switches it back.
     Sliding-window layers also see the first `sinks` tokens of a sequence.  A batch may be padded in front (2-D `attention_mask`, which
     the host reads in every step that passes one); other masks that hide or show more than the causal or sliding one are refused.  A step without a mask can be
     recorded in a graph; its replays go on from the lengths on the device, and past the pages of `max_len` write nothing.  Eager steps may
     follow them (each then waits for the device to tell the lengths).  `cache.reset()` empties it."""
     from . import hf_cache
-    return hf_cache.build(model, batch, max_len, page, group, sinks)
+    return hf_cache.build(model, batch, max_len, page, group, sinks, bits, block, pages)
 
 
 def dense_twin(model: nn.Module, dtype: Optional[torch.dtype] = None) -> nn.Module:
