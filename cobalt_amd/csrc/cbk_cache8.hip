@@ -56,18 +56,36 @@ __device__ inline void transpose4(uint32_t (&x)[4]) {
   x[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
+// The sequence that row t (the same in all lanes) belongs to or would: the last offset at or before it, found a 64th of the list a step
+__device__ inline int sequence_of(const DRows& r, int t, int lane) {
+  if (!r.starts) return t / r.per;
+  int lo = 0;                                                       // the first offset that passes t is in [lo, lo + width]
+  for (int width = r.seqs + 1; width > 0;) {
+    const int step = (width + 63) / 64;
+    const int64_t at = lo + (int64_t)(lane + 1) * step - 1;
+    const uint64_t m = __ballot(at > r.seqs || r.starts[at] > t);
+    lo += (m ? __ffsll((unsigned long long)m) - 1 : 64) * step;
+    width = step - 1;
+  }
+  return min(lo, r.seqs + 1) - 1;
+}
+
 // What begins among rows [t, end): calls f(first row, rows, sequence, position of the first) for each run of one sequence's rows in
 // one block of 2^shift tokens.  Uniform over the workgroup.
 template <class F>
 __device__ inline void runs_from(const DRows& r, int t, int end, int shift, int lane, F f) {
-  int b = seq_at(r, t, lane);
+  int b = sequence_of(r, t, lane);
   while (t < end) {
     if (!r.starts) b = t / r.per;
-    else
-      while (b < r.seqs && r.starts[b + 1] <= t) ++b;               // (-1: in front of the first)
     if (b >= r.seqs) return;
     const Seq s = seq_of(r, max(b, 0));
-    if (b < 0 || t < s.first || t >= s.first + s.n) { ++t; continue; }
+    if (b < 0 || t < s.first || t >= s.first + s.n) {               // in front of the first sequence, or behind this one
+      const int was = b;
+      if (r.starts)
+        while (b < r.seqs && r.starts[b + 1] <= t) ++b;
+      if (b == was) ++t;
+      continue;
+    }
     const int pos = s.pos0 + (t - s.first), in = pos & ((1 << shift) - 1), left = (1 << shift) - in;
     const int rows = min(left, s.first + s.n - t);
     if (t == s.first || in == 0) f(t, rows, b, pos);
@@ -89,13 +107,9 @@ __global__ __launch_bounds__(64 * (NW == 1 ? 4 : NW)) void cache8_write_kernel(D
   const Parts8 at(c, h, D);
   int turn = 0;
   runs_from(r, (int)first, min((int)first + chunk, r.tokens), c.block_shift, lane, [&](int t, int rows, int b, int pos) {
-    const int page = pos < 0 ? -1 : page_of(c, r, b, pos);
-    if (page < 0) return;                                           // (all of the run: a block is on one page)
     const int from = pos & (16 * NW - 1);                           // the run is tokens [from, from + rows) of the block
     const uint32_t in = pos & (c.page - 1) & ~(16 * NW - 1);        // where the block begins in the page
     const bool anew = from == 0;
-    float2* const sc = c.sc + at.scale(page) + (in >> c.block_shift);
-    const float2 was = *sc;
     // ---- the numbers, and the largest magnitudes
     Sixteens<CH> xk[Q][4], xv[Q][4];
     bool is[Q][4];
@@ -112,6 +126,10 @@ __global__ __launch_bounds__(64 * (NW == 1 ? 4 : NW)) void cache8_write_kernel(D
           xv[q][i] = load16<CH>(io.v, row * io.vt + h * io.vh + e * CH);
         }
       }
+    const int page = pos < 0 ? -1 : page_of(c, r, b, pos);          // (looked up while the numbers are on their way)
+    if (page < 0) return;                                           // (all of the run: a block is on one page)
+    float2* const sc = c.sc + at.scale(page) + (in >> c.block_shift);
+    const float2 was = *sc;
     v2s tk = {0, 0}, tv = {0, 0};
     uint32_t nan = 0;                                               // a bit a token
     constexpr uint16_t inf = DT == CBK_F16 ? 0x7c00 : 0x7f80;
@@ -178,6 +196,11 @@ __global__ __launch_bounds__(64 * (NW == 1 ? 4 : NW)) void cache8_write_kernel(D
         const bool bad = nan >> (4 * q + i) & 1;
         uint32_t* const kp = (uint32_t*)(c.kc + code + (uint32_t)((in + 4 * quad + i) * D + e * CH));
         uint32_t kw[T::W];
+        if (__ballot(is[q][i]) == 0 && !grown_k) {                  // (single tokens: three of four)
+#pragma unroll
+          for (int w = 0; w < T::W; ++w) vw[w][i] = 0;
+          continue;
+        }
 #pragma unroll
         for (int w = 0; w < T::W; ++w) {
           float x[4], y[4];
