@@ -294,10 +294,13 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
   return p;
 }
 
-// Which of the two kernels: that of cbk_cache8_prompt.hip takes tiles of 256 rows, filled or not
+// Which of the two kernels.  That of cbk_cache8_prompt.hip takes tiles of 256 rows, filled or not, and wins from about 50 rows a sequence (128 channels, 8
+// cache heads, 16 sequences of 4096 tokens, bf16: 32 rows 69 against 56 us here, 64 rows 72 against 94, 128 rows 80 against 168; fp16: 88 and 55, 91 and 95, 99 and 168), but
+// only where there is work for the chip: it starts and joins more slowly (one sequence of 8192 tokens: 256 rows 62 against 40 us here, 384 rows 59 against 72;
+// of 1024 tokens: 2048 rows 53 against 36, 4096 rows 46 against 61).
 static bool many_rows(const DCache8& c, const DRows& r, int ratio) {
   const int64_t rows = (int64_t)r.tokens * ratio;
-  if (rows <= (int64_t)112 * r.seqs) return false;
+  if (rows <= (int64_t)48 * r.seqs) return false;
   const Load8 w = load_of(c, r, ratio);
   return w.tiles * (w.units + EXTRA) > (int64_t)16 * w.chip;
 }
