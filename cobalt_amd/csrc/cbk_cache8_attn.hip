@@ -33,9 +33,14 @@ struct Held8 {                              // a wavefront's 32 tokens: two sixt
   float2 s[2];                              // scales of their keys and values
 };
 
-template <int D, bool BF>
-__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_attn_kernel(DCache8 c, DRows r, AttnArgs a) {
-  constexpr int R = 16, KS = D / 32, VU = D / 64, TILES = D / 16;
+// Workgroups of R rows a tile that run at once on a CU, by the registers and the LDS they take
+template <int D, int R>
+constexpr int RESIDENT = R == 16 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : D == 128 ? 2 : 3;
+
+// R rows a tile: one or two sixteens of columns, which share what is widened
+template <int D, int R, bool BF>
+__global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCache8 c, DRows r, AttnArgs a) {
+  constexpr int NC = R / 16, KS = D / 32, VU = D / 64, TILES = D / 16;
   __shared__ float o_sh[4][R][D + 4];
   __shared__ float m_sh[4][R], l_sh[4][R];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,37 +128,43 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
     pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
 
     // ---- queries: fragments, positions and factors
-    v8h q[KS];
-    float cs;
-    Sight sight;
-    const int row = row0 + col;
-    const bool is = col < valid;
-    const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
-    sight = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
-    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
-    v4u raw[KS];
+    v8h q[NC][KS];
+    float cs[NC];
+    Sight sight[NC];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 64 * (k >> 1) + 16 * h4 + 8 * (k & 1)) : v4u{};
-    float top = 0.f, down;
+    for (int n = 0; n < NC; ++n) {
+      const int row = row0 + 16 * n + col;
+      const bool is = 16 * n + col < valid;
+      const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
+      sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
+      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
+      v4u raw[KS];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
-    top = across_max(top);
-    cs = a.scale * row_factor(top, down);
+      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 64 * (k >> 1) + 16 * h4 + 8 * (k & 1)) : v4u{};
+      float top = 0.f, down;
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+      top = across_max(top);
+      cs[n] = a.scale * row_factor(top, down);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t two = raw[k][i];
-        const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
-        q[k][2 * i] = (_Float16)(x0 * down);
-        q[k][2 * i + 1] = (_Float16)(x1 * down);
-      }
-    cs = fminf(fmaxf(cs, 1e-30f), 0x1.fffffep127f);                 // (a smaller one has every score at 0, a larger one every difference past any weight; a masked one stays -inf)
-    v4f o[TILES];
-    float m, l;
-    m = FLOOR; l = 0.f;
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = raw[k][i];
+          const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
+          q[n][k][2 * i] = (_Float16)(x0 * down);
+          q[n][k][2 * i + 1] = (_Float16)(x1 * down);
+        }
+      cs[n] = fminf(fmaxf(cs[n], 1e-30f), 0x1.fffffep127f);         // (a smaller one has every score at 0, a larger one every difference past any weight; a masked one stays -inf)
+    }
+    v4f o[NC][TILES];
+    float m[NC], l[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      m[n] = FLOOR; l[n] = 0.f;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
 
     for (int u = u0; u < u1; ++u) {
       const int tok = token_of(u), tok_next = token_of(min(u + 1, u1 - 1));
@@ -162,15 +173,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
       // every row sees all 32 tokens, and all of them are there
       const bool whole = p0 && p1 && tok + 32 <= s.held && tok + 31 <= pos_lo &&
                          (a.window <= 0 || tok > pos_hi - a.window || tok + 32 <= a.sinks);
-      v4f sc[2];
+      v4f sc[NC][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        sc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NC; ++n) sc[n][t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           const v4u w4 = x.k[t][k >> 1];
           const v8h f = octet8(w4[2 * (k & 1)], w4[2 * (k & 1) + 1], x.s[t].x, x.s[t].x);
-          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], sc[t], 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[n][k], sc[n][t], 0, 0, 0);
         }
       }
       if (u + 1 < u1) fetch_keys(tok_next, pg_next);
@@ -180,7 +193,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = tok + 16 * t + 4 * h4 + i;
-            sc[t][i] = key < s.held && (t ? p1 : p0) && sees(sight, key) ? sc[t][i] : -__builtin_inff();
+            const bool there = key < s.held && (t ? p1 : p0);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) sc[n][t][i] = there && sees(sight[n], key) ? sc[n][t][i] : -__builtin_inff();
           }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {                               // whatever stands where no token is: its value is 0
@@ -189,31 +204,34 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
           for (int v = 0; v < VU; ++v) x.v[t][v] &= keep;
         }
       }
-      v8h p, rest;
-      float e[8], top;
+      v8h p[NC], rest[NC];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = rounded_product(sc[i >> 2][i & 3], cs);
-      top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-      top = across_max(top);
-      if (__ballot(top > m + P_SLACK)) {                       // the maximum follows when p would leave its range
-        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
-        m = up;
-        l *= f;
+      for (int n = 0; n < NC; ++n) {
+        float e[8], top;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) o[t] *= f;
-      }
-      const float shift = P_BITS - m;
+        for (int i = 0; i < 8; ++i) e[i] = rounded_product(sc[n][i >> 2][i & 3], cs[n]);
+        top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+        top = across_max(top);
+        if (__ballot(top > m[n] + P_SLACK)) {                       // the maximum follows when p would leave its range
+          const float up = fmaxf(m[n], top), f = __builtin_amdgcn_exp2f(m[n] - up);
+          m[n] = up;
+          l[n] *= f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i] + shift);
+          for (int t = 0; t < TILES; ++t) o[n][t] *= f;
+        }
+        const float shift = P_BITS - m[n];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
-        l = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
-        p[2 * i] = ph.x; p[2 * i + 1] = ph.y;
-        if constexpr (!BF) {
-          const v2h pl = rest_of(ph, e[2 * i], e[2 * i + 1]);
-          rest[2 * i] = pl.x; rest[2 * i + 1] = pl.y;
-          l = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(e[i] + shift);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v2h ph = {(_Float16)e[2 * i], (_Float16)e[2 * i + 1]};
+          l[n] = __builtin_amdgcn_fdot2(ph, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
+          p[n][2 * i] = ph.x; p[n][2 * i + 1] = ph.y;
+          if constexpr (!BF) {
+            const v2h pl = rest_of(ph, e[2 * i], e[2 * i + 1]);
+            rest[n][2 * i] = pl.x; rest[n][2 * i + 1] = pl.y;
+            l[n] = __builtin_amdgcn_fdot2(pl, v2h{(_Float16)1.f, (_Float16)1.f}, l[n], false);
+          }
         }
       }
 #pragma unroll
@@ -221,9 +239,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                               // channels 64 v + 4 n + i
           const v8h f = octet8(x.v[0][v][i], x.v[1][v][i], x.s[0].y, x.s[1].y);
-          o[4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[4 * v + i], 0, 0, 0);
-          if constexpr (!BF)
-            o[4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest, o[4 * v + i], 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            o[n][4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[n], o[n][4 * v + i], 0, 0, 0);
+            if constexpr (!BF)
+              o[n][4 * v + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, rest[n], o[n][4 * v + i], 0, 0, 0);
+          }
         }
       if (u + 1 < u1) {
         fetch_values(tok_next, pg_next);
@@ -234,13 +255,16 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
 
     // ---- the four wavefronts' parts together
     __syncthreads();                                                // (the reads of the last item)
-    l = across_sum(l);
-    if (h4 == 0) { m_sh[wave][col] = m; l_sh[wave][col] = l; }
 #pragma unroll
-    for (int v = 0; v < VU; ++v)
+    for (int n = 0; n < NC; ++n) {
+      l[n] = across_sum(l[n]);
+      if (h4 == 0) { m_sh[wave][16 * n + col] = m[n]; l_sh[wave][16 * n + col] = l[n]; }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)                                   // row n = 4 h4 + i of four tiles: channels 64 v + 4 n ..
-        *(v4f*)&o_sh[wave][col][64 * v + 16 * h4 + 4 * i] = v4f{o[4 * v][i], o[4 * v + 1][i], o[4 * v + 2][i], o[4 * v + 3][i]};
+      for (int v = 0; v < VU; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)                                 // row 4 h4 + i of four tiles: channels 64 v + 4 (4 h4 + i) ..
+          *(v4f*)&o_sh[wave][16 * n + col][64 * v + 16 * h4 + 4 * i] = v4f{o[n][4 * v][i], o[n][4 * v + 1][i], o[n][4 * v + 2][i], o[n][4 * v + 3][i]};
+    }
     __syncthreads();
     const bool direct = u0 == 0 && u1 == g.units;
     const int slot = is_first ? 0 : 1;
@@ -276,21 +300,30 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache8_a
 }
 
 // ------------------------------------------------------------------ launch
-// Every tile of 16 rows, at most; its units, if all sequences were as long as the table allows; the workgroups that run at once:
-// four, three or two a CU, by the registers and the LDS they take.
-struct Load8 { int64_t tiles, units; int chip; };
+// Every tile of `rows` rows, at most; its units, if all sequences were as long as the table allows; the workgroups that run at once.
+struct Load8 { int64_t tiles, units; int rows, chip; };
 static Load8 load_of(const DCache8& c, const DRows& r, int ratio) {
-  return {((int64_t)r.tokens * ratio / 16 + r.seqs) * c.heads, r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1, 256 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2)};
+  const int64_t rows = (int64_t)r.tokens * ratio;
+  Load8 w{(rows / 16 + r.seqs) * c.heads, r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1, 16,
+          256 * (c.dim == 64 ? RESIDENT<64, 16> : c.dim == 128 ? RESIDENT<128, 16> : RESIDENT<256, 16>)};
+  // Tiles of 32 rows read a head's tokens once where two of 16 would read them twice: from 17 rows a sequence, and four units a workgroup, which else have
+  // what they start and end with to win back (128 channels, 8 cache heads, 4 query heads on one: 16 sequences of 4000 tokens, 5 tokens 49 us
+  // against 60, 8 tokens 52 against 62, 4 tokens 47 against 45; 2 of 100000, 8 tokens 91 against 140; one of 8000, 8 tokens 27 against 25).  256 channels have no
+  // registers for it (one workgroup a CU: 43 against 38).
+  if (c.dim < 256 && rows > (int64_t)16 * r.seqs && w.tiles * (w.units + EXTRA) > (int64_t)4 * w.chip)
+    w = Load8{(rows / 32 + r.seqs) * c.heads, w.units, 32, 256 * (c.dim == 64 ? RESIDENT<64, 32> : RESIDENT<128, 32>)};
+  return w;
 }
-struct Plan8 { int grid; bool split; size_t bytes; };
+struct Plan8 { int grid, rows; bool split; size_t bytes; };
 static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
   const Load8 w = load_of(c, r, ratio);
   Plan8 p;
+  p.rows = w.rows;
   // Tiles of few units stay in one piece, which saves the second launch
   p.split = w.units > 8 || (w.units > 4 && 2 * w.tiles < w.chip);
   const int64_t most = p.split ? w.tiles * (w.units + EXTRA) : w.tiles;
   p.grid = (int)(most < w.chip ? most : w.chip);
-  p.bytes = p.split ? attn_bytes(p.grid, 16, c.dim) : 0;
+  p.bytes = p.split ? attn_bytes(p.grid, p.rows, c.dim) : 0;
   return p;
 }
 
@@ -301,17 +334,23 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
 static bool many_rows(const DCache8& c, const DRows& r, int ratio) {
   const int64_t rows = (int64_t)r.tokens * ratio;
   if (rows <= (int64_t)48 * r.seqs) return false;
-  const Load8 w = load_of(c, r, ratio);
-  return w.tiles * (w.units + EXTRA) > (int64_t)16 * w.chip;
+  const int64_t tiles = (rows / 16 + r.seqs) * c.heads, units = r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1;
+  return tiles * (units + EXTRA) > (int64_t)4096 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2);
 }
 size_t cache8_attn_workspace(const DCache8& c, const DRows& r, int ratio) {
   return many_rows(c, r, ratio) ? plan_prompt8(c, r, ratio).bytes : plan_few(c, r, ratio).bytes;
 }
 
+template <int D, int R>
+static void few(const Plan8& p, const DCache8& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
+  if (a.bf) hipLaunchKernelGGL((cache8_attn_kernel<D, R, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  else hipLaunchKernelGGL((cache8_attn_kernel<D, R, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+}
 template <int D>
 static void few(const Plan8& p, const DCache8& c, const DRows& r, const AttnArgs& a, hipStream_t st) {
-  if (a.bf) hipLaunchKernelGGL((cache8_attn_kernel<D, true>), dim3(p.grid), dim3(256), 0, st, c, r, a);
-  else hipLaunchKernelGGL((cache8_attn_kernel<D, false>), dim3(p.grid), dim3(256), 0, st, c, r, a);
+  if constexpr (D < 256)
+    if (p.rows == 32) return few<D, 32>(p, c, r, a, st);
+  few<D, 16>(p, c, r, a, st);
 }
 int launch_cache8_attn(const DCache8& c, const DRows& r, AttnArgs a, size_t ws_bytes, hipStream_t st) {
   const size_t need = cache8_attn_workspace(c, r, a.ratio);
@@ -323,7 +362,7 @@ int launch_cache8_attn(const DCache8& c, const DRows& r, AttnArgs a, size_t ws_b
   if (c.dim == 64) few<64>(p, c, r, a, st);
   else if (c.dim == 128) few<128>(p, c, r, a, st);
   else few<256>(p, c, r, a, st);
-  if (p.split) launch_cache_join(c.dim, a, p.grid, 16, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, p.rows, st);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

@@ -392,9 +392,9 @@ __device__ inline void add_part(const AttnArgs& a, int grid, int64_t part, int r
 // Rows of a tile that several workgroups have parts of.  Workgroup (x, y) takes row y of the tile that begins in workgroup x: D/4 threads a
 // part, 1024/D parts side by side, there may be hundreds.  (x is turned by y: tiles often begin every so many workgroups, and workgroups go to
 // the XCDs in turn.  512 rows in 16 parts each took one XCD 68 us.)
-template <int D>
+template <int D, int R>
 __global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid) {
-  constexpr int C = D / 4, P = 256 / C, R = 16;
+  constexpr int C = D / 4, P = 256 / C;
   __shared__ float sh[P][D + 4];
   const int64_t w = (blockIdx.x + blockIdx.y) % gridDim.x;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
@@ -471,7 +471,8 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
 }
 template <int D>
 static void join1(const AttnArgs& a, int grid, int rows, hipStream_t st) {
-  if (rows == 16) hipLaunchKernelGGL((cache_attn_join_kernel<D>), dim3(grid, 16), dim3(256), 0, st, a, grid);
+  if (rows == 16) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16>), dim3(grid, 16), dim3(256), 0, st, a, grid);
+  else if (rows == 32) hipLaunchKernelGGL((cache_attn_join_kernel<D, 32>), dim3(grid, 32), dim3(256), 0, st, a, grid);
   else hipLaunchKernelGGL((cache_prompt_join_kernel<D>), dim3(grid, 16), dim3(256), 0, st, a, grid);
 }
 void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, hipStream_t st) {

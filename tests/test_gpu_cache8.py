@@ -399,6 +399,30 @@ def test_chunks_behind_long_histories_are_cut_and_joined(dim, dtype):
     s.attend([270, 1, 100], 4, window=1500, sinks=100)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,page,block", [(64, 64, 16), (128, 16, 16), (128, 64, 64)])
+def test_drafts_of_more_than_sixteen_rows_a_head(dim, page, block, dtype):
+    """Tiles of 32 rows, which long histories take: part of one, two sixteens, more than a tile; some of their pages missing, and a NaN."""
+    def fill(s):
+        s.v[5200 + 4100 - 3, 2, 1] = float("nan")                  # seen by the second sequence's last three rows
+    s = Setup([5200, 4100, 17, 5000, 0, 3000], 8, dim, page, block, dtype, seed=dim + block, fill=fill)
+    new = [5, 8, 5, 9, 0, 1]
+    q, out = s.attend([5, 0, 5, 9, 0, 8], 4)
+    s.attend([5, 0, 5, 9, 0, 8], 4, window=1000, sinks=70)
+    q = torch.randn(sum(new), 32, dim, device=DEV).to(dtype)
+    out = ops.cache_attention(s.cache, q, s.rows(new))
+    nan = out.isnan().any(-1)
+    assert bool(nan[10:13, 8:12].all()) and int(nan.sum()) == 12
+    there = [np.ones(n, bool) for n in s.lens]
+    table = s.table.clone()
+    for b, i in ((0, 3), (3, 0), (3, 5000 // page)):
+        table[b, i] = -1
+        there[b][page * i:page * i + page] = False
+    new = [5, 0, 5, 9, 0, 8]
+    q = torch.randn(sum(new), 32, dim, device=DEV).to(dtype)
+    s.check(q, ops.cache_attention(s.cache, q, s.rows(new)._replace(table=table)), new, there=there)
+
+
 @pytest.mark.parametrize("lens,heads,ratio", [([20011], 1, 4), ([9000, 3, 12345], 2, 2), ([4097], 8, 4)])
 def test_long_histories_are_cut_and_joined(lens, heads, ratio):
     s = Setup(lens, heads, 128, 64, 16, BF16, seed=5)
