@@ -80,10 +80,12 @@ __device__ inline void runs_from(const DRows& r, int t, int end, int shift, int 
     if (b >= r.seqs) return;
     const Seq s = seq_of(r, max(b, 0));
     if (b < 0 || t < s.first || t >= s.first + s.n) {               // in front of the first sequence, or behind this one
-      const int was = b;
-      if (r.starts)
-        while (b < r.seqs && r.starts[b + 1] <= t) ++b;
-      if (b == was) ++t;
+      if (r.starts && r.starts[b + 1] <= t) {                       // the next one's, or, where some are empty, a later one's
+        ++b;
+        if (b < r.seqs && r.starts[b + 1] <= t) b = max(b, sequence_of(r, t, lane));
+      } else {
+        ++t;
+      }
       continue;
     }
     const int pos = s.pos0 + (t - s.first), in = pos & ((1 << shift) - 1), left = (1 << shift) - in;

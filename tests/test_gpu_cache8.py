@@ -276,6 +276,37 @@ def test_rows_of_many_blocks_and_of_few(block):
     s.check_held((BF16,))
 
 
+def test_many_empty_sequences_between():
+    """A million sequences, of which a few have rows, some of them one behind the other; and rows in front of the first and behind the last."""
+    seqs, page = 1 << 20, 16
+    have = {0: 5, 1: 1, 77777: 20, 77778: 3, 500000: 33, seqs - 1: 2}
+    lens = torch.zeros(seqs, dtype=torch.int32)
+    new = torch.zeros(seqs, dtype=torch.int64)
+    table = torch.full((seqs, 3), -1, dtype=torch.int32)
+    at, small = 0, []
+    for b, n in have.items():
+        lens[b] = new[b] = n
+        table[b, :-(-n // page)] = torch.arange(at, at + -(-n // page), dtype=torch.int32)
+        at += -(-n // page)
+        small.append(n)
+    starts = (torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)]) + 2).int()
+    rows = KVRows(table.to(DEV), lens.to(DEV), starts.to(DEV))
+    total = sum(small) + 5
+    k, v = (torch.randn(total, 1, 64).half() for _ in range(2))
+    cache, ref = KVCache8(at, 1, 64, page=page, device=DEV), R8.Pool(at, 1, 64, page, 16)
+    ops.cache_write(cache, k.to(DEV), v.to(DEV), rows)
+    ref.write([table[b].tolist() for b in have], small, [x + 2 for x in cut(small)], k.float().numpy(), v.float().numpy())
+    out = tuple(torch.full((total, 1, 64), 7.0, device=DEV) for _ in range(2))
+    ops.cache_read(cache, rows, total, torch.float32, out=out)
+    held = [ref.read([table[b].tolist() for b in have], i, range(n)) for i, n in enumerate(small)]
+    for i in range(2):
+        np.testing.assert_array_equal(out[i][2:-3].cpu().numpy(), np.concatenate([h[i] for h in held]).astype(np.float32))
+        assert bool((out[i][:2] == 7).all()) and bool((out[i][-3:] == 7).all())
+    slots, positions = ops.cache_slots(cache, rows, total)
+    want = [int(table[b, j // page]) * page + j % page for b, n in have.items() for j in range(n)]
+    assert slots.tolist() == [-1, -1] + want + [-1] * 3 and positions.tolist() == [0, 0] + [j for n in small for j in range(n)] + [0] * 3
+
+
 def test_a_write_touches_its_own_blocks_only():
     s = Setup([37, 20], 3, 128, 16, 16, F16, spare=3)
     k, v = (torch.randn(3, 3, 128).half() for _ in range(2))
