@@ -10,7 +10,8 @@
 //
 // Slots.  Row t of sequence b is its token j = len_b - rows_b + (t - starts_b), on place table[b][j / page] * page + j % page.
 //
-// Both move few bytes; they are bound by their launches and by the loads that wait for one another.
+// Both move few bytes; they are bound by their launches and by the loads that wait for one another: a step of 32 sequences 3.5 us in one kernel, 1024
+// sequences of up to 60000 tokens in pages of 16 (3.8 million entries, 15 % of them end, 15 % begin) 4.7 + 6.5 us; slots of 32 rows 2.8, of a million rows 6.6 us.
 #include "cbk_cache_attn.h"
 #include "cbk_cache_check.h"
 
@@ -26,7 +27,10 @@ struct PagePlan { int64_t count, gone, taken, moves; };
 // Behind the plan in the workspace, or in LDS: running sums over the sequences, and the entry that a sequence's pages leave from or go to
 struct PageEnds { int32_t *gone, *more, *first; };
 
-constexpr int INLINE_ENTRIES = 8192, INLINE_SEQS = 1024;            // entries and rows of a table whose pages the first launch moves
+// Entries and rows of a table whose pages the first launch moves.  A step moves few of a table's pages, and one launch takes 6.4 us with 256 threads, 7.8 with
+// 1024 (timed with the call), two 10 to 11; where all move, one workgroup is the bottleneck: 2048 entries 10.2 and 8.5 us, 4096 entries 14 and 9.6, 8192
+// entries 24 and 12, 32768 entries 76 and 28.  So 256 threads to a quarter of the entries, 1024 to all of them, two launches above.
+constexpr int INLINE_ENTRIES = 8192, INLINE_SEQS = 1024;
 
 struct Change { int len, now, have, need; };                        // tokens before and asked for, and their pages
 __device__ inline Change change_of(const DPages& p, const int32_t* want, int b) {
@@ -78,6 +82,33 @@ __device__ inline int share_of(const int32_t* ends, int lo, int hi, int x) {
 // The entry of the table that the x-th page of a list leaves or goes to, if sequence b has it
 __device__ inline int32_t* entry_of(const DPages& p, const int32_t* ends, const int32_t* first, int b, int x) {
   return p.table + (int64_t)b * p.ld + first[b] + (x - (b ? ends[b - 1] : 0));
+}
+
+// The pages from the base-th on, U a thread of T, neighbours side by side, from the place each leaves (the table, or the stack) to the one it goes
+// to (the stack, the table): the loads of all first.  Those given back are of sequences g0 to g1, those taken of m0 to m1.
+template <int U, int T>
+__device__ inline void move_pages(const DPages& p, const PagePlan& plan, const PageEnds& ends, int64_t base, int g0, int g1, int m0, int m1) {
+  int32_t id[U];
+  int32_t* from[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t x = base + u * T + threadIdx.x, place = plan.count + plan.gone - 1 - x;   // from the top of the stack, with what is given back on it
+    from[u] = nullptr;
+    if (x >= plan.moves || place < 0 || place >= p.pages) continue; // (more given back than the pool has pages: not a table of this pool)
+    if (x < plan.gone) from[u] = entry_of(p, ends.gone, ends.first, share_of(ends.gone, g0, g1, (int)x), (int)x);
+    id[u] = *(x < plan.gone ? from[u] : p.free + place);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t x = base + u * T + threadIdx.x, place = plan.count + plan.gone - 1 - x;
+    if (x >= plan.moves || place < 0 || place >= p.pages) continue;
+    int32_t* const to = x < plan.taken ? entry_of(p, ends.more, ends.first, share_of(ends.more, m0, m1, (int)x), (int)x) : nullptr;
+    if (x < plan.gone) {
+      *from[u] = -1;
+      p.free[place] = id[u];
+    }
+    if (to) *to = id[u];
+  }
 }
 
 // T threads; ONE: no more sequences than that, one a thread; HERE: the pages are moved too, not by a second launch
@@ -140,20 +171,7 @@ __global__ __launch_bounds__(T) void pages_plan_kernel(DPages p, const int32_t* 
     return;
   }
   __syncthreads();
-  for (int x = tid; x < plan.moves; x += T) {                       // (as in pages_move_kernel)
-    const int64_t place = plan.count + plan.gone - 1 - x;
-    if (place < 0 || place >= p.pages) continue;
-    int32_t id;
-    if (x < plan.gone) {
-      int32_t* const from = entry_of(p, ends.gone, ends.first, share_of(ends.gone, 0, p.seqs - 1, x), x);
-      id = *from;
-      *from = -1;
-      p.free[place] = id;
-    } else {
-      id = p.free[place];
-    }
-    if (x < plan.taken) *entry_of(p, ends.more, ends.first, share_of(ends.more, 0, p.seqs - 1, x), x) = id;
-  }
+  for (int64_t base = 0; base < plan.moves; base += T) move_pages<1, T>(p, plan, ends, base, 0, p.seqs - 1, 0, p.seqs - 1);
 }
 
 // For two numbers that are the same in all lanes, the first i < n whose entry of an ascending list passes them (n: none does):
@@ -173,54 +191,34 @@ __device__ inline void first_above(int n, int lane, int x0, int x1, int& i0, int
   i0 = min(lo0, n); i1 = min(lo1, n);
 }
 
-constexpr int MOVES = 2;                    // pages a thread at a time
+constexpr int MOVES = 2;                    // pages a thread at a time (half a million moved: 1 22.2 us, 2 21.8, 4 22.4)
 
-// The x-th page from the place it leaves (the table, or the stack) to the one it goes to (the stack, the table).  A workgroup takes neighbours, of few
-// sequences.  SMALL: at most INLINE_SEQS sequences, whose sums come into LDS at once instead of by loads that wait for one another.
+// A workgroup takes neighbours, of few sequences.  SMALL: at most INLINE_SEQS sequences, whose sums come into LDS at once instead of by loads that wait for one another.
 template <bool SMALL>
-__global__ __launch_bounds__(256) void pages_move_kernel(DPages p, const uint8_t* ws) {
+__global__ __launch_bounds__(256) void pages_move_kernel(DPages p, uint8_t* ws) {
   __shared__ int32_t of_sh[SMALL ? 3 * INLINE_SEQS : 1];
-  const int32_t* of = (const int32_t*)(ws + sizeof(PagePlan));
+  int32_t* const of = (int32_t*)(ws + sizeof(PagePlan));
   const int lane = threadIdx.x & 63;
   constexpr int N = SMALL ? 3 * INLINE_SEQS / 256 : 1;
-  int32_t sums[N];
+  int32_t part[N];
   if constexpr (SMALL)
 #pragma unroll
-    for (int i = 0; i < N; ++i) sums[i] = of[min(i * 256 + (int)threadIdx.x, 3 * p.seqs - 1)];
+    for (int i = 0; i < N; ++i) part[i] = of[min(i * 256 + (int)threadIdx.x, 3 * p.seqs - 1)];
   const PagePlan plan = *(const PagePlan*)ws;
   if ((int64_t)blockIdx.x * (256 * MOVES) >= plan.moves) return;
   if constexpr (SMALL) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) of_sh[i * 256 + threadIdx.x] = sums[i];
+    for (int i = 0; i < N; ++i) of_sh[i * 256 + threadIdx.x] = part[i];
     __syncthreads();
   }
-  const int32_t *const gone = SMALL ? of_sh : of, *const more = gone + p.seqs, *const first = gone + 2 * p.seqs;
+  int32_t* const sums = SMALL ? of_sh : of;
+  const PageEnds ends{sums, sums + p.seqs, sums + 2 * p.seqs};
   for (int64_t base = (int64_t)blockIdx.x * (256 * MOVES); base < plan.moves; base += (int64_t)gridDim.x * (256 * MOVES)) {
     const int x0 = (int)base, x1 = (int)min(base + 256 * MOVES, plan.moves) - 1;
     int g0 = 0, g1 = 0, m0 = 0, m1 = 0;                             // the sequences that they can be of
-    if (x0 < plan.gone) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.gone - 1), g0, g1, [&](int i, int x) { return gone[i] > x; });
-    if (x0 < plan.taken) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.taken - 1), m0, m1, [&](int i, int x) { return more[i] > x; });
-    int32_t id[MOVES];
-    int32_t* from[MOVES];
-#pragma unroll
-    for (int u = 0; u < MOVES; ++u) {
-      const int64_t x = base + u * 256 + threadIdx.x, place = plan.count + plan.gone - 1 - x;   // from the top of the stack, with what is given back on it
-      from[u] = nullptr;
-      if (x >= plan.moves || place < 0 || place >= p.pages) continue;   // (more given back than the pool has pages: not a table of this pool)
-      if (x < plan.gone) from[u] = entry_of(p, gone, first, share_of(gone, g0, g1, (int)x), (int)x);
-      id[u] = *(x < plan.gone ? from[u] : p.free + place);
-    }
-#pragma unroll
-    for (int u = 0; u < MOVES; ++u) {
-      const int64_t x = base + u * 256 + threadIdx.x, place = plan.count + plan.gone - 1 - x;
-      if (x >= plan.moves || place < 0 || place >= p.pages) continue;
-      int32_t* const to = x < plan.taken ? entry_of(p, more, first, share_of(more, m0, m1, (int)x), (int)x) : nullptr;
-      if (x < plan.gone) {
-        *from[u] = -1;
-        p.free[place] = id[u];
-      }
-      if (to) *to = id[u];
-    }
+    if (x0 < plan.gone) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.gone - 1), g0, g1, [&](int i, int x) { return ends.gone[i] > x; });
+    if (x0 < plan.taken) first_above(p.seqs, lane, x0, (int)min((int64_t)x1, plan.taken - 1), m0, m1, [&](int i, int x) { return ends.more[i] > x; });
+    move_pages<MOVES, 256>(p, plan, ends, base, g0, g1, m0, m1);
   }
 }
 
@@ -245,7 +243,7 @@ static int to_dpages(const cbk_pages* in, DPages* p, bool need_device_ptrs) {
 }
 
 // ------------------------------------------------------------------ slots
-constexpr int SLOT_ROWS = 2;                // rows a thread
+constexpr int SLOT_ROWS = 2;                // rows a thread (a million rows of 1024 sequences: 1 11.1 us, 2 9.6, 4 10.3; of 8 sequences 9.0, 8.3, 8.5)
 
 // SMALL: at most SLOT_SEQS sequences with offsets, which come into LDS at once
 constexpr int SLOT_SEQS = 768;
@@ -326,14 +324,16 @@ int cbk_cache_pages(const cbk_pages* pages, const void* want, void* starts, void
   uint8_t* const ws = need ? (uint8_t*)workspace : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   auto plan = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, st, p, (const int32_t*)want, (int32_t*)starts, ws); };
-  if (p.seqs <= 256) need ? plan(pages_plan_kernel<256, true, false>, 256) : plan(pages_plan_kernel<256, true, true>, 256);
-  else if (p.seqs <= 1024) need ? plan(pages_plan_kernel<1024, true, false>, 1024) : plan(pages_plan_kernel<1024, true, true>, 1024);
+  if (!need && p.seqs <= 256 && (int64_t)p.seqs * p.cols <= INLINE_ENTRIES / 4) plan(pages_plan_kernel<256, true, true>, 256);
+  else if (!need) plan(pages_plan_kernel<1024, true, true>, 1024);
+  else if (p.seqs <= 256) plan(pages_plan_kernel<256, true, false>, 256);
+  else if (p.seqs <= 1024) plan(pages_plan_kernel<1024, true, false>, 1024);
   else plan(pages_plan_kernel<1024, false, false>, 1024);
   if (need) {
     const int64_t most = ((int64_t)p.seqs * p.cols + 256 * MOVES - 1) / (256 * MOVES);   // pages moved, at most
     const dim3 grid((unsigned)(most < 4096 ? (most ? most : 1) : 4096));
-    if (p.seqs <= INLINE_SEQS) hipLaunchKernelGGL(pages_move_kernel<true>, grid, dim3(256), 0, st, p, (const uint8_t*)ws);
-    else hipLaunchKernelGGL(pages_move_kernel<false>, grid, dim3(256), 0, st, p, (const uint8_t*)ws);
+    if (p.seqs <= INLINE_SEQS) hipLaunchKernelGGL(pages_move_kernel<true>, grid, dim3(256), 0, st, p, ws);
+    else hipLaunchKernelGGL(pages_move_kernel<false>, grid, dim3(256), 0, st, p, ws);
   }
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }

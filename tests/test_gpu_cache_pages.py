@@ -79,8 +79,6 @@ def test_a_step_and_back_leaves_everything_as_it_was():
     had = list(t.ref.lens)
     t.resize([max(0, n + rng.randint(-200, 200)) for n in had])
     t.resize(had)
-    for x, y in zip(t.pool.native()[:3:2], keep[:3:2]):
-        pass
     assert torch.equal(t.pool.table, keep[0]) and torch.equal(t.pool.lens, keep[1]) and torch.equal(t.pool.count, keep[3])
     n = int(keep[3])
     assert torch.equal(t.pool.free[:n], keep[2][:n])
