@@ -20,7 +20,9 @@
 // what a workgroup has of a head it does not finish goes to the workspace with its maximum and sum, and a second
 // launch joins the pieces.  Lengths are read on the device: the host knows none of them.
 //
-// Bound by the bytes of the cache where histories are long.
+// Bound by the bytes of the cache where histories are long: two sequences, 269000 tokens (552 MB), 102.5 us and the join 6.3, 5.4 TB/s in the kernel; 32
+// sequences, 115000 tokens (236 MB), 50 and 4.8, of which some 8 are the chain of look-ups before the first load and the joins in LDS at the end.  One token over
+// 700 of history 7.7 us and 2.8, all of it that chain and the launches.
 #include "cbk_cache8.h"
 #include "cbk_cache_attn.h"
 #include "cbk_cache8_attn.h"
@@ -319,8 +321,10 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
   const Load8 w = load_of(c, r, ratio);
   Plan8 p;
   p.rows = w.rows;
-  // Tiles of few units stay in one piece, which saves the second launch
-  p.split = w.units > 8 || (w.units > 4 && 2 * w.tiles < w.chip);
+  // Tiles of few units stay in one piece, which saves the second launch, where there are enough of them: up to 8 units from a tile a CU, up to 16
+  // where they about fill the chip (128 channels, 8 cache heads, single tokens; whole against cut: 1 sequence of 640 tokens 16.2 and 14.1 us, 32 of 640 17.9 and 23.4,
+  // of 1024 22.4 and 26.5; 64 of 2048 54 and 64, of up to 2048 39 and 43; 32 of up to 2048 32 and 28; 256 of up to 2048 132 and 119).
+  p.split = w.units > 16 || (w.units > 8 && (2 * w.tiles < w.chip || w.tiles > 2 * w.chip)) || (w.units > 4 && w.tiles < 256);
   const int64_t most = p.split ? w.tiles * (w.units + EXTRA) : w.tiles;
   p.grid = (int)(most < w.chip ? most : w.chip);
   p.bytes = p.split ? attn_bytes(p.grid, p.rows, c.dim) : 0;

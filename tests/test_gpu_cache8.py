@@ -462,6 +462,16 @@ def test_long_histories_are_cut_and_joined(lens, heads, ratio):
     s.attend([min(n, 3) for n in lens], ratio)
 
 
+@pytest.mark.parametrize("lens,heads,dim", [([1000] + [700, 1, 90] * 13, 8, 128), ([2000] + [1300, 0, 500, 129] * 25, 8, 64), ([1300, 2000, 20] * 25, 8, 128)])
+def test_histories_of_some_length_in_one_piece(lens, heads, dim):
+    """Enough sequences of medium length that no history is cut."""
+    s = Setup(lens, heads, dim, 64, 16, BF16, seed=8)
+    s.attend([min(n, 1) for n in lens], 4)
+    s.attend([min(n, 1) for n in lens], 4, window=600, sinks=100)
+    s.attend([min(n, 3) for n in lens], 4)
+    s.attend([min(n, 7) for n in lens], 4)
+
+
 def test_many_sequences():
     """More sequences than a workgroup has threads, most of them short, some empty."""
     g = np.random.default_rng(0)
