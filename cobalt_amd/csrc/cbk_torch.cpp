@@ -873,10 +873,10 @@ PyObject* py_cache_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const uintptr_t x = (uintptr_t)starts.const_data_ptr(), y = (uintptr_t)t->const_data_ptr();
         if (t->numel() && x < y + 4 * t->numel() && y < x + 4 * starts.numel()) fail(PyExc_ValueError, "starts must not overlap lens or the pool's arrays");
       }
-    for (int i : {0, 2, 3}) {                                       // (lens themselves may be asked for)
+    for (int i = 0; i < 4; ++i) {                                   // (the pool's lens themselves may be asked for)
       const uintptr_t x = (uintptr_t)want.const_data_ptr(), y = (uintptr_t)p.t[i].const_data_ptr();
-      if (want.numel() && p.t[i].numel() && x < y + 4 * p.t[i].numel() && y < x + 4 * want.numel())
-        fail(PyExc_ValueError, "lens must not overlap the pool's table or stack");
+      if (want.numel() && p.t[i].numel() && x < y + 4 * p.t[i].numel() && y < x + 4 * want.numel() && !(i == 1 && x == y))
+        fail(PyExc_ValueError, "lens must not overlap the pool's arrays, unless it is the pool's lens");
     }
     int rc = CBK_OK;
     {

@@ -198,7 +198,8 @@ def cache_write(cache, k, v, rows) -> None:
     KVCache: rounded to 4 bits per group, codes c = rint((x - m) / s) with the fp16 minimum m and scale s of the group, held value m + c s.
     KVCache8: c = e4m3(x / s) with the power of two s of the token's block, which grows with what is written, held value c s.  Magnitudes above
     65280 (KVCache8: 57344) are held as that; a NaN makes its token's key and value of that head NaN.  Rows whose token has no page are
-    left out.  Two rows of a call must not be the same token of the same page (KVCache8: rows of two sequences not of one block)."""
+    left out.  Two rows of a call must not be the same token of the same page (KVCache8: nor, on two
+    sequences or two entries of a table, of the same block)."""
     _lib.native().cache_write(cache.native(), k, v, rows.table, rows.lens, rows.starts)
 
 

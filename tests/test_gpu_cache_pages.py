@@ -264,6 +264,10 @@ def test_refusals():
         ops.cache_pages(t, lens, starts=t.table.view(-1)[:4])
     with pytest.raises(ValueError, match="overlap"):
         ops.cache_pages(t, t.free[:3])
+    both = torch.zeros(4, dtype=torch.int32, device=DEV)
+    t.lens = both[:3]
+    with pytest.raises(ValueError, match="overlap"):
+        ops.cache_pages(t, both[1:])
     with pytest.raises(ValueError, match="unit stride"):
         ops.cache_pages(t, ints([1, 2, 3, 4, 5, 6])[::2])
     rows = ops.cache_pages(t, lens)
