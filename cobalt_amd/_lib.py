@@ -78,12 +78,12 @@ SIGNATURES = {
     "cbk_cache_attention_workspace_bytes": (ctypes.c_size_t, [_CP, _RP, ctypes.c_int]),
     "cbk_cache_attention": (ctypes.c_int, [_CP, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                                                       ctypes.c_int, _P, ctypes.c_size_t, _P]),
-    "cbk_cache8_code_bytes": (ctypes.c_size_t, [_C8P]),
-    "cbk_cache8_scale_bytes": (ctypes.c_size_t, [_C8P]),
-    "cbk_cache8_write": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
-    "cbk_cache8_read": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
-    "cbk_cache8_attention_workspace_bytes": (ctypes.c_size_t, [_C8P, _RP, ctypes.c_int]),
-    "cbk_cache8_attention": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+    "cbk_cache_eight_code_bytes": (ctypes.c_size_t, [_C8P]),
+    "cbk_cache_eight_scale_bytes": (ctypes.c_size_t, [_C8P]),
+    "cbk_cache_eight_write": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache_eight_read": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, _P]),
+    "cbk_cache_eight_attention_workspace_bytes": (ctypes.c_size_t, [_C8P, _RP, ctypes.c_int]),
+    "cbk_cache_eight_attention": (ctypes.c_int, [_C8P, _RP] + _ROWS + _ROWS + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                                                        ctypes.c_int, _P, ctypes.c_size_t, _P]),
     "cbk_cache_pages_workspace_bytes": (ctypes.c_size_t, [_PP]),
     "cbk_cache_pages": (ctypes.c_int, [_PP, _P, _P, _P, ctypes.c_size_t, _P]),

@@ -80,12 +80,12 @@ class KVCache8(_Pool):
     def __init__(self, pages: int, heads: int, head_dim: int, page: int = 64, block: int = 16, device="cuda"):
         self.pages, self.page, self.heads, self.head_dim, self.block = int(pages), int(page), int(heads), int(head_dim), int(block)
         d = _lib.CbkCache8(pages=self.pages, page=self.page, heads=self.heads, head_dim=self.head_dim, block=self.block)
-        codes = _lib.lib().cbk_cache8_code_bytes(ctypes.byref(d))
+        codes = _lib.lib().cbk_cache_eight_code_bytes(ctypes.byref(d))
         if not codes:
             raise ValueError(f"no cache of {pages} pages of {page} tokens, {heads} heads of {head_dim} channels in blocks of {block} tokens: "
                              "pages >= 1; page 16, 32, 64, 128 or 256; head_dim 64, 128 or 256; block 16, 32, 64, 128 or 256, at most page")
         self.k_codes, self.v_codes = (torch.zeros(codes, dtype=torch.uint8, device=device) for _ in range(2))
-        self.scales = torch.zeros(_lib.lib().cbk_cache8_scale_bytes(ctypes.byref(d)), dtype=torch.uint8, device=device)
+        self.scales = torch.zeros(_lib.lib().cbk_cache_eight_scale_bytes(ctypes.byref(d)), dtype=torch.uint8, device=device)
 
     def native(self):
         return (self.k_codes, self.v_codes, self.scales, self.pages, self.page, self.heads, self.head_dim, self.block)

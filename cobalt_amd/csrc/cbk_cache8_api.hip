@@ -51,26 +51,26 @@ using namespace cbk;
 
 extern "C" {
 
-size_t cbk_cache8_code_bytes(const cbk_cache8* cache) {
+size_t cbk_cache_eight_code_bytes(const cbk_cache8* cache) {
   DCache8 c;
   return to_dcache8(cache, &c, false) ? 0 : (size_t)c.pages * c.heads * c.page * c.dim;
 }
-size_t cbk_cache8_scale_bytes(const cbk_cache8* cache) {
+size_t cbk_cache_eight_scale_bytes(const cbk_cache8* cache) {
   DCache8 c;
   return to_dcache8(cache, &c, false) ? 0 : (size_t)c.pages * c.heads * c.blocks * sizeof(float2);
 }
 
-int cbk_cache8_write(const cbk_cache8* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
-                     const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream) {
+int cbk_cache_eight_write(const cbk_cache8* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
+                          const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream) {
   return cache8_io(cache, rows, CacheIo{(void*)k, (void*)v, k_row, k_head, v_row, v_head}, dtype, true, stream);
 }
 
-int cbk_cache8_read(const cbk_cache8* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
-                    void* v, int64_t v_row, int64_t v_head, int dtype, void* stream) {
+int cbk_cache_eight_read(const cbk_cache8* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
+                         void* v, int64_t v_row, int64_t v_head, int dtype, void* stream) {
   return cache8_io(cache, rows, CacheIo{k, v, k_row, k_head, v_row, v_head}, dtype, false, stream);
 }
 
-size_t cbk_cache8_attention_workspace_bytes(const cbk_cache8* cache, const cbk_rows* rows, int q_heads) {
+size_t cbk_cache_eight_attention_workspace_bytes(const cbk_cache8* cache, const cbk_rows* rows, int q_heads) {
   DCache8 c;
   DRows r;
   int ratio;
@@ -78,9 +78,9 @@ size_t cbk_cache8_attention_workspace_bytes(const cbk_cache8* cache, const cbk_r
   return r.tokens && r.seqs ? cache8_attn_workspace(c, r, ratio) : 0;
 }
 
-int cbk_cache8_attention(const cbk_cache8* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
-                         void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
-                         int sinks, void* workspace, size_t workspace_bytes, void* stream) {
+int cbk_cache_eight_attention(const cbk_cache8* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
+                              void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
+                              int sinks, void* workspace, size_t workspace_bytes, void* stream) {
   DCache8 c;
   DRows r;
   AttnArgs a{};

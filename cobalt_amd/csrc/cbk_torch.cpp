@@ -585,17 +585,17 @@ struct Cache {
   int64_t pages;
   int32_t page, heads, head_dim;
   int write(const cbk_rows* r, const void* k, int64_t kr, int64_t kh, const void* v, int64_t vr, int64_t vh, int dt, void* st) const {
-    return bits == 8 ? cbk_cache8_write(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_write(&c, r, k, kr, kh, v, vr, vh, dt, st);
+    return bits == 8 ? cbk_cache_eight_write(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_write(&c, r, k, kr, kh, v, vr, vh, dt, st);
   }
   int read(const cbk_rows* r, void* k, int64_t kr, int64_t kh, void* v, int64_t vr, int64_t vh, int dt, void* st) const {
-    return bits == 8 ? cbk_cache8_read(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_read(&c, r, k, kr, kh, v, vr, vh, dt, st);
+    return bits == 8 ? cbk_cache_eight_read(&c8, r, k, kr, kh, v, vr, vh, dt, st) : cbk_cache_read(&c, r, k, kr, kh, v, vr, vh, dt, st);
   }
   size_t attention_workspace(const cbk_rows* r, int heads) const {
-    return bits == 8 ? cbk_cache8_attention_workspace_bytes(&c8, r, heads) : cbk_cache_attention_workspace_bytes(&c, r, heads);
+    return bits == 8 ? cbk_cache_eight_attention_workspace_bytes(&c8, r, heads) : cbk_cache_attention_workspace_bytes(&c, r, heads);
   }
   int attention(const cbk_rows* r, const void* q, int64_t qr, int64_t qh, void* out, int64_t orow, int64_t oh, int dt, int heads, float scale,
                 int window, int sinks, void* ws, size_t bytes, void* st) const {
-    return bits == 8 ? cbk_cache8_attention(&c8, r, q, qr, qh, out, orow, oh, dt, heads, scale, window, sinks, ws, bytes, st)
+    return bits == 8 ? cbk_cache_eight_attention(&c8, r, q, qr, qh, out, orow, oh, dt, heads, scale, window, sinks, ws, bytes, st)
                      : cbk_cache_attention(&c, r, q, qr, qh, out, orow, oh, dt, heads, scale, window, sinks, ws, bytes, st);
   }
 };
@@ -623,8 +623,8 @@ Cache as_cache(PyObject* o) {
     need[2] = need[3] = cbk_cache_meta_bytes(&r.c);
   } else {
     r.c8 = cbk_cache8{p[0], p[1], p[2], (int64_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4]};
-    need[0] = need[1] = cbk_cache8_code_bytes(&r.c8);
-    need[2] = cbk_cache8_scale_bytes(&r.c8);
+    need[0] = need[1] = cbk_cache_eight_code_bytes(&r.c8);
+    need[2] = cbk_cache_eight_scale_bytes(&r.c8);
   }
   bool enough = need[0] != 0;
   for (int i = 0; i < arrays; ++i) enough = enough && r.t[i].nbytes() >= need[i];

@@ -342,7 +342,7 @@ int cbk_cache_attention(const cbk_cache* cache, const cbk_rows* rows, const void
  * head makes that token's key and value of the head NaN and counts nothing for the scales; infinities are held as +-57344.
  * Writing a block's first token again loses what the block held behind the rows of that call.
  *
- * k_codes and v_codes have cbk_cache8_code_bytes() each, scales cbk_cache8_scale_bytes(), all 16-byte aligned and cleared to zero
+ * k_codes and v_codes have cbk_cache_eight_code_bytes() each, scales cbk_cache_eight_scale_bytes(), all 16-byte aligned and cleared to zero
  * once before their first use; what stands where is the library's own (cbk_cache8.h). */
 typedef struct cbk_cache8 {
   void *k_codes, *v_codes, *scales;
@@ -353,20 +353,20 @@ typedef struct cbk_cache8 {
   int32_t block;       /* tokens a scale: 16, 32, 64, 128 or 256, at most page        */
 } cbk_cache8;
 
-size_t cbk_cache8_code_bytes(const cbk_cache8* cache);    /* 0: not a valid description */
-size_t cbk_cache8_scale_bytes(const cbk_cache8* cache);
+size_t cbk_cache_eight_code_bytes(const cbk_cache8* cache);    /* 0: not a valid description */
+                                  size_t cbk_cache_eight_scale_bytes(const cbk_cache8* cache);
 
 /* As cbk_cache_write, cbk_cache_read and cbk_cache_attention, with the same cbk_rows.  Two sequences of a call must not write into
  * the same block, and tokens * heads is below 2^29 to write or read.  Attention: keys and values are exact as operands; fp16: queries are too, and
  * softmax weights are two fp16; bf16: softmax weights and queries (with the scale in them) may each be rounded once to fp16. */
-int cbk_cache8_write(const cbk_cache8* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
-                     const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
-int cbk_cache8_read(const cbk_cache8* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
-                    void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
-size_t cbk_cache8_attention_workspace_bytes(const cbk_cache8* cache, const cbk_rows* rows, int q_heads);
-int cbk_cache8_attention(const cbk_cache8* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
-                         void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
-                         int sinks, void* workspace, size_t workspace_bytes, void* stream);
+int cbk_cache_eight_write(const cbk_cache8* cache, const cbk_rows* rows, const void* k, int64_t k_row, int64_t k_head,
+                          const void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+int cbk_cache_eight_read(const cbk_cache8* cache, const cbk_rows* rows, void* k, int64_t k_row, int64_t k_head,
+                         void* v, int64_t v_row, int64_t v_head, int dtype, void* stream);
+size_t cbk_cache_eight_attention_workspace_bytes(const cbk_cache8* cache, const cbk_rows* rows, int q_heads);
+int cbk_cache_eight_attention(const cbk_cache8* cache, const cbk_rows* rows, const void* q, int64_t q_row, int64_t q_head,
+                              void* out, int64_t out_row, int64_t out_head, int dtype, int q_heads, float scale, int window,
+                              int sinks, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- which pages belong to which sequence
  * A pool's tables on the device: `table` (seqs rows of table_cols entries, ld_table apart, -1: no page), `lens`, and the pages that belong to

@@ -63,15 +63,15 @@ def _rows(**kw):
 
 
 def _write(c, r, k=0x7000, kr=256, kh=128, dt=1):
-    return _lib.lib().cbk_cache8_write(ctypes.byref(c), ctypes.byref(r), k, kr, kh, 0x8000, 256, 128, dt, None)
+    return _lib.lib().cbk_cache_eight_write(ctypes.byref(c), ctypes.byref(r), k, kr, kh, 0x8000, 256, 128, dt, None)
 
 
 def _read(c, r, k=0x7000, kr=256, kh=128, dt=1):
-    return _lib.lib().cbk_cache8_read(ctypes.byref(c), ctypes.byref(r), k, kr, kh, 0x8000, 256, 128, dt, None)
+    return _lib.lib().cbk_cache_eight_read(ctypes.byref(c), ctypes.byref(r), k, kr, kh, 0x8000, 256, 128, dt, None)
 
 
 def _attend(c, r, q=0x7000, qr=512, qh=128, out=0x8000, dt=1, heads=4, scale=1.0, window=0, sinks=0, ws=0x10000, room=1 << 40):
-    return _lib.lib().cbk_cache8_attention(ctypes.byref(c), ctypes.byref(r), q, qr, qh, out, 512, 128, dt, heads, scale, window, sinks,
+    return _lib.lib().cbk_cache_eight_attention(ctypes.byref(c), ctypes.byref(r), q, qr, qh, out, 512, 128, dt, heads, scale, window, sinks,
                                            ws, room, None)
 
 
@@ -90,7 +90,7 @@ def test_entry_points_refuse_bad_descriptions_before_any_launch(call):
         assert call(_cache(**kw), _rows()) == want, kw
     for kw, want in BAD_ROWS:
         assert call(_cache(), _rows(**kw)) == want, kw
-    assert _lib.lib().cbk_cache8_write(None, None, None, 0, 0, None, 0, 0, 1, None) == -1
+    assert _lib.lib().cbk_cache_eight_write(None, None, None, 0, 0, None, 0, 0, 1, None) == -1
     # nothing to do: no launch either
     assert call(_cache(), _rows(tokens=0)) == 0
     assert call(_cache(), _rows(seqs=0, tokens=5, starts=0x9000)) == 0
@@ -119,7 +119,7 @@ def test_entry_points_refuse_bad_tensors_before_any_launch():
     assert _attend(_cache(), _rows(), sinks=-1) == -3
     assert _attend(_cache(), _rows(), ws=0x10010) == -4
     big = _rows(table_cols=1000, ld_table=1000)
-    need = _lib.lib().cbk_cache8_attention_workspace_bytes(ctypes.byref(_cache()), ctypes.byref(big), 4)
+    need = _lib.lib().cbk_cache_eight_attention_workspace_bytes(ctypes.byref(_cache()), ctypes.byref(big), 4)
     assert need > 0
     assert _attend(_cache(), big, room=need - 1) == -6
     assert _attend(_cache(), big, ws=None, room=0) == -6
@@ -131,9 +131,9 @@ def test_entry_points_refuse_bad_tensors_before_any_launch():
 def test_sizes():
     L = _lib.lib()
     c = _cache(pages=7, page=64, heads=3, head_dim=256, block=32)
-    assert L.cbk_cache8_code_bytes(ctypes.byref(c)) == 7 * 64 * 3 * 256
-    assert L.cbk_cache8_scale_bytes(ctypes.byref(c)) == 7 * 3 * 2 * 8
-    assert L.cbk_cache8_code_bytes(ctypes.byref(_cache(block=48))) == 0
+    assert L.cbk_cache_eight_code_bytes(ctypes.byref(c)) == 7 * 64 * 3 * 256
+    assert L.cbk_cache_eight_scale_bytes(ctypes.byref(c)) == 7 * 3 * 2 * 8
+    assert L.cbk_cache_eight_code_bytes(ctypes.byref(_cache(block=48))) == 0
     for kw in (dict(head_dim=80), dict(block=8), dict(block=128), dict(page=20), dict(pages=0), dict(heads=0)):
         args = {**dict(pages=2, heads=2, head_dim=128), **kw}
         with pytest.raises(ValueError):
