@@ -354,7 +354,7 @@ typedef struct cbk_cache8 {
 } cbk_cache8;
 
 size_t cbk_cache_eight_code_bytes(const cbk_cache8* cache);    /* 0: not a valid description */
-                                  size_t cbk_cache_eight_scale_bytes(const cbk_cache8* cache);
+size_t cbk_cache_eight_scale_bytes(const cbk_cache8* cache);
 
 /* As cbk_cache_write, cbk_cache_read and cbk_cache_attention, with the same cbk_rows.  Two sequences of a call must not write into
  * the same block, and tokens * heads is below 2^29 to write or read.  Attention: keys and values are exact as operands; fp16: queries are too, and
