@@ -326,11 +326,12 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(DCache8 c, DRows r, Ca
 // Rows a wavefront (or, in wide blocks, a workgroup) walks through: one, whose wavefront ends at once if it begins no block, or all that fit a block.
 // One after the other they cost their loads (256 sequences' single tokens: 52 us against 9), wavefronts that end their start (a prompt of 16384 tokens: 173 against 24;
 // 16 x 64 tokens 17 against 8.6; 64 x 8 tokens 11.5 against 17.6, 256 x 12 tokens 33 against 17.5).  All from half a chip of wavefronts on if the
-// sequences fill blocks, from all of it if they have eight rows.  (8 heads of 128 channels, blocks of 16.)
+// sequences fill blocks, from all of it if they have eight rows; not more than a sequence has on average.  (8 heads of 128 channels, blocks of 16.)
 static int chunk_of(const DCache8& c, const DRows& r, int block) {
   const int64_t waves = (int64_t)r.tokens * c.heads * (block / 16);
   const int64_t each = r.seqs ? r.tokens / r.seqs : 0;
-  return (each >= block && waves >= 4096) || (each >= 8 && waves > 8192) || waves >= (int64_t)1 << 25 ? block : 1;   // (a launch has fewer than 2^32 threads)
+  if (waves >= (int64_t)1 << 25) return block;                      // (a launch has fewer than 2^32 threads)
+  return (each >= block && waves >= 4096) || (each >= 8 && waves > 8192) ? (int)(each < block ? each : block) : 1;
 }
 
 template <int D, int DT, int NW>

@@ -4,6 +4,6 @@
 #include "cbk_cache_attn.h"
 
 namespace cbk {
-PromptPlan plan_prompt8(const DCache8&, const DRows&, int ratio);
+PromptPlan plan_prompt8(const DCache8&, const DRows&, int ratio, bool cut);
 int launch_cache8_prompt(const PromptPlan&, const DCache8&, const DRows&, const AttnArgs&, hipStream_t);
 }  // namespace cbk

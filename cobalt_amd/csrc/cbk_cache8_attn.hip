@@ -302,23 +302,29 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
 }
 
 // ------------------------------------------------------------------ launch
-// Every tile of `rows` rows, at most; its units, if all sequences were as long as the table allows; the workgroups that run at once.
+// Tokens that the rows of a sequence see: all that the table holds, if there is no window, else about the window, what is new, and the sinks
+static int seen_of(const DRows& r, int window, int sinks) {
+  if (window <= 0) return r.cap;
+  const int64_t s = (int64_t)window + r.tokens / r.seqs + UNIT + ((int64_t)sinks + UNIT - 1) / UNIT * UNIT;
+  return (int)(s < r.cap ? s : r.cap);
+}
+// Every tile of `rows` rows, at most; its units, if all sequences saw `seen` tokens; the workgroups that run at once.
 struct Load8 { int64_t tiles, units; int rows, chip; };
-static Load8 load_of(const DCache8& c, const DRows& r, int ratio) {
+static Load8 load_of(const DCache8& c, const DRows& r, int ratio, int seen) {
   const int64_t rows = (int64_t)r.tokens * ratio;
-  Load8 w{(rows / 16 + r.seqs) * c.heads, r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1, 16,
+  Load8 w{(rows / 16 + r.seqs) * c.heads, seen > UNIT ? (seen + UNIT - 1) / UNIT : 1, 16,
           256 * (c.dim == 64 ? RESIDENT<64, 16> : c.dim == 128 ? RESIDENT<128, 16> : RESIDENT<256, 16>)};
-  // Tiles of 32 rows read a head's tokens once where two of 16 would read them twice: from 17 rows a sequence, and four units a workgroup, which else have
+  // Tiles of 32 rows read a head's tokens once where two of 16 would read them twice: from 17 rows a sequence, and eight units a workgroup, which else have
   // what they start and end with to win back (128 channels, 8 cache heads, 4 query heads on one: 16 sequences of 4000 tokens, 5 tokens 49 us
   // against 60, 8 tokens 52 against 62, 4 tokens 47 against 45; 2 of 100000, 8 tokens 91 against 140; one of 8000, 8 tokens 27 against 25).  256 channels have no
   // registers for it (one workgroup a CU: 43 against 38).
-  if (c.dim < 256 && rows > (int64_t)16 * r.seqs && w.tiles * (w.units + EXTRA) > (int64_t)4 * w.chip)
+  if (c.dim < 256 && rows > (int64_t)16 * r.seqs && w.tiles * (w.units + EXTRA) > (int64_t)8 * w.chip)
     w = Load8{(rows / 32 + r.seqs) * c.heads, w.units, 32, 256 * (c.dim == 64 ? RESIDENT<64, 32> : RESIDENT<128, 32>)};
   return w;
 }
 struct Plan8 { int grid, rows; bool split; size_t bytes; };
-static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
-  const Load8 w = load_of(c, r, ratio);
+static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio, int seen) {
+  const Load8 w = load_of(c, r, ratio, seen);
   Plan8 p;
   p.rows = w.rows;
   // Tiles of few units stay in one piece, which saves the second launch, where there are enough of them: up to 8 units from a tile a CU, up to 16
@@ -331,18 +337,47 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio) {
   return p;
 }
 
-// Which of the two kernels.  That of cbk_cache8_prompt.hip takes tiles of 256 rows, filled or not, and wins from about 50 rows a sequence (128 channels, 8
-// cache heads, 16 sequences of 4096 tokens, bf16: 32 rows 69 against 56 us here, 64 rows 72 against 94, 128 rows 80 against 168; fp16: 88 and 55, 91 and 95, 99 and 168), but
-// only where there is work for the chip: it starts and joins more slowly (one sequence of 8192 tokens: 256 rows 62 against 40 us here, 384 rows 59 against 72;
-// of 1024 tokens: 2048 rows 53 against 36, 4096 rows 46 against 61).
-static bool many_rows(const DCache8& c, const DRows& r, int ratio) {
-  const int64_t rows = (int64_t)r.tokens * ratio;
-  if (rows <= (int64_t)48 * r.seqs) return false;
-  const int64_t tiles = (rows / 16 + r.seqs) * c.heads, units = r.cap > UNIT ? (r.cap + UNIT - 1) / UNIT : 1;
-  return tiles * (units + EXTRA) > (int64_t)4096 * (c.dim == 64 ? 4 : c.dim == 128 ? 3 : 2);
+// What a call is to take, in us, by the launches (their start, and the join behind a cut), the tiles of rows, and the units that each reads.  Which kernel, and
+// whether that for many rows cuts its tiles, is the least of three such times: a tile of 256 rows reads the cache a 16th as often as tiles of 16 and fills two
+// thirds of the chip's rate for an ordinary product, but is one workgroup a CU, filled or not, and a cut leaves 256 rows of float32 in memory for each
+// end.  Constants from 500 calls of 24 rows a sequence and more in all forms (1 to 64 sequences of 1 to 140000 tokens, 1 to 16 cache heads, windows),
+// each in all three ways: the least of the three estimates is within 1.2 % of the fastest on the (geometric) mean and within 9 % for 95 of 100.  For instance
+// (128 channels, bf16 unless said): 61 new of 85 tokens of 46 sequences, 4 cache heads x 4, 256 channels: few rows 104 us, whole 60, cut 103;
+// 1 sequence of 37 new behind 132000, 8 x 4, fp16: 210, 5788, 251; 180 new of 75000, 16 x 16, 256 channels, window of 39: 115, 38, 91; the last 512 of 16384 tokens, 8 x 4:
+// whole 469, cut 174; prompts of 3100 tokens, 8 x 2, fp16: whole 159, cut 124; of 4096, 8 x 4: whole 157, cut 190.
+struct Choice8 { bool many; PromptPlan prompt; Plan8 few; size_t bytes; };
+static Choice8 choose(const DCache8& c, const DRows& r, const AttnArgs& a, int window, int sinks) {
+  const int seen = seen_of(r, window, sinks);
+  const int64_t rows = (int64_t)r.tokens * a.ratio;
+  Choice8 x{};
+  x.few = plan_few(c, r, a.ratio, seen);
+  x.bytes = x.few.bytes;
+  if (rows <= (int64_t)16 * r.seqs) return x;
+  const Load8 w = load_of(c, r, a.ratio, seen);
+  const double slow = c.dim == 256 ? 1.2 : 1., unit = 2 + 1.1 * w.units, filled = (double)w.tiles / w.chip;
+  const double few = x.few.split ? (w.rows == 32 ? 16 : 14) + filled * (w.units + 2) * 2.5 * slow : 9 + fmax(unit, filled * unit * 2.2) * slow;
+  // tokens that a tile of 256 rows sees, in tiles of its own, at most and on average
+  const int keys = c.dim == 256 ? 64 : 128, least = r.cap < keys ? keys : r.cap;
+  const double limit = window > 0 ? fmin(least, (double)window + 256 / a.ratio + sinks + keys) : least;
+  const double mean = fmin(limit, fmax(least - 0.5 * r.tokens / r.seqs, 0.5 * least));
+  const double longest = ceil(limit / keys), usual = ceil(mean / keys), tiles = (double)(rows / 256 + r.seqs) * c.heads / 256;
+  const double step = c.dim == 64 ? (a.bf ? 2.2 : 3.6) : c.dim == 128 ? (a.bf ? 3.4 : 4.3) : a.bf ? 3.4 : 3.8;
+  const double start = c.dim == 64 ? 6 : c.dim == 128 ? 9 : 12, join = c.dim == 64 ? 25 : c.dim == 128 ? 31 : 49;
+  const double whole = 4 + fmax(start + longest * step, tiles * (start + usual * step)), cut = join + tiles * (usual + 2) * step;
+  x.many = fmin(whole, cut) < few;
+  if (x.many) {
+    x.prompt = plan_prompt8(c, r, a.ratio, cut < whole);
+    x.bytes = x.prompt.bytes;
+  }
+  return x;
 }
-size_t cache8_attn_workspace(const DCache8& c, const DRows& r, int ratio) {
-  return many_rows(c, r, ratio) ? plan_prompt8(c, r, ratio).bytes : plan_few(c, r, ratio).bytes;
+size_t cache8_attn_workspace(const DCache8& c, const DRows& r, int ratio) {   // (of either type)
+  AttnArgs a{};
+  a.ratio = ratio;
+  const size_t f16 = choose(c, r, a, 0, 0).bytes;
+  a.bf = 1;
+  const size_t bf16 = choose(c, r, a, 0, 0).bytes;
+  return f16 > bf16 ? f16 : bf16;
 }
 
 template <int D, int R>
@@ -359,9 +394,11 @@ static void few(const Plan8& p, const DCache8& c, const DRows& r, const AttnArgs
 int launch_cache8_attn(const DCache8& c, const DRows& r, AttnArgs a, size_t ws_bytes, hipStream_t st) {
   const size_t need = cache8_attn_workspace(c, r, a.ratio);
   if (need > ws_bytes || (need && !a.ws)) return CBK_ERR_WORKSPACE;
-  if (!need) a.ws = nullptr;
-  if (many_rows(c, r, a.ratio)) return launch_cache8_prompt(plan_prompt8(c, r, a.ratio), c, r, a, st);
-  const Plan8 p = plan_few(c, r, a.ratio);
+  Choice8 x = choose(c, r, a, a.window, a.sinks);
+  if (x.bytes > need) x = choose(c, r, a, 0, 0);                    // (the workspace is asked for without the window)
+  if (!x.bytes) a.ws = nullptr;
+  if (x.many) return launch_cache8_prompt(x.prompt, c, r, a, st);
+  const Plan8 p = x.few;
   a.whole = !p.split;
   if (c.dim == 64) few<64>(p, c, r, a, st);
   else if (c.dim == 128) few<128>(p, c, r, a, st);

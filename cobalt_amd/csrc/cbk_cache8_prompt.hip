@@ -16,7 +16,7 @@
 // bf16 results: queries with the scale of the scores in them and p rounded once to fp16 (an eighth of the result's own step).  fp16 results: queries as
 // they are, and p with its rest as a second operand.
 //
-// Work is dealt out in one of two ways (plan_prompt8).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
+// Work is dealt out in one of two ways (chosen in cbk_cache8_attn.hip).  Whole: a workgroup per tile of rows, the longest first.  Cut: as many
 // workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
 // of a tile that it does not finish is joined by the second launch (cbk_cache_attn.hip).
 //
@@ -440,17 +440,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
 }
 
 // ------------------------------------------------------------------ launch
-PromptPlan plan_prompt8(const DCache8& c, const DRows& r, int ratio) {
+PromptPlan plan_prompt8(const DCache8& c, const DRows& r, int ratio, bool cut) {
   PromptPlan p;
-  // Whole tiles where there are enough of them or where they are prompts, whose tiles are of all lengths and fill the chip one behind the
-  // other; equal shares where a few tiles stand behind long histories.  128 channels, 8 cache heads of 4 query heads, bf16, whole against cut: prompts of
-  // 1024 tokens 47 and 59 us, of 2048 78 and 91, of 4096 158 and 190; the last 512 of 2048 tokens 73 and 57, of 16384 469 and 174; the last 1024 of 4096 130
-  // and 103; 16 tokens of 16 sequences of 4096 110 and 71, of 32 (320 tiles) 115 and 118; 1000 of 6000 tokens of 8 (1060 tiles) 742 and 751.
   const int64_t tiles = ((int64_t)r.tokens * ratio / ROWS + r.seqs) * c.heads;   // at most
-  const bool prompts = 2 * (int64_t)r.tokens > (int64_t)r.cap * r.seqs;          // most of what the table can hold is new
-  p.cut = !prompts && tiles < 3 * CHIP;
-  p.grid = p.cut ? CHIP : tiles;
-  p.bytes = p.cut ? attn_bytes((int)p.grid, ROWS, c.dim) : 0;
+  p.cut = cut;
+  p.grid = cut ? CHIP : tiles;
+  p.bytes = cut ? attn_bytes((int)p.grid, ROWS, c.dim) : 0;
   return p;
 }
 

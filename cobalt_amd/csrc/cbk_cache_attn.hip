@@ -377,16 +377,29 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
   if (a.ws && !joined && tid == 0) desc->count = 0;
 }
 
-// One more part of a row: four channels of it, against the maximum so far
-template <int D>
-__device__ inline void add_part(const AttnArgs& a, int grid, int64_t part, int rows, int row, int d, float& top, float& sum, float (&y)[4]) {
-  const float* const x = attn_part<D>(a.ws, grid, part * rows + row);
-  const float4 o = *(const float4*)(x + d);
-  const float mm = x[D], ll = x[D + 1], up = fmaxf(top, mm);
-  const float f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(mm - up);
-  top = up;
-  sum = sum * f + ll * g;
-  y[0] = y[0] * f + o.x * g; y[1] = y[1] * f + o.y * g; y[2] = y[2] * f + o.z * g; y[3] = y[3] * f + o.w * g;
+// Every P-th part of a row from the p-th on: four channels of each, against the maximum so far.  U of them are loaded at a time, one behind the
+// other they would each cost the way to memory.
+template <int D, int R, int P, int U>
+__device__ inline void add_parts(const AttnArgs& a, int grid, int64_t w, const AttnPiece& e, int p, int row, int d, float& top, float& sum, float (&y)[4]) {
+  for (int i0 = p; i0 < e.count; i0 += U * P) {
+    float4 o[U];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * P, e.count - 1);
+      const float* const x = attn_part<D>(a.ws, grid, ((w + i) * 2 + (i ? 0 : e.slot)) * R + row);
+      o[u] = *(const float4*)(x + d);
+      ml[u] = *(const float2*)(x + D);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * P < e.count) {
+        const float up = fmaxf(top, ml[u].x), f = __builtin_amdgcn_exp2f(top - up), g = __builtin_amdgcn_exp2f(ml[u].x - up);
+        top = up;
+        sum = sum * f + ml[u].y * g;
+        y[0] = y[0] * f + o[u].x * g; y[1] = y[1] * f + o[u].y * g; y[2] = y[2] * f + o[u].z * g; y[3] = y[3] * f + o[u].w * g;
+      }
+  }
 }
 
 // Rows of a tile that several workgroups have parts of.  Workgroup (x, y) takes row y of the tile that begins in workgroup x: D/4 threads a
@@ -401,7 +414,7 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int gr
   const int tid = threadIdx.x, d = 4 * (tid % C), p = tid / C, row = blockIdx.y;
   if (e.count == 0 || row >= e.valid) return;
   float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = p; i < e.count; i += P) add_part<D>(a, grid, (w + i) * 2 + (i ? 0 : e.slot), R, row, d, top, sum, y);
+  add_parts<D, R, P, 4>(a, grid, w, e, p, row, d, top, sum, y);
   *(float4*)&sh[p][d] = make_float4(y[0], y[1], y[2], y[3]);
   if (d == 0) { sh[p][D] = top; sh[p][D + 1] = sum; }
   __syncthreads();
@@ -432,7 +445,7 @@ __global__ __launch_bounds__(256) void cache_prompt_join_kernel(AttnArgs a, int 
   const int end = min(((int)blockIdx.y + 1) * SHARE, e.valid);
   for (int row = blockIdx.y * SHARE + wave; row < end; row += 4) {
     float top = FLOOR, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = p; i < e.count; i += P) add_part<D>(a, grid, (w + i) * 2 + (i ? 0 : e.slot), R, row, d, top, sum, y);
+    add_parts<D, R, P, 4>(a, grid, w, e, p, row, d, top, sum, y);
 #pragma unroll
     for (int by = C; by < 64; by *= 2) {
       const float up = fmaxf(top, __shfl_xor(top, by)), f = __builtin_amdgcn_exp2f(top - up);

@@ -472,6 +472,29 @@ def test_histories_of_some_length_in_one_piece(lens, heads, dim):
     s.attend([min(n, 7) for n in lens], 4)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_drafts_over_many_and_over_long_histories(dim, dtype):
+    """Tiles of 32 rows, in one piece and cut, their last rows empty."""
+    s = Setup([1100, 800, 40] * 13 + [1100], 8, dim, 64, 16, dtype, seed=3)
+    s.attend([min(n, 3) for n in s.lens], 8)
+    s.attend([min(n, 3) for n in s.lens], 8, window=700, sinks=3)
+    s = Setup([11000, 300, 9000, 10000, 8000, 9500, 11000], 8, dim, 64, 64, dtype, seed=4)
+    s.attend([5, 3, 7, 5, 6, 5, 5], 4)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts_and_chunks_of_them(dim, dtype):
+    """The kernel for many rows, a tile of rows one workgroup's and cut."""
+    s = Setup([900, 300, 0, 500], 8, dim, 64, 16, dtype, seed=5)
+    s.attend([900, 300, 0, 500], 4)
+    s.attend([900, 300, 0, 500], 4, window=200, sinks=5)
+    s = Setup([3001, 700], 8, dim, 64, 32, dtype, seed=6)
+    s.attend([300, 500], 4)
+    s.attend([300, 500], 4, window=2500, sinks=100)
+
+
 def test_many_sequences():
     """More sequences than a workgroup has threads, most of them short, some empty."""
     g = np.random.default_rng(0)
