@@ -323,15 +323,17 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(DCache8 c, DRows r, Ca
   });
 }
 
-// Rows a wavefront (or, in wide blocks, a workgroup) walks through: one, whose wavefront ends at once if it begins no block, or all that fit a block.
-// One after the other they cost their loads (256 sequences' single tokens: 52 us against 9), wavefronts that end their start (a prompt of 16384 tokens: 173 against 24;
-// 16 x 64 tokens 17 against 8.6; 64 x 8 tokens 11.5 against 17.6, 256 x 12 tokens 33 against 17.5).  All from half a chip of wavefronts on if the
-// sequences fill blocks, from all of it if they have eight rows; not more than a sequence has on average.  (8 heads of 128 channels, blocks of 16.)
+// Rows a wavefront (or, in wide blocks, a workgroup) walks through: as many as leave 2048 wavefronts, but no more than a sequence has on average, or a block.
+// Those that begin no block end at once, and cost their start; blocks that one wavefront meets one behind the other cost their loads each.  Write, read, 8
+// heads of 128 channels, blocks of 16, us: 512 sequences' 4 tokens a row a wavefront 28 and 26, so 11.6 and 12.4, their single tokens 10.2 and 8.9 (16 rows
+// a wavefront 52 and 42); a prompt of 16384 tokens a row a wavefront 173 and 160, 16 rows 24 and 27; 16 sequences' 48 tokens 14.7, so 9.6, 16 rows 8.4;
+// 64 sequences' 8 tokens 11.6, so 9.6, 16 rows 17.6; 10 of 49 tokens in blocks of 256 28 with 256 rows a workgroup, so 9.8.
 static int chunk_of(const DCache8& c, const DRows& r, int block) {
   const int64_t waves = (int64_t)r.tokens * c.heads * (block / 16);
-  const int64_t each = r.seqs ? r.tokens / r.seqs : 0;
   if (waves >= (int64_t)1 << 25) return block;                      // (a launch has fewer than 2^32 threads)
-  return (each >= block && waves >= 4096) || (each >= 8 && waves > 8192) ? (int)(each < block ? each : block) : 1;
+  const int64_t each = r.seqs ? r.tokens / r.seqs : 1, most = each < block ? each : block, fit = (waves + 2047) / 2048;
+  const int64_t n = fit < most ? fit : most;
+  return n < 1 ? 1 : (int)n;
 }
 
 template <int D, int DT, int NW>

@@ -322,7 +322,7 @@ static Load8 load_of(const DCache8& c, const DRows& r, int ratio, int seen) {
     w = Load8{(rows / 32 + r.seqs) * c.heads, w.units, 32, 256 * (c.dim == 64 ? RESIDENT<64, 32> : RESIDENT<128, 32>)};
   return w;
 }
-struct Plan8 { int grid, rows; bool split; size_t bytes; };
+struct Plan8 { int grid, rows; bool split, wide; size_t bytes; };
 static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio, int seen) {
   const Load8 w = load_of(c, r, ratio, seen);
   Plan8 p;
@@ -334,6 +334,7 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio, int seen) {
   const int64_t most = p.split ? w.tiles * (w.units + EXTRA) : w.tiles;
   p.grid = (int)(most < w.chip ? most : w.chip);
   p.bytes = p.split ? attn_bytes(p.grid, p.rows, c.dim) : 0;
+  p.wide = p.grid > 200 * w.tiles;
   return p;
 }
 
@@ -403,7 +404,7 @@ int launch_cache8_attn(const DCache8& c, const DRows& r, AttnArgs a, size_t ws_b
   if (c.dim == 64) few<64>(p, c, r, a, st);
   else if (c.dim == 128) few<128>(p, c, r, a, st);
   else few<256>(p, c, r, a, st);
-  if (p.split) launch_cache_join(c.dim, a, p.grid, p.rows, st);
+  if (p.split) launch_cache_join(c.dim, a, p.grid, p.rows, st, p.wide);
   return hipGetLastError() == hipSuccess ? CBK_OK : CBK_ERR_HIP;
 }
 

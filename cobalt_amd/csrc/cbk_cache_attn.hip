@@ -403,11 +403,12 @@ __device__ inline void add_parts(const AttnArgs& a, int grid, int64_t w, const A
 }
 
 // Rows of a tile that several workgroups have parts of.  Workgroup (x, y) takes row y of the tile that begins in workgroup x: D/4 threads a
-// part, 1024/D parts side by side, there may be hundreds.  (x is turned by y: tiles often begin every so many workgroups, and workgroups go to
-// the XCDs in turn.  512 rows in 16 parts each took one XCD 68 us.)
-template <int D, int R>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(AttnArgs a, int grid) {
-  constexpr int C = D / 4, P = 256 / C;
+// part, 4T/D parts side by side, there may be hundreds.  (x is turned by y: tiles often begin every so many workgroups, and workgroups go to
+// the XCDs in turn.  512 rows in 16 parts each took one XCD 68 us.)  T: 256, or 1024 where tiles have 200 parts and more on average: one sequence of 120000
+// tokens on one head of 256 channels, 8-bit cache, 35 against 57 us with the launch before it; four of 60000, 192 parts each, 37 against 33.
+template <int D, int R, int T>
+__global__ __launch_bounds__(T) void cache_attn_join_kernel(AttnArgs a, int grid) {
+  constexpr int C = D / 4, P = T / C;
   __shared__ float sh[P][D + 4];
   const int64_t w = (blockIdx.x + blockIdx.y) % gridDim.x;
   const AttnPiece e = ((const AttnPiece*)a.ws)[w];
@@ -483,15 +484,16 @@ static AttnPlan plan_attn(const DCache& c, const DRows& r, int ratio) {
   return p;
 }
 template <int D>
-static void join1(const AttnArgs& a, int grid, int rows, hipStream_t st) {
-  if (rows == 16) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16>), dim3(grid, 16), dim3(256), 0, st, a, grid);
-  else if (rows == 32) hipLaunchKernelGGL((cache_attn_join_kernel<D, 32>), dim3(grid, 32), dim3(256), 0, st, a, grid);
+static void join1(const AttnArgs& a, int grid, int rows, bool wide, hipStream_t st) {
+  if (rows == 16 && wide) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16, 1024>), dim3(grid, 16), dim3(1024), 0, st, a, grid);
+  else if (rows == 16) hipLaunchKernelGGL((cache_attn_join_kernel<D, 16, 256>), dim3(grid, 16), dim3(256), 0, st, a, grid);
+  else if (rows == 32) hipLaunchKernelGGL((cache_attn_join_kernel<D, 32, 256>), dim3(grid, 32), dim3(256), 0, st, a, grid);
   else hipLaunchKernelGGL((cache_prompt_join_kernel<D>), dim3(grid, 16), dim3(256), 0, st, a, grid);
 }
-void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, hipStream_t st) {
-  if (dim == 64) join1<64>(a, grid, rows, st);
-  else if (dim == 128) join1<128>(a, grid, rows, st);
-  else join1<256>(a, grid, rows, st);
+void launch_cache_join(int dim, const AttnArgs& a, int grid, int rows, hipStream_t st, bool wide) {
+  if (dim == 64) join1<64>(a, grid, rows, wide, st);
+  else if (dim == 128) join1<128>(a, grid, rows, wide, st);
+  else join1<256>(a, grid, rows, wide, st);
 }
 
 // Which of the two kernels.  That of cbk_cache_prompt.hip takes tiles of 256 rows, filled or not, and wins from about 100 rows a sequence

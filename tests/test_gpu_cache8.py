@@ -462,6 +462,16 @@ def test_long_histories_are_cut_and_joined(lens, heads, ratio):
     s.attend([min(n, 3) for n in lens], ratio)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_one_tile_in_hundreds_of_pieces(dim, dtype):
+    s = Setup([70001], 1, dim, 128, 32, dtype, seed=7)
+    s.attend([1], 1)
+    s.attend([1], 16)
+    s.attend([5], 3, window=60000, sinks=10)
+
+
+
 @pytest.mark.parametrize("lens,heads,dim", [([1000] + [700, 1, 90] * 13, 8, 128), ([2000] + [1300, 0, 500, 129] * 25, 8, 64), ([1300, 2000, 20] * 25, 8, 128)])
 def test_histories_of_some_length_in_one_piece(lens, heads, dim):
     """Enough sequences of medium length that no history is cut."""
