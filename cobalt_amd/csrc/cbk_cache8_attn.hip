@@ -353,7 +353,7 @@ static Choice8 choose(const DCache8& c, const DRows& r, const AttnArgs& a, int w
   Choice8 x{};
   x.few = plan_few(c, r, a.ratio, seen);
   x.bytes = x.few.bytes;
-  if (rows <= (int64_t)16 * r.seqs) return x;
+  if (rows <= (int64_t)16 * r.seqs || (rows / 256 + r.seqs) * c.heads >= (int64_t)1 << 23) return x;   // (a launch of workgroups of 512 has fewer than 2^32 threads)
   const Load8 w = load_of(c, r, a.ratio, seen);
   const double slow = c.dim == 256 ? 1.2 : 1., unit = 2 + 1.1 * w.units, filled = (double)w.tiles / w.chip;
   const double few = x.few.split ? (w.rows == 32 ? 16 : 14) + filled * (w.units + 2) * 2.5 * slow : 9 + fmax(unit, filled * unit * 2.2) * slow;

@@ -514,6 +514,14 @@ def test_many_sequences():
     s.attend([min(n, 1) for n in lens], 2)
 
 
+@pytest.mark.parametrize("heads,dim", [(1, 64), (4, 128)])
+def test_many_short_prompts(heads, dim):
+    g = np.random.default_rng(1)
+    s = Setup([int(x) for x in g.integers(0, 60, 600)], heads, dim, 16, 16, BF16, seed=9)
+    s.attend(s.lens, 8)
+    s.attend([(n + 1) // 2 for n in s.lens], 8, window=10, sinks=2)
+
+
 def test_rows_that_see_nothing_are_zero():
     s = Setup([100, 40, 30], 2, 128, 16, 16, F16)
     q = torch.randn(5, 4, 128, device=DEV).half()
