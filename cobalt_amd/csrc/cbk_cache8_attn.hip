@@ -125,14 +125,11 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
     // keys of the next step are under way while this one's values are worked on, and the other way round
     int pg[2], pg_next[2];
     pages_of(token_of(u0), pg);
-    fetch_keys(token_of(u0), pg);
-    fetch_values(token_of(u0), pg);
-    pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
-
-    // ---- queries: fragments, positions and factors
+    // ---- queries: loaded while the pages are looked up, made ready while the first codes are on their way
     v8h q[NC][KS];
     float cs[NC];
     Sight sight[NC];
+    v4u raw[NC][KS];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int row = row0 + 16 * n + col;
@@ -140,19 +137,24 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
       const int tok = is ? row / a.ratio : 0, hq = h * a.ratio + (is ? row % a.ratio : 0);
       sight[n] = sight_of(s.pos0 + (is ? tok : (row0 + valid - 1) / a.ratio), s.held, a);
       const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.first + tok) * a.qt + (int64_t)hq * a.qh;
-      v4u raw[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) raw[k] = is ? *(const v4u*)(qp + 64 * (k >> 1) + 16 * h4 + 8 * (k & 1)) : v4u{};
+      for (int k = 0; k < KS; ++k) raw[n][k] = is ? *(const v4u*)(qp + 64 * (k >> 1) + 16 * h4 + 8 * (k & 1)) : v4u{};
+    }
+    fetch_keys(token_of(u0), pg);
+    fetch_values(token_of(u0), pg);
+    pages_of(token_of(min(u0 + 1, u1 - 1)), pg_next);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
       float top = 0.f, down;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) top = bits_top(raw[k], BF, top);
+      for (int k = 0; k < KS; ++k) top = bits_top(raw[n][k], BF, top);
       top = across_max(top);
       cs[n] = a.scale * row_factor(top, down);
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t two = raw[k][i];
+          const uint32_t two = raw[n][k][i];
           const float x0 = BF ? __uint_as_float(two << 16) : h2f((uint16_t)two), x1 = BF ? __uint_as_float(two & 0xffff0000u) : h2f((uint16_t)(two >> 16));
           q[n][k][2 * i] = (_Float16)(x0 * down);
           q[n][k][2 * i + 1] = (_Float16)(x1 * down);
