@@ -49,7 +49,9 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
   const int col = lane & 15, h4 = lane >> 4;
 
   // ---- this workgroup's piece of the list
-  auto units = [&](int b) { return units_of(r, a, c.heads, b, R); };
+  const bool lanes = r.seqs <= 64;                                  // each lane has a sequence, which saves the loads below
+  const Seq mine = lanes ? seq_of(r, min(lane, r.seqs - 1)) : Seq{};
+  auto units = [&](int b) { return units_of(lanes ? mine : seq_of(r, b), a, c.heads, R); };
   const Index list(r.seqs, lane, units);
   const int64_t total = list.total, pieces = min((int64_t)gridDim.x, total);
   const int64_t w = blockIdx.x;
@@ -62,12 +64,12 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
   const int64_t begin = shares.begin(w), end = shares.end(w);
   int64_t base;
   int b = list.find(begin, base, units);
+  Seq s = lanes ? of_lane(mine, b) : seq_of(r, b);
   int64_t at = begin;
   int joined = 0;
 
   while (at < end) {
     // ---- one head's tile of rows and the units of it that are this workgroup's
-    const Seq s = seq_of(r, b);
     const Range g = range_of(s, a);
     const int rows = s.n * a.ratio, tiles = (rows + R - 1) / R;
     const int weight = a.whole ? 1 : g.units + EXTRA;
@@ -75,6 +77,7 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
     if (at >= base + all) {
       base += all;
       if (++b == r.seqs) break;                                     // (there is a next one, unless lengths change under the call)
+      s = seq_of(r, b);
       continue;
     }
     const int64_t item = quotient(at - base, weight), start = base + item * weight;

@@ -42,6 +42,9 @@ __device__ inline int64_t shift_up(int64_t x, int by, int lane) {   // the value
 __device__ inline int64_t of_lane(int64_t x, int l) {
   return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
 }
+__device__ inline Seq of_lane(const Seq& s, int l) {
+  return Seq{__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.pos0, l), __builtin_amdgcn_readlane(s.held, l)};
+}
 __device__ inline int64_t scan64(int64_t x, int lane) {             // sum of the lanes up to this one
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) x += shift_up(x, o, lane);
@@ -181,8 +184,7 @@ __device__ inline Range range_of(const Seq& s, const AttnArgs& a) {
   return g;
 }
 
-__device__ inline int64_t units_of(const DRows& r, const AttnArgs& a, int heads, int b, int rows) {
-  const Seq s = seq_of(r, b);
+__device__ inline int64_t units_of(const Seq& s, const AttnArgs& a, int heads, int rows) {
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
   return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
 }

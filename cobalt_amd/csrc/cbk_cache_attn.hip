@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void cache_at
   const int col = lane & 15, h4 = lane >> 4;
 
   // ---- this workgroup's piece of the list
-  auto units = [&](int b) { return units_of(r, a, c.heads, b, R); };
+  auto units = [&](int b) { return units_of(seq_of(r, b), a, c.heads, R); };
   const Index list(r.seqs, lane, units);
   const int64_t total = list.total, pieces = min((int64_t)gridDim.x, total);
   const int64_t w = blockIdx.x;
