@@ -32,10 +32,10 @@ namespace cbk {
 
 constexpr int OWN8 = 2;                     // tiles of tokens that a tile of rows counts for by itself: its queries, its start and end
 
-// The larger of a lane's number and that of the lane 32 on, without the trip through LDS, which the stores of the next tile keep busy
+// The larger of a lane's number and that of the lane 32 on (not through LDS, which the stores of the next tile keep busy)
 __device__ inline float halves_max(float x) {
-  const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+  const Two h = halves(x);
+  return fmaxf(h.a, h.b);
 }
 
 template <int D>

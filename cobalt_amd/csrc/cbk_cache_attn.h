@@ -35,20 +35,25 @@ __device__ inline float* attn_part(uint8_t* ws, int64_t grid, int64_t row) {
   return (float*)(ws + (grid * (int64_t)sizeof(AttnPiece) + 255) / 256 * 256) + row * attn_row(D);
 }
 
-__device__ inline int64_t shift_up(int64_t x, int by, int lane) {   // the value of the lane `by` below, 0 at the start
-  const int lo = __shfl_up((int)x, by), hi = __shfl_up((int)(x >> 32), by);
-  return lane >= by ? (int64_t)hi << 32 | (uint32_t)lo : 0;
-}
 __device__ inline int64_t of_lane(int64_t x, int l) {
   return (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
 }
 __device__ inline Seq of_lane(const Seq& s, int l) {
   return Seq{__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.pos0, l), __builtin_amdgcn_readlane(s.held, l)};
 }
-__device__ inline int64_t scan64(int64_t x, int lane) {             // sum of the lanes up to this one
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) x += shift_up(x, o, lane);
-  return x;
+// The value of another lane: CTRL says of which, lanes without one and rows (of sixteen lanes) that are not in ROWS get 0
+template <int CTRL, int ROWS>
+__device__ inline int64_t moved(int64_t x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)hi << 32 | (uint32_t)lo;
+}
+__device__ inline int64_t scan64(int64_t x) {                       // sum of the lanes up to this one; all 64 are there
+  x += moved<0x111, 0xf>(x);                                        // 1, 2, 4, 8 lanes on in the row
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);                                        // the last lane of the row before, to the second and fourth
+  return x + moved<0x143, 0xc>(x);                                  // the last of the first half, to the second
 }
 
 // A quotient of numbers that are not negative and nearly always short: a division of 64-bit numbers takes some 150 instructions
@@ -78,7 +83,7 @@ struct Index {
     const int first = lane * each, last = min(first + each, seqs);
 #pragma unroll 4
     for (int b = first; b < last; ++b) sum += units(b);
-    sum = scan64(sum, lane);
+    sum = scan64(sum);
     total = of_lane(sum, 63);
   }
   // the sequence that unit `at` < total is of, and the unit it begins with
@@ -89,7 +94,7 @@ struct Index {
     if (each == 1 || q == 64) return min(q, seqs - 1);              // (64: lengths or offsets that change under the call)
     const int last = min((q + 1) * each, seqs);
     for (int j = q * each; j < last; j += 64) {
-      const int64_t to = scan64(j + lane < last ? units(j + lane) : 0, lane), here = of_lane(to, 63);
+      const int64_t to = scan64(j + lane < last ? units(j + lane) : 0), here = of_lane(to, 63);
       if (at < base + here) {
         const int l = __popcll(__ballot(base + to <= at));
         if (l) base += of_lane(to, l - 1);
@@ -188,13 +193,23 @@ __device__ inline int64_t units_of(const Seq& s, const AttnArgs& a, int heads, i
   const int64_t tiles = ((int64_t)s.n * a.ratio + rows - 1) / rows;
   return tiles * heads * (a.whole ? 1 : range_of(s, a).units + EXTRA);
 }
-__device__ inline float across_max(float x) {                       // over the four quarters of the wavefront
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+// Over the four quarters of the wavefront, without the trip through LDS: neighbouring quarters side by side, then the halves
+struct Two { float a, b; };
+__device__ inline Two quarters(float x) {
+  const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return Two{__uint_as_float(t[0]), __uint_as_float(t[1])};
+}
+__device__ inline Two halves(float x) {
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return Two{__uint_as_float(t[0]), __uint_as_float(t[1])};
+}
+__device__ inline float across_max(float x) {
+  const Two q = quarters(x), h = halves(fmaxf(q.a, q.b));
+  return fmaxf(h.a, h.b);
 }
 __device__ inline float across_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  const Two q = quarters(x), h = halves(q.a + q.b);
+  return h.a + h.b;
 }
 
 // ------------------------------------------------------------------ many rows: tiles of 256
