@@ -51,16 +51,19 @@ __host__ __device__ constexpr int key_dword(int w) {
 // The rows of sequence b: [first, first + n) of the call, token positions pos0 .. pos0 + n - 1, and the tokens the table
 // has pages for.  Offsets that are not ascending give rows that do not belong together, never rows outside the call.
 struct Seq { int first, n, pos0, held; };
-__device__ inline Seq seq_of(const DRows& r, int b) {
+__device__ inline Seq seq_from(const DRows& r, int s0, int s1, int len) {   // of its two offsets and its length
   Seq s;
-  int s0 = b * r.per, s1 = s0 + r.per;
-  if (r.starts) { s0 = r.starts[b]; s1 = r.starts[b + 1]; }
   s0 = min(max(s0, 0), r.tokens);
   s1 = min(max(s1, s0), r.tokens);
-  const int len = max(r.lens[b], 0);
+  len = max(len, 0);
   s.first = s0; s.n = s1 - s0; s.pos0 = len - s.n;
   s.held = min(len, r.cap);
   return s;
+}
+__device__ inline Seq seq_of(const DRows& r, int b) {
+  int s0 = b * r.per, s1 = s0 + r.per;
+  if (r.starts) { s0 = r.starts[b]; s1 = r.starts[b + 1]; }
+  return seq_from(r, s0, s1, r.lens[b]);
 }
 
 // page of token `pos` (not negative) of sequence b; -1: the table has none

@@ -45,6 +45,24 @@ __device__ inline Sixteens<CH> load16(const void* p, int64_t i) {
   return x;
 }
 __device__ inline v2s magnitudes(uint32_t w) { return __builtin_bit_cast(v2s, w & 0x7fff7fffu); }
+// The maxima over all lanes, without trips through LDS: neighbours, pairs, mirrored eights and sixteens, then quarters and halves
+template <int CTRL>
+__device__ inline v2s with_moved(v2s x) {
+  const uint32_t y = __builtin_amdgcn_update_dpp(0, (int)__builtin_bit_cast(uint32_t, x), CTRL, 0xf, 0xf, false);
+  return __builtin_elementwise_max(x, __builtin_bit_cast(v2s, y));
+}
+__device__ inline v2s across_lanes(v2s x) {
+  x = with_moved<0xb1>(x);
+  x = with_moved<0x4e>(x);
+  x = with_moved<0x141>(x);
+  x = with_moved<0x140>(x);
+  uint32_t w = __builtin_bit_cast(uint32_t, x);
+  const auto q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  x = __builtin_elementwise_max(__builtin_bit_cast(v2s, (uint32_t)q[0]), __builtin_bit_cast(v2s, (uint32_t)q[1]));
+  w = __builtin_bit_cast(uint32_t, x);
+  const auto h = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __builtin_elementwise_max(__builtin_bit_cast(v2s, (uint32_t)h[0]), __builtin_bit_cast(v2s, (uint32_t)h[1]));
+}
 template <int DT>
 __device__ inline float from16(uint16_t b) { return DT == CBK_F16 ? h2f(b) : bf2f(b); }
 
@@ -75,12 +93,18 @@ __device__ inline int sequence_of(const DRows& r, int t, int lane) {
 // What begins among rows [t, end): calls f(first row, rows, sequence, position of the first) for each run of one sequence's rows in
 // one block of 2^shift tokens.  Uniform over the workgroup.
 template <class F>
-__device__ inline void runs_from(const DRows& r, int t, int end, int shift, int lane, F f) {
-  int b = sequence_of(r, t, lane);
+__device__ inline void runs_from(const DRows& r, int t, int end, int shift, int lane, bool may, F f) {
+  // Up to 63 sequences: a lane has an offset and a length each, so that one load does not wait for the other (write and read, 16 sequences of 16 tokens 9.1 and
+  // 9.8 -> 8.3 and 9.4 us, with the event; 16 of 4000 70.3 and 77.4 -> 68.0 and 76.7; a read of 87000 tokens of 16 heads 184 -> 189, so not there)
+  const bool lanes = may && r.starts && r.seqs < 64;
+  const int offset = lanes ? r.starts[min(lane, r.seqs)] : 0, length = lanes ? r.lens[min(lane, r.seqs - 1)] : 0;
+  int b = lanes ? __popcll(__ballot(lane <= r.seqs && offset <= t)) - 1 : sequence_of(r, t, lane);
   while (t < end) {
     if (!r.starts) b = t / r.per;
     if (b >= r.seqs) return;
-    const Seq s = seq_of(r, max(b, 0));
+    const int at = max(b, 0);
+    const Seq s = lanes ? seq_from(r, __builtin_amdgcn_readlane(offset, at), __builtin_amdgcn_readlane(offset, at + 1), __builtin_amdgcn_readlane(length, at))
+                        : seq_of(r, at);
     if (b < 0 || t < s.first || t >= s.first + s.n) {               // in front of the first sequence, or behind this one
       if (r.starts && r.starts[b + 1] <= t) {                       // the next one's, or, where some are empty, a later one's
         ++b;
@@ -110,7 +134,7 @@ __global__ __launch_bounds__(64 * (NW == 1 ? 4 : NW)) void cache8_write_kernel(D
   if (first >= r.tokens) return;
   const Parts8 at(c, h, D);
   int turn = 0;
-  runs_from(r, (int)first, min((int)first + chunk, r.tokens), c.block_shift, lane, [&](int t, int rows, int b, int pos) {
+  runs_from(r, (int)first, min((int)first + chunk, r.tokens), c.block_shift, lane, true, [&](int t, int rows, int b, int pos) {
     const int from = pos & (16 * NW - 1);                           // the run is tokens [from, from + rows) of the block
     const uint32_t in = pos & (c.page - 1) & ~(16 * NW - 1);        // where the block begins in the page
     const bool anew = from == 0;
@@ -169,11 +193,7 @@ __global__ __launch_bounds__(64 * (NW == 1 ? 4 : NW)) void cache8_write_kernel(D
           }
     }
     v2s top = {tk.x > tk.y ? tk.x : tk.y, tv.x > tv.y ? tv.x : tv.y};
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const uint32_t other = __shfl_xor(__builtin_bit_cast(uint32_t, top), o);
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(v2s, other));
-    }
+    top = across_lanes(top);
     if constexpr (NW > 1) {                                         // (two places in turn: a wavefront may be a run ahead)
       if (lane == 0) top_sh[turn][part] = __builtin_bit_cast(uint32_t, top);
       __syncthreads();
@@ -255,7 +275,8 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(DCache8 c, DRows r, Ca
   const int64_t first = item / c.heads * chunk;
   if (first >= r.tokens) return;
   const Parts8 at(c, h, D);
-  runs_from(r, (int)first, min((int)first + chunk, r.tokens), 4, lane, [&](int t, int rows, int b, int pos) {
+  const bool few = (int64_t)r.tokens * c.heads < (int64_t)chunk << 15;   // wavefronts
+  runs_from(r, (int)first, min((int)first + chunk, r.tokens), 4, lane, few, [&](int t, int rows, int b, int pos) {
     const int page = pos < 0 ? -1 : page_of(c, r, b, pos), from = pos & 15;
     const uint32_t in = pos & (c.page - 1) & ~15;
     const uint64_t code = page < 0 ? 0 : at.code(page);
