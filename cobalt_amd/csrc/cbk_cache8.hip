@@ -14,8 +14,8 @@
 // whose row begins none end at once; large ones have one per `block` rows and walk through what begins there.
 //
 // Both kernels only move data (2 B in and 1 B out per number, or the other way round) and are bound by the bytes: 28600 tokens of 8 heads of 128 channels, bf16,
-// written in 35.4 us and read in 30.4 (5.0 and 5.8 TB/s; a large copy reaches 5.1); 32 single tokens, bound by a chain of look-ups (sequence, length, page, scale),
-// in 4.7 and 4.8 us.
+// written in 35.6 us and read in 29.6 (4.9 and 5.9 TB/s; a large copy reaches 5.1); 32 single tokens, bound by a chain of look-ups (sequence, length, page, scale),
+// in 4.4 and 4.8 us.
 #include "cbk_cache_io.h"
 #include "cbk_cache8.h"
 

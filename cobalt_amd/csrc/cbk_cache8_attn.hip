@@ -20,9 +20,9 @@
 // what a workgroup has of a head it does not finish goes to the workspace with its maximum and sum, and a second
 // launch joins the pieces.  Lengths are read on the device: the host knows none of them.
 //
-// Bound by the bytes of the cache where histories are long: two sequences, 269000 tokens (552 MB), 102.5 us and the join 6.3, 5.4 TB/s in the kernel; 32
-// sequences, 115000 tokens (236 MB), 50 and 4.8, of which some 8 are the chain of look-ups before the first load and the joins in LDS at the end.  One token over
-// 700 of history 7.7 us and 2.8, all of it that chain and the launches.
+// Bound by the bytes of the cache where histories are long: two sequences, 269000 tokens (552 MB), 101 us and the join 5.5, 5.5 TB/s in the kernel; 32
+// sequences, 115000 tokens (236 MB), 49 and 4.8, of which some 7 are the chain of look-ups before the first load and the joins in LDS at the end.  One token over
+// 700 of history 7.2 us and 2.8, all of it that chain and the launches.
 #include "cbk_cache8.h"
 #include "cbk_cache_attn.h"
 #include "cbk_cache8_attn.h"
@@ -350,7 +350,7 @@ static Plan8 plan_few(const DCache8& c, const DRows& r, int ratio, int seen) {
 // each in all three ways: the least of the three estimates is within 1.2 % of the fastest on the (geometric) mean and within 9 % for 95 of 100.  For instance
 // (128 channels, bf16 unless said): 61 new of 85 tokens of 46 sequences, 4 cache heads x 4, 256 channels: few rows 104 us, whole 60, cut 103;
 // 1 sequence of 37 new behind 132000, 8 x 4, fp16: 210, 5788, 251; 180 new of 75000, 16 x 16, 256 channels, window of 39: 115, 38, 91; the last 512 of 16384 tokens, 8 x 4:
-// whole 469, cut 174; prompts of 3100 tokens, 8 x 2, fp16: whole 159, cut 124; of 4096, 8 x 4: whole 157, cut 190.
+// whole 469, cut 174; prompts of 3100 tokens, 8 x 2, fp16: whole 159, cut 124; of 4096, 8 x 4: whole 155, cut 190.
 struct Choice8 { bool many; PromptPlan prompt; Plan8 few; size_t bytes; };
 static Choice8 choose(const DCache8& c, const DRows& r, const AttnArgs& a, int window, int sinks) {
   const int seen = seen_of(r, window, sinks);

@@ -20,7 +20,7 @@
 // workgroups as the chip holds, each with an equal share of the one list of all tiles of rows and their tokens; what a workgroup has
 // of a tile that it does not finish is joined by the second launch (cbk_cache_attn.hip).
 //
-// A 4096-token prompt of 32 query heads on 8, 128 channels: bf16 158 us, 870 TFLOP/s (a large library product reaches 1200), fp16 230 us with its half more
+// A 4096-token prompt of 32 query heads on 8, 128 channels: bf16 155 us, 890 TFLOP/s (a large library product reaches 1200), fp16 230 us with its half more
 // products; of 8192 tokens and 64 channels 366 and 555 us, where an exponential and five instructions a score bound it; 4096 tokens of 16 heads on
 // 4, 256 channels, 242 and 316 us.
 #include <type_traits>
