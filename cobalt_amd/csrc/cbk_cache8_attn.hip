@@ -11,8 +11,9 @@
 // its share.
 //
 // Held values are fp16 numbers, so keys and values are exact as operands: one instruction widens two codes and multiplies them
-// with their block's scale.  Query rows are operands as they are (bf16 of ordinary size is exact in fp16), rows of very large or small
-// numbers after division by a power of two; scores are exact up to float32.  p is kept at 2^7.5 times its size against the running
+// with their block's scale.  fp16 query rows are operands as they are; bf16 ones are rounded once to fp16, those whose largest number is below
+// 2^-6 or from 2^15 on divided by a power of two first: exact down to 2^-14 and off by 2^-25 at most below it, of rows that are divided 2^-40 of the
+// largest.  Scores are exact up to float32 but for that.  p is kept at 2^7.5 times its size against the running
 // maximum, so that what an fp16 cannot hold lies 2^-31 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
 // bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
 //
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(256, (RESIDENT<D, R>)) void cache8_attn_kernel(DCac
 #pragma unroll
       for (int k = 0; k < KS; ++k) top = bits_top(raw[n][k], BF, top);
       top = across_max(top);
-      cs[n] = a.scale * row_factor(top, down);
+      cs[n] = a.scale * row_factor8<BF>(top, down);
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll

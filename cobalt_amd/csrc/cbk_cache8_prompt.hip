@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache8_prompt_kernel(DCache8 c,
     top = fmaxf(top, __shfl_xor(top, 32));
     const float times = BF ? a.scale : 1.f;
     const float size = BF && top < __builtin_inff() ? fminf(top * times, 0x1.fffffep127f) : top;   // (of what `times` leaves)
-    grow = row_factor(size, down) * (BF ? 1.f : a.scale);
+    grow = row_factor8<BF>(size, down) * (BF ? 1.f : a.scale);
     if (!BF) grow = fminf(fmaxf(grow, 1e-30f), 0x1.fffffep127f);    // (a smaller one has every score at 0, a larger one every difference past any weight)
 #pragma unroll
     for (int k = 0; k < T::KS; ++k)

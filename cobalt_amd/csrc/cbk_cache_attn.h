@@ -122,13 +122,15 @@ __device__ inline v2h rest_of(v2h rounded, float e0, float e1) {
   return v2h{(_Float16)r0, (_Float16)r1};
 }
 
-// Power of two that a query row is divided by, and `down`, its reciprocal, for a largest magnitude `top`: 1 if the row (and sums of
-// 128 of its elements) is an ordinary fp16 row without it, else one that leaves [1, 2).  Also 1 for zeros and NaN.  An infinity makes the whole
+// Power of two that a query row is divided by, and `down`, its reciprocal, for a largest magnitude `top`: 1 if the row is an ordinary fp16 row
+// without it, from 2^-6 to 2^BITS (8 where sums of 128 of its elements are fp16 too), else one that leaves [2^(BITS - 1), 2^BITS): the larger what is
+// left, the smaller the elements beside `top` that an fp16 still holds, to 2^-(24 + BITS) of it.  Also 1 for zeros and NaN.  An infinity makes the whole
 // row NaN (`down` is): products that are -inf alone would leave a row without weights, which is a row that saw nothing.
+template <int BITS = 8>
 __device__ inline float row_factor(float top, float& down) {
   int e = 0;
-  if (!(top >= 0x1p-6f && top < 0x1p8f) && top > 0.f && top < __builtin_inff())
-    e = min(max((int)(__float_as_uint(top) >> 23), 1) - 127, 126);  // (e = 127 would need 2^-127, which is no normal number: [2, 4) then)
+  if (!(top >= 0x1p-6f && top < (float)(1 << BITS)) && top > 0.f && top < __builtin_inff())
+    e = max((int)(__float_as_uint(top) >> 23) - 126 - BITS, -126);
   down = top < __builtin_inff() ? __uint_as_float((uint32_t)(127 - e) << 23) : __builtin_nanf("");
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }

@@ -319,9 +319,9 @@ int cbk_cache_read(const cbk_cache* cache, const cbk_rows* rows, void* k, int64_
  *   out[t, hq] = sum_j softmax_j(scale q[t, hq] . k_j) v_j,   head hq reads cache head hq / (q_heads / heads),
  * over the tokens j <= i that the cache holds, i the row's own position, and with window > 0 only those with j > i - window
  * or j < sinks.  A row that sees no token is 0.  fp16 or bf16 in and out; scores, their maximum and all sums
- * in float32, operands of the products in fp16.  fp16: exact codes and queries, values rounded once, softmax weights as two
- * fp16.  bf16: keys, values, softmax weights and queries (with the scale in them) may each be rounded once to fp16, an eighth of
- * the result's own step.  A query with an infinity or a NaN gives NaN where it sees a token.  scale in [1e-30, 1e30], scores in the range of float32, q_heads at most 256 heads; out must not overlap q.  The result is the same from call to call, also on
+ * in float32, operands of the products in fp16.  fp16: exact codes, exact queries (in rows that pass 2^8, up to 2^-32 of
+ * their largest), values rounded once, softmax weights as two fp16.  bf16: keys, values, softmax weights and queries (with the scale
+ * in them) may each be rounded once to fp16, an eighth of the result's own step.  A query with an infinity or a NaN gives NaN where it sees a token.  scale in [1e-30, 1e30], scores in the range of float32, q_heads at most 256 heads; out must not overlap q.  The result is the same from call to call, also on
  * another workspace.  The workspace holds nothing between calls and needs no clearing:
  * cbk_cache_attention_workspace_bytes(), 256-byte aligned, one per call in flight. */
 size_t cbk_cache_attention_workspace_bytes(const cbk_cache* cache, const cbk_rows* rows, int q_heads);

@@ -432,6 +432,30 @@ def test_rows_of_all_sizes_side_by_side(n, dtype):
         s.check(q, ops.cache_attention(s.cache, q, s.rows([n]), scale=scale), [n], scale=scale)
 
 
+@pytest.mark.parametrize("large", [300.0, 4096.0, 60000.0])
+@pytest.mark.parametrize("dim,n,heads", [(64, 4, 2), (128, 4, 2), (256, 4, 2), (64, 700, 8), (128, 700, 8), (256, 700, 8)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_large_channel_leaves_the_small_ones(dtype, dim, n, heads, large):
+    """One channel of the queries thousands of times the others, over a group of keys that are 0: the scores are the others' alone.  Rows that pass 2^8 leave
+    [2^7, 2^8) and are held with steps of 2^-24, so that each element is off by 2^-25 max(1, large / 2^7) at most; bf16 ones may have the scale in them."""
+    def fill(s):
+        s.k *= 4
+        s.k[..., :32] = 0
+    s = Setup([700], heads, dim, 64, 32, dtype, outliers=False, seed=11, fill=fill)
+    q = 0.05 * torch.randn(n, 2 * heads, dim, generator=torch.Generator().manual_seed(12))
+    q[..., 5] = large
+    q = q.to(dtype)
+    out = ops.cache_attention(s.cache, q.to(DEV), s.rows([n]))
+    scale, qn, on = dim ** -0.5, q.double().numpy(), out.double().cpu().numpy()
+    for h in range(0, 2 * heads, 2 * heads - 1):
+        k = s.hk[:, h // 2]
+        o, spread, size, reach = R.attention(qn[:, h], k, s.hv[:, h // 2], np.arange(700 - n, 700), np.ones(700, bool), scale)
+        e = (SCORE[dtype] * reach + U + 2.0 ** -16)[:, None] + 2.0 ** -25 * max(1.0, large / 2 ** 7 * scale) * np.abs(k).sum(1).max()
+        tol = e / (1 - e) * spread + U * size
+        tol = tol + HALF[dtype] * (np.abs(o) + tol) + 2.0 ** -25
+        assert (np.abs(on[:, h] - o) <= tol).all(), (h, (np.abs(on[:, h] - o) / tol).max())
+
+
 def test_one_token_outweighs_a_long_history():
     """Weights 2^-20 of the largest, 30000 of them: 3 % of the sum, in p that fp16 could not tell from 0 as it is."""
     def fill(s):

@@ -670,6 +670,33 @@ def test_rows_of_all_sizes_side_by_side(n, heads, dtype):
             s.check(q, ops.cache_attention(s.cache, q, s.rows([n]), scale=scale), [n], scale=scale)
 
 
+@pytest.mark.parametrize("large", [300.0, 4096.0, 60000.0, 2.0 ** 20])
+@pytest.mark.parametrize("dim,n,heads", [(64, 4, 2), (128, 4, 2), (256, 4, 2), (64, 1100, 16), (128, 1100, 16), (256, 1100, 16)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_large_channel_leaves_the_small_ones(dtype, dim, n, heads, large):
+    """One channel of the queries thousands of times the others, over keys that are 0 there: the scores are the others' alone.  fp16 queries are exact operands;
+    bf16 ones are held with steps of 2^-24, times what leaves the largest in [2^14, 2^15), so that each is off by 2^-25 max(1, large / 2^14) at most."""
+    if dtype == F16 and large > 65504:
+        large = 65504.0
+
+    def fill(s):
+        s.k *= 4
+        s.k[..., 5] = 0
+    s = Setup([1100], heads, dim, 64, 32, dtype, outliers=False, seed=11, fill=fill)
+    q = 0.05 * torch.randn(n, 2 * heads, dim, generator=torch.Generator().manual_seed(12))
+    q[..., 5] = large
+    q = q.to(dtype)
+    out = ops.cache_attention(s.cache, q.to(DEV), s.rows([n]))
+    scale, qn, on = dim ** -0.5, q.double().numpy(), out.double().cpu().numpy()
+    for h in range(0, 2 * heads, 2 * heads - 1):
+        o, spread, size, reach = R8.attention(qn[:, h], s.hk[:, h // 2], s.hv[:, h // 2], np.arange(1100 - n, 1100), np.ones(1100, bool), scale)
+        tol = bound(o, spread, size, reach, dim, 1100, dtype)
+        if dtype == BF16:
+            e = 2.0 ** -25 * max(1.0, large / 2 ** 14) * np.abs(s.hk[:, h // 2]).sum(1).max()
+            tol = tol + 1.01 * e / (1 - e) * spread
+        assert (np.abs(on[:, h] - o) <= tol).all(), (h, (np.abs(on[:, h] - o) / tol).max())
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_scales_at_the_ends_of_their_range(dtype):
     s = Setup([1100], 16, 128, 32, 32, dtype, outliers=False, seed=3)
