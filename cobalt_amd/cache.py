@@ -15,7 +15,8 @@ from . import _lib
 class KVRows(NamedTuple):
     """Whose tokens the rows of a call are.  Dense tensors are [rows, heads, head_dim], the newest tokens of the sequences
     packed one behind the other: sequence b owns rows starts[b] to starts[b + 1] (`starts` None: equally many each), and the
-    last of them is its token lens[b] - 1.  Token j of sequence b is on page table[b, j // page].
+    last of them is its token lens[b] - 1.  Token j of sequence b is on page table[b, j // page].  A call may have fewer rows than the
+    offsets name: those it has are the same tokens as in a call with all of them.
 
     All three are int32 tensors on the cache's device and are read when the kernels run: nothing here is copied to the host,
     and a call recorded in a graph follows them; they must not change while it runs.  A table entry outside the pool (-1) is a page

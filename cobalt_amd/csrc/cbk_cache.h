@@ -49,14 +49,16 @@ __host__ __device__ constexpr int key_dword(int w) {
 }
 
 // The rows of sequence b: [first, first + n) of the call, token positions pos0 .. pos0 + n - 1, and the tokens the table
-// has pages for.  Offsets that are not ascending give rows that do not belong together, never rows outside the call.
+// has pages for.  Its offsets may name rows in front of the call's or behind them: those that are there keep their positions.  Offsets that are
+// not ascending give rows that do not belong together, never rows outside the call.
 struct Seq { int first, n, pos0, held; };
 __device__ inline Seq seq_from(const DRows& r, int s0, int s1, int len) {   // of its two offsets and its length
   Seq s;
   s0 = min(max(s0, 0), r.tokens);
-  s1 = min(max(s1, s0), r.tokens);
+  s1 = max(s1, s0);
   len = max(len, 0);
-  s.first = s0; s.n = s1 - s0; s.pos0 = len - s.n;
+  s.first = s0; s.n = min(s1, r.tokens) - s0;
+  s.pos0 = max(len - (s1 - s0), -(1 << 30));                        // (further down no row of fewer than 2^30 reaches token 0, and windows fit an int)
   s.held = min(len, r.cap);
   return s;
 }

@@ -293,7 +293,8 @@ typedef struct cbk_cache {
  * table[b * ld_table + j / page] of the pool.  All of these are DEVICE arrays of int32, read when the kernels
  * run: a recorded call follows them, and they must not change while it runs.  Nothing in them can lead outside the arrays: a table
  * entry outside [0, pages), or a token behind the table's last column, is a token the cache does not hold.  A row before
- * starts[0] or behind starts[seqs] belongs to no sequence and stays as it was. */
+ * starts[0] or behind starts[seqs] belongs to no sequence and stays as it was.  Of a sequence whose offsets pass the call's rows, those
+ * that are there are the tokens they would be in a call that has them all. */
 typedef struct cbk_rows {
   const void* table;
   int64_t ld_table;

@@ -211,6 +211,49 @@ def test_requests_through_tables_cache_and_attention(kind):
     assert tables.table.tolist() == ref.table
 
 
+@pytest.mark.parametrize("kind", ["4bit", "8bit"])
+@pytest.mark.parametrize("lens,starts,counts", [([40, 70, 33], [0, 5, 30, 42], [36, 20, 5, 3, 41]), ([40, 70, 33], [-3, 5, 30, 42], [36, 42]),
+                                                ([350, 400, 330], [0, 300, 620, 930], [800, 450, 929]), ([7, 40, 20], [0, 12, 30, 70], [50, 69])])
+def test_rows_that_the_call_does_not_have(kind, lens, starts, counts):
+    """Offsets that end behind the call's rows: those that are there are written, read and attended over as the tokens that `cache_slots` names."""
+    heads, dim, page = 2, 64, 16
+    per = [-(-n // page) for n in lens]
+    cols = max(per) + 1
+    table = [[sum(per[:b]) + i if i < per[b] else -1 for i in range(cols)] for b in range(len(lens))]
+    make = (lambda: KVCache(sum(per), heads, dim, page=page, device=DEV)) if kind == "4bit" else (lambda: KVCache8(sum(per), heads, dim, page=page, device=DEV))
+    rows = KVRows(ints(table), ints(lens), ints(starts))
+    full = KVRows(rows.table, rows.lens, ints([0, lens[0], lens[0] + lens[1], sum(lens)]))
+    bits = 1 << torch.arange(dim) % 10
+    named = lambda n: 1.0 + ((torch.arange(n)[:, None, None] & bits) != 0).expand(n, heads, dim).half()      # a row's number in its channels, 1 and 2
+    number = lambda x: ((x.cpu()[..., :10] > 1.5) * bits[:10]).sum(-1) - (x.cpu()[..., 0] < 0.5).int()       # (nothing held: -1)
+    first = torch.zeros(sum(lens), heads, dim)                      # values: 1 for each sequence's first token, of its mean a row tells how many it sees
+    first[[0, lens[0], lens[0] + lens[1]]] = 1
+    whole = make()
+    ops.cache_write(whole, torch.zeros(sum(lens), heads, dim).half().to(DEV), first.half().to(DEV), full)
+    for n in counts:
+        want = [-1] * sum(lens)
+        pos = []
+        for t in range(n):
+            b = max(i for i in range(3) if starts[i] <= t)
+            pos.append(lens[b] - (starts[b + 1] - t))
+            if pos[-1] >= 0:
+                want[sum(lens[:b]) + pos[-1]] = t
+        slots, positions = ops.cache_slots(whole, rows, n)
+        assert positions.tolist() == [max(j, 0) for j in pos]
+        cache = make()
+        x = named(n).to(DEV)
+        ops.cache_write(cache, x, x, rows)
+        for held in ops.cache_read(cache, full, sum(lens), torch.float32):
+            assert number(held).tolist() == [[w, w] for w in want]
+        for held in ops.cache_read(cache, rows, n, torch.float32):
+            assert number(held).tolist() == [[t if j >= 0 else -1] * heads for t, j in enumerate(pos)]
+        for ratio in (1, 16):                                       # few rows a sequence, and many
+            out = ops.cache_attention(whole, torch.zeros(n, heads * ratio, dim).half().to(DEV), rows).double().cpu()
+            seen = torch.where(out > 0, 1 / out.clamp(min=1e-9), torch.zeros_like(out))
+            # 1 / (pos + 1), of weights and a result that fp16 rounds: 2^-10 off at most, of 400 less than a half
+            assert torch.equal(seen.round().long(), torch.tensor([max(j + 1, 0) for j in pos])[:, None, None].expand_as(out))
+
+
 def test_a_recorded_step_takes_pages_as_it_grows():
     tables = KVPages(30, 3, 120, page=16, device=DEV)
     ref = R8.Tables(30, 3, 120, 16)
