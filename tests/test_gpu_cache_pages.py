@@ -123,6 +123,36 @@ def test_tables_that_do_not_belong_to_their_pool_stay_inside_it():
     assert guard == [x.numel() for x in t.native()[:4]]
 
 
+@pytest.mark.parametrize("seqs,cols,pages", [(2, 7, 8), (300, 20, 50), (200, 50, 900), (1024, 9, 100), (1500, 8, 64), (70000, 3, 1000)])
+def test_nothing_around_the_arrays_of_a_table_is_touched(seqs, cols, pages):
+    """Lengths, counts, entries and stacks of all kinds, as no pool has them, in one launch and in two: the arrays stand in one buffer, with other numbers between."""
+    rng, page, cap = random.Random(seqs), 16, 16 * cols
+    sizes = {"table": seqs * cols, "lens": seqs, "free": pages, "count": 1, "starts": seqs + 1, "want": seqs}
+    gap, at, place = 64, 64, {}
+    for name, n in sizes.items():
+        place[name] = (at, at + n)
+        at += n + gap
+    buffer = torch.full((at,), 0x5a5a5a5a, dtype=torch.int32, device=DEV)
+    part = {name: buffer[a:b] for name, (a, b) in place.items()}
+    t = KVPages(pages, seqs, cap, page=page, device=DEV)
+    t.table, t.lens, t.free, t.count = part["table"].view(seqs, cols), part["lens"], part["free"], part["count"]
+    between = torch.ones(at, dtype=torch.bool, device=DEV)
+    for a, b in place.values():
+        between[a:b] = False
+    ends = [-(1 << 31), -1, 0, 1, cap - 1, cap, cap + 1, 1 << 30, (1 << 31) - 1]
+    some = lambda n, top: [rng.choice(ends) if rng.random() < 0.3 else rng.randint(0, top) for _ in range(n)]
+    entries, stack = ints(some(sizes["table"], pages)), ints(some(pages, pages))
+    for count in (pages, 0, -3, pages // 2, 10 * pages, -(1 << 31), (1 << 31) - 1):
+        for lens, want in (([cap] * seqs, [0] * seqs), ([0] * seqs, [cap] * seqs), (some(seqs, cap), some(seqs, cap)), ([1] * seqs, some(seqs, 40)), (some(seqs, 40), [-1] * seqs)):
+            for name, x in (("lens", ints(lens)), ("want", ints(want)), ("count", ints([count])), ("table", entries), ("free", stack)):
+                part[name].copy_(x)
+            rows = ops.cache_pages(t, part["want"], starts=part["starts"])
+            ops.cache_slots(t, rows, 50)
+            assert bool((buffer[between] == 0x5a5a5a5a).all())
+            assert part["want"].tolist() == want
+            assert 0 <= int(t.count) <= pages and 0 <= int(t.lens.min()) and int(t.lens.max()) <= cap
+
+
 def test_slots_of_rows_of_all_kinds():
     table = ints([[3, 1, -1, 70], [0, 2, 9, -5], [4, 5, 6, 7]])
     pool = KVPages(8, 3, 64, page=16, device=DEV)
