@@ -882,7 +882,8 @@ PyObject* py_cache_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
       const GilRelease other_threads_run;
       const c10::DeviceGuard guard(p.t[0].device());
-      if (!starts.defined()) starts = p.p.seqs ? at::empty({p.p.seqs + 1}, p.t[0].options()) : at::zeros({1}, p.t[0].options());
+      if (!starts.defined()) starts = at::empty({p.p.seqs + 1}, p.t[0].options());
+      if (!p.p.seqs) starts.zero_();                                // (a call without sequences launches nothing)
       const at::Tensor ws = scratch(p.t[0], cbk_cache_pages_workspace_bytes(&p.p));
       rc = cbk_cache_pages(&p.p, want.const_data_ptr(), starts.mutable_data_ptr(), ws.defined() ? ws.mutable_data_ptr() : nullptr,
                            ws.defined() ? ws.nbytes() : 0, stream_of(p.t[0]));

@@ -387,8 +387,8 @@ typedef struct cbk_pages {
  * entries, the first on top; then the sequences take pages from the top in their order.  Once the pages do not last for a sequence, it and
  * all behind it that lack pages keep their lengths; a length that the table has no entries for is refused in the same way, alone.  lens
  * is what came of it.  starts (seqs + 1, or NULL): where the new rows of each sequence begin, when what they gained is packed one
- * behind the other, for a cbk_rows of table, lens and starts.  Nothing is waited for and nothing read by the host; calls on one pool
- * follow one another on a stream.  want may be lens itself, and else overlaps none of the pool's arrays; starts overlaps nothing.
+ * behind the other, for a cbk_rows of table, lens and starts.  Without sequences nothing
+ * is done, starts stays as it was.  Nothing is waited for and nothing read by the host; calls on one pool follow one another on a stream.  want may be lens itself, and else overlaps none of the pool's arrays; starts overlaps nothing.
  * The workspace holds nothing between calls: cbk_cache_pages_workspace_bytes() (0 for small tables), 256-byte aligned. */
 size_t cbk_cache_pages_workspace_bytes(const cbk_pages* pages);
 int cbk_cache_pages(const cbk_pages* pages, const void* want, void* starts, void* workspace, size_t workspace_bytes, void* stream);

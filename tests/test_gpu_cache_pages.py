@@ -153,6 +153,15 @@ def test_nothing_around_the_arrays_of_a_table_is_touched(seqs, cols, pages):
             assert 0 <= int(t.count) <= pages and 0 <= int(t.lens.min()) and int(t.lens.max()) <= cap
 
 
+def test_offsets_of_no_sequences():
+    t = KVPages(8, 1, 64, page=16, device=DEV)
+    t.table, t.lens = t.table[:0], t.lens[:0]
+    starts = torch.full((3,), 7, dtype=torch.int32, device=DEV)
+    rows = ops.cache_pages(t, ints([]), starts=starts[:1])
+    assert rows.starts.tolist() == [0] and starts.tolist() == [0, 7, 7]
+    assert ops.cache_pages(t, ints([])).starts.tolist() == [0] and int(t.count) == 8
+
+
 def test_slots_of_rows_of_all_kinds():
     table = ints([[3, 1, -1, 70], [0, 2, 9, -5], [4, 5, 6, 7]])
     pool = KVPages(8, 3, 64, page=16, device=DEV)
