@@ -348,7 +348,8 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(DCache8 c, DRows r, Ca
 // Those that begin no block end at once, and cost their start; blocks that one wavefront meets one behind the other cost their loads each.  Write, read, 8
 // heads of 128 channels, blocks of 16, us: 512 sequences' 4 tokens a row a wavefront 28 and 26, so 11.6 and 12.4, their single tokens 10.2 and 8.9 (16 rows
 // a wavefront 52 and 42); a prompt of 16384 tokens a row a wavefront 173 and 160, 16 rows 24 and 27; 16 sequences' 48 tokens 14.7, so 9.6, 16 rows 8.4;
-// 64 sequences' 8 tokens 11.6, so 9.6, 16 rows 17.6; 10 of 49 tokens in blocks of 256 28 with 256 rows a workgroup, so 9.8.
+// 64 sequences' 8 tokens 11.6, so 9.6, 16 rows 17.6; 10 of 49 tokens in blocks of 256 28 with 256 rows a workgroup, so 9.8.  Not helped by it: few rows into
+// wide blocks, a wavefront for each sixteen of which is started (256 sequences' 12 rows in blocks of 256, 128, 64 and 16: written in 34, 18, 11 and 6.5, read in 7).
 static int chunk_of(const DCache8& c, const DRows& r, int block) {
   const int64_t waves = (int64_t)r.tokens * c.heads * (block / 16);
   if (waves >= (int64_t)1 << 25) return block;                      // (a launch has fewer than 2^32 threads)

@@ -12,7 +12,7 @@
 //
 // Held values are fp16 numbers, so keys and values are exact as operands: one instruction widens two codes and multiplies them
 // with their block's scale.  fp16 query rows are operands as they are; bf16 ones are rounded once to fp16, those whose largest number is below
-// 2^-6 or from 2^15 on divided by a power of two first: exact down to 2^-14 and off by 2^-25 at most below it, of rows that are divided 2^-40 of the
+// 2^-6 or from 2^15 on divided by a power of two first: exact down to 2^-17 and off by 2^-25 at most below it, of rows that are divided 2^-39 of the
 // largest.  Scores are exact up to float32 but for that.  p is kept at 2^7.5 times its size against the running
 // maximum, so that what an fp16 cannot hold lies 2^-31 below the largest; for an fp16 result the rest p - fp16(p) is a second operand, for a
 // bf16 one, whose own step is eight times as large, it is left out, and the sum adds the rounded p.
